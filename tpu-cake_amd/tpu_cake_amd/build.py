@@ -1,4 +1,4 @@
-"""Build ``librpa.so`` for gfx950 in-tree with hipcc (``python -m tpu_cake_amd.build``).
+"""Build ``librpa.so`` and ``librpa_sparse.so`` for gfx950 in-tree with hipcc (``python -m tpu_cake_amd.build``).
 
 Also builds ``librpa_timeline.so``: the same sources with ``-DRPA_TIMELINE``, whose attention
 kernel records a per-workgroup timeline (read by ``tpu_cake_amd.timeline``); the product path
@@ -19,7 +19,9 @@ CSRC = PKG.parent / "csrc"
 INCLUDE = ROOT / "include"
 SOURCES = [CSRC / "rpa_kernels.hip"]
 HEADERS = [CSRC / "rpa_schedule.h", INCLUDE / "rpa.h"]
+SPARSE_SOURCES = [CSRC / "rpa_sparse.hip"]  # page allocation, K/V append, sparse attention (include/rpa_sparse.h)
 OUTPUT = PKG / "librpa.so"
+SPARSE_OUTPUT = PKG / "librpa_sparse.so"
 TIMELINE_OUTPUT = PKG / "librpa_timeline.so"
 ARCH = "gfx950"
 
@@ -29,6 +31,16 @@ def hipcc() -> str:
         if cand and pathlib.Path(cand).exists():
             return cand
     raise RuntimeError("hipcc not found")
+
+
+def sparse_command(output: pathlib.Path = SPARSE_OUTPUT) -> list[str]:
+    """As ``command``, without its no-NaN assumption: what the append and the choice of pages do
+    with NaN inputs is defined."""
+    return [
+        hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared",
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+        f"-I{INCLUDE}", f"-I{CSRC}", *[str(s) for s in SPARSE_SOURCES], "-o", str(output),
+    ]
 
 
 def command(output: pathlib.Path = OUTPUT, extra: list[str] | None = None) -> list[str]:
@@ -44,9 +56,9 @@ def command(output: pathlib.Path = OUTPUT, extra: list[str] | None = None) -> li
     ]
 
 
-def _start(output: pathlib.Path, extra: list[str]):
+def _start(output: pathlib.Path, make, *args):
     tmp = output.with_suffix(".so.tmp")
-    cmd = command(tmp, extra)
+    cmd = make(tmp, *args)
     return output, tmp, cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
 
 
@@ -62,11 +74,12 @@ def _finish(job, verbose: bool) -> pathlib.Path:
 
 
 def build(verbose: bool = False, timeline: bool = True) -> pathlib.Path:
-    """Compile every HIP source into ``librpa.so`` (always recompiles), and (``timeline``) the
-    timeline variant beside it, the two compilations in parallel.  Returns the product path."""
-    jobs = [_start(OUTPUT, [])]
+    """Compile every HIP source into ``librpa.so`` and ``librpa_sparse.so`` (always recompiles), and
+    (``timeline``) the timeline variant beside them, the compilations in parallel.  Returns the path
+    of ``librpa.so``."""
+    jobs = [_start(OUTPUT, command, []), _start(SPARSE_OUTPUT, sparse_command)]
     if timeline:
-        jobs.append(_start(TIMELINE_OUTPUT, ["-DRPA_TIMELINE"]))
+        jobs.append(_start(TIMELINE_OUTPUT, command, ["-DRPA_TIMELINE"]))
     out = [_finish(j, verbose) for j in jobs]
     return out[0]
 
