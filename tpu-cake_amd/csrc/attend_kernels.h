@@ -1,0 +1,388 @@
+// Attention over chosen pages: for each (token, kv head) a list of logical pages of its sequence.
+//
+// Mathematics: softmax over the keys x of the listed pages up to the token's position, one pass with a
+// running maximum m and sum l in fp32 (exp2 domain):  o = sum_x 2^(s_x - m) v_x / sum_x 2^(s_x - m).
+// On v_mfma_f32_16x16x32_bf16, 32 keys at a time: S = K Q^T (A: 16 keys x 32 dims, B: the group's heads as
+// 16 columns), O^T += V^T P^T (A: 16 dims x 32 keys).  A lane's scores are the keys its P operand needs,
+// so P moves between no lanes; V passes through LDS as key rows and comes back transposed
+// (ds_read_b64_tr_b16).  P is split into two bf16 parts, hi = bf16(p) and bf16(p - hi), each with its own
+// MFMA: nothing is rounded to 8 bits, and the second product hides behind the loads.  fp8 codes are exact
+// in bf16; K scales multiply the scores and V scales P, both in fp32.
+//
+// Every listed key of a row is read once, 2 D elem bytes at 2 Hkv D elem apart: HBM bounds decode rows.
+// Rows choose apart, so rows are what workgroups share nothing of: one row (its up to 16 heads) a
+// workgroup, its keys over four waves, each with its own (m, l, O), joined at the end through LDS.  With
+// few rows the list is split over workgroups as well, and a second launch joins their parts.
+#pragma once
+
+#include "select_kernels.h"
+
+namespace rpa_sparse {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.4028234663852886e38f;
+constexpr float kRescale = 8.f;      // the running maximum moves when a score passes it by more (log2)
+constexpr int kAttendWaves = 4;
+constexpr int kMaxBlocks = 1024;     // list blocks of a workgroup
+
+// What keys that do not exist read: zeros, so that P = 0 never meets a NaN.
+__device__ uint4 g_zero_row[64];
+
+struct AttendParams {
+  const uint16_t* q;
+  const uint8_t* kv;
+  const float* scales;
+  const int32_t *picked, *kv_lens, *table, *cu, *num_seqs;
+  uint16_t* out;
+  float* parts;  // splits > 1: (m, l) of 16 rows, then the rows' O, for each (row, split)
+  long long q_token, q_head;
+  int T, Hkv, G, D, P, S, N, PPS, K;
+  int tiles;                // 16-head tiles of a group
+  int width, subs, blocks;  // keys of a list block (a page, or 64 keys of one), blocks of a page, of a list
+  uint32_t magic;           // ceil(2^32 / width): v / width for v < 2^26 (width > 1)
+  int per, splits;          // blocks of a workgroup
+  float scale, cap, v_scale;  // scale: of q.k; times log2 e where cap is 0
+};
+
+__device__ __forceinline__ float swap_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float swap_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A wave's LDS accesses execute in order; this keeps the compiler from reordering them.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ u32x4 bf16_of_codes(uint32_t a, uint32_t b) {  // eight e4m3 codes, exactly
+  u32x4 w;
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true));
+  w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false));
+  w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
+  return w;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+// DP: dims of a row in registers and LDS (64, 128 or 256), FULL: D == DP.
+template <int DP, bool FULL, bool FP8>
+__global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams p) {
+  constexpr int kRow = DP * 2 + 32;                    // an LDS key row of V
+  constexpr int kWave = 32 * kRow;                     // a wave's V; later its 16 rows of O in fp32
+  constexpr int kORow = DP + 4;                        // floats
+  constexpr int kElem = FP8 ? 1 : 2;
+  constexpr int kLoads = DP * kElem / 64;              // 16-byte loads of a lane for a key row's K (or V)
+  constexpr int kSteps = DP / 32;
+  static_assert(16 * kORow * 4 <= kWave, "O rows fit the wave's V region");
+  extern __shared__ __align__(16) uint8_t lds[];
+  int* const s_row = (int*)lds;                        // a block's first pool row
+  int* const s_len = s_row + p.per;                    // its keys that the token sees
+  float* const s_ks = (float*)(s_len + p.per);         // fp8: its scales
+  float* const s_vs = s_ks + p.per;
+  uint8_t* const s_v = lds + ((size_t)p.per * (FP8 ? 16 : 8) + 15) / 16 * 16;
+  __shared__ float s_m[kAttendWaves][16], s_l[kAttendWaves][16];
+  __shared__ int s_end;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, j = lane / 16;
+  const int tile = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, h = pair % p.Hkv, t = pair / p.Hkv;
+  const int split = blockIdx.y;
+  if (tid == 0) s_end = 0;
+  const Place at = place_of(p.cu, p.num_seqs, p.kv_lens, p.N, t);
+  const int newest = newest_page(at, p.S, p.PPS);
+  __syncthreads();
+  if (newest >= 0) {
+    const int32_t* list = p.picked + (size_t)pair * p.K;
+    const int32_t* table = p.table + (size_t)at.seq * p.PPS;
+    for (int b = tid; b < p.per; b += 64 * kAttendWaves) {
+      const int block = split * p.per + b;
+      int row = 0, len = 0;
+      float ks = 0.f, vs = 0.f;
+      if (block < p.blocks) {
+        const int entry = block / p.subs, sub = block % p.subs;
+        const int page = list[entry];
+        if (page >= 0 && page <= newest) {
+          const int first = sub * p.width;
+          len = min(min(p.S - first, p.width), at.pos + 1 - (page * p.S + first));
+          len = max(len, 0);
+          const int phys = table[page];
+          if (phys < 0 || phys >= p.P) {
+            flag_error(RPA_SPARSE_ERR_PAGE);
+            len = 0;
+          } else {
+            row = phys * p.S + first;
+            if (FP8) {
+              const float* s = p.scales ? p.scales + ((size_t)phys * p.Hkv + h) * 2 : nullptr;
+              ks = s ? s[0] : 1.f, vs = s ? s[1] : 1.f;
+            }
+          }
+        }
+      }
+      s_row[b] = row;
+      s_len[b] = len;
+      if (FP8) s_ks[b] = ks, s_vs[b] = vs;
+      if (len > 0) atomicMax(&s_end, b + 1);
+    }
+  }
+  __syncthreads();
+  const int units = (s_end * p.width + 31) / 32;
+
+  // the group's queries, B operand: column n, dims of k-slot group j
+  bf16x8 q[kSteps];
+  {
+    const int head = tile * 16 + n;
+    const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + head) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int dim = FP8 ? 64 * (s / 2) + 16 * j + 8 * (s % 2) : 32 * s + 8 * j;
+      u32x4 w = {0, 0, 0, 0};
+      if (head < p.G && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+      q[s] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+
+  const int row_bytes = p.D * kElem;
+  const auto block_of = [&](int v) { return p.width == 1 ? v : (int)__umulhi((uint32_t)v, p.magic); };
+  u32x4 k[2][kLoads], v[2][kLoads];
+  uint32_t seen[2];  // bit n: key n of the 16 exists
+  const auto load = [&](int unit) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int key = unit * 32 + 16 * b + n, block = block_of(key), off = key - block * p.width;
+      const bool ok = block < p.per && off < s_len[min(block, p.per - 1)];
+      seen[b] = (uint32_t)__ballot(ok) & 0xffffu;
+      const uint8_t* src = (const uint8_t*)g_zero_row;
+      if (ok) src = p.kv + ((size_t)(s_row[block] + off) * (2 * p.Hkv) + 2 * h) * row_bytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int byte = 64 * i + 16 * j;
+        if (FULL || byte < row_bytes) {
+          k[b][i] = *(const u32x4*)(src + byte);
+          v[b][i] = *(const u32x4*)(src + row_bytes + byte);
+        } else {
+          k[b][i] = v[b][i] = u32x4{0, 0, 0, 0};
+        }
+      }
+    }
+  };
+
+  uint8_t* const tile_v = s_v + wave * kWave;
+  f32x4 o[DP / 16];
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = kLowest, l = 0.f;
+  int unit = wave;
+  if (unit < units) load(unit);
+  for (; unit < units; unit += kAttendWaves) {
+    f32x4 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const u32x4 a = FP8 ? bf16_of_codes(k[b][i / 2][2 * (i % 2)], k[b][i / 2][2 * (i % 2) + 1]) : k[b][FP8 ? 0 : i];
+        s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], s[b], 0, 0, 0);
+      }
+    }
+    wave_fence();  // the last unit's V has been read
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        uint8_t* dst = tile_v + (16 * b + n) * kRow + (FP8 ? 128 * i + 32 * j : 64 * i + 16 * j);
+        if (FP8) {
+          *(u32x4*)dst = bf16_of_codes(v[b][i][0], v[b][i][1]);
+          *(u32x4*)(dst + 16) = bf16_of_codes(v[b][i][2], v[b][i][3]);
+        } else {
+          *(u32x4*)dst = v[b][i];
+        }
+      }
+    wave_fence();
+    const uint32_t here[2] = {seen[0] >> (4 * j), seen[1] >> (4 * j)};
+    if (unit + kAttendWaves < units) load(unit + kAttendWaves);
+
+    float vs[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float ks[4] = {1.f, 1.f, 1.f, 1.f};
+      if (FP8) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int block = min(block_of(unit * 32 + 16 * b + 4 * j + r), p.per - 1);
+          ks[r] = s_ks[block], vs[b][r] = s_vs[block];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = s[b][r] * p.scale;
+        if (FP8) x *= ks[r];
+        if (p.cap != 0.f) x = p.cap * tanhf(x / p.cap) * kLog2e;
+        s[b][r] = here[b] >> r & 1 ? x : -__builtin_inff();
+      }
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    top = swap_max(top);
+    if (__ballot(top > m + kRescale)) {
+      const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[d] *= f;
+    }
+    u32x4 hi, lo;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float e[4], rest[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
+        l += e[r];
+        if (FP8) e[r] *= vs[b][r];
+        rest[r] = e[r] - (float)(__bf16)e[r];
+      }
+      hi[2 * b] = pack_bf16(e[0], e[1]), hi[2 * b + 1] = pack_bf16(e[2], e[3]);
+      lo[2 * b] = pack_bf16(rest[0], rest[1]), lo[2 * b + 1] = pack_bf16(rest[2], rest[3]);
+    }
+    typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+    const uint8_t* vt = tile_v + (4 * j + n / 4) * kRow + 8 * (n % 4);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
+      const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kRow + 32 * d));
+      const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
+    }
+  }
+
+  // join the waves
+  l = swap_sum(l);
+  if (j == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+  __syncthreads();  // every wave is done with its V, too
+  float all = s_m[0][n];
+#pragma unroll
+  for (int w = 1; w < kAttendWaves; ++w) all = fmaxf(all, s_m[w][n]);
+  const float f = __builtin_amdgcn_exp2f(m - all);
+  float* const mine = (float*)tile_v + n * kORow;
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) *(f32x4*)(mine + 16 * d + 4 * j) = o[d] * f;
+  __syncthreads();
+  const int rows = min(p.G - tile * 16, 16), quads = p.D / 4;
+  const size_t part = (size_t)blockIdx.x * p.splits + split;
+  float* const parts = p.parts + part * (32 + (size_t)min(p.G, 16) * p.D);
+  for (int i = tid; i < rows * quads; i += 64 * kAttendWaves) {
+    const int r = i / quads, d = i % quads * 4;
+    float top = s_m[0][r], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kAttendWaves; ++w) top = fmaxf(top, s_m[w][r]);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kAttendWaves; ++w) {
+      sum += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
+      x += *(const f32x4*)((const float*)(s_v + w * kWave) + r * kORow + d);
+    }
+    if (p.splits > 1) {
+      if (d == 0) parts[2 * r] = top, parts[2 * r + 1] = sum;
+      if (sum != 0.f) *(f32x4*)(parts + 32 + r * p.D + d) = x;
+      continue;
+    }
+    const float g = sum == 0.f ? 0.f : p.v_scale / sum;
+    *(u32x2*)(p.out + ((size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r) * p.D + d) =
+        sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x[0] * g, x[1] * g), pack_bf16(x[2] * g, x[3] * g)};
+  }
+}
+
+// The split form's second launch: one workgroup a (row, head tile), a thread for every four dims.
+__global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
+  const int tile = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, h = pair % p.Hkv, t = pair / p.Hkv;
+  const int rows = min(p.G - tile * 16, 16), quads = p.D / 4;
+  const size_t stride = 32 + (size_t)min(p.G, 16) * p.D;
+  const float* const first = p.parts + (size_t)blockIdx.x * p.splits * stride;
+  for (int i = threadIdx.x; i < rows * quads; i += 256) {
+    const int r = i / quads, d = i % quads * 4;
+    float top = kLowest;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, first[s * stride + 2 * r]);
+    float sum = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+      const float* part = first + s * stride;
+      const float l = part[2 * r + 1];
+      if (l == 0.f) continue;  // a part without keys has no O
+      const float f = __builtin_amdgcn_exp2f(part[2 * r] - top);
+      sum += l * f;
+      x += *(const f32x4*)(part + 32 + r * p.D + d) * f;
+    }
+    const float g = sum == 0.f ? 0.f : p.v_scale / sum;
+    *(u32x2*)(p.out + ((size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r) * p.D + d) =
+        sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x[0] * g, x[1] * g), pack_bf16(x[2] * g, x[3] * g)};
+  }
+}
+
+// ---- host side ----
+int check_attend(const rpa_sparse_shape_t* s) {
+  const int rc = check_sparse(s);
+  if (rc) return rc;
+  const long long subs = s->page_size <= 64 ? 1 : (s->page_size + 63) / 64;
+  if (s->num_tokens * (long long)s->num_q_heads > 0x7fffffffll)
+    return fail(RPA_E_INVALID, "num_tokens * num_q_heads overflows int32");
+  if (s->num_pages * subs > 1 << 24) return fail(RPA_E_UNSUPPORTED, "a list of more than 2^24 pages or 64-key parts of pages");
+  return RPA_OK;
+}
+
+struct AttendPlan {
+  int tiles, width, subs, per, splits;
+  long long blocks, rows;
+  size_t bytes;
+};
+
+constexpr long long kAttendFill = 1024;  // workgroups that fill the card: four on each of 256 CUs
+
+AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
+  AttendPlan r = {};
+  const int G = s.num_q_heads / s.num_kv_heads;
+  r.tiles = (G + 15) / 16;
+  r.rows = (long long)s.num_tokens * s.num_kv_heads * r.tiles;
+  r.width = s.page_size <= 64 ? s.page_size : 64;
+  r.subs = (s.page_size + r.width - 1) / r.width;
+  r.blocks = (long long)s.num_pages * r.subs;
+  // a workgroup's part: at least 128 keys, one unit a wave, and at most kMaxBlocks blocks
+  const long long least = (128 + r.width - 1) / r.width;
+  long long splits = r.rows ? (kAttendFill + r.rows - 1) / r.rows : 1;
+  if (splits > (r.blocks + least - 1) / least) splits = (r.blocks + least - 1) / least;
+  long long per = (r.blocks + splits - 1) / splits;
+  if (per > kMaxBlocks) per = kMaxBlocks;
+  r.per = (int)per;
+  r.splits = (int)((r.blocks + per - 1) / per);
+  if (r.splits > 1) r.bytes = (size_t)r.rows * r.splits * (32 + (size_t)(G < 16 ? G : 16) * s.head_dim) * 4;
+  return r;
+}
+
+template <int DP, bool FULL, bool FP8>
+void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t stream) {
+  const size_t lds = ((size_t)plan.per * (FP8 ? 16 : 8) + 15) / 16 * 16 + (size_t)kAttendWaves * 32 * (DP * 2 + 32);
+  attend_kernel<DP, FULL, FP8><<<dim3((unsigned)plan.rows, plan.splits), 64 * kAttendWaves, lds, stream>>>(p);
+}
+
+}  // namespace
+}  // namespace rpa_sparse

@@ -19,44 +19,6 @@
 namespace rpa_sparse {
 namespace {
 
-constexpr uint32_t kSumCap = 1u << 30;  // sums saturate here: limits (pages, tokens) are below this
-
-__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) {
-  const uint32_t s = a + b;  // a, b <= 2^30
-  return s < kSumCap ? s : kSumCap;
-}
-
-struct Pair {
-  uint32_t a, b;
-};
-
-// Exclusive sums of a pair over the workgroup's threads, and the workgroup's totals.  Saturating
-// addition of non-negative numbers is associative, so any order gives the same.
-template <int WAVES>
-__device__ __forceinline__ Pair scan_pairs(Pair v, Pair& total, Pair (*lds)) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  Pair inc = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t a = __shfl_up(inc.a, d), b = __shfl_up(inc.b, d);
-    if (lane >= d) inc = {sat_add(inc.a, a), sat_add(inc.b, b)};
-  }
-  __syncthreads();  // the last use of lds
-  if (lane == 63) lds[wave] = inc;
-  __syncthreads();
-  Pair before = {0, 0};
-  total = {0, 0};
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const Pair t = lds[w];
-    if (w == wave) before = total;
-    total = {sat_add(total.a, t.a), sat_add(total.b, t.b)};
-  }
-  Pair up = {__shfl_up(inc.a, 1), __shfl_up(inc.b, 1)};
-  if (lane == 0) up = {0, 0};
-  return {sat_add(before.a, up.a), sat_add(before.b, up.b)};
-}
-
 struct AssignParams {
   const int32_t *cached, *fresh;
   int32_t* table;

@@ -2,7 +2,10 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include "attend_kernels.h"
+#include "page_index.h"
 #include "paging_kernels.h"
+#include "select_kernels.h"
 
 using namespace rpa_sparse;
 
@@ -63,6 +66,116 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
   const int grid = (shape->num_requests - 1) / kReleaseSlice + 1;
   release_kernel<<<grid, kReleaseThreads, 0, (hipStream_t)stream>>>(p);
   return launched("release_pages");
+}
+
+int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void* values, const int32_t* slot_mapping,
+                  void* kv_pages, const float* kv_scales, float k_scale, float v_scale, int8_t* bounds,
+                  int8_t* exponents, void* stream) {
+  int rc = check_append(shape);
+  if (rc) return rc;
+  if (shape->num_tokens == 0) return RPA_OK;
+  if (!keys || !values || !slot_mapping || !kv_pages || !bounds != !exponents)
+    return fail(RPA_E_INVALID, "NULL tensor pointer");
+  if ((rc = check_strides("keys", keys, shape->k_token_stride, shape->k_head_stride))) return rc;
+  if ((rc = check_strides("values", values, shape->v_token_stride, shape->v_head_stride))) return rc;
+  if (!aligned16(kv_pages) || !aligned16(bounds)) return fail(RPA_E_INVALID, "kv_pages and bounds must be 16-byte aligned");
+  const AppendParams p = {(const uint16_t*)keys, (const uint16_t*)values, slot_mapping, (uint8_t*)kv_pages, kv_scales, k_scale,
+                          v_scale, bounds, exponents, shape->k_token_stride, shape->k_head_stride, shape->v_token_stride,
+                          shape->v_head_stride, (long long)shape->total_pages * shape->page_size, shape->num_tokens,
+                          shape->num_kv_heads, shape->head_dim, shape->page_size};
+  const int threads = 64 * (shape->num_kv_heads < 8 ? shape->num_kv_heads : 8);
+  const auto kernel = shape->kv_dtype == RPA_KV_FP8_E4M3 ? append_kernel<true> : append_kernel<false>;
+  kernel<<<shape->num_tokens, threads, 0, (hipStream_t)stream>>>(p);
+  return launched("append_kv");
+}
+
+size_t rpa_select_workspace_size(const rpa_sparse_shape_t* shape) {
+  return check_sparse(shape) == RPA_OK ? plan_select(*shape).bytes : 0;
+}
+
+int rpa_select_pages(const rpa_sparse_shape_t* shape, int32_t sink_pages, int32_t recent_pages, const void* q,
+                     const int8_t* bounds, const int8_t* exponents, const int32_t* kv_lens,
+                     const int32_t* page_indices, const int32_t* cu_q_lens, const int32_t* num_seqs,
+                     int32_t* selected_pages, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_sparse(shape);
+  if (rc) return rc;
+  if (sink_pages < 0 || recent_pages < 0 || (long long)sink_pages + recent_pages > shape->num_pages)
+    return fail(RPA_E_INVALID, "sink_pages and recent_pages must not be negative nor more than num_pages together");
+  if (shape->num_tokens == 0) return RPA_OK;
+  if (!q || !bounds || !exponents || !kv_lens || !page_indices || !cu_q_lens || !num_seqs || !selected_pages)
+    return fail(RPA_E_INVALID, "NULL tensor pointer");
+  if ((rc = check_strides("q", q, shape->q_token_stride, shape->q_head_stride))) return rc;
+  if (!aligned16(bounds)) return fail(RPA_E_INVALID, "bounds must be 16-byte aligned");
+  const SelectPlan plan = plan_select(*shape);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
+    return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  const SelectParams p = {(const uint16_t*)q, bounds, exponents, kv_lens, page_indices, cu_q_lens, num_seqs, selected_pages,
+                          (uint32_t*)workspace, shape->q_token_stride, shape->q_head_stride, shape->num_tokens,
+                          shape->num_kv_heads, shape->num_q_heads / shape->num_kv_heads, shape->head_dim,
+                          shape->total_pages, shape->page_size, shape->max_num_seqs, shape->pages_per_seq,
+                          shape->num_pages, sink_pages, recent_pages, plan.gp, plan.tokens, plan.stride, 0};
+  const hipStream_t s = (hipStream_t)stream;
+  return plan.steps == 2 ? launch_select<2>(plan, p, s) : plan.steps == 4 ? launch_select<4>(plan, p, s)
+                                                                          : launch_select<8>(plan, p, s);
+}
+
+size_t rpa_sparse_workspace_size(const rpa_sparse_shape_t* shape) {
+  return check_attend(shape) == RPA_OK ? plan_attend(*shape).bytes : 0;
+}
+
+int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse_options_t* options, const void* q,
+                               const void* kv_pages, const float* kv_scales, const int32_t* selected_pages,
+                               const int32_t* kv_lens, const int32_t* page_indices, const int32_t* cu_q_lens,
+                               const int32_t* num_seqs, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  int rc = check_attend(shape);
+  if (rc) return rc;
+  if (!options) return fail(RPA_E_INVALID, "options is NULL");
+  if (shape->num_tokens == 0) return RPA_OK;
+  if (!q || !kv_pages || !selected_pages || !kv_lens || !page_indices || !cu_q_lens || !num_seqs || !out)
+    return fail(RPA_E_INVALID, "NULL tensor pointer");
+  const bool fp8 = shape->kv_dtype == RPA_KV_FP8_E4M3;
+  if (kv_scales && !fp8) return fail(RPA_E_INVALID, "kv_scales requires fp8 kv_pages");
+  if ((rc = check_strides("q", q, shape->q_token_stride, shape->q_head_stride))) return rc;
+  if (!aligned16(kv_pages) || !aligned16(out)) return fail(RPA_E_INVALID, "kv_pages and out must be 16-byte aligned");
+  if (out == q) return fail(RPA_E_INVALID, "out must not be q");
+  const AttendPlan plan = plan_attend(*shape);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
+    return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  const float cap = options->soft_cap < 0.f ? -options->soft_cap : options->soft_cap;
+  AttendParams p = {};
+  p.q = (const uint16_t*)q, p.kv = (const uint8_t*)kv_pages, p.scales = kv_scales;
+  p.picked = selected_pages, p.kv_lens = kv_lens, p.table = page_indices, p.cu = cu_q_lens, p.num_seqs = num_seqs;
+  p.out = (uint16_t*)out, p.parts = (float*)workspace;
+  p.q_token = shape->q_token_stride, p.q_head = shape->q_head_stride;
+  p.T = shape->num_tokens, p.Hkv = shape->num_kv_heads, p.G = shape->num_q_heads / shape->num_kv_heads;
+  p.D = shape->head_dim, p.P = shape->total_pages, p.S = shape->page_size, p.N = shape->max_num_seqs;
+  p.PPS = shape->pages_per_seq, p.K = shape->num_pages;
+  p.tiles = plan.tiles, p.width = plan.width, p.subs = plan.subs, p.blocks = (int)plan.blocks;
+  p.magic = plan.width > 1 ? (uint32_t)((0x100000000ull + plan.width - 1) / plan.width) : 0;
+  p.per = plan.per, p.splits = plan.splits;
+  p.scale = options->sm_scale * options->k_scale * (cap != 0.f ? 1.f : kLog2e), p.cap = cap;
+  p.v_scale = options->v_scale;
+  const hipStream_t s = (hipStream_t)stream;
+  const int D = p.D;
+  if (fp8) {
+    if (D == 256) launch_attend<256, true, true>(plan, p, s);
+    else if (D == 128) launch_attend<128, true, true>(plan, p, s);
+    else if (D == 64) launch_attend<64, true, true>(plan, p, s);
+    else launch_attend<128, false, true>(plan, p, s);
+  } else {
+    if (D == 256) launch_attend<256, true, false>(plan, p, s);
+    else if (D == 128) launch_attend<128, true, false>(plan, p, s);
+    else if (D == 64) launch_attend<64, true, false>(plan, p, s);
+    else if (D < 64) launch_attend<64, false, false>(plan, p, s);
+    else launch_attend<128, false, false>(plan, p, s);
+  }
+  if ((rc = launched("sparse_paged_attention"))) return rc;
+  if (plan.splits > 1) {
+    join_kernel<<<(unsigned)plan.rows, 256, 0, s>>>(p);
+    return launched("sparse_paged_attention (join)");
+  }
+  return RPA_OK;
 }
 
 }  // extern "C"

@@ -8,7 +8,7 @@ reference's fused-plan surface (``tpu_cake_amd.fused``); the v1 Inkling decode
 contract (``experiment inkling-rpa``) runs through ``tpu_cake_amd.inkling``.
 """
 
-from . import fused, inkling, paging  # noqa: F401
+from . import fused, inkling, paging, sparse  # noqa: F401
 
 from .ops import (  # noqa: F401
     DEFAULT_MASK_VALUE,
@@ -30,6 +30,7 @@ __all__ = [
     "fused",
     "inkling",
     "paging",
+    "sparse",
     "dynamic_validate_inputs",
     "gather_kv",
     "ragged_paged_attention",

@@ -11,7 +11,7 @@ import os
 import pathlib
 import threading
 
-from ._lib import RpaError
+from ._lib import RPA_KV_BF16, RPA_KV_FP8_E4M3, RpaError  # noqa: F401
 
 LIB_PATH = pathlib.Path(__file__).with_name("librpa_sparse.so")
 ABI_VERSION = 1
@@ -28,6 +28,13 @@ def _struct(name: str, *fields: tuple) -> type:
 
 RpaPagingShape = _struct("RpaPagingShape", *((n, _i32) for n in (
     "num_requests", "pages_per_seq", "page_size", "free_capacity", "max_tokens")))
+RpaAppendShape = _struct("RpaAppendShape", *((n, _i32) for n in (
+    "num_tokens", "num_kv_heads", "head_dim", "total_pages", "page_size", "kv_dtype")), *((n, ctypes.c_int64) for n in (
+        "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")))
+RpaSparseShape = _struct("RpaSparseShape", *((n, _i32) for n in (
+    "num_tokens", "num_q_heads", "num_kv_heads", "head_dim", "total_pages", "page_size", "max_num_seqs", "pages_per_seq",
+    "kv_dtype", "num_pages")), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64))
+RpaSparseOptions = _struct("RpaSparseOptions", *((n, ctypes.c_float) for n in ("sm_scale", "soft_cap", "k_scale", "v_scale")))
 
 # name -> (result, argument types): every symbol include/rpa_sparse.h declares
 _SIGNATURES = {
@@ -36,6 +43,12 @@ _SIGNATURES = {
     "rpa_sparse_read_error_word": (ctypes.c_int, [ctypes.POINTER(_i32), _i32, _vp]),
     "rpa_assign_pages": (ctypes.c_int, [ctypes.POINTER(RpaPagingShape)] + [_vp] * 12),
     "rpa_release_pages": (ctypes.c_int, [ctypes.POINTER(RpaPagingShape)] + [_vp] * 8),
+    "rpa_append_kv": (ctypes.c_int, [ctypes.POINTER(RpaAppendShape)] + [_vp] * 5 + [ctypes.c_float] * 2 + [_vp] * 3),
+    "rpa_select_workspace_size": (_sz, [ctypes.POINTER(RpaSparseShape)]),
+    "rpa_select_pages": (ctypes.c_int, [ctypes.POINTER(RpaSparseShape), _i32, _i32] + [_vp] * 9 + [_sz, _vp]),
+    "rpa_sparse_workspace_size": (_sz, [ctypes.POINTER(RpaSparseShape)]),
+    "rpa_sparse_paged_attention": (ctypes.c_int, [ctypes.POINTER(RpaSparseShape), ctypes.POINTER(RpaSparseOptions)]
+                                   + [_vp] * 10 + [_sz, _vp]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
