@@ -2,6 +2,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "attend_kernels.h"
 #include "page_index.h"
 #include "paging_kernels.h"
@@ -113,7 +115,8 @@ int rpa_select_pages(const rpa_sparse_shape_t* shape, int32_t sink_pages, int32_
                           (uint32_t*)workspace, shape->q_token_stride, shape->q_head_stride, shape->num_tokens,
                           shape->num_kv_heads, shape->num_q_heads / shape->num_kv_heads, shape->head_dim,
                           shape->total_pages, shape->page_size, shape->max_num_seqs, shape->pages_per_seq,
-                          shape->num_pages, sink_pages, recent_pages, plan.gp, plan.tokens, plan.stride, 0};
+                          shape->num_pages, sink_pages, recent_pages, plan.gp, plan.gp == 4 ? 2 : plan.gp == 8 ? 3 : 4, plan.tokens, plan.stride, 0,
+                          (uint32_t)(0x100000000ull / (shape->head_dim / 8) + 1)};
   const hipStream_t s = (hipStream_t)stream;
   return plan.steps == 2 ? launch_select<2>(plan, p, s) : plan.steps == 4 ? launch_select<4>(plan, p, s)
                                                                           : launch_select<8>(plan, p, s);

@@ -61,6 +61,42 @@ __device__ __forceinline__ Pair scan_pairs(Pair v, Pair& total, Pair (*lds)) {
   return {sat_add(before.a, up.a), sat_add(before.b, up.b)};
 }
 
+// A wave's LDS accesses execute in order; this keeps the compiler from reordering them.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float swap_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float swap_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The largest of a value over the wave.
+__device__ __forceinline__ float wave_max(float v) {
+  const auto step = [&](auto dpp) {
+    v = fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(v), __float_as_uint(v), dpp(), 0xf, 0xf, false)));
+  };
+  step([] { return 0xB1; });   // quad_perm 1 0 3 2
+  step([] { return 0x4E; });   // quad_perm 2 3 0 1
+  step([] { return 0x141; });  // row_half_mirror
+  step([] { return 0x140; });  // row_mirror
+  return swap_max(v);
+}
+
 // ---- host side ----
 // The message of the thread's last failure: a fixed buffer, so that reporting one cannot throw.
 thread_local char g_last_error[256];
