@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
   const int split = blockIdx.y;
   if (tid == 0) s_end = 0;
   const Place at = place_of(p.cu, p.num_seqs, p.kv_lens, p.N, t);
-  const int newest = newest_page(at, p.S, p.PPS);
+  const int newest = newest_page(at.pos, p.S, p.PPS);
   __syncthreads();
   if (newest >= 0) {
     const int32_t* list = p.picked + (size_t)pair * p.K;

@@ -33,9 +33,9 @@ struct SelectParams {
   int T, Hkv, G, D, P, S, N, PPS, K, sink, recent;
   int gp;      // columns a token takes: G rounded up to 4, 8 or a multiple of 16
   int shift;   // log2 of gp, at most 4
-  int tokens;  // tokens a workgroup scores together
+  int tokens;  // tokens of a tile: consecutive ones of a sequence that a workgroup scores together
   long long stride;  // keys of a token's row: PPS rounded up to 16
-  int first;   // the split form's first token
+  int first;   // the split form's first tile
   uint32_t chunk_magic;  // ceil(2^32 / (D / 8)): i / (D / 8) for i < 2^27
 };
 
@@ -73,9 +73,50 @@ __device__ __forceinline__ Place place_of(const int32_t* cu, const int32_t* num_
   return t < begin || t >= end ? Place{-1, -1} : Place{lo, kv_lens[lo] - (end - t)};
 }
 
-__device__ __forceinline__ int newest_page(const Place& at, int S, int PPS) {
-  if (at.pos < 0) return -1;
-  const int page = at.pos / S;
+// The index-th tile of `size` (a power of two) consecutive tokens of one sequence: sequences in order,
+// ceil(q_len / size) tiles each, then the tokens past the last (seq -1).  There are at most
+// ceil(T / size) + N tiles.  count: its tokens, pos: its first token's position.
+struct Tile {
+  int seq, first, count, pos;
+};
+
+__device__ __forceinline__ Tile tile_of(const int32_t* cu, const int32_t* num_seqs, const int32_t* kv_lens, int N, int T, int size,
+                                        int index) {
+  if (size == 1) {
+    const Place at = index < T ? place_of(cu, num_seqs, kv_lens, N, index) : Place{-1, -1};
+    return {at.seq, index, index < T, at.pos};
+  }
+  const int lane = threadIdx.x % 64, shift = __builtin_ctz(size);
+  int begin = cu[min(lane, N - 1)], end = cu[min(lane, N - 1) + 1], len = kv_lens[min(lane, N - 1)];
+  const int n = min(max(*num_seqs, 0), N);
+  int before = 0;  // tiles of the sequences before this window's
+  for (int base = 0; base < n; base += 64) {
+    const int s = base + lane;
+    const int own = s < n && end > begin ? (end - begin + size - 1) >> shift : 0;
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(upto, d);
+      upto += lane >= d ? o : 0;
+    }
+    const int here = __popcll(__ballot(before + upto <= index));  // sequences of the window that lie before
+    if (here < 64) {
+      const int b = __shfl(begin, here), e = __shfl(end, here), l = __shfl(len, here);
+      const int first = b + ((index - before - __shfl(upto - own, here)) << shift);
+      return {base + here, first, first < 0 ? 0 : max(min(min(size, e - first), T - first), 0), l - (e - first)};
+    }
+    before += __shfl(upto, 63);
+    const int next = min(s + 64, N - 1);
+    begin = cu[next], end = cu[next + 1], len = kv_lens[next];
+  }
+  const int first = (n ? max(cu[n], 0) : 0) + ((index - before) << shift);
+  return {-1, first, max(min(size, T - first), 0), -1};
+}
+
+// The newest page of a token at `pos` (-1: it sees no key).
+__device__ __forceinline__ int newest_page(int pos, int S, int PPS) {
+  if (pos < 0) return -1;
+  const int page = pos / S;
   if (page >= PPS) {
     flag_error(RPA_SPARSE_ERR_LEN);
     return PPS - 1;
@@ -164,23 +205,24 @@ __device__ __forceinline__ int max_over(int v, int width) {
   return v;
 }
 
-// The keys of pages [begin, end) of one sequence (begin a multiple of 16; the last 16 may pass end) for
-// its local tokens [from, to), 16 pages a wave and turn, by wave `rank` of `waves`.  last[i]: local token
-// i's newest page.  keys: token i's row at i * p.stride (LDS or global).  The next turn's page ids are
+// The keys of pages [begin, end) of a sequence (begin a multiple of 16; the last 16 may pass end) for the
+// `count` tokens of a tile, 16 pages a wave and turn.  last[i]: token i's newest page.  keys: token i's row
+// at i * p.stride (LDS or global).  The next turn's page ids are
 // loaded behind this turn's index rows.  The code is kept short: every workgroup runs it a few times
 // only, and at first fetches it line by line.
-template <int STEPS>
+template <int STEPS, int WAVES>
 __device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int h, const int8_t* rows, const int* last,
-                                            int from, int to, int begin, int end, int rank, int waves, uint32_t* keys) {
+                                            int count, int begin, int end, uint32_t* keys) {
   constexpr int kRow = STEPS * 64 + 16;
   const int lane = threadIdx.x % 64, n = lane % 16, j = lane / 16;
   const int width = 1 << p.shift;
-  const int tile0 = from * p.gp / 16, tile1 = (to * p.gp + 15) / 16;  // column tiles of the tokens
+  const int columns = (count * p.gp + 15) / 16;  // tiles of 16
   const int32_t* table = p.table + (size_t)seq * p.PPS;
-  const int stride = waves * 16;
-  int next = table[min(begin + rank * 16 + n, end - 1)];
+  constexpr int kStride = WAVES * 16;
+  const int start = begin + threadIdx.x / 64 * 16;
+  int next = table[min(start + n, end - 1)];
 #pragma unroll 1
-  for (int first = begin + rank * 16; first < end; first += stride) {
+  for (int first = start; first < end; first += kStride) {
     int phys = next;
     if (phys < 0 || phys >= p.P) {
       flag_error(RPA_SPARSE_ERR_PAGE);
@@ -195,13 +237,13 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int 
       a[s] = off < 2 * p.D ? *(const i32x4*)(row + off) : i32x4{0, 0, 0, 0};
     }
     const int e = p.exps[at];
-    next = table[min(first + stride + n, end - 1)];
+    next = table[min(first + kStride + n, end - 1)];
     // a token's columns share its four pages: column i of 4, 8 or 16 writes page i % 4
     const int i = n % 4, page = first + 4 * j + i;
     const float grid = pow2(min(max(__shfl(e, 4 * j + i), kExpMin), kExpMax));
     int best[4];
 #pragma unroll 1
-    for (int c = tile0; c < tile1; ++c) {
+    for (int c = 0; c < columns; ++c) {
       i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -211,11 +253,11 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int m = max_over(acc[k], width);
-        best[k] = p.gp > 16 && c > tile0 ? max(best[k], m) : m;
+        best[k] = p.gp > 16 && c > 0 ? max(best[k], m) : m;
       }
-      if (p.gp > 16 && c + 1 < tile1) continue;  // one token over several tiles
+      if (p.gp > 16 && c + 1 < columns) continue;  // one token over several tiles
       const int token = p.gp > 16 ? 0 : (16 * c + n) >> p.shift;
-      if (token < from || token >= to) continue;
+      if (token >= count) continue;
       const int newest = last[token];
       const int value = i & 2 ? (i & 1 ? best[3] : best[2]) : (i & 1 ? best[1] : best[0]);
       const uint32_t k = ordered((float)value * grid);
@@ -225,111 +267,25 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int 
   }
 }
 
-// The scores of a workgroup's local tokens over pages [begin, begin + pages): runs of tokens of one
-// sequence are scored apart, by waves of their own where there are fewer runs than waves.
-template <int STEPS, int WAVES>
-__device__ __forceinline__ void score_tokens(const SelectParams& p, int h, const int8_t* rows, const int* seq, const int* last,
-                                             int begin, int pages, uint32_t* keys) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int runs = 0;
-  for (int i = 0; i < p.tokens; ++i) runs += i == 0 || seq[i] != seq[i - 1];
-  const int teams = min(runs, WAVES);
-  int run = -1;
-  for (int i = 0; i < p.tokens;) {
-    int to = i + 1;
-    while (to < p.tokens && seq[to] == seq[i]) ++to;
-    ++run;
-    const int visible = seq[i] < 0 ? 0 : last[to - 1] + 1;
-    if (run % teams == wave % teams && visible > p.K && visible > begin)
-      score_pages<STEPS>(p, seq[i], h, rows, last, i, to, begin, min(visible, begin + pages), wave / teams,
-                         (WAVES - wave % teams + teams - 1) / teams, keys);
-    i = to;
-  }
-}
-
 constexpr int kFew = 128;  // candidates that one wave ranks
 
-// What one wave shares with itself while it chooses for a row, and a workgroup.
 struct WaveTeam {
   alignas(16) uint32_t key[kFew + 4];
   int page[kFew];
 };
+
+// What a workgroup shares while it chooses for a row.
 template <int THREADS>
 struct Team {
   static constexpr int kGroups = 256;  // maxima that bound the choice
   int count[64];                       // zeroed before
-  Pair scan[THREADS / 64];
   uint32_t bound;                      // zeroed before
+  int found;                           // zeroed before
+  Pair scan[THREADS / 64];
   alignas(16) uint32_t top[kGroups];
-  alignas(16) uint32_t key[THREADS + 4];
-  int page[THREADS];
+  alignas(16) unsigned long long key[THREADS + 2];  // candidates: key, then the page's complement
+  alignas(16) int page[THREADS + 4];                // chosen pages by rank
 };
-
-// Of `found` candidates in page order, `need` < found or equal: this thread's (number c) is chosen if
-// fewer than `need` are higher, equal ones before it counting as higher.
-__device__ __forceinline__ bool ranks_among(const uint32_t* key, int found, int need, int c) {
-  const uint32_t k = c < found ? key[c] : 0u;
-  int rank = 0;
-#pragma unroll 4
-  for (int i = 0; i < (found + 3) / 4; ++i) {
-    const u32x4 o = ((const u32x4*)key)[i];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) rank += o[e] + (4 * i + e < c) > k;
-  }
-  return c < found && rank < need;
-}
-
-// A threshold that at least `need` of the team's keys reach, found two bits a step from the top by
-// counting; fewer than `need` keys are above the one of 16 steps.  Ends early when at most `enough` keys
-// reach it.  key(i), i < per: this thread's keys.
-template <int THREADS, int PER, typename Key>
-__device__ __forceinline__ uint32_t search(const Key& key, int per, int need, int enough, int steps, int* count) {
-  uint32_t threshold = 0;
-  for (int step = 0; step < steps; ++step) {
-    const int shift = 30 - 2 * step;
-    const uint32_t t1 = threshold | 1u << shift, t2 = threshold | 2u << shift, t3 = threshold | 3u << shift;
-    int c1 = 0, c2 = 0, c3 = 0;
-#pragma unroll
-    for (int i = 0; i < (PER ? PER : per); ++i) {
-      const uint32_t k = key(i);
-      c1 += __popcll(__ballot(k >= t1));
-      c2 += __popcll(__ballot(k >= t2));
-      c3 += __popcll(__ballot(k >= t3));
-    }
-    if (THREADS > 64) {
-      if (threadIdx.x % 64 == 0) {
-        atomicAdd(count + 4 * step, c1);
-        atomicAdd(count + 4 * step + 1, c2);
-        atomicAdd(count + 4 * step + 2, c3);
-      }
-      __syncthreads();
-      c1 = count[4 * step], c2 = count[4 * step + 1], c3 = count[4 * step + 2];
-    }
-    threshold = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : threshold;
-    const int reach = c3 >= need ? c3 : c2 >= need ? c2 : c1 >= need ? c1 : enough + 1;
-    if (reach <= enough) break;
-  }
-  return threshold;
-}
-
-// Writes the `need` highest of the team's keys' pages, ascending, of equal keys the first ones; more
-// than `need` keys are not 0.  Threads own consecutive keys; page(i): of this thread's i-th.
-template <int THREADS, int PER, typename Key, typename Page>
-__device__ __forceinline__ void take(const Key& key, const Page& page, int per, int need, int32_t* out, int* count, Pair* scan) {
-  const uint32_t threshold = search<THREADS, PER>(key, per, need, need, 16, count);
-  Pair own = {0, 0}, total;
-#pragma unroll
-  for (int i = 0; i < (PER ? PER : per); ++i) own.a += key(i) > threshold, own.b += key(i) == threshold;
-  Pair at = scan_pairs<THREADS / 64>(own, total, scan);
-  const uint32_t ties = (uint32_t)need - total.a;  // of the threshold's own key, the first ones
-#pragma unroll
-  for (int i = 0; i < (PER ? PER : per); ++i) {
-    const uint32_t k = key(i);
-    const bool above = k > threshold, equal = k == threshold;
-    if (above | (equal & (at.b < ties))) out[at.a + min(at.b, ties)] = page(i);
-    at.a += above, at.b += equal;
-  }
-}
 
 // The rows that list every page, and the forced pages of the others: before and behind the rest.
 // Returns how many of the others are wanted, 0: nothing is left to do.
@@ -345,46 +301,63 @@ __device__ __forceinline__ int choose_forced(const SelectParams& p, int n, int32
   return p.K - p.sink - p.recent;  // n > K >= sink + recent
 }
 
-// One wave writes the chosen pages of one row, ascending, from its n <= 64 * KPT keys.
+// The largest threshold that `need` of a wave's n keys reach, two bits a step from the top.
+template <typename Key>
+__device__ __forceinline__ uint32_t search_wave(const Key& key, int n, int need) {
+  uint32_t threshold = 0;
+  for (int shift = 30; shift >= 0; shift -= 2) {
+    const uint32_t t1 = threshold | 1u << shift, t2 = threshold | 2u << shift, t3 = threshold | 3u << shift;
+    int c1 = 0, c2 = 0, c3 = 0;
+    for (int i = 0; i < n; i += 64) {
+      const uint32_t k = key(i);
+      c1 += __popcll(__ballot(k >= t1));
+      c2 += __popcll(__ballot(k >= t2));
+      c3 += __popcll(__ballot(k >= t3));
+    }
+    threshold = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : threshold;
+  }
+  return threshold;
+}
+
+// One wave writes the chosen pages of one row, ascending, from its n keys.
 //
 // Few keys survive a cheap bound: where the 64 lanes' maxima hold `need` values of at least x, so do the
 // keys, and none below x is chosen.  x is the need-th largest maximum to 16 bits; of n random keys not many
 // more than `need` survive.  They are moved together and each is ranked against all of them.
-template <int KPT>
 __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_t* keys, int n, int32_t* out, WaveTeam& team) {
   const int lane = threadIdx.x % 64;
+  const unsigned long long below = (1ull << lane) - 1;
   const int need = choose_forced<64>(p, n, out);
   if (need == 0) return;
   out += p.sink;
-  uint32_t held[KPT], top = 0;  // pages lane, lane + 64, ...
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    held[i] = 0;
-    if (64 * i < n) held[i] = keys[min(64 * i + lane, n - 1)];
-  }
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {  // forced pages count as absent
-    held[i] = 64 * i + lane < n && held[i] != kForced ? held[i] : 0u;
-    top = max(top, held[i]);
-  }
-  const auto count = [&](uint32_t t) { return __popcll(__ballot(top >= t)); };
+  const auto key = [&](int i) {  // of page i + lane; forced pages and those past the row count as absent
+    const uint32_t k = keys[min(i + lane, n - 1)];
+    return i + lane < n && k != kForced ? k : 0u;
+  };
+  uint32_t top = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 64) top = max(top, key(i));
   uint32_t bound = 0;
+#pragma unroll 1
   for (int shift = 30; need <= 64 && shift >= 16; shift -= 2) {
     const uint32_t t1 = bound | 1u << shift, t2 = bound | 2u << shift, t3 = bound | 3u << shift;
-    const int c1 = count(t1), c2 = count(t2), c3 = count(t3);
+    const int c1 = __popcll(__ballot(top >= t1)), c2 = __popcll(__ballot(top >= t2)), c3 = __popcll(__ballot(top >= t3));
     bound = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : bound;
     if ((c3 >= need ? c3 : c2 >= need ? c2 : c1) == need) break;
   }
   bound = max(bound, 1u);
   int found = 0;
+  for (int i = 0; i < n; i += 256) {
+    uint32_t k[4];
 #pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    if (64 * i >= n) break;
-    const bool is = held[i] >= bound;
-    const unsigned long long who = __ballot(is);
-    const int to = found + __popcll(who & ((1ull << lane) - 1));
-    if (is && to < kFew) team.key[to] = held[i], team.page[to] = 64 * i + lane;
-    found += __popcll(who);
+    for (int u = 0; u < 4; ++u) k[u] = key(i + 64 * u);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned long long who = __ballot(k[u] >= bound);
+      const int to = found + __popcll(who & below);
+      if (k[u] >= bound && to < kFew) team.key[to] = k[u], team.page[to] = i + 64 * u + lane;
+      found += __popcll(who);
+    }
   }
   int written = 0;
   if (found <= kFew) {
@@ -392,63 +365,55 @@ __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_
     wave_fence();
 #pragma unroll 1
     for (int c = lane; c - lane < found; c += 64) {
-      const bool chosen = ranks_among(team.key, found, need, c);
+      const uint32_t k = c < found ? team.key[c] : 0u;
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < (found + 3) / 4; ++i) {
+        const u32x4 o = ((const u32x4*)team.key)[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += o[e] + (4 * i + e < c) > k;  // an equal key of an earlier page, too
+      }
+      const bool chosen = c < found && rank < need;
       const unsigned long long who = __ballot(chosen);
-      if (chosen) out[written + __popcll(who & ((1ull << lane) - 1))] = team.page[c];
+      if (chosen) out[written + __popcll(who & below)] = team.page[c];
       written += __popcll(who);
     }
     wave_fence();
     return;
   }
-  // too many: the threshold that `need` of all keys reach, its own key's first pages as far as they go
-  const uint32_t threshold = search<64, KPT>([&](int i) { return held[i]; }, KPT, need, need, 16, nullptr);
+  // too many: the threshold that `need` of all keys reach, and its own key's first pages as far as they go
+  const uint32_t threshold = search_wave(key, n, need);
   int above = 0, ties = 0;
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) above += __popcll(__ballot(held[i] > threshold));
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    const unsigned long long equal = __ballot(held[i] == threshold);
-    const bool chosen = held[i] > threshold ||
-                        (held[i] == threshold && ties + __popcll(equal & ((1ull << lane) - 1)) < need - above);
+  for (int i = 0; i < n; i += 64) above += __popcll(__ballot(key(i) > threshold));
+  for (int i = 0; i < n; i += 64) {
+    const uint32_t k = key(i);
+    const unsigned long long equal = __ballot(k == threshold);
+    const bool chosen = (k > threshold) | ((k == threshold) & (ties + __popcll(equal & below) < need - above));
     const unsigned long long who = __ballot(chosen);
-    if (chosen) out[written + __popcll(who & ((1ull << lane) - 1))] = 64 * i + lane;
+    if (chosen) out[written + __popcll(who & below)] = i + lane;
     written += __popcll(who), ties += __popcll(equal);
   }
 }
 
-// The same by a workgroup, for more keys, with barriers between its steps: 64 or 256 maxima bound the
-// choice, and each thread ranks one candidate.  KPT: keys a thread holds in registers, consecutive ones, a
-// multiple of 4; 0: any number, read again each time.  The row is allocated to a multiple of 16 keys.
-template <int THREADS, int KPT>
+// The same by a workgroup, for longer rows.  64 or 256 maxima bound the choice; candidates come together in
+// any order, each is ranked by key and page against all of them, and the chosen ones by page among
+// themselves, so the order of the atomics leaves no trace.
+template <int THREADS>
 __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* keys, int n, int32_t* out, Team<THREADS>& team) {
+  constexpr int kWaves = THREADS / 64;
   const int tid = threadIdx.x, lane = tid % 64;
   const int need = choose_forced<THREADS>(p, n, out);
   if (need == 0) return;
   out += p.sink;
-  const int per = KPT ? KPT : (n + THREADS - 1) / THREADS;
-  const int own = tid * per;
-  uint32_t held[KPT ? KPT : 4];
-  if (KPT) {
-#pragma unroll
-    for (int i = 0; i < KPT; i += 4) {
-      const u32x4 w = *(const u32x4*)(keys + (own + i < n ? own + i : 0));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) held[i + e] = w[e];
-    }
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) held[i] = own + i < n && held[i] != kForced ? held[i] : 0u;  // forced: absent
-  }
   const auto key = [&](int i) {
-    if (KPT) return held[KPT ? i : 0];
-    const uint32_t k = own + i < n ? keys[own + i] : 0u;
-    return k == kForced ? 0u : k;
+    const uint32_t k = keys[min(i, n - 1)];
+    return i < n && k != kForced ? k : 0u;
   };
-  const auto page = [&](int i) { return own + i; };
   const int groups = need <= 48 ? 64 : Team<THREADS>::kGroups;
   if (need <= groups / 4 * 3) {
     uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < (KPT ? KPT : per); ++i) top = max(top, key(i));
+#pragma unroll 8
+    for (int i = 0; i < n; i += THREADS) top = max(top, key(i + tid));
     const int wide = THREADS / groups;  // threads of a group, a power of two
     for (int d = 1; d < wide; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     if (tid % wide == 0) team.top[tid / wide] = top;
@@ -466,114 +431,161 @@ __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* ke
     }
     __syncthreads();
     const uint32_t bound = max(1u, team.bound);
-    Pair mine = {0, 0}, total;
+    for (int i = 0; i < n; i += 8 * THREADS) {
+      uint32_t k[8];
 #pragma unroll
-    for (int i = 0; i < (KPT ? KPT : per); ++i) mine.a += key(i) >= bound;
-    const Pair at = scan_pairs<THREADS / 64>(mine, total, team.scan);
-    const int found = (int)total.a;
+      for (int u = 0; u < 8; ++u) k[u] = key(i + THREADS * u + tid);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k[u] >= bound) {
+          const int to = atomicAdd(&team.found, 1);
+          if (to < THREADS) team.key[to] = (unsigned long long)k[u] << 32 | (uint32_t)~(i + THREADS * u + tid);
+        }
+    }
+    __syncthreads();
+    const int found = team.found;
     if (found <= THREADS) {
-      uint32_t to = at.a;
-      if (mine.a) {
-#pragma unroll
-        for (int i = 0; i < (KPT ? KPT : per); ++i)
-          if (key(i) >= bound) team.key[to] = key(i), team.page[to] = own + i, ++to;
-      }
-      if (tid < 4) team.key[found + tid] = 0;  // what the last four-word read passes
+      if (tid == 0) team.key[found] = 0;  // what the last two-word read passes
       __syncthreads();
-      const bool chosen = tid - lane < found && ranks_among(team.key, found, need, tid);
-      const unsigned long long who = __ballot(chosen);
-      int written = 0;
-      if (found > 64) {
-        if (lane == 0) team.top[tid / 64] = __popcll(who);
-        __syncthreads();
-        for (int w = 0; w < tid / 64; ++w) written += team.top[w];
+      if (tid < found) {
+        const unsigned long long mine = team.key[tid];
+        int rank = 0;
+#pragma unroll 4
+        for (int i = 0; i < found; i += 2) rank += (team.key[i] > mine) + (team.key[i + 1] > mine);
+        if (rank < need) team.page[rank] = ~(uint32_t)mine;
       }
-      if (chosen) out[written + __popcll(who & ((1ull << lane) - 1))] = team.page[tid];
+      if (tid < 4) team.page[need + tid] = 0x7fffffff;
+      __syncthreads();
+      for (int r = tid; r < need; r += THREADS) {
+        const int page = team.page[r];
+        int at = 0;
+#pragma unroll 4
+        for (int i = 0; i < need; i += 4) {
+          const i32x4 o = *(const i32x4*)(team.page + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) at += o[e] < page;
+        }
+        out[at] = page;
+      }
       return;
     }
   }
+  // too many: a search by thresholds with a barrier a step, over consecutive keys of each thread
+  const int per = (n + THREADS - 1) / THREADS, own = tid * per, end = min(own + per, n);
+  uint32_t threshold = 0;
   __syncthreads();
-  take<THREADS, KPT>(key, page, per, need, out, team.count, team.scan);
-}
-
-// Places the workgroup's tokens and rounds their queries.
-template <int STEPS, int WAVES>
-__device__ __forceinline__ void prepare_tokens(const SelectParams& p, int t0, int h, int* seq, int* last, int8_t* rows) {
-  const int wave = threadIdx.x / 64;
-  for (int i = wave; i < p.tokens; i += WAVES) {
-    const int t = t0 + i;
-    int8_t* const mine = rows + (size_t)i * p.gp * (STEPS * 64 + 16);
-    Place at = {-1, -1};
-    if (t < p.T) {
-      u32x4 w[kHeld];
-      load_queries(p, t, h, w);  // beside the metadata
-      at = place_of(p.cu, p.num_seqs, p.kv_lens, p.N, t);
-      round_queries<STEPS>(p, t, h, w, mine);
-    } else {
-      zero_queries<STEPS>(p, mine);
+#pragma unroll 1
+  for (int step = 0; step < 16; ++step) {
+    const int shift = 30 - 2 * step;
+    const uint32_t t1 = threshold | 1u << shift, t2 = threshold | 2u << shift, t3 = threshold | 3u << shift;
+    int c1 = 0, c2 = 0, c3 = 0;
+    for (int i = own; i < end; ++i) {
+      const uint32_t k = key(i);
+      c1 += k >= t1, c2 += k >= t2, c3 += k >= t3;
     }
-    const int newest = newest_page(at, p.S, p.PPS);
-    if (threadIdx.x % 64 == 0) seq[i] = newest < 0 ? -1 : at.seq, last[i] = newest;
+    if (c1) atomicAdd(&team.count[4 * step], c1);
+    if (c2) atomicAdd(&team.count[4 * step + 1], c2);
+    if (c3) atomicAdd(&team.count[4 * step + 2], c3);
+    __syncthreads();
+    c1 = team.count[4 * step], c2 = team.count[4 * step + 1], c3 = team.count[4 * step + 2];
+    threshold = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : threshold;
+  }
+  Pair mine = {0, 0}, total;
+  for (int i = own; i < end; ++i) mine.a += key(i) > threshold, mine.b += key(i) == threshold;
+  Pair at = scan_pairs<kWaves>(mine, total, team.scan);
+  const uint32_t ties = (uint32_t)need - total.a;  // of the threshold's own key, the first ones
+  for (int i = own; i < end; ++i) {
+    const uint32_t k = key(i);
+    const bool above = k > threshold, equal = k == threshold;
+    if (above | (equal & (at.b < ties))) out[at.a + min(at.b, ties)] = i;
+    at.a += above, at.b += equal;
   }
 }
 
-// One launch for rows whose keys fit the LDS: p.tokens consecutive tokens of a head share each page's index
-// row (one token a sequence in decode batches).  WAVE: rows of up to 64 * KPT keys, chosen by a wave each;
-// otherwise by the whole workgroup.
-template <int STEPS, int KPT, bool WAVE>
+// Rounds a tile's queries, a wave a token, and notes the tokens' newest pages.
+template <int STEPS, int WAVES>
+__device__ __forceinline__ void prepare_tile(const SelectParams& p, const Tile& tile, int h, int* last, int8_t* rows) {
+  for (int i = threadIdx.x / 64; i < p.tokens; i += WAVES) {
+    int8_t* const mine = rows + (size_t)i * p.gp * (STEPS * 64 + 16);
+    const bool live = i < tile.count && tile.seq >= 0;
+    if (live) {
+      u32x4 w[kHeld];
+      load_queries(p, tile.first + i, h, w);
+      round_queries<STEPS>(p, tile.first + i, h, w, mine);
+    } else {
+      zero_queries<STEPS>(p, mine);
+    }
+    const int newest = live ? newest_page(tile.pos + i, p.S, p.PPS) : -1;
+    if (threadIdx.x % 64 == 0) last[i] = newest;
+  }
+}
+
+// One launch for rows whose keys fit the LDS: a workgroup scores a tile's tokens, or in decode batches one
+// token, for a head.  WAVE: a row is chosen by a wave, otherwise (one token) by the whole workgroup.
+template <int STEPS, bool WAVE>
 __global__ __launch_bounds__(512) void select_kernel(SelectParams p) {
   constexpr int kThreads = 512, kWaves = kThreads / 64;
   extern __shared__ __align__(16) uint8_t lds[];
   uint32_t* const keys = (uint32_t*)lds;
   int8_t* const rows = (int8_t*)(lds + (size_t)p.tokens * p.stride * 4);
-  __shared__ int s_seq[16], s_last[16];
+  __shared__ int s_last[16];
   __shared__ typename std::conditional<WAVE, WaveTeam, Team<kThreads>>::type s_team[WAVE ? kWaves : 1];
   const int tid = threadIdx.x, wave = tid / 64;
-  const int h = blockIdx.x % p.Hkv, t0 = blockIdx.x / p.Hkv * p.tokens;
-  if constexpr (!WAVE)
-    if (tid < 64) s_team[0].count[tid] = 0, s_team[0].bound = 0;
-  prepare_tokens<STEPS, kWaves>(p, t0, h, s_seq, s_last, rows);
+  const int h = blockIdx.x % p.Hkv;
+  if constexpr (!WAVE) {
+    if (tid < 64) s_team[0].count[tid] = 0;
+    if (tid == 0) s_team[0].bound = 0, s_team[0].found = 0;
+  }
+  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, blockIdx.x / p.Hkv);
+  if (tile.count == 0) return;  // uniform
+  prepare_tile<STEPS, kWaves>(p, tile, h, s_last, rows);
   __syncthreads();
-  score_tokens<STEPS, kWaves>(p, h, rows, s_seq, s_last, 0, p.PPS, keys);
+  const int visible = s_last[tile.count - 1] + 1;
+  if (visible > p.K) score_pages<STEPS, kWaves>(p, tile.seq, h, rows, s_last, tile.count, 0, visible, keys);
   __syncthreads();
-  int32_t* const out = p.out + ((size_t)t0 * p.Hkv + h) * p.K;
+  int32_t* const out = p.out + ((size_t)tile.first * p.Hkv + h) * p.K;
   if constexpr (WAVE) {
-    for (int i = wave; i < p.tokens && t0 + i < p.T; i += kWaves)
-      choose_wave<KPT>(p, keys + (size_t)i * p.stride, s_last[i] + 1, out + (size_t)i * p.Hkv * p.K, s_team[wave]);
+    for (int i = wave; i < tile.count; i += kWaves)
+      choose_wave(p, keys + (size_t)i * p.stride, s_last[i] + 1, out + (size_t)i * p.Hkv * p.K, s_team[wave]);
   } else {
-    choose<kThreads, KPT>(p, keys, s_last[0] + 1, out, s_team[0]);  // one token
+    choose<kThreads>(p, keys, s_last[0] + 1, out, s_team[0]);
   }
 }
 
 constexpr int kSplitPages = 512;  // pages a workgroup of the split form scores
 
 // The split form, for few rows or rows past the LDS: keys to global memory, then a launch that chooses.
+// Token i of the z-th tile and head h have row (z * p.tokens + i) * Hkv + h of the keys.
 template <int STEPS>
 __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
   constexpr int kWaves = 4;
   extern __shared__ __align__(16) uint8_t lds[];
   int8_t* const rows = (int8_t*)lds;
-  __shared__ int s_seq[16], s_last[16];
-  const int h = blockIdx.y, local = blockIdx.z * p.tokens, begin = blockIdx.x * kSplitPages;
-  prepare_tokens<STEPS, kWaves>(p, p.first + local, h, s_seq, s_last, rows);
+  __shared__ int s_last[16];
+  const int h = blockIdx.y, begin = blockIdx.x * kSplitPages;
+  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, p.first + blockIdx.z);
+  if (tile.seq < 0 || tile.count == 0 || (tile.pos + tile.count - 1) / p.S < begin) return;  // uniform
+  prepare_tile<STEPS, kWaves>(p, tile, h, s_last, rows);
   __syncthreads();
-  // token i's row of head h is row (local + i) * Hkv + h of the keys
-  uint32_t* const keys = p.keys + ((size_t)local * p.Hkv + h) * p.stride;
+  const int visible = s_last[tile.count - 1] + 1;
+  if (visible <= p.K || visible <= begin) return;
+  uint32_t* const keys = p.keys + ((size_t)blockIdx.z * p.tokens * p.Hkv + h) * p.stride;
   p.stride *= p.Hkv;
-  score_tokens<STEPS, kWaves>(p, h, rows, s_seq, s_last, begin, kSplitPages, keys);
+  score_pages<STEPS, kWaves>(p, tile.seq, h, rows, s_last, tile.count, begin, min(visible, begin + kSplitPages), keys);
 }
 
-template <int KPT>
 __global__ __launch_bounds__(1024) void choose_kernel(SelectParams p) {
   constexpr int kThreads = 1024;
   __shared__ Team<kThreads> s_team;
-  const int h = blockIdx.x % p.Hkv, local = blockIdx.x / p.Hkv, t = p.first + local;
-  if (threadIdx.x < 64) s_team.count[threadIdx.x] = 0, s_team.bound = 0;
-  const Place at = place_of(p.cu, p.num_seqs, p.kv_lens, p.N, t);
-  const int newest = newest_page(at, p.S, p.PPS);
+  const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv, i = row % p.tokens;
+  if (tid < 64) s_team.count[tid] = 0;
+  if (tid == 0) s_team.bound = 0, s_team.found = 0;
+  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, p.first + row / p.tokens);
+  if (i >= tile.count) return;  // uniform
+  const int newest = tile.seq < 0 ? -1 : newest_page(tile.pos + i, p.S, p.PPS);
   __syncthreads();
-  choose<kThreads, KPT>(p, p.keys + ((size_t)local * p.Hkv + h) * p.stride, newest + 1,
-                        p.out + ((size_t)t * p.Hkv + h) * p.K, s_team);
+  choose<kThreads>(p, p.keys + (size_t)blockIdx.x * p.stride, newest + 1, p.out + ((size_t)(tile.first + i) * p.Hkv + h) * p.K,
+                   s_team);
 }
 
 // ---- host side ----
@@ -601,10 +613,12 @@ struct SelectPlan {
   long long stride;
   bool tile, split;
   size_t lds;       // dynamic, of the scoring kernel
-  long long batch;  // split: tokens scored before their pages are chosen
+  long long tiles;
+  long long batch;  // split: tiles scored before their pages are chosen
   size_t bytes;     // split: workspace
 };
 
+constexpr long long kWaveRow = 2048;  // keys of a row that one wave chooses from
 constexpr size_t kSelectLds = 60 * 1024;
 constexpr size_t kSelectWorkspace = 256u << 20;  // the split form works through more rows in turns
 
@@ -623,7 +637,7 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
     const size_t token = r.gp * row;
     for (r.tokens = 16; r.tokens > least && r.tokens * (token + keys) > kSelectLds; r.tokens /= 2) {
     }
-    r.split = r.tokens * (token + keys) > kSelectLds || r.stride > 2048;
+    r.split = r.tokens * (token + keys) > kSelectLds || r.stride > kWaveRow;
     for (r.tokens = r.split ? 16 : r.tokens; r.tokens > least && r.tokens * token > kSelectLds; r.tokens /= 2) {
     }
     r.lds = r.tokens * (token + (r.split ? 0 : keys));
@@ -633,13 +647,12 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
     r.split = r.gp * row + keys > kSelectLds || (rows < 256 && r.stride > 1024);
     r.lds = r.gp * row + (r.split ? 0 : keys);
   }
+  r.tiles = r.tokens == 1 ? s.num_tokens : ((long long)s.num_tokens + r.tokens - 1) / r.tokens + s.max_num_seqs;
   if (r.split) {
-    const long long token = (long long)s.num_kv_heads * keys, most = (long long)kSelectWorkspace / token;
-    r.batch = most < r.tokens ? r.tokens : most / r.tokens * r.tokens;
-    if (r.batch > 65535ll * r.tokens) r.batch = 65535ll * r.tokens;
-    const long long all = ((long long)s.num_tokens + r.tokens - 1) / r.tokens * r.tokens;
-    if (r.batch > all) r.batch = all;
-    r.bytes = (size_t)(r.batch * token);
+    const long long tile = r.tokens * (long long)s.num_kv_heads * keys, most = (long long)kSelectWorkspace / tile;
+    r.batch = most < 1 ? 1 : most > 65535 ? 65535 : most;
+    if (r.batch > r.tiles) r.batch = r.tiles;
+    r.bytes = (size_t)(r.batch * tile);
   }
   return r;
 }
@@ -647,23 +660,16 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
 template <int STEPS>
 int launch_select(const SelectPlan& plan, SelectParams p, hipStream_t stream) {
   if (!plan.split) {
-    const int grid = (p.T + plan.tokens - 1) / plan.tokens * p.Hkv;
-    const auto kernel = plan.stride <= 512    ? select_kernel<STEPS, 8, true>
-                        : plan.stride <= 2048 ? select_kernel<STEPS, 32, true>
-                        : plan.stride <= 8192 ? select_kernel<STEPS, 16, false>
-                                              : select_kernel<STEPS, 32, false>;
-    kernel<<<grid, 512, plan.lds, stream>>>(p);
+    const auto kernel = plan.stride <= kWaveRow ? select_kernel<STEPS, true> : select_kernel<STEPS, false>;
+    kernel<<<(unsigned)(plan.tiles * p.Hkv), 512, plan.lds, stream>>>(p);
     return launched("select_pages");
   }
-  for (long long first = 0; first < p.T; first += plan.batch) {
+  for (long long first = 0; first < plan.tiles; first += plan.batch) {
     p.first = (int)first;
-    const int tokens = (int)(p.T - first < plan.batch ? p.T - first : plan.batch);
-    const dim3 grid((p.PPS + kSplitPages - 1) / kSplitPages, p.Hkv, (tokens + plan.tokens - 1) / plan.tokens);
+    const int tiles = (int)(plan.tiles - first < plan.batch ? plan.tiles - first : plan.batch);
+    const dim3 grid((p.PPS + kSplitPages - 1) / kSplitPages, p.Hkv, tiles);
     score_kernel<STEPS><<<grid, 256, plan.lds, stream>>>(p);
-    const auto kernel = plan.stride <= 8192    ? choose_kernel<8>
-                        : plan.stride <= 32768 ? choose_kernel<32>
-                                               : choose_kernel<0>;
-    kernel<<<tokens * p.Hkv, 1024, 0, stream>>>(p);
+    choose_kernel<<<tiles * plan.tokens * p.Hkv, 1024, 0, stream>>>(p);
     const int rc = launched("select_pages");
     if (rc) return rc;
   }
