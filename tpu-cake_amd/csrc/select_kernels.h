@@ -132,61 +132,41 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 // Rounds one token's group of queries to int8: positive parts in columns' first D bytes, negative parts
 // in the next D, zeros up to the row's end.  The columns past G repeat head 0, which leaves a maximum.
-// One wave; w: the group's first values, 16 bytes a lane and 64 lanes a step, loaded beforehand.
-constexpr int kHeld = 2;
-
-__device__ __forceinline__ void load_queries(const SelectParams& p, int t, int h, u32x4 w[kHeld]) {
-  const int lane = threadIdx.x % 64, chunks = p.D / 8;
-  const uint16_t* q = p.q + t * p.q_token + (long long)h * p.G * p.q_head;
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) {
-    const int i = lane + 64 * k, col = __umulhi((uint32_t)i, p.chunk_magic);
-    w[k] = u32x4{0, 0, 0, 0};
-    if (i < p.G * chunks) w[k] = *(const u32x4*)(q + col * p.q_head + 8 * (i - col * chunks));
-  }
-}
-
+// One wave, 8 values a lane and step; the second pass finds them in the L1.
 template <int STEPS>
-__device__ __forceinline__ void round_queries(const SelectParams& p, int t, int h, const u32x4 w[kHeld], int8_t* rows) {
+__device__ __forceinline__ void round_queries(const SelectParams& p, int t, int h, int8_t* rows) {
   constexpr int kRow = STEPS * 64 + 16;
   const int lane = threadIdx.x % 64, chunks = p.D / 8, total = p.G * chunks;
   const uint16_t* q = p.q + t * p.q_token + (long long)h * p.G * p.q_head;
-  const auto at = [&](int i) {
-    const int col = __umulhi((uint32_t)i, p.chunk_magic);
-    return *(const u32x4*)(q + col * p.q_head + 8 * (i - col * chunks));
-  };
   float amax = 0.f;
-  const auto widen = [&](u32x4 v) {
+#pragma unroll 1
+  for (int i = lane; i < total; i += 64) {
+    const int col = __umulhi((uint32_t)i, p.chunk_magic);
     float x[8];
-    unpack8(v, x);
+    unpack8(*(const u32x4*)(q + col * p.q_head + 8 * (i - col * chunks)), x);
 #pragma unroll
     for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));  // fmaxf drops NaN
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) widen(w[k]);
-  for (int i = lane + 64 * kHeld; i < total; i += 64) widen(at(i));
+  }
   const float inv = pow2(-grid_exponent(wave_max(amax)));
-  const auto put = [&](int i, u32x4 v) {
+#pragma unroll 1
+  for (int i = lane; i < total; i += 64) {
     const int col = __umulhi((uint32_t)i, p.chunk_magic), c = i - col * chunks;
     float x[8];
-    unpack8(v, x);
-    u32x2 pos, neg;
+    unpack8(*(const u32x4*)(q + col * p.q_head + 8 * c), x);
+    u32x2 pos = {0, 0}, neg = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int r = x[k] == x[k] ? (int)fminf(fmaxf(rintf(x[k] * inv), -127.f), 127.f) : 0;
-      const uint32_t a = (uint32_t)(max(r, 0) & 255) << (8 * (k % 4)), b = (uint32_t)(min(r, 0) & 255) << (8 * (k % 4));
-      if (k % 4 == 0) pos[k / 4] = a, neg[k / 4] = b;
-      else pos[k / 4] |= a, neg[k / 4] |= b;
+    for (int k = 0; k < 8; ++k) {  // the conversion to a byte turns negative values to 0
+      const float y = x[k] == x[k] ? rintf(__builtin_amdgcn_fmed3f(x[k] * inv, -127.f, 127.f)) : 0.f;
+      pos[k / 4] = __builtin_amdgcn_cvt_pk_u8_f32(y, k % 4, pos[k / 4]);
+      neg[k / 4] = __builtin_amdgcn_cvt_pk_u8_f32(-y, k % 4, neg[k / 4]);
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) neg[k] = (0x80808080u - neg[k]) ^ 0x80808080u;  // minus each byte: they are at most 127
     for (int to = col; to < p.gp; to = to < p.G && to > 0 ? p.gp : max(to + 1, p.G)) {  // head 0's also past G
       *(u32x2*)(rows + to * kRow + 8 * c) = pos;
       *(u32x2*)(rows + to * kRow + p.D + 8 * c) = neg;
     }
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (lane + 64 * k < total) put(lane + 64 * k, w[k]);
-  for (int i = lane + 64 * kHeld; i < total; i += 64) put(i, at(i));
+  }
   const int tail = (STEPS * 64 - 2 * p.D) / 8;
   for (int i = lane; i < p.gp * tail; i += 64) *(u32x2*)(rows + i / tail * kRow + 2 * p.D + 8 * (i % tail)) = u32x2{0, 0};
 }
@@ -400,8 +380,8 @@ __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_
 // themselves, so the order of the atomics leaves no trace.
 template <int THREADS>
 __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* keys, int n, int32_t* out, Team<THREADS>& team) {
-  constexpr int kWaves = THREADS / 64;
-  const int tid = threadIdx.x, lane = tid % 64;
+  constexpr int kWaves = THREADS / 64, kBatch = 16;  // keys of a thread in flight
+  const int tid = threadIdx.x;
   const int need = choose_forced<THREADS>(p, n, out);
   if (need == 0) return;
   out += p.sink;
@@ -412,8 +392,13 @@ __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* ke
   const int groups = need <= 48 ? 64 : Team<THREADS>::kGroups;
   if (need <= groups / 4 * 3) {
     uint32_t top = 0;
-#pragma unroll 8
-    for (int i = 0; i < n; i += THREADS) top = max(top, key(i + tid));
+    for (int i = 0; i < n; i += kBatch * THREADS) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) k[u] = key(i + THREADS * u + tid);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) top = max(top, k[u]);
+    }
     const int wide = THREADS / groups;  // threads of a group, a power of two
     for (int d = 1; d < wide; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     if (tid % wide == 0) team.top[tid / wide] = top;
@@ -431,12 +416,12 @@ __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* ke
     }
     __syncthreads();
     const uint32_t bound = max(1u, team.bound);
-    for (int i = 0; i < n; i += 8 * THREADS) {
-      uint32_t k[8];
+    for (int i = 0; i < n; i += kBatch * THREADS) {
+      uint32_t k[kBatch];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) k[u] = key(i + THREADS * u + tid);
+      for (int u = 0; u < kBatch; ++u) k[u] = key(i + THREADS * u + tid);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < kBatch; ++u)
         if (k[u] >= bound) {
           const int to = atomicAdd(&team.found, 1);
           if (to < THREADS) team.key[to] = (unsigned long long)k[u] << 32 | (uint32_t)~(i + THREADS * u + tid);
@@ -502,29 +487,31 @@ __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* ke
   }
 }
 
-// Rounds a tile's queries, a wave a token, and notes the tokens' newest pages.
+// The workgroup's tile, its queries rounded, a wave a token, and its tokens' newest pages.
 template <int STEPS, int WAVES>
-__device__ __forceinline__ void prepare_tile(const SelectParams& p, const Tile& tile, int h, int* last, int8_t* rows) {
+__device__ __forceinline__ Tile prepare_tile(const SelectParams& p, int index, int h, int* last, int8_t* rows) {
+  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, index);
   for (int i = threadIdx.x / 64; i < p.tokens; i += WAVES) {
     int8_t* const mine = rows + (size_t)i * p.gp * (STEPS * 64 + 16);
     const bool live = i < tile.count && tile.seq >= 0;
     if (live) {
-      u32x4 w[kHeld];
-      load_queries(p, tile.first + i, h, w);
-      round_queries<STEPS>(p, tile.first + i, h, w, mine);
+      round_queries<STEPS>(p, tile.first + i, h, mine);
     } else {
       zero_queries<STEPS>(p, mine);
     }
     const int newest = live ? newest_page(tile.pos + i, p.S, p.PPS) : -1;
     if (threadIdx.x % 64 == 0) last[i] = newest;
   }
+  return tile;
 }
 
 // One launch for rows whose keys fit the LDS: a workgroup scores a tile's tokens, or in decode batches one
 // token, for a head.  WAVE: a row is chosen by a wave, otherwise (one token) by the whole workgroup.
+constexpr int kSelectThreads = 1024;
+
 template <int STEPS, bool WAVE>
-__global__ __launch_bounds__(512) void select_kernel(SelectParams p) {
-  constexpr int kThreads = 512, kWaves = kThreads / 64;
+__global__ __launch_bounds__(kSelectThreads, 8) void select_kernel(SelectParams p) {
+  constexpr int kThreads = kSelectThreads, kWaves = kThreads / 64;
   extern __shared__ __align__(16) uint8_t lds[];
   uint32_t* const keys = (uint32_t*)lds;
   int8_t* const rows = (int8_t*)(lds + (size_t)p.tokens * p.stride * 4);
@@ -536,9 +523,8 @@ __global__ __launch_bounds__(512) void select_kernel(SelectParams p) {
     if (tid < 64) s_team[0].count[tid] = 0;
     if (tid == 0) s_team[0].bound = 0, s_team[0].found = 0;
   }
-  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, blockIdx.x / p.Hkv);
+  const Tile tile = prepare_tile<STEPS, kWaves>(p, blockIdx.x / p.Hkv, h, s_last, rows);
   if (tile.count == 0) return;  // uniform
-  prepare_tile<STEPS, kWaves>(p, tile, h, s_last, rows);
   __syncthreads();
   const int visible = s_last[tile.count - 1] + 1;
   if (visible > p.K) score_pages<STEPS, kWaves>(p, tile.seq, h, rows, s_last, tile.count, 0, visible, keys);
@@ -563,9 +549,8 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
   int8_t* const rows = (int8_t*)lds;
   __shared__ int s_last[16];
   const int h = blockIdx.y, begin = blockIdx.x * kSplitPages;
-  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, p.first + blockIdx.z);
-  if (tile.seq < 0 || tile.count == 0 || (tile.pos + tile.count - 1) / p.S < begin) return;  // uniform
-  prepare_tile<STEPS, kWaves>(p, tile, h, s_last, rows);
+  const Tile tile = prepare_tile<STEPS, kWaves>(p, p.first + blockIdx.z, h, s_last, rows);
+  if (tile.seq < 0 || tile.count == 0) return;  // uniform
   __syncthreads();
   const int visible = s_last[tile.count - 1] + 1;
   if (visible <= p.K || visible <= begin) return;
@@ -661,7 +646,7 @@ template <int STEPS>
 int launch_select(const SelectPlan& plan, SelectParams p, hipStream_t stream) {
   if (!plan.split) {
     const auto kernel = plan.stride <= kWaveRow ? select_kernel<STEPS, true> : select_kernel<STEPS, false>;
-    kernel<<<(unsigned)(plan.tiles * p.Hkv), 512, plan.lds, stream>>>(p);
+    kernel<<<(unsigned)(plan.tiles * p.Hkv), kSelectThreads, plan.lds, stream>>>(p);
     return launched("select_pages");
   }
   for (long long first = 0; first < plan.tiles; first += plan.batch) {
