@@ -67,6 +67,67 @@ def test_chunk_tokens_see_their_own_keys_only(cuda):
     _check(b, 13, hole=0.0)  # all pages: causal attention
 
 
+@pytest.mark.parametrize("kind,dim", [("bf16", 128), ("bf16", 64), ("bf16", 256), ("bf16", 32), ("bf16", 40), ("bf16", 96),
+                                      ("fp8", 128), ("fp8", 64), ("fp8", 256), ("fp8", 80)])
+@pytest.mark.parametrize("page", [1, 7, 16, 64, 100, 256])
+def test_chunks_of_dims_and_pages(cuda, kind, dim, page):
+    b = Batch(dim + page, [90, 30, 1000, 64, 0, 257, 5], [33, 1, 70, 64, 0, 16, 2], page, 8, 2, dim, spare=1, pad=5)
+    _check(b, 6, kind)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 8, 9, 16, 17])
+def test_chunks_of_groups(cuda, group):
+    _check(Batch(group, [400, 77, 3], [50, 9, 3], 16, group * 2, 2, 64, pad=1), 8, soft_cap=30.0)
+
+
+def test_chunk_with_long_lists(cuda):
+    """Unions of more pages than a workgroup holds, and lists of their own that long."""
+    _check(Batch(31, [4000], [12], 1, 4, 1, 64), 1500)
+    _check(Batch(32, [1900, 3000], [9, 8], 1, 8, 1, 64), 300)
+
+
+def test_chunk_over_a_table_past_the_bitmaps(cuda):
+    _check(Batch(33, [33000], [9], 1, 4, 1, 32), 20)
+
+
+def test_chunk_over_huge_pages(cuda):
+    """Pages of more parts than a tile indexes."""
+    _check(Batch(34, [140000, 90], [3, 5], 131072, 2, 1, 32), 2)
+
+
+def test_chunk_pages_listed_twice_count_twice(cuda):
+    b = Batch(35, [200, 300], [20, 40], 16, 8, 2, 64)
+    picked = b.lists(7)
+    picked[3, 0, 5] = picked[3, 0, 1]
+    picked[33, 1] = picked[33, 1, 0]
+    _check(b, 7, picked=picked)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_chunk_nan_that_other_tokens_see(cuda, kind):
+    """A key that one token lists, or is far enough to see, holds NaN or infinities: only that token's rows show it."""
+    b = Batch(36, [80, 70], [40, 30], 16, 8, 2, 128)
+    pool, scales, keys, values = b.pool(kind)
+    picked = b.lists(5, hole=0.0)
+    picked[:40][picked[:40] == 1] = -1
+    picked[7, 0, 0] = 1  # token 7 of the first sequence alone lists its page 1, for kv head 0
+    held = pool.view(torch.uint8) if kind == "fp8" else pool
+    held[b.table[0, 1], 3, :2] = 0x7F if kind == "fp8" else float("nan")
+    held[b.table[1, 4], 1, 2:] = 0x7F if kind == "fp8" else float("inf")  # position 65 of 70, kv head 1
+    pool = held.view(pool.dtype)
+    kw = dict(sm_scale=0.1, kv_scales=None if scales is None else torch.from_numpy(scales).cuda())
+    got = sparse.sparse_paged_attention(b.q.cuda(), pool.cuda(), i32(picked), *b.meta(), **kw).double().cpu().numpy()
+    bad = np.zeros((70, 8), bool)
+    bad[7, :4] = True
+    for t, (i, pos) in enumerate(orc.positions(b.lens, b.cu, b.n, 70)):
+        if i == 1 and pos >= 65 and (picked[t, 1] == 4).any():
+            bad[t, 4:] = True
+    assert bad.sum() > 8 and (~np.isfinite(got).all(-1) == bad).all()
+    want = orc.sparse_attention(b.q.double().numpy(), keys, values, picked, b.lens, b.table, b.cu, b.n, 0.1)
+    tol = _tolerance(want, b.q, keys, values, 80, 0.1)
+    assert (np.abs(got - want) <= tol)[~bad].all()
+
+
 @pytest.mark.parametrize("soft_cap", [None, 20.0, -20.0])
 @pytest.mark.parametrize("sm_scale", [1.0, -0.3, 0.0])
 def test_scales_and_caps(cuda, soft_cap, sm_scale):

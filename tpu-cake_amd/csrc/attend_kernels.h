@@ -315,6 +315,319 @@ __global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
   }
 }
 
+// Prompt chunks: a workgroup takes a tile of up to 64 columns of one sequence -- `tokens` consecutive tokens,
+// gp columns each, 16 columns a wave -- and the union of their lists, each page of which is read once, into
+// LDS, for all of them.  Neighbouring tokens choose mostly the same pages (in the measured chunk 16 tokens of
+// 32 pages each name about 58), so the L2 gives up a ninth of the bytes that rows of their own would ask
+// for, and every wave multiplies whole 16-column tiles.  Per 32 keys the four waves read 64 KB of K and V out
+// of LDS (512 cycles at 128 B a cycle) beside 384 cycles of MFMA each.  A key counts for a column if its page
+// is on the token's own list and it is not past the token's position; a wave passes over 32 keys that none of
+// its columns counts.  A page one token lists and another does not may hold infinities or NaN, and P = 0 does
+// not silence those: where an output is not finite the tile is done again token by token, each reading its own
+// keys only.  Lists that name a page twice are done so at once.
+struct TileParams {
+  AttendParams a;
+  int tokens, gp, shift;      // of a tile; columns of a token and their log2
+  uint32_t sub_magic;         // ceil(2^32 / subs)
+};
+
+constexpr int kTilePages = 1024;       // pages of a list that a workgroup holds at once
+constexpr int kTileColumns = 32768;    // page table columns whose bitmaps fit beside them
+constexpr int kTileParts = 2048;       // 64-key parts of a page: below it, block / subs by sub_magic is exact
+
+struct TileEntry {
+  int row, base, mask;  // the page's first pool row, its first position, the tokens that list it
+};
+
+template <int DP, bool FULL, bool FP8>
+__global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
+  const AttendParams& p = tp.a;
+  constexpr int kThreads = 256;
+  constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;  // LDS key rows
+  constexpr int kBuffer = 32 * (kKRow + kVRow);
+  constexpr int kElem = FP8 ? 1 : 2;
+  constexpr int kChunks = DP * kElem / 16;                 // 16-byte chunks of a key row
+  constexpr int kLoads = (kChunks + 7) / 8;                // of a thread: 8 threads a key
+  constexpr int kSteps = DP / 32;
+  extern __shared__ __align__(16) uint8_t lds[];
+  uint8_t* const s_kv = lds;                               // two buffers
+  TileEntry* const s_entry = (TileEntry*)(lds + 2 * kBuffer);
+  float* const s_scale = (float*)(s_entry + kTilePages);   // fp8: K and V scales of the entries
+  const int words = (p.PPS + 31) / 32;
+  uint32_t* const s_bits = (uint32_t*)(s_scale + (FP8 ? 2 * kTilePages : 0));
+  uint32_t* const s_before = s_bits + words;
+  __shared__ Pair s_scan[kThreads / 64];
+  __shared__ int s_flag[2];  // a page listed twice; an output that is not finite
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, j = lane / 16;
+  const int h = blockIdx.x % p.Hkv;
+  const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, tp.tokens, blockIdx.x / p.Hkv);
+  if (tile.count == 0) return;  // uniform
+  if (tile.seq < 0 || tile.pos + tile.count <= 0) {
+    for (int i = tid; i < tile.count * p.G * p.D / 8; i += kThreads) {
+      const int t = i / (p.G * p.D / 8), c = i % (p.G * p.D / 8);
+      *(u32x4*)(p.out + ((size_t)(tile.first + t) * p.Hkv + h) * p.G * p.D + 8 * c) = u32x4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const int32_t* const table = p.table + (size_t)tile.seq * p.PPS;
+  const int32_t* const lists = p.picked + ((size_t)tile.first * p.Hkv + h) * p.K;
+  const size_t list_stride = (size_t)p.Hkv * p.K;
+
+  // this lane's column
+  const int column = wave * 16 + n, token = column >> tp.shift, head = column & (tp.gp - 1);
+  const bool live = token < tile.count && head < p.G;
+  const int pos = live ? tile.pos + token : -1;
+  bf16x8 q[kSteps];
+  {
+    const uint16_t* src = p.q + (tile.first + token) * p.q_token + ((long long)h * p.G + head) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int dim = 32 * s + 8 * j;
+      u32x4 w = {0, 0, 0, 0};
+      if (live && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+      q[s] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+
+  const int row_bytes = p.D * kElem;
+  f32x4 o[DP / 16];
+  float m, l;
+  const auto reset = [&] {
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = kLowest, l = 0.f;
+  };
+
+  // Attends to the keys of `pages` entries up to position `last`.
+  const auto attend = [&](int pages, int last) {
+    const int keys = pages * p.subs * p.width, units = (keys + 31) / 32;
+    struct Key {
+      int entry, base, off;  // off: in its page
+    };
+    const auto locate = [&](int v) {
+      const int block = p.width == 1 ? v : (int)__umulhi((uint32_t)v, p.magic);
+      const int entry = p.subs == 1 ? block : (int)__umulhi((uint32_t)block, tp.sub_magic);
+      const int off = v - block * p.width + (block - entry * p.subs) * p.width;
+      return Key{entry, 0, off};
+    };
+    u32x4 k[kLoads], v[kLoads];
+    const auto load = [&](int unit) {  // thread: key tid / 8, chunks tid % 8, + 8, ...
+      const int at = unit * 32 + tid / 8;
+      const Key x = locate(min(at, keys - 1));
+      const TileEntry e = s_entry[x.entry];
+      const uint8_t* src = (const uint8_t*)g_zero_row;
+      if (at < keys && e.mask && x.off < p.S && e.base + x.off <= last)
+        src = p.kv + ((size_t)(e.row + x.off) * (2 * p.Hkv) + 2 * h) * row_bytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int byte = 16 * (tid % 8 + 8 * i);
+        k[i] = v[i] = u32x4{0, 0, 0, 0};
+        if (byte < (FULL ? DP * kElem : row_bytes)) {
+          k[i] = *(const u32x4*)(src + byte);
+          v[i] = *(const u32x4*)(src + row_bytes + byte);
+        }
+      }
+    };
+    const auto store = [&](int unit) {
+      uint8_t* const kt = s_kv + (unit & 1) * kBuffer + tid / 8 * kKRow;
+      uint8_t* const vt = s_kv + (unit & 1) * kBuffer + 32 * kKRow + tid / 8 * kVRow;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int byte = 16 * (tid % 8 + 8 * i);
+        if (byte >= DP * kElem) break;
+        if (FP8) {
+          *(u32x4*)(kt + 2 * byte) = bf16_of_codes(k[i][0], k[i][1]);
+          *(u32x4*)(kt + 2 * byte + 16) = bf16_of_codes(k[i][2], k[i][3]);
+          *(u32x4*)(vt + 2 * byte) = bf16_of_codes(v[i][0], v[i][1]);
+          *(u32x4*)(vt + 2 * byte + 16) = bf16_of_codes(v[i][2], v[i][3]);
+        } else {
+          *(u32x4*)(kt + byte) = k[i];
+          *(u32x4*)(vt + byte) = v[i];
+        }
+      }
+    };
+    load(0);
+    store(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int unit = 0; unit < units; ++unit) {
+      if (unit + 1 < units) load(unit + 1);
+      // which of the lane's keys (16 b + 4 j + r) count for its column
+      uint32_t counts = 0;
+      float ks[2][4], vs[2][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = unit * 32 + 16 * b + 4 * j + r;
+          const Key x = locate(min(at, keys - 1));
+          const TileEntry e = s_entry[x.entry];
+          if (at < keys && (e.mask >> token & 1) && x.off < p.S && e.base + x.off <= pos) counts |= 1u << (4 * b + r);
+          if (FP8) ks[b][r] = s_scale[2 * x.entry], vs[b][r] = s_scale[2 * x.entry + 1];
+        }
+      if (__ballot(counts != 0)) {
+        const uint8_t* const kt = s_kv + (unit & 1) * kBuffer;
+        f32x4 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            const u32x4 a = *(const u32x4*)(kt + (16 * b + n) * kKRow + 64 * i + 16 * j);
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], s[b], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float x = s[b][r] * p.scale;
+            if (FP8) x *= ks[b][r];
+            if (p.cap != 0.f) x = p.cap * tanhf(x / p.cap) * kLog2e;
+            s[b][r] = counts >> (4 * b + r) & 1 ? x : -__builtin_inff();
+          }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = swap_max(top);
+        if (__ballot(top > m + kRescale)) {
+          const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+          m = next;
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) o[d] *= f;
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          float e[4], rest[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
+            l += e[r];
+            if (FP8) e[r] *= vs[b][r];
+            rest[r] = e[r] - (float)(__bf16)e[r];
+          }
+          hi[2 * b] = pack_bf16(e[0], e[1]), hi[2 * b + 1] = pack_bf16(e[2], e[3]);
+          lo[2 * b] = pack_bf16(rest[0], rest[1]), lo[2 * b + 1] = pack_bf16(rest[2], rest[3]);
+        }
+        typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+        const uint8_t* const vt = kt + 32 * kKRow + (4 * j + n / 4) * kVRow + 8 * (n % 4);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
+          const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kVRow + 32 * d));
+          const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
+        }
+      }
+      if (unit + 1 < units) store(unit + 1);
+      __syncthreads();
+    }
+  };
+
+  const auto finite = [&] {
+    bool ok = true;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ok &= fabsf(o[d][r]) < __builtin_inff();
+    return ok;
+  };
+  // The columns' rows, normalised: those of token `only`, or all (-1).
+  const auto write = [&](int only) {
+    const float sum = swap_sum(l), g = sum == 0.f ? 0.f : p.v_scale / sum;
+    if (!live || (only >= 0 && token != only)) return;
+    uint16_t* const row = p.out + (((size_t)(tile.first + token) * p.Hkv + h) * p.G + head) * p.D;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      const int dim = 16 * d + 4 * j;
+      if (FULL || dim < p.D)
+        *(u32x2*)(row + dim) = sum == 0.f ? u32x2{0, 0}
+                                          : u32x2{pack_bf16(o[d][0] * g, o[d][1] * g), pack_bf16(o[d][2] * g, o[d][3] * g)};
+    }
+  };
+  const auto entry = [&](int i, int page, int mask) {
+    const int phys = table[page];
+    const bool ok = phys >= 0 && phys < p.P;
+    if (!ok) flag_error(RPA_SPARSE_ERR_PAGE);
+    s_entry[i] = {ok ? phys * p.S : 0, page * p.S, ok ? mask : 0};
+    if (FP8) {
+      const float* s = p.scales && ok ? p.scales + ((size_t)phys * p.Hkv + h) * 2 : nullptr;
+      s_scale[2 * i] = s ? s[0] : 1.f, s_scale[2 * i + 1] = s ? s[1] : 1.f;
+    }
+  };
+
+  // the union of the lists, as a bitmap
+  const int entries = tile.count * p.K;
+  const auto listed = [&](int i, int& t) {  // the page of entry i of all lists, -1: none that its token sees
+    t = i / p.K;
+    const int page = lists[t * list_stride + (i - t * p.K)];
+    return page >= 0 && page <= newest_page(tile.pos + t, p.S, p.PPS) ? page : -1;
+  };
+  for (int i = tid; i < words; i += kThreads) s_bits[i] = 0;
+  if (tid < 2) s_flag[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < entries; i += kThreads) {
+    int t;
+    const int page = listed(i, t);
+    if (page >= 0) atomicOr(&s_bits[page / 32], 1u << (page % 32));
+  }
+  __syncthreads();
+  const int each = (words + kThreads - 1) / kThreads;
+  Pair found = {0, 0}, total;
+  for (int i = tid * each; i < min((tid + 1) * each, words); ++i) found.a += __popc(s_bits[i]);
+  uint32_t before = scan_pairs<kThreads / 64>(found, total, s_scan).a;
+  for (int i = tid * each; i < min((tid + 1) * each, words); ++i) s_before[i] = before, before += __popc(s_bits[i]);
+  reset();
+  for (int first = 0; first < (int)total.a; first += kTilePages) {
+    const int pages = min((int)total.a - first, kTilePages);
+    __syncthreads();
+    for (int i = tid; i < pages; i += kThreads) s_entry[i].mask = 0;
+    __syncthreads();
+    for (int i = tid; i < entries; i += kThreads) {
+      int t;
+      const int page = listed(i, t);
+      if (page < 0) continue;
+      const int at = (int)(s_before[page / 32] + __popc(s_bits[page / 32] & ((1u << (page % 32)) - 1))) - first;
+      if (at < 0 || at >= pages) continue;
+      const int old = atomicOr(&s_entry[at].mask, 1 << t);
+      if (old >> t & 1) s_flag[0] = 1;
+      s_entry[at].base = page;  // every lister writes the same
+    }
+    __syncthreads();
+    if (s_flag[0]) break;  // uniform: a page listed twice
+    for (int i = tid; i < pages; i += kThreads) entry(i, s_entry[i].base, s_entry[i].mask);
+    __syncthreads();
+    attend(pages, tile.pos + tile.count - 1);
+  }
+  if (!s_flag[0]) {
+    if (!finite()) s_flag[1] = 1;
+    __syncthreads();
+  }
+  if (!s_flag[0] && !s_flag[1]) {
+    write(-1);
+    return;
+  }
+  // token by token
+  for (int t = 0; t < tile.count; ++t) {
+    reset();
+    for (int first = 0; first < p.K; first += kTilePages) {
+      const int pages = min(p.K - first, kTilePages);
+      __syncthreads();
+      for (int i = tid; i < pages; i += kThreads) {
+        int own;
+        const int page = listed(t * p.K + first + i, own);
+        if (page >= 0) entry(i, page, 1 << t);
+        else s_entry[i] = {0, 0, 0};
+      }
+      __syncthreads();
+      attend(pages, tile.pos + t);
+    }
+    write(t);
+  }
+}
+
 // ---- host side ----
 int check_attend(const rpa_sparse_shape_t* s) {
   const int rc = check_sparse(s);
@@ -327,6 +640,9 @@ int check_attend(const rpa_sparse_shape_t* s) {
 }
 
 struct AttendPlan {
+  bool chunk;           // tiles of tokens
+  int tokens, gp;       // of a tile
+  long long grid;       // its workgroups
   int tiles, width, subs, per, splits;
   long long blocks, rows;
   size_t bytes;
@@ -342,6 +658,13 @@ AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
   r.width = s.page_size <= 64 ? s.page_size : 64;
   r.subs = (s.page_size + r.width - 1) / r.width;
   r.blocks = (long long)s.num_pages * r.subs;
+  if (s.num_tokens > 2 * s.max_num_seqs && G <= 16 && s.pages_per_seq <= kTileColumns && r.subs < kTileParts) {
+    r.chunk = true;
+    r.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
+    r.tokens = 64 / r.gp;
+    r.grid = (((long long)s.num_tokens + r.tokens - 1) / r.tokens + s.max_num_seqs) * s.num_kv_heads;
+    return r;
+  }
   // a workgroup's part: at least 128 keys, one unit a wave, and at most kMaxBlocks blocks
   const long long least = (128 + r.width - 1) / r.width;
   long long splits = r.rows ? (kAttendFill + r.rows - 1) / r.rows : 1;
@@ -356,6 +679,14 @@ AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
 
 template <int DP, bool FULL, bool FP8>
 void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t stream) {
+  if (plan.chunk) {
+    const TileParams tp = {p, plan.tokens, plan.gp, plan.gp == 4 ? 2 : plan.gp == 8 ? 3 : 4,
+                           (uint32_t)(0x100000000ull / plan.subs + 1)};
+    const size_t lds = 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
+                       (size_t)((p.PPS + 31) / 32) * 8;
+    attend_tile_kernel<DP, FULL, FP8><<<(unsigned)plan.grid, 256, lds, stream>>>(tp);
+    return;
+  }
   const size_t lds = ((size_t)plan.per * (FP8 ? 16 : 8) + 15) / 16 * 16 + (size_t)kAttendWaves * 32 * (DP * 2 + 32);
   attend_kernel<DP, FULL, FP8><<<dim3((unsigned)plan.rows, plan.splits), 64 * kAttendWaves, lds, stream>>>(p);
 }
