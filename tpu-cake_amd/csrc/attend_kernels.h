@@ -62,6 +62,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
+// Two values as two bf16 each: the nearest ones, and what is left.
+__device__ __forceinline__ u32x2 split_bf16(float a, float b) {
+  const uint32_t hi = pack_bf16(a, b);
+  return u32x2{hi, pack_bf16(a - bf16_lo(hi), b - bf16_hi(hi))};
+}
+
+__device__ __forceinline__ void cap_scores(f32x4 s[2], float cap) {
+#pragma unroll 1
+  for (int b = 0; b < 2; ++b) {
+    f32x4 x = b ? s[1] : s[0];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = cap * tanhf(x[r] / cap) * kLog2e;
+    if (b) s[1] = x;
+    else s[0] = x;
+  }
+}
+
 // DP: dims of a row in registers and LDS (64, 128 or 256), FULL: D == DP.
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams p) {
@@ -209,13 +226,13 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = s[b][r] * p.scale;
-        if (FP8) x *= ks[r];
-        if (p.cap != 0.f) x = p.cap * tanhf(x / p.cap) * kLog2e;
-        s[b][r] = here[b] >> r & 1 ? x : -__builtin_inff();
-      }
+      for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[r] : p.scale;
     }
+    if (p.cap != 0.f) cap_scores(s, p.cap);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[b][r] = here[b] >> r & 1 ? s[b][r] : -__builtin_inff();
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = swap_max(top);
@@ -229,16 +246,16 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
     u32x4 hi, lo;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      float e[4], rest[4];
+      float e[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
         l += e[r];
         if (FP8) e[r] *= vs[b][r];
-        rest[r] = e[r] - (float)(__bf16)e[r];
       }
-      hi[2 * b] = pack_bf16(e[0], e[1]), hi[2 * b + 1] = pack_bf16(e[2], e[3]);
-      lo[2 * b] = pack_bf16(rest[0], rest[1]), lo[2 * b + 1] = pack_bf16(rest[2], rest[3]);
+      const u32x2 first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
+      hi[2 * b] = first[0], hi[2 * b + 1] = second[0];
+      lo[2 * b] = first[1], lo[2 * b + 1] = second[1];
     }
     typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
     const uint8_t* vt = tile_v + (4 * j + n / 4) * kRow + 8 * (n % 4);
@@ -331,7 +348,7 @@ struct TileParams {
   uint32_t sub_magic;         // ceil(2^32 / subs)
 };
 
-constexpr int kTilePages = 1024;       // pages of a list that a workgroup holds at once
+constexpr int kTilePages = 512;        // pages of a list that a workgroup holds at once
 constexpr int kTileColumns = 32768;    // page table columns whose bitmaps fit beside them
 constexpr int kTileParts = 2048;       // 64-key parts of a page: below it, block / subs by sub_magic is exact
 
@@ -339,10 +356,17 @@ struct TileEntry {
   int row, base, mask;  // the page's first pool row, its first position, the tokens that list it
 };
 
+// Groups of four waves take every so manieth 32 keys and join at the end.  Latency bounds a turn (entry,
+// K, softmax, V, barrier), so the card is filled with the waves that registers and LDS allow: one group took
+// 140 us for 500 tokens of 32 pages of 64 keys (32 heads, 8 kv heads), two 130, three 113; 354, 354 and 302
+// for 2000 tokens.
+constexpr int tile_groups(int dp) { return dp == 256 ? 2 : 3; }
+
 template <int DP, bool FULL, bool FP8>
-__global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
+__global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(TileParams tp) {
   const AttendParams& p = tp.a;
-  constexpr int kThreads = 256;
+  constexpr int kGroups = tile_groups(DP);
+  constexpr int kThreads = 256 * kGroups;
   constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;  // LDS key rows
   constexpr int kBuffer = 32 * (kKRow + kVRow);
   constexpr int kElem = FP8 ? 1 : 2;
@@ -350,15 +374,18 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
   constexpr int kLoads = (kChunks + 7) / 8;                // of a thread: 8 threads a key
   constexpr int kSteps = DP / 32;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* const s_kv = lds;                               // two buffers
-  TileEntry* const s_entry = (TileEntry*)(lds + 2 * kBuffer);
+  static_assert(4 * 16 * (DP + 4) * 4 <= 2 * kBuffer, "a group's rows of O fit its buffers");
+  TileEntry* const s_entry = (TileEntry*)(lds + kGroups * 2 * kBuffer);
   float* const s_scale = (float*)(s_entry + kTilePages);   // fp8: K and V scales of the entries
   const int words = (p.PPS + 31) / 32;
   uint32_t* const s_bits = (uint32_t*)(s_scale + (FP8 ? 2 * kTilePages : 0));
   uint32_t* const s_before = s_bits + words;
   __shared__ Pair s_scan[kThreads / 64];
   __shared__ int s_flag[2];  // a page listed twice; an output that is not finite
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = lane % 16, j = lane / 16;
+  __shared__ float s_m[kGroups][64], s_l[kGroups][64];
+  const int tid = threadIdx.x, lane = tid % 64, n = lane % 16, j = lane / 16;
+  const int group = tid / 256, wave = tid / 64 % 4, member = tid % 256;
+  uint8_t* const s_kv = lds + group * 2 * kBuffer;  // two buffers of the group's own
   const int h = blockIdx.x % p.Hkv;
   const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, tp.tokens, blockIdx.x / p.Hkv);
   if (tile.count == 0) return;  // uniform
@@ -402,17 +429,17 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
   const auto attend = [&](int pages, int last) {
     const int keys = pages * p.subs * p.width, units = (keys + 31) / 32;
     struct Key {
-      int entry, base, off;  // off: in its page
+      int entry, off;  // off: in its page
     };
     const auto locate = [&](int v) {
       const int block = p.width == 1 ? v : (int)__umulhi((uint32_t)v, p.magic);
       const int entry = p.subs == 1 ? block : (int)__umulhi((uint32_t)block, tp.sub_magic);
       const int off = v - block * p.width + (block - entry * p.subs) * p.width;
-      return Key{entry, 0, off};
+      return Key{entry, off};
     };
     u32x4 k[kLoads], v[kLoads];
-    const auto load = [&](int unit) {  // thread: key tid / 8, chunks tid % 8, + 8, ...
-      const int at = unit * 32 + tid / 8;
+    const auto load = [&](int unit) {  // a thread: key member / 8, chunks member % 8, + 8, ...
+      const int at = unit * 32 + member / 8;
       const Key x = locate(min(at, keys - 1));
       const TileEntry e = s_entry[x.entry];
       const uint8_t* src = (const uint8_t*)g_zero_row;
@@ -420,7 +447,7 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
         src = p.kv + ((size_t)(e.row + x.off) * (2 * p.Hkv) + 2 * h) * row_bytes;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int byte = 16 * (tid % 8 + 8 * i);
+        const int byte = 16 * (member % 8 + 8 * i);
         k[i] = v[i] = u32x4{0, 0, 0, 0};
         if (byte < (FULL ? DP * kElem : row_bytes)) {
           k[i] = *(const u32x4*)(src + byte);
@@ -428,12 +455,12 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
         }
       }
     };
-    const auto store = [&](int unit) {
-      uint8_t* const kt = s_kv + (unit & 1) * kBuffer + tid / 8 * kKRow;
-      uint8_t* const vt = s_kv + (unit & 1) * kBuffer + 32 * kKRow + tid / 8 * kVRow;
+    const auto store = [&](int turn) {
+      uint8_t* const kt = s_kv + (turn & 1) * kBuffer + member / 8 * kKRow;
+      uint8_t* const vt = s_kv + (turn & 1) * kBuffer + 32 * kKRow + member / 8 * kVRow;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int byte = 16 * (tid % 8 + 8 * i);
+        const int byte = 16 * (member % 8 + 8 * i);
         if (byte >= DP * kElem) break;
         if (FP8) {
           *(u32x4*)(kt + 2 * byte) = bf16_of_codes(k[i][0], k[i][1]);
@@ -446,27 +473,43 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
         }
       }
     };
-    load(0);
-    store(0);
+    if (group < units) load(group), store(0);
     __syncthreads();
 #pragma unroll 1
-    for (int unit = 0; unit < units; ++unit) {
-      if (unit + 1 < units) load(unit + 1);
+    for (int turn = 0, unit = group; turn * kGroups < units; ++turn, unit += kGroups) {
+      if (unit + kGroups < units) load(unit + kGroups);
       // which of the lane's keys (16 b + 4 j + r) count for its column
       uint32_t counts = 0;
       float ks[2][4], vs[2][4];
+      if (unit >= units) {
+      } else if (p.width % 16 == 0) {  // 16 keys lie in one page
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int at = unit * 32 + 16 * b + 4 * j + r;
+        for (int b = 0; b < 2; ++b) {
+          const int at = unit * 32 + 16 * b;
           const Key x = locate(min(at, keys - 1));
           const TileEntry e = s_entry[x.entry];
-          if (at < keys && (e.mask >> token & 1) && x.off < p.S && e.base + x.off <= pos) counts |= 1u << (4 * b + r);
-          if (FP8) ks[b][r] = s_scale[2 * x.entry], vs[b][r] = s_scale[2 * x.entry + 1];
+          const int most = min(pos - e.base, p.S - 1) - x.off - 4 * j;  // of the lane's four, 0 .. most count
+          if (at < keys && (e.mask >> token & 1) && most >= 0) counts |= (most < 3 ? (2u << most) - 1 : 15u) << (4 * b);
+          if (FP8) {
+            const float kx = s_scale[2 * x.entry], vx = s_scale[2 * x.entry + 1];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ks[b][r] = kx, vs[b][r] = vx;
+          }
         }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = unit * 32 + 16 * b + 4 * j + r;
+            const Key x = locate(min(at, keys - 1));
+            const TileEntry e = s_entry[x.entry];
+            if (at < keys && (e.mask >> token & 1) && x.off < p.S && e.base + x.off <= pos) counts |= 1u << (4 * b + r);
+            if (FP8) ks[b][r] = s_scale[2 * x.entry], vs[b][r] = s_scale[2 * x.entry + 1];
+          }
+      }
       if (__ballot(counts != 0)) {
-        const uint8_t* const kt = s_kv + (unit & 1) * kBuffer;
+        const uint8_t* const kt = s_kv + (turn & 1) * kBuffer;
         f32x4 s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -480,12 +523,12 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = s[b][r] * p.scale;
-            if (FP8) x *= ks[b][r];
-            if (p.cap != 0.f) x = p.cap * tanhf(x / p.cap) * kLog2e;
-            s[b][r] = counts >> (4 * b + r) & 1 ? x : -__builtin_inff();
-          }
+          for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[b][r] : p.scale;
+        if (p.cap != 0.f) cap_scores(s, p.cap);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[b][r] = counts >> (4 * b + r) & 1 ? s[b][r] : -__builtin_inff();
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         top = swap_max(top);
@@ -499,16 +542,16 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
         u32x4 hi, lo;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          float e[4], rest[4];
+          float e[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
             l += e[r];
             if (FP8) e[r] *= vs[b][r];
-            rest[r] = e[r] - (float)(__bf16)e[r];
           }
-          hi[2 * b] = pack_bf16(e[0], e[1]), hi[2 * b + 1] = pack_bf16(e[2], e[3]);
-          lo[2 * b] = pack_bf16(rest[0], rest[1]), lo[2 * b + 1] = pack_bf16(rest[2], rest[3]);
+          const u32x2 first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
+          hi[2 * b] = first[0], hi[2 * b + 1] = second[0];
+          lo[2 * b] = first[1], lo[2 * b + 1] = second[1];
         }
         typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
         const uint8_t* const vt = kt + 32 * kKRow + (4 * j + n / 4) * kVRow + 8 * (n % 4);
@@ -521,9 +564,33 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
           o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
         }
       }
-      if (unit + 1 < units) store(unit + 1);
+      if (unit + kGroups < units) store(turn + 1);
       __syncthreads();
     }
+  };
+  // The first group's waves take the others' (m, l, O) in.
+  const auto join = [&] {
+    float* const rows = (float*)(s_kv + wave * 16 * (DP + 4) * 4) + n * (DP + 4);
+    if (group) {
+      l = swap_sum(l);
+      if (j == 0) s_m[group][wave * 16 + n] = m, s_l[group][wave * 16 + n] = l;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) *(f32x4*)(rows + 16 * d + 4 * j) = o[d];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) {
+        const float other = s_m[g][wave * 16 + n], next = fmaxf(m, other);
+        const float mine = __builtin_amdgcn_exp2f(m - next), its = __builtin_amdgcn_exp2f(other - next);
+        m = next;
+        l = l * mine + (j == 0 ? s_l[g][wave * 16 + n] * its : 0.f);
+        const float* const from = rows + g * 2 * kBuffer / 4;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) o[d] = o[d] * mine + *(const f32x4*)(from + 16 * d + 4 * j) * its;
+      }
+    }
+    __syncthreads();
   };
 
   const auto finite = [&] {
@@ -537,7 +604,7 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
   // The columns' rows, normalised: those of token `only`, or all (-1).
   const auto write = [&](int only) {
     const float sum = swap_sum(l), g = sum == 0.f ? 0.f : p.v_scale / sum;
-    if (!live || (only >= 0 && token != only)) return;
+    if (!live || group || (only >= 0 && token != only)) return;
     uint16_t* const row = p.out + (((size_t)(tile.first + token) * p.Hkv + h) * p.G + head) * p.D;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
@@ -602,7 +669,8 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
     attend(pages, tile.pos + tile.count - 1);
   }
   if (!s_flag[0]) {
-    if (!finite()) s_flag[1] = 1;
+    join();
+    if (group == 0 && !finite()) s_flag[1] = 1;
     __syncthreads();
   }
   if (!s_flag[0] && !s_flag[1]) {
@@ -624,6 +692,7 @@ __global__ __launch_bounds__(256) void attend_tile_kernel(TileParams tp) {
       __syncthreads();
       attend(pages, tile.pos + t);
     }
+    join();
     write(t);
   }
 }
@@ -682,9 +751,10 @@ void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t st
   if (plan.chunk) {
     const TileParams tp = {p, plan.tokens, plan.gp, plan.gp == 4 ? 2 : plan.gp == 8 ? 3 : 4,
                            (uint32_t)(0x100000000ull / plan.subs + 1)};
-    const size_t lds = 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
+    constexpr int kGroups = tile_groups(DP);
+    const size_t lds = kGroups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
                        (size_t)((p.PPS + 31) / 32) * 8;
-    attend_tile_kernel<DP, FULL, FP8><<<(unsigned)plan.grid, 256, lds, stream>>>(tp);
+    attend_tile_kernel<DP, FULL, FP8><<<(unsigned)plan.grid, 256 * kGroups, lds, stream>>>(tp);
     return;
   }
   const size_t lds = ((size_t)plan.per * (FP8 ? 16 : 8) + 15) / 16 * 16 + (size_t)kAttendWaves * 32 * (DP * 2 + 32);

@@ -79,118 +79,161 @@ struct AppendParams {
   long long k_token, k_head, v_token, v_head;  // strides, in values
   long long rows;                              // P * S
   int T, Hkv, D, S;
+  uint32_t chunk_magic, row_magic;  // ceil(2^32 / n) for n = D / 8 and 2 D / 8: i / n for i < 2^26
 };
 
-// One workgroup per token, one wave per kv head (each wave takes heads wave, wave + W, ...): the rows
-// are copied (or quantised) 16 bytes a lane.  A token that is the first of its page's new rows -- row 0
-// of a page, or a slot that does not follow the previous token's -- also widens the page's bounds by
-// the whole run of consecutive slots, reading their keys once more (L2) with 64 / (D / 8) rows in
-// flight per wave; decode rows are runs of one.  Runs of one page are the work of one wave, so no
-// atomics and no order decide the result.
-template <bool FP8>
+// A workgroup takes TOKENS tokens, a wave one kv head of them at a time (heads wave, wave + W, ...).  The rows
+// are copied, or quantised, 16 bytes a lane with four loads in flight; K and V do not wait for the slots.
+// A token that is the first of its page's new rows -- row 0 of a page, or a slot that does not follow the
+// previous token's -- also widens the page's bounds by the whole run of consecutive slots, reading their keys
+// once more with 64 / (D / 8) rows in flight; decode rows are runs of one.  A run is one wave's work, so no
+// atomics and no order decide the result.  Quantising is monotone: the bounds of an fp8 page come from the
+// largest and smallest inputs, quantised.
+//
+// Decode batches are bound by latency (slots, then the page's old bounds) and take a workgroup a token; long
+// batches by the turnover of workgroups: 8 tokens each (12 chunks of 333 to 1000 tokens into an fp8 pool,
+// 8 heads of 128: XX us, 91 with one).
+template <bool FP8, int TOKENS>
 __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
-  const int lane = threadIdx.x % 64, t = blockIdx.x;
-  const int slot = p.slots[t];
-  if (slot == -1) return;
-  if (slot < 0 || slot >= p.rows) {
-    if (threadIdx.x == 0) flag_error(RPA_SPARSE_ERR_SLOT);
-    return;
-  }
-  const int page = slot / p.S, row = slot % p.S;
-  const int chunks = p.D / 8;
-  int run = 0;  // new rows of this page from here on, 0: they belong to an earlier token's run
-  if (p.bounds && (row == 0 || t == 0 || p.slots[t - 1] != slot - 1)) {
-    const int most = min(p.S - row, p.T - t);
-    run = most;
-    for (int base = 1; base < most; base += 64) {
-      const int i = base + lane;
-      const unsigned long long end = __ballot(i >= most || p.slots[t + i] != slot + i);
-      if (end) {
-        run = base + __builtin_ctzll(end);
-        break;
-      }
-    }
-  }
-  for (int h = threadIdx.x / 64; h < p.Hkv; h += blockDim.x / 64) {
-    float scale[2] = {p.k_scale, p.v_scale};
-    if (FP8 && p.scales) {
-      const float* s = p.scales + ((size_t)page * p.Hkv + h) * 2;
-      scale[0] = s[0], scale[1] = s[1];
-    }
-    for (int i = lane; i < 2 * chunks; i += 64) {
-      const int part = i >= chunks, c = i - part * chunks;
-      const uint16_t* src = part ? p.v + t * p.v_token + h * p.v_head : p.k + t * p.k_token + h * p.k_head;
-      const u32x4 w = *(const u32x4*)(src + 8 * c);
-      const size_t at = ((size_t)slot * (2 * p.Hkv) + 2 * h + part) * p.D + 8 * c;
-      if (FP8) {
-        float x[8];
-        unpack8(w, x);
-        *(u32x2*)(p.kv + at) = fp8_codes(x, part ? scale[1] : scale[0]);
-      } else {
-        *(u32x4*)(p.kv + 2 * at) = w;
-      }
-    }
-    if (run == 0) continue;
-    const int teams = 64 / chunks, team = lane / chunks, c = lane % chunks;
-    float hi[8], lo[8];
+  const int lane = threadIdx.x % 64, t0 = blockIdx.x * TOKENS;
+  const int chunks = p.D / 8, row_chunks = 2 * chunks;
+  const int items = min(TOKENS, p.T - t0) * row_chunks;
+  const int wave = threadIdx.x / 64, waves = blockDim.x / 64;
+  constexpr int kHold = 4;
+  u32x4 w[kHold];
+  const auto load = [&](int h, int base) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi[i] = -__builtin_inff(), lo[i] = __builtin_inff();
-    if (team < teams) {
-      const uint16_t* src = p.k + (t + team) * p.k_token + h * p.k_head + 8 * c;
-#pragma unroll 4
-      for (int r = team; r < run; r += teams, src += teams * p.k_token) {
-        float x[8];
-        unpack8(*(const u32x4*)src, x);
-        if (FP8) fp8_values(fp8_codes(x, scale[0]), scale[0], x);
+    for (int u = 0; u < kHold; ++u) {
+      const int idx = min(base + 64 * u + lane, items - 1);
+      const int i = __umulhi((uint32_t)idx, p.row_magic), c = idx - i * row_chunks, part = c >= chunks;
+      const uint16_t* src = part ? p.v + (t0 + i) * p.v_token + h * p.v_head : p.k + (t0 + i) * p.k_token + h * p.k_head;
+      w[u] = *(const u32x4*)(src + 8 * (c - part * chunks));
+    }
+  };
+  load(wave, 0);
+  // the slots from here on, a lane each
+  const int mine = t0 + lane < p.T ? p.slots[t0 + lane] : -2;
+  const int left = t0 > 0 ? p.slots[t0 - 1] : -2;
+  const int prev = lane ? __shfl_up(mine, 1) : left;
+  const bool valid = mine >= 0 && mine < p.rows;
+  if (wave == 0 && lane < TOKENS && mine != -1 && !valid && t0 + lane < p.T) flag_error(RPA_SPARSE_ERR_SLOT);
+  const unsigned long long leads =
+      p.bounds ? __ballot(lane < TOKENS && valid && (mine % p.S == 0 || prev != mine - 1)) : 0ull;
+#pragma unroll 1
+  for (int h = wave; h < p.Hkv; h += waves) {
+#pragma unroll 1
+    for (int base = 0; base < items; base += 64 * kHold) {
+      if (h != wave || base) load(h, base);
+      int slot[kHold];
+      float scale[kHold];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = x[i] == x[i] ? x[i] : 0.f;  // NaN counts as 0
-          hi[i] = fmaxf(hi[i], y);
-          lo[i] = fminf(lo[i], y);
+      for (int u = 0; u < kHold; ++u) {
+        const int idx = min(base + 64 * u + lane, items - 1);
+        const int i = __umulhi((uint32_t)idx, p.row_magic), part = idx - i * row_chunks >= chunks;
+        slot[u] = __shfl(mine, i);
+        if (slot[u] < 0 || slot[u] >= p.rows || base + 64 * u + lane >= items) slot[u] = -1;
+        scale[u] = part ? p.v_scale : p.k_scale;
+        if (FP8 && p.scales) scale[u] = p.scales[((size_t)(max(slot[u], 0) / p.S) * p.Hkv + h) * 2 + part];
+      }
+#pragma unroll
+      for (int u = 0; u < kHold; ++u) {
+        if (slot[u] < 0) continue;
+        const int idx = base + 64 * u + lane;
+        const int i = __umulhi((uint32_t)idx, p.row_magic), c = idx - i * row_chunks, part = c >= chunks;
+        const size_t at = ((size_t)slot[u] * (2 * p.Hkv) + 2 * h + part) * p.D + 8 * (c - part * chunks);
+        if (FP8) {
+          float x[8];
+          unpack8(w[u], x);
+          *(u32x2*)(p.kv + at) = fp8_codes(x, scale[u]);
+        } else {
+          *(u32x4*)(p.kv + 2 * at) = w[u];
         }
       }
     }
-    float amax = 0.f;
-    if (team < min(teams, run))
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
-#pragma unroll
-    for (int d = 32; d; d /= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    for (int g = 1; g < min(teams, run); ++g)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        hi[i] = fmaxf(hi[i], __shfl(hi[i], g * chunks + c));
-        lo[i] = fminf(lo[i], __shfl(lo[i], g * chunks + c));
-      }
-    const size_t at = (size_t)page * p.Hkv + h;
-    int e = grid_exponent(amax);
-    const int old = row == 0 ? kExpMin : min(max((int)p.exps[at], kExpMin), kExpMax);
-    e = max(e, old);
-    if (lane < chunks) {
+#pragma unroll 1
+    for (unsigned long long todo = leads; todo; todo &= todo - 1) {
+      const int first = __builtin_ctzll(todo), t = t0 + first;
+      const int slot = __builtin_amdgcn_readlane(mine, first), page = slot / p.S, row = slot % p.S;
+      // the run: within the 64 slots at hand, then further
+      const int most = min(p.S - row, p.T - t);
+      const unsigned long long follows = __ballot(mine == slot + lane - first && lane - first < most) >> first;
+      int run = ~follows ? __builtin_ctzll(~follows) : 64;
+      if (first + run == 64)
+        for (; run < most; run += 64) {
+          const int i = run + lane;
+          const unsigned long long end = __ballot(i >= most || p.slots[t + i] != slot + i);
+          if (end) {
+            run += __builtin_ctzll(end);
+            break;
+          }
+        }
+      run = min(run, most);
+      const size_t at = (size_t)page * p.Hkv + h;
+      const int team = __umulhi((uint32_t)lane, p.chunk_magic), c = lane - team * chunks;
+      const int teams = min(__umulhi(64u, p.chunk_magic), (uint32_t)run);  // that have a row
       int8_t* const up = p.bounds + at * 2 * p.D + 8 * c;
       int8_t* const down = up + p.D;
-      u32x2 was_up = {0, 0}, was_down = {0, 0}, now_up, now_down;
-      if (row) was_up = *(const u32x2*)up, was_down = *(const u32x2*)down;
-      const float inv = pow2(-e);
-      const int shift = min(e - old, 31);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int u = grid_up(hi[i], inv), d = grid_down(lo[i], inv);
-        if (row) {
-          const int pu = (int8_t)(was_up[i / 4] >> (8 * (i % 4))), pd = (int8_t)(was_down[i / 4] >> (8 * (i % 4)));
-          u = max(u, -(-pu >> shift));
-          d = min(d, pd >> shift);
-        }
-        const uint32_t ub = (uint32_t)(u & 255) << (8 * (i % 4)), db = (uint32_t)(d & 255) << (8 * (i % 4));
-        if (i % 4 == 0) now_up[i / 4] = ub, now_down[i / 4] = db;
-        else now_up[i / 4] |= ub, now_down[i / 4] |= db;
+      u32x2 was_up = {0, 0}, was_down = {0, 0};
+      int old = kExpMin;
+      if (row) {  // a page begun earlier
+        old = min(max((int)p.exps[at], kExpMin), kExpMax);
+        if (lane < chunks) was_up = *(const u32x2*)up, was_down = *(const u32x2*)down;
       }
-      *(u32x2*)up = now_up;
-      *(u32x2*)down = now_down;
+      float hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hi[i] = -__builtin_inff(), lo[i] = __builtin_inff();
+      if (team < teams) {
+        const uint16_t* src = p.k + (t + team) * p.k_token + h * p.k_head + 8 * c;
+        const long long step = teams * p.k_token;
+#pragma unroll 4
+        for (int r = team; r < run; r += teams, src += step) {
+          float x[8];
+          unpack8(*(const u32x4*)src, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float y = x[i] == x[i] ? x[i] : 0.f;  // NaN counts as 0
+            hi[i] = fmaxf(hi[i], y);
+            lo[i] = fminf(lo[i], y);
+          }
+        }
+      }
+      for (int g = 1; g < teams; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hi[i] = fmaxf(hi[i], __shfl(hi[i], g * chunks + c));
+          lo[i] = fminf(lo[i], __shfl(lo[i], g * chunks + c));
+        }
+      if (FP8) {
+        const float scale = p.scales ? p.scales[2 * at] : p.k_scale;
+        fp8_values(fp8_codes(hi, scale), scale, hi);
+        fp8_values(fp8_codes(lo, scale), scale, lo);
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+      const int e = max(grid_exponent(wave_max(team == 0 ? amax : 0.f)), old);
+      if (lane < chunks) {
+        const float inv = pow2(-e);
+        const int shift = min(e - old, 31);
+        u32x2 now_up = {0, 0}, now_down = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          int u = grid_up(hi[i], inv), d = grid_down(lo[i], inv);
+          const int pu = (int8_t)(was_up[i / 4] >> (8 * (i % 4))), pd = (int8_t)(was_down[i / 4] >> (8 * (i % 4)));
+          u = row ? max(u, -(-pu >> shift)) : u;
+          d = row ? min(d, pd >> shift) : d;
+          now_up[i / 4] |= (uint32_t)(u & 255) << (8 * (i % 4));
+          now_down[i / 4] |= (uint32_t)(d & 255) << (8 * (i % 4));
+        }
+        *(u32x2*)up = now_up;
+        *(u32x2*)down = now_down;
+      }
+      if (lane == 0) p.exps[at] = (int8_t)e;
     }
-    if (lane == 0) p.exps[at] = (int8_t)e;
   }
 }
+
+constexpr int kAppendTokens = 8, kAppendLong = 2048;  // tokens of a workgroup, in batches longer than that
 
 int check_heads(int hkv, int d, int kv_dtype) {
   if (hkv <= 0) return fail(RPA_E_INVALID, "non-positive dimension in shape");
