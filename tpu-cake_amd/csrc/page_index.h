@@ -69,6 +69,9 @@ __device__ __forceinline__ void fp8_values(u32x2 w, float scale, float x[8]) {
   }
 }
 
+constexpr int kAppendTokens = 8, kAppendLong = 2048;  // tokens of a workgroup, in batches longer than that
+constexpr int kAppendRounds = 4;
+
 struct AppendParams {
   const uint16_t *k, *v;
   const int32_t* slots;
@@ -79,23 +82,15 @@ struct AppendParams {
   long long k_token, k_head, v_token, v_head;  // strides, in values
   long long rows;                              // P * S
   int T, Hkv, D, S;
+  int wide;  // workgroups that widen bounds
   uint32_t chunk_magic, row_magic;  // ceil(2^32 / n) for n = D / 8 and 2 D / 8: i / n for i < 2^26
 };
 
-// A workgroup takes TOKENS tokens, a wave one kv head of them at a time (heads wave, wave + W, ...).  The rows
-// are copied, or quantised, 16 bytes a lane with four loads in flight; K and V do not wait for the slots.
-// A token that is the first of its page's new rows -- row 0 of a page, or a slot that does not follow the
-// previous token's -- also widens the page's bounds by the whole run of consecutive slots, reading their keys
-// once more with 64 / (D / 8) rows in flight; decode rows are runs of one.  A run is one wave's work, so no
-// atomics and no order decide the result.  Quantising is monotone: the bounds of an fp8 page come from the
-// largest and smallest inputs, quantised.
-//
-// Decode batches are bound by latency (slots, then the page's old bounds) and take a workgroup a token; long
-// batches by the turnover of workgroups: 8 tokens each (12 chunks of 333 to 1000 tokens into an fp8 pool,
-// 8 heads of 128: XX us, 91 with one).
+// Copies, or quantises, the rows of TOKENS tokens, a wave one kv head of them at a time (heads wave, wave + W,
+// ...), 16 bytes a lane with four loads in flight.  K and V do not wait for the slots.
 template <bool FP8, int TOKENS>
-__global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
-  const int lane = threadIdx.x % 64, t0 = blockIdx.x * TOKENS;
+__device__ __forceinline__ void copy_rows(const AppendParams& p, int t0) {
+  const int lane = threadIdx.x % 64;
   const int chunks = p.D / 8, row_chunks = 2 * chunks;
   const int items = min(TOKENS, p.T - t0) * row_chunks;
   const int wave = threadIdx.x / 64, waves = blockDim.x / 64;
@@ -111,14 +106,8 @@ __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
     }
   };
   load(wave, 0);
-  // the slots from here on, a lane each
-  const int mine = t0 + lane < p.T ? p.slots[t0 + lane] : -2;
-  const int left = t0 > 0 ? p.slots[t0 - 1] : -2;
-  const int prev = lane ? __shfl_up(mine, 1) : left;
-  const bool valid = mine >= 0 && mine < p.rows;
-  if (wave == 0 && lane < TOKENS && mine != -1 && !valid && t0 + lane < p.T) flag_error(RPA_SPARSE_ERR_SLOT);
-  const unsigned long long leads =
-      p.bounds ? __ballot(lane < TOKENS && valid && (mine % p.S == 0 || prev != mine - 1)) : 0ull;
+  const int mine = lane < TOKENS && t0 + lane < p.T ? p.slots[t0 + lane] : -1;
+  if (wave == 0 && mine != -1 && (mine < 0 || mine >= p.rows)) flag_error(RPA_SPARSE_ERR_SLOT);
 #pragma unroll 1
   for (int h = wave; h < p.Hkv; h += waves) {
 #pragma unroll 1
@@ -150,90 +139,143 @@ __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
         }
       }
     }
-#pragma unroll 1
-    for (unsigned long long todo = leads; todo; todo &= todo - 1) {
-      const int first = __builtin_ctzll(todo), t = t0 + first;
-      const int slot = __builtin_amdgcn_readlane(mine, first), page = slot / p.S, row = slot % p.S;
-      // the run: within the 64 slots at hand, then further
-      const int most = min(p.S - row, p.T - t);
-      const unsigned long long follows = __ballot(mine == slot + lane - first && lane - first < most) >> first;
-      int run = ~follows ? __builtin_ctzll(~follows) : 64;
-      if (first + run == 64)
-        for (; run < most; run += 64) {
-          const int i = run + lane;
-          const unsigned long long end = __ballot(i >= most || p.slots[t + i] != slot + i);
-          if (end) {
-            run += __builtin_ctzll(end);
-            break;
-          }
-        }
-      run = min(run, most);
-      const size_t at = (size_t)page * p.Hkv + h;
-      const int team = __umulhi((uint32_t)lane, p.chunk_magic), c = lane - team * chunks;
-      const int teams = min(__umulhi(64u, p.chunk_magic), (uint32_t)run);  // that have a row
-      int8_t* const up = p.bounds + at * 2 * p.D + 8 * c;
-      int8_t* const down = up + p.D;
-      u32x2 was_up = {0, 0}, was_down = {0, 0};
-      int old = kExpMin;
-      if (row) {  // a page begun earlier
-        old = min(max((int)p.exps[at], kExpMin), kExpMax);
-        if (lane < chunks) was_up = *(const u32x2*)up, was_down = *(const u32x2*)down;
-      }
-      float hi[8], lo[8];
+  }
+}
+
+// One run of new rows -- `run` tokens from t on, from `row` of `page` on -- for all teams of a wave (alone: the
+// same one, each a share of its rows), or one a team (run 0: none).
+template <bool FP8>
+__device__ __forceinline__ void widen_runs(const AppendParams& p, int t, int page, int row, int run, bool alone, int team,
+                                           int teams, int c) {
+  const int chunks = p.D / 8;
+  const int step = alone ? min(teams, run) : min(run, 1), from = alone ? team : 0;
+  const bool merges = run > 0 && (!alone || team == 0);
+  for (int h = threadIdx.x / 64; h < p.Hkv; h += blockDim.x / 64) {
+    const size_t at = (size_t)page * p.Hkv + h;
+    int8_t* const up = p.bounds + at * 2 * p.D + 8 * c;
+    int8_t* const down = up + p.D;
+    u32x2 was_up = {0, 0}, was_down = {0, 0};
+    int old = kExpMin;
+    if (merges && row) {  // a page begun earlier
+      old = min(max((int)p.exps[at], kExpMin), kExpMax);
+      was_up = *(const u32x2*)up, was_down = *(const u32x2*)down;
+    }
+    const float scale = FP8 ? (p.scales ? p.scales[2 * at] : p.k_scale) : 1.f;
+    float hi[8], lo[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = -__builtin_inff(), lo[i] = __builtin_inff();
-      if (team < teams) {
-        const uint16_t* src = p.k + (t + team) * p.k_token + h * p.k_head + 8 * c;
-        const long long step = teams * p.k_token;
+    for (int i = 0; i < 8; ++i) hi[i] = -__builtin_inff(), lo[i] = __builtin_inff();
+    if (from < step) {
+      const uint16_t* src = p.k + (t + from) * p.k_token + h * p.k_head + 8 * c;
 #pragma unroll 4
-        for (int r = team; r < run; r += teams, src += step) {
-          float x[8];
-          unpack8(*(const u32x4*)src, x);
+      for (int r = from; r < run; r += step, src += step * p.k_token) {
+        float x[8];
+        unpack8(*(const u32x4*)src, x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float y = x[i] == x[i] ? x[i] : 0.f;  // NaN counts as 0
-            hi[i] = fmaxf(hi[i], y);
-            lo[i] = fminf(lo[i], y);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float y = x[i] == x[i] ? x[i] : 0.f;  // NaN counts as 0
+          hi[i] = fmaxf(hi[i], y);
+          lo[i] = fminf(lo[i], y);
         }
       }
-      for (int g = 1; g < teams; ++g)
+    }
+    if (alone)
+      for (int g = 1; g < step; ++g)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           hi[i] = fmaxf(hi[i], __shfl(hi[i], g * chunks + c));
           lo[i] = fminf(lo[i], __shfl(lo[i], g * chunks + c));
         }
-      if (FP8) {
-        const float scale = p.scales ? p.scales[2 * at] : p.k_scale;
-        fp8_values(fp8_codes(hi, scale), scale, hi);
-        fp8_values(fp8_codes(lo, scale), scale, lo);
-      }
-      float amax = 0.f;
+    if (FP8) {
+      fp8_values(fp8_codes(hi, scale), scale, hi);
+      fp8_values(fp8_codes(lo, scale), scale, lo);
+    }
+    float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
-      const int e = max(grid_exponent(wave_max(team == 0 ? amax : 0.f)), old);
-      if (lane < chunks) {
-        const float inv = pow2(-e);
-        const int shift = min(e - old, 31);
-        u32x2 now_up = {0, 0}, now_down = {0, 0};
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+    float most = amax;
+    for (int i = 1; i < chunks; ++i) most = fmaxf(most, __shfl(amax, min(team * chunks + (c + i < chunks ? c + i : c + i - chunks), 63)));
+    const int e = max(grid_exponent(most), old);
+    if (merges) {
+      const float inv = pow2(-e);
+      const int shift = min(e - old, 31);
+      u32x2 now_up = {0, 0}, now_down = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          int u = grid_up(hi[i], inv), d = grid_down(lo[i], inv);
-          const int pu = (int8_t)(was_up[i / 4] >> (8 * (i % 4))), pd = (int8_t)(was_down[i / 4] >> (8 * (i % 4)));
-          u = row ? max(u, -(-pu >> shift)) : u;
-          d = row ? min(d, pd >> shift) : d;
-          now_up[i / 4] |= (uint32_t)(u & 255) << (8 * (i % 4));
-          now_down[i / 4] |= (uint32_t)(d & 255) << (8 * (i % 4));
-        }
-        *(u32x2*)up = now_up;
-        *(u32x2*)down = now_down;
+      for (int i = 0; i < 8; ++i) {
+        int u = grid_up(hi[i], inv), d = grid_down(lo[i], inv);
+        const int pu = (int8_t)(was_up[i / 4] >> (8 * (i % 4))), pd = (int8_t)(was_down[i / 4] >> (8 * (i % 4)));
+        u = row ? max(u, -(-pu >> shift)) : u;
+        d = row ? min(d, pd >> shift) : d;
+        now_up[i / 4] |= (uint32_t)(u & 255) << (8 * (i % 4));
+        now_down[i / 4] |= (uint32_t)(d & 255) << (8 * (i % 4));
       }
-      if (lane == 0) p.exps[at] = (int8_t)e;
+      *(u32x2*)up = now_up;
+      *(u32x2*)down = now_down;
+      if (c == 0) p.exps[at] = (int8_t)e;
     }
   }
 }
 
-constexpr int kAppendTokens = 8, kAppendLong = 2048;  // tokens of a workgroup, in batches longer than that
+// Widens the bounds of the pages that `count` tokens from t0 on are the first new rows of: row 0 of a page, or
+// a slot that does not follow the previous token's.  Such a token stands for its whole run of consecutive slots
+// in the page, and a run is the work of one wave, so no atomics and no order decide the result.  A wave takes a
+// kv head; its teams of D / 8 lanes take a run each, or, where there is one only (prompts), every so manieth of
+// its rows.  Quantising is monotone: the bounds of an fp8 page come from the largest and smallest inputs,
+// quantised.
+template <bool FP8>
+__device__ __forceinline__ void widen_bounds(const AppendParams& p, int t0, int count) {
+  const int lane = threadIdx.x % 64, chunks = p.D / 8;
+  const int team = __umulhi((uint32_t)lane, p.chunk_magic), c = lane - team * chunks;
+  const int teams = __umulhi(64u, p.chunk_magic);
+  // the slots from here on, a lane each
+  const int mine = t0 + lane < p.T ? p.slots[t0 + lane] : -2;
+  const int left = t0 > 0 ? p.slots[t0 - 1] : -2;
+  const int before = __shfl_up(mine, 1), prev = lane ? before : left;
+  const unsigned long long leads =
+      __ballot(lane < count && mine >= 0 && mine < p.rows && (mine % p.S == 0 || prev != mine - 1));
+  if (leads == 0) return;
+  // each slot's run as far as the slots at hand go: rows of its page at consecutive slots
+  const int after = __shfl_down(mine, 1);
+  const bool joins = lane < 63 && after == mine + 1 && after % p.S != 0;
+  const unsigned long long breaks = ~__ballot(joins) >> lane;  // bit i: slot lane + i is the last of its run
+  const int length = breaks ? 1 + __builtin_ctzll(breaks) : 64;
+  const bool is_lead = leads >> lane & 1;
+  // short runs: a team each; long ones: one after another, all teams on each
+  const bool apart = __ballot(is_lead && (length > 16 || lane + length > 63)) == 0 && (leads & (leads - 1));
+  for (unsigned long long todo = leads; todo; todo = apart ? 0 : todo & (todo - 1)) {
+    const int first = apart ? min(team, count - 1) : __builtin_ctzll(todo), t = t0 + first;
+    const bool lead = team < teams && (!apart || (team < count && (leads >> first & 1)));
+    const int slot = max(__shfl(mine, first), 0), row = slot % p.S, most = min(p.S - row, p.T - t);
+    int run = __shfl(length, first);
+    if (!apart && first + run > 63)  // further than the slots at hand
+      for (run = 64 - first; run < most; run += 64) {
+        const int i = run + lane;
+        const unsigned long long end = __ballot(i >= most || p.slots[t + i] != slot + i);
+        if (end) {
+          run += __builtin_ctzll(end);
+          break;
+        }
+      }
+    widen_runs<FP8>(p, t, slot / p.S, row, lead ? min(run, most) : 0, !apart, team, teams, c);
+  }
+}
+
+// One launch: the first `wide` workgroups (with an index) widen bounds, the others copy rows beside them.  Decode
+// batches are bound by latency: a token a workgroup, or a team.  Long batches are bound by the turnover of
+// workgroups and by runs that start late: eight tokens, and four rounds of teams first.
+template <bool FP8, int TOKENS>
+__global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
+  const int block = blockIdx.x, teams = __umulhi(64u, p.chunk_magic);
+  if (block < p.wide) {
+    constexpr int kRounds = TOKENS > 1 ? kAppendRounds : 1;
+    for (int r = 0; r < kRounds; ++r) {
+      const int t0 = (block * kRounds + r) * teams;
+      if (t0 < p.T) widen_bounds<FP8>(p, t0, min(teams, p.T - t0));
+    }
+  } else {
+    copy_rows<FP8, TOKENS>(p, (block - p.wide) * TOKENS);
+  }
+}
+
 
 int check_heads(int hkv, int d, int kv_dtype) {
   if (hkv <= 0) return fail(RPA_E_INVALID, "non-positive dimension in shape");

@@ -81,18 +81,19 @@ int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void*
   if ((rc = check_strides("keys", keys, shape->k_token_stride, shape->k_head_stride))) return rc;
   if ((rc = check_strides("values", values, shape->v_token_stride, shape->v_head_stride))) return rc;
   if (!aligned16(kv_pages) || !aligned16(bounds)) return fail(RPA_E_INVALID, "kv_pages and bounds must be 16-byte aligned");
+  const int chunks = shape->head_dim / 8, tokens = shape->num_tokens > kAppendLong ? kAppendTokens : 1;
+  const int ahead = 64 / chunks * (tokens > 1 ? kAppendRounds : 1);  // tokens of a workgroup that widens bounds
+  const int wide = bounds ? (shape->num_tokens - 1) / ahead + 1 : 0;
   const AppendParams p = {(const uint16_t*)keys, (const uint16_t*)values, slot_mapping, (uint8_t*)kv_pages, kv_scales, k_scale,
                           v_scale, bounds, exponents, shape->k_token_stride, shape->k_head_stride, shape->v_token_stride,
                           shape->v_head_stride, (long long)shape->total_pages * shape->page_size, shape->num_tokens,
-                          shape->num_kv_heads, shape->head_dim, shape->page_size,
-                          (uint32_t)(0x100000000ull / (shape->head_dim / 8) + 1),
-                          (uint32_t)(0x100000000ull / (shape->head_dim / 4) + 1)};
+                          shape->num_kv_heads, shape->head_dim, shape->page_size, wide,
+                          (uint32_t)(0x100000000ull / chunks + 1), (uint32_t)(0x100000000ull / (2 * chunks) + 1)};
   const int threads = 64 * (shape->num_kv_heads < 8 ? shape->num_kv_heads : 8);
-  const int tokens = shape->num_tokens > kAppendLong ? kAppendTokens : 1;
   const auto kernel = shape->kv_dtype == RPA_KV_FP8_E4M3
                           ? (tokens > 1 ? append_kernel<true, kAppendTokens> : append_kernel<true, 1>)
                           : (tokens > 1 ? append_kernel<false, kAppendTokens> : append_kernel<false, 1>);
-  kernel<<<(shape->num_tokens - 1) / tokens + 1, threads, 0, (hipStream_t)stream>>>(p);
+  kernel<<<wide + (shape->num_tokens - 1) / tokens + 1, threads, 0, (hipStream_t)stream>>>(p);
   return launched("append_kv");
 }
 
