@@ -28,6 +28,7 @@ struct AssignParams {
 };
 
 constexpr int kItems = 4;  // requests per thread and turn
+constexpr int kSmallBatch = 256 * kItems;  // requests that one turn of a 256-thread workgroup sums
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void assign_kernel(AssignParams p) {
@@ -150,7 +151,7 @@ struct ReleaseParams {
   int N, PPS, S, F;
 };
 
-constexpr int kReleaseThreads = 256;
+constexpr int kReleaseThreads = 1024;
 constexpr int kReleaseSlice = 64;  // requests per workgroup
 
 // A workgroup owns a slice of the requests: it sums the pages that earlier requests give back, then
@@ -162,13 +163,16 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const int i0 = blockIdx.x * kReleaseSlice;
   const long long capacity = (long long)p.PPS * p.S;
-  const auto pages_of = [&](int i) {
-    if (!p.finished[i]) return 0;
-    const int len = p.cached[i];
-    return len <= 0 ? 0 : ceil_div((int)min((long long)len, capacity), p.S);
+  const auto pages_of = [&](bool finished, int len) {
+    return !finished || len <= 0 ? 0 : ceil_div((int)min((long long)len, capacity), p.S);
   };
   uint32_t before = 0;
-  for (int i = tid; i < i0; i += kReleaseThreads) before = sat_add(before, (uint32_t)pages_of(i));
+#pragma unroll 4
+  for (int i = tid; i < i0; i += kReleaseThreads) {
+    const bool finished = p.finished[i];
+    const int len = p.cached[i];  // beside it, not after it
+    before = sat_add(before, (uint32_t)pages_of(finished, len));
+  }
   for (int d = 32; d; d /= 2) before = sat_add(before, __shfl_xor(before, d));
   if (lane == 0) s_sum[wave] = before;
   __syncthreads();
@@ -177,7 +181,9 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
     for (int w = 0; w < kReleaseThreads / 64; ++w) before = sat_add(before, s_sum[w]);
     const int i = i0 + lane;
     const bool live = i < p.N;
-    const int pages = live ? pages_of(i) : 0;
+    const bool finished = live && p.finished[i];
+    const int len = live ? p.cached[i] : 0;
+    const int pages = pages_of(finished, len);
     uint32_t inc = (uint32_t)pages;
     for (int d = 1; d < 64; d *= 2) {
       const uint32_t o = __shfl_up(inc, d);
@@ -186,9 +192,8 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
     s_pages[lane] = pages;
     s_off[lane] = sat_add(before, inc - (uint32_t)pages);
     if (live) {
-      const int len = p.cached[i];
-      if (p.finished[i] && (len < 0 || len > capacity)) flag_error(RPA_SPARSE_ERR_LEN);
-      p.cached_out[i] = p.finished[i] ? 0 : len;
+      if (finished && (len < 0 || len > capacity)) flag_error(RPA_SPARSE_ERR_LEN);
+      p.cached_out[i] = finished ? 0 : len;
     }
     if (i0 + kReleaseSlice >= p.N && lane == 63) {
       const long long end = (long long)max(*p.free_count, 0) + sat_add(before, inc);

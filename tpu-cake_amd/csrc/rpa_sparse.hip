@@ -47,9 +47,11 @@ int rpa_assign_pages(const rpa_paging_shape_t* shape, const int32_t* cached_lens
   const AssignParams p = {cached_lens, new_tokens, page_table, free_pages, free_count, kv_lens, cu_q_lens, num_seqs,
                           slot_mapping, positions, free_count_out, shape->num_requests, shape->pages_per_seq,
                           shape->page_size, shape->free_capacity, shape->max_tokens};
-  constexpr int kThreads = 1024;
-  const int grid = shape->max_tokens > 0 ? (shape->max_tokens + kThreads - 1) / kThreads : 1;
-  assign_kernel<kThreads><<<grid, kThreads, 0, (hipStream_t)stream>>>(p);
+  // small batches take small workgroups: their scans' barriers cost less
+  const int threads = shape->num_requests <= kSmallBatch ? 256 : 1024;
+  const int grid = shape->max_tokens > 0 ? (shape->max_tokens - 1) / threads + 1 : 1;
+  if (threads == 256) assign_kernel<256><<<grid, threads, 0, (hipStream_t)stream>>>(p);
+  else assign_kernel<1024><<<grid, threads, 0, (hipStream_t)stream>>>(p);
   return launched("assign_pages");
 }
 

@@ -62,12 +62,11 @@ def _separate(outs: dict, ins: dict) -> None:
                 raise ValueError(f"{a} overlaps {b}: outputs need memory of their own")
 
 
+# one allocation for a call's outputs: views of it, without the bookkeeping that gradients would need
+_parts = torch.unsafe_split_with_sizes
+
 # shapes that passed the checks -> the call's shape struct
 _plans: dict[tuple, object] = {}
-
-
-def _signature(*tensors) -> tuple:
-    return tuple((t.shape, t.dtype, t.get_device(), t.is_contiguous()) for t in tensors)
 
 
 def _keep(sig: tuple, plan):
@@ -97,7 +96,12 @@ def assign_pages(
     (``cu_q_lens`` does not grow): bring it again in a later step.  Its j-th new page is the next from
     the top of the stack.  Invalid lengths set ``ERR_LEN`` in the error word (``read_error_word``).
     """
-    sig = ("assign", _signature(cached_lens, new_tokens, page_table, free_pages, free_count), page_size, max_tokens)
+    # what the checks go by: written out, as a call costs less than a helper's calls would
+    sig = (page_table.shape, page_table.dtype, page_table.get_device(), page_table.is_contiguous(),
+           cached_lens.shape, cached_lens.dtype, cached_lens.get_device(), cached_lens.is_contiguous(),
+           new_tokens.shape, new_tokens.dtype, new_tokens.get_device(), new_tokens.is_contiguous(),
+           free_pages.shape, free_pages.dtype, free_pages.get_device(), free_pages.is_contiguous(),
+           free_count.shape, free_count.dtype, free_count.get_device(), free_count.is_contiguous(), page_size, max_tokens)
     plan = _plans.get(sig)
     if plan is None:
         n = page_table.shape[0]
@@ -110,11 +114,12 @@ def assign_pages(
         if free_pages.numel() >= 1 << 30:
             raise ValueError("free_pages must have fewer than 2^30 entries")
         plan = _keep(sig, (_sparse_lib.RpaPagingShape(n, page_table.shape[1], page_size, free_pages.numel(), max_tokens),
-                           [n, n + 1, 1, max_tokens, max_tokens, 1], _sparse_lib.load().rpa_assign_pages))
-    shape, sizes, fn = plan
+                           [n, n + 1, 1, max_tokens, max_tokens, 1], 2 * n + 3 + 2 * max_tokens,
+                           _sparse_lib.load().rpa_assign_pages))
+    shape, sizes, total, fn = plan
     dev = page_table.get_device()
     if out is None:
-        out = StepMetadata(*torch.empty(sum(sizes), dtype=torch.int32, device=page_table.device).split(sizes))
+        out = StepMetadata(*_parts(page_table.new_empty(total), sizes))
     else:
         names = dict(zip(StepMetadata._fields, out))
         _check({k: (t, (n,), torch.int32) for (k, t), n in zip(names.items(), sizes)}, page_table, 1, page_size)
@@ -146,7 +151,11 @@ def release_pages(
     """Pushes the pages of finished requests on the free stack, in order; returns (lengths, with 0 for
     the finished ones, and the new count).  Pages past ``free_pages``' capacity are dropped and set
     ``ERR_FREE`` in the error word."""
-    sig = ("release", _signature(cached_lens, finished, page_table, free_pages, free_count), page_size)
+    sig = (page_table.shape, page_table.dtype, page_table.get_device(), page_table.is_contiguous(),
+           cached_lens.shape, cached_lens.dtype, cached_lens.get_device(), cached_lens.is_contiguous(),
+           finished.shape, finished.dtype, finished.get_device(), finished.is_contiguous(),
+           free_pages.shape, free_pages.dtype, free_pages.get_device(), free_pages.is_contiguous(),
+           free_count.shape, free_count.dtype, free_count.get_device(), free_count.is_contiguous(), page_size)
     plan = _plans.get(sig)
     if plan is None:
         n = page_table.shape[0]
@@ -161,7 +170,7 @@ def release_pages(
     shape, sizes, fn = plan
     dev = page_table.get_device()
     if out is None:
-        out = torch.empty(sum(sizes), dtype=torch.int32, device=page_table.device).split(sizes)
+        out = _parts(page_table.new_empty(sizes[0] + 1), sizes)
     else:
         names = {"out lengths": out[0], "out count": out[1]}
         _check({k: (t, (n,), torch.int32) for (k, t), n in zip(names.items(), sizes)}, page_table, 1, page_size)

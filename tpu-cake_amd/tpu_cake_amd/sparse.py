@@ -43,6 +43,7 @@ def make_page_index(kv_pages: torch.Tensor) -> PageIndex:
                      torch.zeros((pages, combined // 2), dtype=torch.int8, device=kv_pages.device))
 
 
+# what passed the checks -> the call's structs; signatures of different entry points differ in length
 _plans: dict[tuple, tuple] = {}
 
 
@@ -51,10 +52,6 @@ def _keep(sig: tuple, plan: tuple) -> tuple:
         _plans.clear()
     _plans[sig] = plan
     return plan
-
-
-def _sig(t: torch.Tensor) -> tuple:
-    return t.shape, t.dtype, t.get_device(), t.is_contiguous()
 
 
 def _tensor(name: str, t, dtype, shape, device, *, rows: bool = False) -> None:
@@ -152,8 +149,14 @@ def append_kv(
     differ and the new rows of one page have to be consecutive tokens, as ``paging.assign_pages`` lays
     them out; ``preflight_append`` checks it on the host.
     """
-    sig = ("append", _sig(k), k.stride(), _sig(v), v.stride(), _sig(kv_pages), _sig(slot_mapping),
-           kv_scales is not None and _sig(kv_scales), k_scale, v_scale, index is not None and (_sig(index[0]), _sig(index[1])))
+    # what the checks go by: written out, as a call costs less than a helper's calls would
+    sig = (k.shape, k.dtype, k.get_device(), k.stride(), v.shape, v.dtype, v.get_device(), v.stride(),
+           kv_pages.shape, kv_pages.dtype, kv_pages.get_device(), kv_pages.is_contiguous(),
+           slot_mapping.shape, slot_mapping.dtype, slot_mapping.get_device(), slot_mapping.is_contiguous(),
+           None if kv_scales is None else (kv_scales.shape, kv_scales.dtype, kv_scales.get_device(), kv_scales.is_contiguous()),
+           k_scale, v_scale,
+           None if index is None else (index[0].shape, index[0].dtype, index[0].get_device(), index[0].is_contiguous(),
+                                       index[1].shape, index[1].dtype, index[1].get_device(), index[1].is_contiguous()))
     plan = _plans.get(sig)
     if plan is None:
         pages, page_size, heads, dim, code = _pool(kv_pages)
@@ -223,8 +226,14 @@ def select_pages(
     two: the choice does not depend on an order of summation.  Tokens at or past ``cu_q_lens[num_seqs]``
     get no page.
     """
-    sig = ("select", q.shape, q.dtype, q.get_device(), q.stride(), _sig(index[0]), _sig(index[1]), _sig(kv_lens),
-           _sig(page_indices), _sig(cu_q_lens), _sig(num_seqs), page_size, num_pages, sink_pages, recent_pages)
+    bounds, exponents = index
+    sig = (q.shape, q.dtype, q.get_device(), q.stride(), bounds.shape, bounds.dtype, bounds.get_device(), bounds.is_contiguous(),
+           exponents.shape, exponents.dtype, exponents.get_device(), exponents.is_contiguous(),
+           kv_lens.shape, kv_lens.dtype, kv_lens.get_device(), kv_lens.is_contiguous(),
+           page_indices.shape, page_indices.dtype, page_indices.get_device(), page_indices.is_contiguous(),
+           cu_q_lens.shape, cu_q_lens.dtype, cu_q_lens.get_device(), cu_q_lens.is_contiguous(),
+           num_seqs.shape, num_seqs.dtype, num_seqs.get_device(), num_seqs.is_contiguous(),
+           page_size, num_pages, sink_pages, recent_pages)
     plan = _plans.get(sig)
     if plan is None:
         _index(index, None, None, None, None)
@@ -248,15 +257,15 @@ def select_pages(
     shape, out_shape, need, fn = plan
     dev = q.get_device()
     if out is None:
-        out = torch.empty(out_shape, dtype=torch.int32, device=q.device)
+        out = kv_lens.new_empty(out_shape)
     else:
         _tensor("out", out, torch.int32, out_shape, q.device)
     if dev != _get_device():
         with torch.cuda.device(dev):
             return select_pages(q, index, kv_lens, page_indices, cu_q_lens, num_seqs, page_size=page_size, num_pages=num_pages,
                                 sink_pages=sink_pages, recent_pages=recent_pages, out=out)
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    rc = fn(shape, sink_pages, recent_pages, q.data_ptr(), index[0].data_ptr(), index[1].data_ptr(), kv_lens.data_ptr(),
+    scratch = bounds.new_empty(need) if need else None  # bytes
+    rc = fn(shape, sink_pages, recent_pages, q.data_ptr(), bounds.data_ptr(), exponents.data_ptr(), kv_lens.data_ptr(),
             page_indices.data_ptr(), cu_q_lens.data_ptr(), num_seqs.data_ptr(), out.data_ptr(),
             scratch.data_ptr() if need else None, need, _current_stream(dev))
     if rc:
@@ -290,9 +299,15 @@ def sparse_paged_attention(
     for the product with V; scaled keys and values are not rounded (the dense operator rounds them to
     bf16).
     """
-    sig = ("attend", q.shape, q.dtype, q.get_device(), q.stride(), _sig(kv_pages), _sig(selected_pages), _sig(kv_lens),
-           _sig(page_indices), _sig(cu_q_lens), _sig(num_seqs), sm_scale, soft_cap, k_scale, v_scale,
-           kv_scales is not None and _sig(kv_scales))
+    sig = (q.shape, q.dtype, q.get_device(), q.stride(),
+           kv_pages.shape, kv_pages.dtype, kv_pages.get_device(), kv_pages.is_contiguous(), selected_pages.shape,
+           selected_pages.dtype, selected_pages.get_device(), selected_pages.is_contiguous(),
+           kv_lens.shape, kv_lens.dtype, kv_lens.get_device(), kv_lens.is_contiguous(),
+           page_indices.shape, page_indices.dtype, page_indices.get_device(), page_indices.is_contiguous(),
+           cu_q_lens.shape, cu_q_lens.dtype, cu_q_lens.get_device(), cu_q_lens.is_contiguous(),
+           num_seqs.shape, num_seqs.dtype, num_seqs.get_device(), num_seqs.is_contiguous(),
+           sm_scale, soft_cap, k_scale, v_scale,
+           None if kv_scales is None else (kv_scales.shape, kv_scales.dtype, kv_scales.get_device(), kv_scales.is_contiguous()))
     plan = _plans.get(sig)
     if plan is None:
         pages, page_size, heads, dim, code = _pool(kv_pages)
@@ -317,7 +332,7 @@ def sparse_paged_attention(
     shape, options, need, fn = plan
     dev = q.get_device()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     else:
         _tensor("out", out, torch.bfloat16, q.shape, q.device)
         if out.data_ptr() == q.data_ptr():
