@@ -306,25 +306,35 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
   }
 }
 
-// The split form's second launch: one workgroup a (row, head tile), a thread for every four dims.
+// The split form's second launch: one workgroup a (row, head tile), a thread for every four dims, the loads of
+// kParts parts at once.
 __global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
+  constexpr int kParts = 8;
   const int tile = blockIdx.x % p.tiles, pair = blockIdx.x / p.tiles, h = pair % p.Hkv, t = pair / p.Hkv;
   const int rows = min(p.G - tile * 16, 16), quads = p.D / 4;
   const size_t stride = 32 + (size_t)min(p.G, 16) * p.D;
   const float* const first = p.parts + (size_t)blockIdx.x * p.splits * stride;
   for (int i = threadIdx.x; i < rows * quads; i += 256) {
     const int r = i / quads, d = i % quads * 4;
-    float top = kLowest;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, first[s * stride + 2 * r]);
-    float sum = 0.f;
+    float top = kLowest, sum = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-      const float* part = first + s * stride;
-      const float l = part[2 * r + 1];
-      if (l == 0.f) continue;  // a part without keys has no O
-      const float f = __builtin_amdgcn_exp2f(part[2 * r] - top);
-      sum += l * f;
-      x += *(const f32x4*)(part + 32 + r * p.D + d) * f;
+    for (int s = 0; s < p.splits; s += kParts) {
+      float m[kParts], l[kParts];
+      f32x4 o[kParts];
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) {
+        const float* part = first + min(s + u, p.splits - 1) * stride;
+        m[u] = part[2 * r], l[u] = s + u < p.splits ? part[2 * r + 1] : 0.f;
+        o[u] = *(const f32x4*)(part + 32 + r * p.D + d);
+      }
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) {
+        if (l[u] == 0.f) continue;  // a part without keys has no O
+        const float next = fmaxf(top, m[u]), mine = __builtin_amdgcn_exp2f(top - next), its = __builtin_amdgcn_exp2f(m[u] - next);
+        top = next;
+        sum = sum * mine + l[u] * its;
+        x = x * mine + o[u] * its;
+      }
     }
     const float g = sum == 0.f ? 0.f : p.v_scale / sum;
     *(u32x2*)(p.out + ((size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r) * p.D + d) =
@@ -717,7 +727,7 @@ struct AttendPlan {
   size_t bytes;
 };
 
-constexpr long long kAttendFill = 1024;  // workgroups that fill the card: four on each of 256 CUs
+constexpr long long kAttendFill = 256;  // workgroups below which lists are split: one a CU
 
 AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
   AttendPlan r = {};
