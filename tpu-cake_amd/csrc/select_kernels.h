@@ -258,14 +258,21 @@ struct WaveTeam {
 template <int THREADS>
 struct Team {
   static constexpr int kGroups = 256;  // maxima that bound the choice
+  static constexpr int kMost = 512;    // candidates ranked
   int count[64];                       // zeroed before
-  uint32_t bound;                      // zeroed before
+  uint32_t bound;
   int found;                           // zeroed before
   Pair scan[THREADS / 64];
   alignas(16) uint32_t top[kGroups];
-  alignas(16) unsigned long long key[THREADS + 2];  // candidates: key, then the page's complement
-  alignas(16) int page[THREADS + 4];                // chosen pages by rank
+  unsigned long long key[kMost];  // candidates: key, then the page's complement
+  int page[kGroups];           // chosen pages by rank
 };
+
+template <int THREADS>
+__device__ __forceinline__ void clear_team(Team<THREADS>& team) {
+  if (threadIdx.x < 64) team.count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) team.found = 0;
+}
 
 // The rows that list every page, and the forced pages of the others: before and behind the rest.
 // Returns how many of the others are wanted, 0: nothing is left to do.
@@ -375,13 +382,15 @@ __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_
   }
 }
 
-// The same by a workgroup, for longer rows.  64 or 256 maxima bound the choice; candidates come together in
-// any order, each is ranked by key and page against all of them, and the chosen ones by page among
-// themselves, so the order of the atomics leaves no trace.
-template <int THREADS>
+// The same by a workgroup, for longer rows.  256 maxima bound the choice, searched by one wave; candidates come
+// together in any order, each is ranked by key and page against all of them, and the chosen ones by page among
+// themselves, so the order of the atomics leaves no trace.  Rows of up to kBatch keys a thread are read
+// once.
+template <int THREADS, int kBatch>  // kBatch: keys of a thread in flight
 __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* keys, int n, int32_t* out, Team<THREADS>& team) {
-  constexpr int kWaves = THREADS / 64, kBatch = 16;  // keys of a thread in flight
-  const int tid = threadIdx.x;
+  constexpr int kWaves = THREADS / 64;
+  constexpr int kGroups = Team<THREADS>::kGroups, kMost = Team<THREADS>::kMost;
+  const int tid = threadIdx.x, lane = tid % 64;
   const int need = choose_forced<THREADS>(p, n, out);
   if (need == 0) return;
   out += p.sink;
@@ -389,68 +398,80 @@ __device__ __forceinline__ void choose(const SelectParams& p, const uint32_t* ke
     const uint32_t k = keys[min(i, n - 1)];
     return i < n && k != kForced ? k : 0u;
   };
-  const int groups = need <= 48 ? 64 : Team<THREADS>::kGroups;
-  if (need <= groups / 4 * 3) {
-    uint32_t top = 0;
-    for (int i = 0; i < n; i += kBatch * THREADS) {
-      uint32_t k[kBatch];
+  if (need <= kGroups / 4 * 3) {
+    uint32_t k[kBatch], top = 0;
+    const auto load = [&](int i) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) k[u] = key(i + THREADS * u + tid);
+      for (int u = 0; u < kBatch; ++u) k[u] = i + THREADS * u < n ? keys[min(i + THREADS * u + tid, n - 1)] : 0u;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) k[u] = i + THREADS * u + tid < n && k[u] != kForced ? k[u] : 0u;
+    };
+    for (int i = 0; i < n; i += kBatch * THREADS) {
+      load(i);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) top = max(top, k[u]);
     }
-    const int wide = THREADS / groups;  // threads of a group, a power of two
-    for (int d = 1; d < wide; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    if (tid % wide == 0) team.top[tid / wide] = top;
+    constexpr int kWide = THREADS / kGroups;  // threads of a group: 4
+    static_assert(kWide == 4, "a quad");
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xf, 0xf, false));  // quad_perm 1 0 3 2
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xf, 0xf, false));  // quad_perm 2 3 0 1
+    if (tid % kWide == 0) team.top[tid / kWide] = top;
     __syncthreads();
-    if (tid < groups) {
-      const uint32_t mine = team.top[tid];
-      int reach = 0;
-#pragma unroll 4
-      for (int i = 0; i < groups / 4; ++i) {
-        const u32x4 o = ((const u32x4*)team.top)[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) reach += o[k] >= mine;
+    if (tid < 64) {
+      const u32x4 mine = ((const u32x4*)team.top)[lane];
+      const auto count = [&](uint32_t t) {
+        return __popcll(__ballot(mine[0] >= t)) + __popcll(__ballot(mine[1] >= t)) + __popcll(__ballot(mine[2] >= t)) +
+               __popcll(__ballot(mine[3] >= t));
+      };
+      uint32_t bound = 0;
+#pragma unroll 1
+      for (int shift = 30; shift >= 14; shift -= 2) {
+        const uint32_t t1 = bound | 1u << shift, t2 = bound | 2u << shift, t3 = bound | 3u << shift;
+        const int c1 = count(t1), c2 = count(t2), c3 = count(t3);
+        bound = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : bound;
+        if ((c3 >= need ? c3 : c2 >= need ? c2 : c1) == need) break;
       }
-      if (reach >= need) atomicMax(&team.bound, mine);
+      if (lane == 0) team.bound = max(bound, 1u);
     }
     __syncthreads();
-    const uint32_t bound = max(1u, team.bound);
+    const uint32_t bound = team.bound;
     for (int i = 0; i < n; i += kBatch * THREADS) {
-      uint32_t k[kBatch];
+      if (n > kBatch * THREADS) load(i);
+      int own = 0;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) k[u] = key(i + THREADS * u + tid);
+      for (int u = 0; u < kBatch; ++u) own += k[u] >= bound;
+      if (own) {
+        int to = atomicAdd(&team.found, own);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (k[u] >= bound) {
-          const int to = atomicAdd(&team.found, 1);
-          if (to < THREADS) team.key[to] = (unsigned long long)k[u] << 32 | (uint32_t)~(i + THREADS * u + tid);
-        }
+        for (int u = 0; u < kBatch; ++u)
+          if (k[u] >= bound) {
+            if (to < kMost) team.key[to] = (unsigned long long)k[u] << 32 | (uint32_t)~(i + THREADS * u + tid);
+            ++to;
+          }
+      }
     }
     __syncthreads();
     const int found = team.found;
-    if (found <= THREADS) {
-      if (tid == 0) team.key[found] = 0;  // what the last two-word read passes
-      __syncthreads();
-      if (tid < found) {
-        const unsigned long long mine = team.key[tid];
+    if (found <= kMost) {
+      // each candidate against every kWide-th of them
+      for (int c = tid / kWide; c < found; c += kGroups) {
+        const unsigned long long mine = team.key[c];
         int rank = 0;
 #pragma unroll 4
-        for (int i = 0; i < found; i += 2) rank += (team.key[i] > mine) + (team.key[i + 1] > mine);
-        if (rank < need) team.page[rank] = ~(uint32_t)mine;
+        for (int i = tid % kWide; i < found; i += kWide) rank += team.key[i] > mine;
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xf, 0xf, false);
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xf, 0xf, false);
+        if (tid % kWide == 0 && rank < need) team.page[rank] = ~(uint32_t)mine;
       }
-      if (tid < 4) team.page[need + tid] = 0x7fffffff;
       __syncthreads();
-      for (int r = tid; r < need; r += THREADS) {
+      for (int r = tid / kWide; r < need; r += kGroups) {
         const int page = team.page[r];
         int at = 0;
 #pragma unroll 4
-        for (int i = 0; i < need; i += 4) {
-          const i32x4 o = *(const i32x4*)(team.page + i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) at += o[e] < page;
-        }
-        out[at] = page;
+        for (int i = tid % kWide; i < need; i += kWide) at += team.page[i] < page;
+        at += __builtin_amdgcn_update_dpp(0, at, 0xB1, 0xf, 0xf, false);
+        at += __builtin_amdgcn_update_dpp(0, at, 0x4E, 0xf, 0xf, false);
+        if (tid % kWide == 0) out[at] = page;
       }
       return;
     }
@@ -519,10 +540,7 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_kernel(SelectParams 
   __shared__ typename std::conditional<WAVE, WaveTeam, Team<kThreads>>::type s_team[WAVE ? kWaves : 1];
   const int tid = threadIdx.x, wave = tid / 64;
   const int h = blockIdx.x % p.Hkv;
-  if constexpr (!WAVE) {
-    if (tid < 64) s_team[0].count[tid] = 0;
-    if (tid == 0) s_team[0].bound = 0, s_team[0].found = 0;
-  }
+  if constexpr (!WAVE) clear_team(s_team[0]);
   const Tile tile = prepare_tile<STEPS, kWaves>(p, blockIdx.x / p.Hkv, h, s_last, rows);
   if (tile.count == 0) return;  // uniform
   __syncthreads();
@@ -534,11 +552,12 @@ __global__ __launch_bounds__(kSelectThreads, 8) void select_kernel(SelectParams 
     for (int i = wave; i < tile.count; i += kWaves)
       choose_wave(p, keys + (size_t)i * p.stride, s_last[i] + 1, out + (size_t)i * p.Hkv * p.K, s_team[wave]);
   } else {
-    choose<kThreads>(p, keys, s_last[0] + 1, out, s_team[0]);
+    choose<kThreads, 4>(p, keys, s_last[0] + 1, out, s_team[0]);  // from LDS
   }
 }
 
-constexpr int kSplitPages = 512;  // pages a workgroup of the split form scores
+constexpr int kSplitPages = 256;  // pages a workgroup of the split form scores (two rows of 31 000 pages of 16 keys
+                                   // 49.5 us, one of them 28.2; 49.8 and 30.8 with 512, 55.7 and 36.7 with 1024)
 
 // The split form, for few rows or rows past the LDS: keys to global memory, then a launch that chooses.
 // Token i of the z-th tile and head h have row (z * p.tokens + i) * Hkv + h of the keys.
@@ -562,14 +581,13 @@ __global__ __launch_bounds__(256) void score_kernel(SelectParams p) {
 __global__ __launch_bounds__(1024) void choose_kernel(SelectParams p) {
   constexpr int kThreads = 1024;
   __shared__ Team<kThreads> s_team;
-  const int tid = threadIdx.x, h = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv, i = row % p.tokens;
-  if (tid < 64) s_team.count[tid] = 0;
-  if (tid == 0) s_team.bound = 0, s_team.found = 0;
+  const int h = blockIdx.x % p.Hkv, row = blockIdx.x / p.Hkv, i = row % p.tokens;
+  clear_team(s_team);
   const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, p.tokens, p.first + row / p.tokens);
   if (i >= tile.count) return;  // uniform
   const int newest = tile.seq < 0 ? -1 : newest_page(tile.pos + i, p.S, p.PPS);
   __syncthreads();
-  choose<kThreads>(p, p.keys + (size_t)blockIdx.x * p.stride, newest + 1, p.out + ((size_t)(tile.first + i) * p.Hkv + h) * p.K,
+  choose<kThreads, 32>(p, p.keys + (size_t)blockIdx.x * p.stride, newest + 1, p.out + ((size_t)(tile.first + i) * p.Hkv + h) * p.K,
                    s_team);
 }
 
