@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
 // Prompt chunks: a workgroup takes a tile of up to 64 columns of one sequence -- `tokens` consecutive tokens,
 // gp columns each, 16 columns a wave -- and the union of their lists, each page of which is read once, into
 // LDS, for all of them.  Neighbouring tokens choose mostly the same pages (in the measured chunk 16 tokens of
-// 32 pages each name about 58), so the L2 gives up a ninth of the bytes that rows of their own would ask
+// 32 pages each name about 40), so the L2 gives up a twelfth of the bytes that rows of their own would ask
 // for, and every wave multiplies whole 16-column tiles.  Per 32 keys the four waves read 64 KB of K and V out
 // of LDS (512 cycles at 128 B a cycle) beside 384 cycles of MFMA each.  A key counts for a column if its page
 // is on the token's own list and it is not past the token's position; a wave passes over 32 keys that none of
@@ -358,24 +358,23 @@ struct TileParams {
   uint32_t sub_magic;         // ceil(2^32 / subs)
 };
 
-constexpr int kTilePages = 512;        // pages of a list that a workgroup holds at once
+constexpr int kTilePages = 384;        // pages of a union that a workgroup holds at once: two workgroups' LDS fit a CU
 constexpr int kTileColumns = 32768;    // page table columns whose bitmaps fit beside them
 constexpr int kTileParts = 2048;       // 64-key parts of a page: below it, block / subs by sub_magic is exact
 
-struct TileEntry {
-  int row, base, mask;  // the page's first pool row, its first position, the tokens that list it
+struct alignas(16) TileEntry {
+  int row, base, mask, unused;  // the page's first pool row, its first position, the tokens that list it
 };
 
-// Groups of four waves take every so manieth 32 keys and join at the end.  Latency bounds a turn (entry,
-// K, softmax, V, barrier), so the card is filled with the waves that registers and LDS allow: one group took
-// 140 us for 500 tokens of 32 pages of 64 keys (32 heads, 8 kv heads), two 130, three 113; 354, 354 and 302
-// for 2000 tokens.
-constexpr int tile_groups(int dp) { return dp == 256 ? 2 : 3; }
-
-template <int DP, bool FULL, bool FP8>
-__global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(TileParams tp) {
+// kGroups groups of four waves take every kGroups-th 32 keys and join at the end.  A turn is bound by what a SIMD
+// issues (24 MFMA of 16 cycles and some 150 VALU instructions a wave) and by waiting for the slowest wave, not by
+// memory: 500 tokens of 32 pages of 64 keys (32 heads, 8 kv heads, 128 dims) take 107 us with 3 groups, one workgroup
+// a CU, and 99 with 2 groups of 128 registers, two workgroups a CU; 2000 tokens 286 and 244; 60 and 250 tokens, too
+// few to fill a CU twice, 64 and 83.  fp8 needs registers for its conversion, 109 us with 3 groups and 154 with 2
+// (spills), and 256 dims the LDS for one workgroup a CU.
+template <int DP, bool FULL, bool FP8, int kGroups>
+__global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGroups) void attend_tile_kernel(TileParams tp) {
   const AttendParams& p = tp.a;
-  constexpr int kGroups = tile_groups(DP);
   constexpr int kThreads = 256 * kGroups;
   constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;  // LDS key rows
   constexpr int kBuffer = 32 * (kKRow + kVRow);
@@ -394,7 +393,8 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
   __shared__ int s_flag[2];  // a page listed twice; an output that is not finite
   __shared__ float s_m[kGroups][64], s_l[kGroups][64];
   const int tid = threadIdx.x, lane = tid % 64, n = lane % 16, j = lane / 16;
-  const int group = tid / 256, wave = tid / 64 % 4, member = tid % 256;
+  const int group = __builtin_amdgcn_readfirstlane(tid / 256), wave = __builtin_amdgcn_readfirstlane(tid / 64 % 4);
+  const int member = tid % 256;
   uint8_t* const s_kv = lds + group * 2 * kBuffer;  // two buffers of the group's own
   const int h = blockIdx.x % p.Hkv;
   const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, tp.tokens, blockIdx.x / p.Hkv);
@@ -450,10 +450,16 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
     u32x4 k[kLoads], v[kLoads];
     const auto load = [&](int unit) {  // a thread: key member / 8, chunks member % 8, + 8, ...
       const int at = unit * 32 + member / 8;
-      const Key x = locate(min(at, keys - 1));
+      Key x;
+      if (p.width % 32 == 0) {  // a page's own 32 keys: found once a wave
+        x = locate(unit * 32);
+        x.off += member / 8;
+      } else {
+        x = locate(min(at, keys - 1));
+      }
       const TileEntry e = s_entry[x.entry];
       const uint8_t* src = (const uint8_t*)g_zero_row;
-      if (at < keys && e.mask && x.off < p.S && e.base + x.off <= last)
+      if ((at < keys) & (e.mask != 0) & (x.off < p.S) & (e.base + x.off <= last))
         src = p.kv + ((size_t)(e.row + x.off) * (2 * p.Hkv) + 2 * h) * row_bytes;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
@@ -499,7 +505,8 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
           const Key x = locate(min(at, keys - 1));
           const TileEntry e = s_entry[x.entry];
           const int most = min(pos - e.base, p.S - 1) - x.off - 4 * j;  // of the lane's four, 0 .. most count
-          if (at < keys && (e.mask >> token & 1) && most >= 0) counts |= (most < 3 ? (2u << most) - 1 : 15u) << (4 * b);
+          const uint32_t four = (1u << min(max(most + 1, 0), 4)) - 1;
+          counts |= ((at < keys) & (e.mask >> token & 1) ? four : 0u) << (4 * b);
           if (FP8) {
             const float kx = s_scale[2 * x.entry], vx = s_scale[2 * x.entry + 1];
 #pragma unroll
@@ -514,7 +521,8 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
             const int at = unit * 32 + 16 * b + 4 * j + r;
             const Key x = locate(min(at, keys - 1));
             const TileEntry e = s_entry[x.entry];
-            if (at < keys && (e.mask >> token & 1) && x.off < p.S && e.base + x.off <= pos) counts |= 1u << (4 * b + r);
+            const bool count = (at < keys) & (e.mask >> token & 1) & (x.off < p.S) & (e.base + x.off <= pos);
+            counts |= (uint32_t)count << (4 * b + r);
             if (FP8) ks[b][r] = s_scale[2 * x.entry], vs[b][r] = s_scale[2 * x.entry + 1];
           }
       }
@@ -535,10 +543,12 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[b][r] : p.scale;
         if (p.cap != 0.f) cap_scores(s, p.cap);
+        if (__ballot(counts != 255)) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] = counts >> (4 * b + r) & 1 ? s[b][r] : -__builtin_inff();
+            for (int r = 0; r < 4; ++r) s[b][r] = counts >> (4 * b + r) & 1 ? s[b][r] : -__builtin_inff();
+        }
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         top = swap_max(top);
@@ -628,7 +638,7 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
     const int phys = table[page];
     const bool ok = phys >= 0 && phys < p.P;
     if (!ok) flag_error(RPA_SPARSE_ERR_PAGE);
-    s_entry[i] = {ok ? phys * p.S : 0, page * p.S, ok ? mask : 0};
+    s_entry[i] = {ok ? phys * p.S : 0, page * p.S, ok ? mask : 0, 0};
     if (FP8) {
       const float* s = p.scales && ok ? p.scales + ((size_t)phys * p.Hkv + h) * 2 : nullptr;
       s_scale[2 * i] = s ? s[0] : 1.f, s_scale[2 * i + 1] = s ? s[1] : 1.f;
@@ -697,7 +707,7 @@ __global__ __launch_bounds__(256 * tile_groups(DP)) void attend_tile_kernel(Tile
         int own;
         const int page = listed(t * p.K + first + i, own);
         if (page >= 0) entry(i, page, 1 << t);
-        else s_entry[i] = {0, 0, 0};
+        else s_entry[i] = {0, 0, 0, 0};
       }
       __syncthreads();
       attend(pages, tile.pos + t);
@@ -727,6 +737,7 @@ struct AttendPlan {
   size_t bytes;
 };
 
+constexpr long long kTileFill = 257;   // tiles from which two workgroups share a CU
 constexpr long long kAttendFill = 256;  // workgroups below which lists are split: one a CU
 
 AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
@@ -761,10 +772,19 @@ void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t st
   if (plan.chunk) {
     const TileParams tp = {p, plan.tokens, plan.gp, plan.gp == 4 ? 2 : plan.gp == 8 ? 3 : 4,
                            (uint32_t)(0x100000000ull / plan.subs + 1)};
-    constexpr int kGroups = tile_groups(DP);
-    const size_t lds = kGroups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
-                       (size_t)((p.PPS + 31) / 32) * 8;
-    attend_tile_kernel<DP, FULL, FP8><<<(unsigned)plan.grid, 256 * kGroups, lds, stream>>>(tp);
+    const auto launch = [&](auto kernel, int groups) {
+      const size_t lds = groups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
+                         (size_t)((p.PPS + 31) / 32) * 8;
+      kernel<<<(unsigned)plan.grid, 256 * groups, lds, stream>>>(tp);
+    };
+    if constexpr (DP == 256) {
+      launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
+    } else if constexpr (FP8) {
+      launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
+    } else {
+      if (plan.grid < kTileFill) launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
+      else launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
+    }
     return;
   }
   const size_t lds = ((size_t)plan.per * (FP8 ? 16 : 8) + 15) / 16 * 16 + (size_t)kAttendWaves * 32 * (DP * 2 + 32);
