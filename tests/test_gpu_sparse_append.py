@@ -159,6 +159,32 @@ def test_slots_outside_the_pool_are_skipped_and_flagged(cuda):
     assert torch.equal(pool, want)
 
 
+@pytest.mark.parametrize("tokens", [6, 64])  # one workgroup's teams, and several workgroups'
+def test_slots_outside_an_fp8_pool_read_no_scales(cuda, tokens):
+    """Far slots beside pages that begin: per-page scales and bounds of the pool's pages only."""
+    rng = np.random.default_rng(tokens)
+    pages = tokens // 2
+    pool = torch.zeros((pages, 4, 4, 128), dtype=torch.float8_e4m3fn, device="cuda")
+    index = sparse.make_page_index(pool)
+    scales = rng.uniform(0.002, 0.02, (pages, 2, 2)).astype(np.float32)
+    x = torch.from_numpy(rng.standard_normal((tokens, 2, 128)).astype(np.float32)).to(torch.bfloat16)
+    slots = np.full(tokens, 2**31 - 1, np.int64)
+    slots[::2] = 4 * np.arange(pages)
+    slots[1] = -7
+    sparse.read_error_word(clear=True)
+    sparse.append_kv(x.cuda(), x.cuda(), pool, i32(slots), kv_scales=torch.from_numpy(scales).cuda(), index=index)
+    assert sparse.read_error_word(clear=True) == sparse._sparse_lib.ERR_SLOT
+    codes = _codes(x[::2].float().numpy(), scales[:, :, :1])
+    got = pool.double().cpu().numpy()
+    np.testing.assert_array_equal(got[:, 0, ::2], codes)
+    assert (got[:, 1:] == 0).all()
+    for p in range(pages):
+        for h in range(2):
+            bounds, e = orc.page_bounds((codes[p, h].astype(np.float32) * scales[p, h, 0])[None])
+            assert index.exponents[p, h].item() == e
+            np.testing.assert_array_equal(index.bounds[p, h].cpu().numpy(), bounds)
+
+
 def test_rows_past_a_page_that_grows_are_left_alone(cuda):
     pool = torch.full((3, 8, 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")
     x = torch.randn((3, 1, 128), device="cuda").to(torch.bfloat16)

@@ -151,7 +151,7 @@ __device__ __forceinline__ void widen_runs(const AppendParams& p, int t, int pag
   const int step = alone ? min(teams, run) : min(run, 1), from = alone ? team : 0;
   const bool merges = run > 0 && (!alone || team == 0);
   for (int h = threadIdx.x / 64; h < p.Hkv; h += blockDim.x / 64) {
-    const size_t at = (size_t)page * p.Hkv + h;
+    const size_t at = (size_t)(run ? page : 0) * p.Hkv + h;  // without a run the page may be any number
     int8_t* const up = p.bounds + at * 2 * p.D + 8 * c;
     int8_t* const down = up + p.D;
     u32x2 was_up = {0, 0}, was_down = {0, 0};
