@@ -28,7 +28,7 @@ extern "C" {
 enum {
   RPA_SPARSE_ERR_PAGE = 1,  /* a page id outside the pool */
   RPA_SPARSE_ERR_SLOT = 2,  /* a slot outside the pool (not -1, which means: no row) */
-  RPA_SPARSE_ERR_LEN = 4,   /* a negative length, or one past the page table */
+  RPA_SPARSE_ERR_LEN = 4,   /* a length past the page table; given to the paging calls, also a negative one */
   RPA_SPARSE_ERR_FREE = 8   /* the free stack's count or capacity exceeded */
 };
 
@@ -79,7 +79,7 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
  * are rounded up to that grid and the smallest down, clamped to [-127, 127]; NaN counts as 0.  Keys of
  * an fp8 pool are code * K scale. */
 typedef struct rpa_append_shape {
-  int32_t num_tokens;
+  int32_t num_tokens;  /* below 2^30 */
   int32_t num_kv_heads;
   int32_t head_dim;    /* as rpa_shape_t: 256, or a multiple of 8 in [32, 128] (fp8: of 16 in [64, 128]) */
   int32_t total_pages;
@@ -92,7 +92,8 @@ typedef struct rpa_append_shape {
 /* Writes token t's key and value rows (bf16) to row slot_mapping[t] % page_size of page
  * slot_mapping[t] / page_size of kv_pages (rpa.h's layout); -1: no row.  fp8 pools hold
  * e4m3(x / scale), saturated, with the scale of the row's page and head in kv_scales (float
- * [total_pages, num_kv_heads, 2]) or, where that is NULL, k_scale and v_scale (ignored for bf16).
+ * [total_pages, num_kv_heads, 2]) or, where that is NULL, k_scale and v_scale, positive and finite
+ * (ignored for bf16).
  * bounds and exponents: the pool's index, or both NULL.  A page whose row 0 is written starts its
  * bounds anew, other pages' widen.  The slots (other than -1) have to differ, and the new rows of one
  * page have to be consecutive tokens at consecutive slots. */
@@ -135,8 +136,8 @@ typedef struct rpa_sparse_options {
  * its kv head: selected_pages int32 [num_tokens, num_kv_heads, num_pages], logical pages in any order,
  * entries outside the token's pages (-1) list nothing, a page listed twice counts twice.  Keys and values
  * of an fp8 pool are code * scale, not rounded; kv_scales as in rpa.h or NULL.
- * out bf16 [num_tokens, num_q_heads, head_dim], contiguous; rows without a key, and rows at or past
- * cu_q_lens[num_seqs], are zero. */
+ * out bf16 [num_tokens, num_q_heads, head_dim], contiguous; rows without a key or without a score
+ * above -infinity, and rows at or past cu_q_lens[num_seqs], are zero. */
 size_t rpa_sparse_workspace_size(const rpa_sparse_shape_t* shape);
 int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse_options_t* options, const void* q,
                                const void* kv_pages, const float* kv_scales, const int32_t* selected_pages,

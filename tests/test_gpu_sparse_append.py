@@ -147,6 +147,23 @@ def test_extreme_keys_in_the_index(cuda):
             np.testing.assert_array_equal(index.bounds[p, h].cpu().numpy(), bounds, err_msg=f"{p} {h}")
 
 
+def test_extreme_scales_in_the_index(cuda):
+    """Page scales of 0, NaN and infinity: keys that the pool holds as NaN times them count as 0."""
+    rng = np.random.default_rng(1)
+    x = torch.from_numpy(rng.choice([0.0, 1.0, -2.5, 3e38, -np.inf, np.nan], (40, 1, 64)).astype(np.float32)).to(torch.bfloat16)
+    scales = np.array([0.0, np.nan, np.inf, 1e-30, 1e30], np.float32)
+    pool = torch.zeros((5, 8, 2, 64), dtype=torch.float8_e4m3fn, device="cuda")
+    index = sparse.make_page_index(pool)
+    both = torch.from_numpy(np.repeat(scales[:, None, None], 2, axis=2)).contiguous().cuda()
+    sparse.append_kv(x.cuda(), x.cuda(), pool, i32(np.arange(40)), kv_scales=both, index=index)
+    with np.errstate(all="ignore"):
+        keys = pool[:, :, 0].double().cpu().numpy().astype(np.float32) * scales[:, None, None]
+    for p in range(5):
+        bounds, e = orc.page_bounds(keys[p])
+        assert index.exponents[p, 0].item() == e, p
+        np.testing.assert_array_equal(index.bounds[p, 0].cpu().numpy(), bounds, err_msg=str(p))
+
+
 def test_slots_outside_the_pool_are_skipped_and_flagged(cuda):
     sparse.read_error_word(clear=True)
     pool = torch.zeros((2, 4, 2, 64), dtype=torch.bfloat16, device="cuda")

@@ -84,6 +84,28 @@ def test_append_refuses_pointers(lib):
     assert lib.rpa_append_kv(None, *FAKE[:5], 1.0, 1.0, *FAKE[5:7], None) == -1
 
 
+@pytest.mark.parametrize("bad", [0.0, -0.5, float("inf"), float("nan")])
+def test_append_refuses_scales(lib, monkeypatch, anywhere, bad):
+    ok = ctypes.byref(_append(kv_dtype=1))
+    for scales in ((bad, 1.0), (1.0, bad)):
+        assert lib.rpa_append_kv(ok, *FAKE[:4], None, *scales, *FAKE[5:7], None) == -1
+        assert b"positive and finite" in lib.rpa_sparse_last_error()
+    real = sparse._tensor
+    monkeypatch.setattr(sparse, "_tensor", lambda *a, **kw: real(*a))
+    pool = torch.zeros((4, 16, 4, 128), dtype=torch.uint8)
+    for scales in (dict(k_scale=bad), dict(v_scale=bad)):
+        with pytest.raises(ValueError, match="positive and finite"):
+            sparse.append_kv(_bf(3, 2, 128), _bf(3, 2, 128), pool, _i(3), **scales)
+
+
+def test_counts_that_pass_32_bits_are_refused(lib):
+    many = ctypes.byref(_append(num_tokens=1 << 30))
+    assert lib.rpa_append_kv(many, *FAKE[:5], 1.0, 1.0, *FAKE[5:7], None) == -1 and b"2^30" in lib.rpa_sparse_last_error()
+    wide = ctypes.byref(_sparse(max_num_seqs=1 << 27))
+    assert lib.rpa_select_pages(wide, 1, 1, *FAKE[:9], 1 << 40, None) == -1 and b"max_num_seqs" in lib.rpa_sparse_last_error()
+    assert lib.rpa_sparse_workspace_size(wide) == 0
+
+
 def _sparse(**kw):
     return _sparse_lib.RpaSparseShape(**{**dict(num_tokens=4, num_q_heads=8, num_kv_heads=2, head_dim=128, total_pages=64, page_size=16,
                                                 max_num_seqs=4, pages_per_seq=8, kv_dtype=0, num_pages=6, q_token_stride=1024,

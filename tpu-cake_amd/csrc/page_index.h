@@ -188,6 +188,11 @@ __device__ __forceinline__ void widen_runs(const AppendParams& p, int t, int pag
     if (FP8) {
       fp8_values(fp8_codes(hi, scale), scale, hi);
       fp8_values(fp8_codes(lo, scale), scale, lo);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // a scale of 0 or none that is a number: 0, as other NaN
+        hi[i] = hi[i] == hi[i] ? hi[i] : 0.f;
+        lo[i] = lo[i] == lo[i] ? lo[i] : 0.f;
+      }
     }
     float amax = 0.f;
 #pragma unroll
@@ -305,6 +310,7 @@ int check_strides(const char* name, const void* p, long long token, long long he
 int check_append(const rpa_append_shape_t* s) {
   if (!s) return fail(RPA_E_INVALID, "shape is NULL");
   if (s->num_tokens < 0) return fail(RPA_E_INVALID, "negative num_tokens");
+  if (s->num_tokens >= 1 << 30) return fail(RPA_E_INVALID, "num_tokens must be below 2^30");
   const int rc = check_heads(s->num_kv_heads, s->head_dim, s->kv_dtype);
   return rc ? rc : check_pool(s->total_pages, s->page_size);
 }

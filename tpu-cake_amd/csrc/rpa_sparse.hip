@@ -1,4 +1,5 @@
 // librpa_sparse: the C ABI of include/rpa_sparse.h over its kernels.
+#include <float.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -83,6 +84,9 @@ int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void*
   if ((rc = check_strides("keys", keys, shape->k_token_stride, shape->k_head_stride))) return rc;
   if ((rc = check_strides("values", values, shape->v_token_stride, shape->v_head_stride))) return rc;
   if (!aligned16(kv_pages) || !aligned16(bounds)) return fail(RPA_E_INVALID, "kv_pages and bounds must be 16-byte aligned");
+  const auto usable = [](float x) { return x > 0.f && x <= FLT_MAX; };
+  if (shape->kv_dtype == RPA_KV_FP8_E4M3 && !kv_scales && !(usable(k_scale) && usable(v_scale)))
+    return fail(RPA_E_INVALID, "k_scale and v_scale must be positive and finite");
   const int chunks = shape->head_dim / 8, tokens = shape->num_tokens > kAppendLong ? kAppendTokens : 1;
   const int ahead = 64 / chunks * (tokens > 1 ? kAppendRounds : 1);  // tokens of a workgroup that widens bounds
   const int wide = bounds ? (shape->num_tokens - 1) / ahead + 1 : 0;

@@ -606,6 +606,8 @@ int check_sparse(const rpa_sparse_shape_t* s) {
     return fail(RPA_E_INVALID, "pages_per_seq * page_size overflows int32");
   if ((long long)s->num_tokens * s->num_kv_heads > 0x7fffffffll)
     return fail(RPA_E_INVALID, "num_tokens * num_kv_heads overflows int32");
+  if (s->num_tokens + 16ll * s->max_num_seqs > 0x7fffffffll)
+    return fail(RPA_E_INVALID, "num_tokens + 16 * max_num_seqs overflows int32");
   if (s->num_q_heads / s->num_kv_heads > 256) return fail(RPA_E_UNSUPPORTED, "more than 256 query heads per kv head");
   return RPA_OK;
 }

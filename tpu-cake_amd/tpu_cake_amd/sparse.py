@@ -167,6 +167,9 @@ def append_kv(
         _scales(kv_scales, k_scale, v_scale, pages, heads, code, device)
         if code != _sparse_lib.RPA_KV_FP8_E4M3 and (k_scale is not None or v_scale is not None):
             raise ValueError("k_scale and v_scale require fp8 kv_pages")
+        for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if x is not None and not 0.0 < x < float("inf"):
+                raise ValueError(f"{name}={x!r} must be positive and finite")
         if index is not None:
             _index(index, pages, heads, dim, device)
         shape = _sparse_lib.RpaAppendShape(k.shape[0], heads, dim, pages, page_size, code, k.stride(0), k.stride(1),
@@ -294,8 +297,8 @@ def sparse_paged_attention(
     token's sequence in any order, -1 or other entries outside its pages list nothing, a page listed
     twice counts twice).
 
-    Returns bf16 [T, Hq, D] (or fills ``out``); rows without a key, and rows at or past
-    ``cu_q_lens[num_seqs]``, are zero.  Scores, softmax and sums are fp32 and probabilities keep 16 bits
+    Returns bf16 [T, Hq, D] (or fills ``out``); rows without a key or without a score above -infinity,
+    and rows at or past ``cu_q_lens[num_seqs]``, are zero.  Scores, softmax and sums are fp32 and probabilities keep 16 bits
     for the product with V; scaled keys and values are not rounded (the dense operator rounds them to
     bf16).
     """
