@@ -32,6 +32,22 @@ constexpr int kMaxBlocks = 1024;     // list blocks of a workgroup
 // What keys that do not exist read: zeros, so that P = 0 never meets a NaN.
 __device__ uint4 g_zero_row[64];
 
+typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
+
+// Its address, kept in registers: the compiler would load it from the code object's table in every turn.
+__device__ __forceinline__ global_bytes zero_row() {
+  uint64_t at = (uint64_t)g_zero_row;
+  asm volatile("" : "+s"(at));
+  return (global_bytes)at;
+}
+
+__device__ __forceinline__ u32x4 load16(global_bytes at) {
+  return *(const __attribute__((address_space(1))) u32x4*)at;
+}
+
+// The larger one, or the one that is a number; fmaxf spends instructions on signalling NaN first.
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
+
 struct AttendParams {
   const uint16_t* q;
   const uint8_t* kv;
@@ -46,6 +62,7 @@ struct AttendParams {
   uint32_t magic;           // ceil(2^32 / width): v / width for v < 2^26 (width > 1)
   int per, splits;          // blocks of a workgroup
   float scale, cap, v_scale;  // scale: of q.k; times log2 e where cap is 0
+  int late;                   // the scale is applied behind the mask, with the exponential: bf16, no cap, scale > 0
 };
 
 __device__ __forceinline__ u32x4 bf16_of_codes(uint32_t a, uint32_t b) {  // eight e4m3 codes, exactly
@@ -427,6 +444,9 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
   }
 
   const int row_bytes = p.D * kElem;
+  const uint32_t row_stride = 2u * p.Hkv * row_bytes;
+  const global_bytes zero = zero_row(), rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
+  const float late = p.late ? p.scale : 1.f;
   f32x4 o[DP / 16];
   float m, l;
   const auto reset = [&] {
@@ -458,16 +478,15 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
         x = locate(min(at, keys - 1));
       }
       const TileEntry e = s_entry[x.entry];
-      const uint8_t* src = (const uint8_t*)g_zero_row;
-      if ((at < keys) & (e.mask != 0) & (x.off < p.S) & (e.base + x.off <= last))
-        src = p.kv + ((size_t)(e.row + x.off) * (2 * p.Hkv) + 2 * h) * row_bytes;
+      const bool exists = (at < keys) & (e.mask != 0) & (x.off < p.S) & (e.base + x.off <= last);
+      const global_bytes key = rows + (uint64_t)(uint32_t)(e.row + x.off) * row_stride, src = exists ? key : zero;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int byte = 16 * (member % 8 + 8 * i);
         k[i] = v[i] = u32x4{0, 0, 0, 0};
         if (byte < (FULL ? DP * kElem : row_bytes)) {
-          k[i] = *(const u32x4*)(src + byte);
-          v[i] = *(const u32x4*)(src + row_bytes + byte);
+          k[i] = load16(src + byte);
+          v[i] = load16(src + row_bytes + byte);
         }
       }
     };
@@ -497,7 +516,28 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
       // which of the lane's keys (16 b + 4 j + r) count for its column
       uint32_t counts = 0;
       float ks[2][4], vs[2][4];
+      bool inside = false;  // all of the keys lie before the tile's first token
       if (unit >= units) {
+      } else if (p.width % 32 == 0) {  // 32 keys lie in one page
+        const Key x = locate(unit * 32);
+        const TileEntry e = s_entry[x.entry];
+        const int base = __builtin_amdgcn_readfirstlane(e.base), mask = __builtin_amdgcn_readfirstlane(e.mask);
+        inside = base + x.off + 31 <= tile.pos && x.off + 31 < p.S;
+        if (inside) {
+          counts = 255;
+        } else {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int most = min(pos - base, p.S - 1) - x.off - 16 * b - 4 * j;  // of the lane's four, 0 .. most count
+            counts |= ((1u << min(max(most + 1, 0), 4)) - 1) << (4 * b);
+          }
+        }
+        counts = mask >> token & 1 ? counts : 0u;
+        if (FP8) {
+          const float kx = s_scale[2 * x.entry], vx = s_scale[2 * x.entry + 1];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) ks[r / 4][r % 4] = kx, vs[r / 4][r % 4] = vx;
+        }
       } else if (p.width % 16 == 0) {  // 16 keys lie in one page
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -538,21 +578,27 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], s[b], 0, 0, 0);
           }
         }
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[b][r] : p.scale;
-        if (p.cap != 0.f) cap_scores(s, p.cap);
-        if (__ballot(counts != 255)) {
+        if (FP8 || !p.late) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[b][r] = counts >> (4 * b + r) & 1 ? s[b][r] : -__builtin_inff();
+            for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[b][r] : p.scale;
+          if (p.cap != 0.f) cap_scores(s, p.cap);
         }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = swap_max(top);
-        if (__ballot(top > m + kRescale)) {
+        if (__ballot(counts != 255)) {
+          if (inside) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) s[r / 4][r % 4] = counts ? s[r / 4][r % 4] : -__builtin_inff();
+          } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) s[r / 4][r % 4] = counts >> r & 1 ? s[r / 4][r % 4] : -__builtin_inff();
+          }
+        }
+        float top = max_of(max_of(max_of(s[0][0], s[0][1]), max_of(s[0][2], s[0][3])),
+                           max_of(max_of(s[1][0], s[1][1]), max_of(s[1][2], s[1][3])));
+        if (!FP8) top *= late;
+        if (__ballot(top > m + kRescale)) {  // of the lane's own keys: any lane's
+          top = swap_max(top);
           const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
           m = next;
           l *= f;
@@ -565,7 +611,7 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
           float e[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
+            e[r] = __builtin_amdgcn_exp2f(FP8 ? s[b][r] - m : __builtin_fmaf(s[b][r], late, -m));
             l += e[r];
             if (FP8) e[r] *= vs[b][r];
           }
