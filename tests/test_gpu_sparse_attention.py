@@ -202,6 +202,25 @@ def test_scores_at_the_ends_of_the_range(cuda):
     assert (np.abs(got.double().cpu().numpy() - want) <= 2.0**-8 * np.abs(want) + 5 * 2.0**-15).all()
 
 
+@pytest.mark.parametrize("size", [1e37, 3e9, -3e9, -1e37])
+@pytest.mark.parametrize("scale", [1.0, 0.7])
+def test_large_scores_in_chunks(cuda, size, scale):
+    """Tied scores of any size and scale: the mean of the values, in tiles of a chunk's tokens too."""
+    b = Batch(20, [96], [32], 16, 2, 1, 64)
+    pool, _, _, _ = b.pool()
+    held = pool.view(b.total, 16, 1, 2, 64)
+    held[:, :, :, 0] = 0
+    held[:, :, :, 0, 0] = 1.0
+    b.q[:] = 0
+    b.q[:, :, 0] = size
+    picked = np.tile(np.arange(6), (b.tokens, 1, 1))
+    got = sparse.sparse_paged_attention(b.q.cuda(), pool.cuda(), i32(picked), *b.meta(), sm_scale=scale)
+    x = held.double().numpy()
+    want = orc.sparse_attention(b.q.double().numpy(), x[:, :, :, 0], x[:, :, :, 1], picked, b.lens, b.table, b.cu, b.n, scale)
+    # half a step of the result, and two parts of 2^-17 of each value's weight
+    assert (np.abs(got.double().cpu().numpy() - want) <= 2.0**-8 * np.abs(want) + 2.0**-16 * np.abs(x[:, :, :, 1]).max()).all()
+
+
 def test_whole_lists_equal_the_dense_operator(cuda):
     """With every page listed the dense operator's result, within both operators' roundings."""
     b = Batch(18, [300, 90, 1, 600], [1, 40, 1, 1], 16, 8, 2, 128)

@@ -62,7 +62,6 @@ struct AttendParams {
   uint32_t magic;           // ceil(2^32 / width): v / width for v < 2^26 (width > 1)
   int per, splits;          // blocks of a workgroup
   float scale, cap, v_scale;  // scale: of q.k; times log2 e where cap is 0
-  int late;                   // the scale is applied behind the mask, with the exponential: bf16, no cap, scale > 0
 };
 
 __device__ __forceinline__ u32x4 bf16_of_codes(uint32_t a, uint32_t b) {  // eight e4m3 codes, exactly
@@ -85,12 +84,19 @@ __device__ __forceinline__ u32x2 split_bf16(float a, float b) {
   return u32x2{hi, pack_bf16(a - bf16_lo(hi), b - bf16_hi(hi))};
 }
 
+// A product that rounds by itself: joined with the subtraction of the maximum into one operation, the maximum's own
+// rounding would remain, 2^100 and more for the largest scores.
+__device__ __forceinline__ float scaled(float x, float scale) {
+#pragma clang fp contract(off)
+  return x * scale;
+}
+
 __device__ __forceinline__ void cap_scores(f32x4 s[2], float cap) {
 #pragma unroll 1
   for (int b = 0; b < 2; ++b) {
     f32x4 x = b ? s[1] : s[0];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = cap * tanhf(x[r] / cap) * kLog2e;
+    for (int r = 0; r < 4; ++r) x[r] = scaled(cap * tanhf(x[r] / cap), kLog2e);
     if (b) s[1] = x;
     else s[0] = x;
   }
@@ -172,6 +178,8 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
   }
 
   const int row_bytes = p.D * kElem;
+  const uint32_t row_stride = 2u * p.Hkv * row_bytes;
+  const global_bytes zero = zero_row(), keys = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
   const auto block_of = [&](int v) { return p.width == 1 ? v : (int)__umulhi((uint32_t)v, p.magic); };
   u32x4 k[2][kLoads], v[2][kLoads];
   uint32_t seen[2];  // bit n: key n of the 16 exists
@@ -179,16 +187,16 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int key = unit * 32 + 16 * b + n, block = block_of(key), off = key - block * p.width;
-      const bool ok = block < p.per && off < s_len[min(block, p.per - 1)];
+      const int entry = min(block, p.per - 1);
+      const bool ok = (block < p.per) & (off < s_len[entry]);
       seen[b] = (uint32_t)__ballot(ok) & 0xffffu;
-      const uint8_t* src = (const uint8_t*)g_zero_row;
-      if (ok) src = p.kv + ((size_t)(s_row[block] + off) * (2 * p.Hkv) + 2 * h) * row_bytes;
+      const global_bytes key_row = keys + (uint64_t)(uint32_t)(s_row[entry] + off) * row_stride, src = ok ? key_row : zero;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int byte = 64 * i + 16 * j;
         if (FULL || byte < row_bytes) {
-          k[b][i] = *(const u32x4*)(src + byte);
-          v[b][i] = *(const u32x4*)(src + row_bytes + byte);
+          k[b][i] = load16(src + byte);
+          v[b][i] = load16(src + row_bytes + byte);
         } else {
           k[b][i] = v[b][i] = u32x4{0, 0, 0, 0};
         }
@@ -228,6 +236,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
         }
       }
     wave_fence();
+    const bool whole = (seen[0] & seen[1]) == 0xffffu;  // before the next unit's
     const uint32_t here[2] = {seen[0] >> (4 * j), seen[1] >> (4 * j)};
     if (unit + kAttendWaves < units) load(unit + kAttendWaves);
 
@@ -243,17 +252,19 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[r] : p.scale;
+      for (int r = 0; r < 4; ++r) s[b][r] = scaled(s[b][r], FP8 ? p.scale * ks[r] : p.scale);
     }
     if (p.cap != 0.f) cap_scores(s, p.cap);
+    if (!whole) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[b][r] = here[b] >> r & 1 ? s[b][r] : -__builtin_inff();
-    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    top = swap_max(top);
-    if (__ballot(top > m + kRescale)) {
+        for (int r = 0; r < 4; ++r) s[b][r] = here[b] >> r & 1 ? s[b][r] : -__builtin_inff();
+    }
+    float top = max_of(max_of(max_of(s[0][0], s[0][1]), max_of(s[0][2], s[0][3])),
+                       max_of(max_of(s[1][0], s[1][1]), max_of(s[1][2], s[1][3])));
+    if (__ballot(top > m + kRescale)) {  // of the lane's own keys: any lane's
+      top = swap_max(top);
       const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
       m = next;
       l *= f;
@@ -446,7 +457,6 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
   const int row_bytes = p.D * kElem;
   const uint32_t row_stride = 2u * p.Hkv * row_bytes;
   const global_bytes zero = zero_row(), rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
-  const float late = p.late ? p.scale : 1.f;
   f32x4 o[DP / 16];
   float m, l;
   const auto reset = [&] {
@@ -578,13 +588,11 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], s[b], 0, 0, 0);
           }
         }
-        if (FP8 || !p.late) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[b][r] *= FP8 ? p.scale * ks[b][r] : p.scale;
-          if (p.cap != 0.f) cap_scores(s, p.cap);
-        }
+          for (int r = 0; r < 4; ++r) s[b][r] = scaled(s[b][r], FP8 ? p.scale * ks[b][r] : p.scale);
+        if (p.cap != 0.f) cap_scores(s, p.cap);
         if (__ballot(counts != 255)) {
           if (inside) {
 #pragma unroll
@@ -596,7 +604,6 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
         }
         float top = max_of(max_of(max_of(s[0][0], s[0][1]), max_of(s[0][2], s[0][3])),
                            max_of(max_of(s[1][0], s[1][1]), max_of(s[1][2], s[1][3])));
-        if (!FP8) top *= late;
         if (__ballot(top > m + kRescale)) {  // of the lane's own keys: any lane's
           top = swap_max(top);
           const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
@@ -611,7 +618,7 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
           float e[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(FP8 ? s[b][r] - m : __builtin_fmaf(s[b][r], late, -m));
+            e[r] = __builtin_amdgcn_exp2f(s[b][r] - m);
             l += e[r];
             if (FP8) e[r] *= vs[b][r];
           }

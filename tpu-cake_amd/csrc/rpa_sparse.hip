@@ -171,7 +171,6 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
   p.per = plan.per, p.splits = plan.splits;
   p.scale = options->sm_scale * options->k_scale * (cap != 0.f ? 1.f : kLog2e), p.cap = cap;
   p.v_scale = options->v_scale;
-  p.late = !fp8 && cap == 0.f && p.scale > 0.f;
   const hipStream_t s = (hipStream_t)stream;
   const int D = p.D;
   if (fp8) {
