@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
 // Prompt chunks: a workgroup takes a tile of up to 64 columns of one sequence -- `tokens` consecutive tokens,
 // gp columns each, 16 columns a wave -- and the union of their lists, each page of which is read once, into
 // LDS, for all of them.  Neighbouring tokens choose mostly the same pages (in the measured chunk 16 tokens of
-// 32 pages each name about 40), so the L2 gives up a twelfth of the bytes that rows of their own would ask
+// 32 pages each name 44 to 48), so the L2 gives up a tenth of the bytes that rows of their own would ask
 // for, and every wave multiplies whole 16-column tiles.  Per 32 keys the four waves read 64 KB of K and V out
 // of LDS (512 cycles at 128 B a cycle) beside 384 cycles of MFMA each.  A key counts for a column if its page
 // is on the token's own list and it is not past the token's position; a wave passes over 32 keys that none of
@@ -395,11 +395,11 @@ struct alignas(16) TileEntry {
 };
 
 // kGroups groups of four waves take every kGroups-th 32 keys and join at the end.  A turn is bound by what a SIMD
-// issues (24 MFMA of 16 cycles and some 150 VALU instructions a wave) and by waiting for the slowest wave, not by
-// memory: 500 tokens of 32 pages of 64 keys (32 heads, 8 kv heads, 128 dims) take 107 us with 3 groups, one workgroup
-// a CU, and 99 with 2 groups of 128 registers, two workgroups a CU; 2000 tokens 286 and 244; 60 and 250 tokens, too
-// few to fill a CU twice, 64 and 83.  fp8 needs registers for its conversion, 109 us with 3 groups and 154 with 2
-// (spills), and 256 dims the LDS for one workgroup a CU.
+// issues (24 MFMA of 16 cycles and some 120 VALU instructions a wave), by its chain of LDS reads, products and
+// exponentials and by waiting for the slowest wave, not by memory: 500 tokens of 32 pages of 64 keys (32 heads, 8
+// kv heads, 128 dims) take 100 us with 3 groups, one workgroup a CU, and 92 with 2 groups of 128 registers, two
+// workgroups a CU; 2000 tokens 264 and 228; 60 and 250 tokens, too few to fill a CU twice, 60 and 79.  fp8 needs
+// registers for its conversion, 104 us with 3 groups, and spills with 2; 256 dims fill the LDS with one workgroup.
 template <int DP, bool FULL, bool FP8, int kGroups>
 __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGroups) void attend_tile_kernel(TileParams tp) {
   const AttendParams& p = tp.a;
