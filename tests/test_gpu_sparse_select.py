@@ -80,6 +80,21 @@ def test_ties_go_to_the_earlier_page(cuda):
     _check(b, 20, index=(bounds, exps))
 
 
+@pytest.mark.parametrize("num_pages", [34, 35, 64, 100, 193, 194, 250, 700])
+@pytest.mark.parametrize("tied", [False, True])
+def test_wide_lists(cuda, num_pages, tied):
+    """Lists of every way that a wave or a workgroup bounds its candidates, also where all of them tie."""
+    b = Batch(num_pages, [1200, 400, 380, 1400, 130], [20, 9, 1, 1, 30], 2, 4, 2, 64)
+    decode = Batch(num_pages, [2000, 1100, 700, 380], [1] * 4, 2, 4, 2, 64)
+    for rows in (b, decode):
+        bounds, exps = rows.index()
+        if tied:
+            bounds[:, :, :, 2:] = 0  # scores of few different values
+            bounds //= 50
+            exps[:] = -5
+        _check(rows, num_pages, index=(bounds, exps))
+
+
 def test_exponents_at_their_ends(cuda):
     b = Batch(3, [800, 500], [1, 40], 4, 4, 2, 128)
     bounds, exps = b.index(spread=(-100, 101))

@@ -247,11 +247,11 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int seq, int 
   }
 }
 
-constexpr int kFew = 128;  // candidates that one wave ranks
+constexpr int kFew = 192;  // candidates that one wave ranks
 
 struct WaveTeam {
   alignas(16) uint32_t key[kFew + 4];
-  int page[kFew];
+  uint16_t page[kFew];  // of a row of at most kWaveRow
 };
 
 // What a workgroup shares while it chooses for a row.
@@ -308,9 +308,9 @@ __device__ __forceinline__ uint32_t search_wave(const Key& key, int n, int need)
 
 // One wave writes the chosen pages of one row, ascending, from its n keys.
 //
-// Few keys survive a cheap bound: where the 64 lanes' maxima hold `need` values of at least x, so do the
-// keys, and none below x is chosen.  x is the need-th largest maximum to 16 bits; of n random keys not many
-// more than `need` survive.  They are moved together and each is ranked against all of them.
+// Few keys survive a cheap bound: where 64 lanes' maxima, or four of each lane, hold `need` values of at least x,
+// so do the keys, and none below x is chosen.  x is the need-th largest maximum to 16 bits; of n random keys not
+// many more than `need` survive.  They are moved together and each is ranked against all of them.
 __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_t* keys, int n, int32_t* out, WaveTeam& team) {
   const int lane = threadIdx.x % 64;
   const unsigned long long below = (1ull << lane) - 1;
@@ -321,14 +321,23 @@ __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_
     const uint32_t k = keys[min(i + lane, n - 1)];
     return i + lane < n && k != kForced ? k : 0u;
   };
-  uint32_t top = 0;
-#pragma unroll 4
-  for (int i = 0; i < n; i += 64) top = max(top, key(i));
+  uint32_t top[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int i = 0; i < n; i += 256)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top[u] = max(top[u], key(i + 64 * u));
+  const bool quick = need <= 32;  // 1000 tokens choose 30 of 512 pages in 32.8 us by 64 maxima, 33.8 by 256; 50 in 44 and 39
+  if (quick) top[0] = max(max(top[0], top[1]), max(top[2], top[3]));
+  const auto count = [&](uint32_t t) {
+    int c = __popcll(__ballot(top[0] >= t));
+    if (!quick) c += __popcll(__ballot(top[1] >= t)) + __popcll(__ballot(top[2] >= t)) + __popcll(__ballot(top[3] >= t));
+    return c;
+  };
   uint32_t bound = 0;
 #pragma unroll 1
-  for (int shift = 30; need <= 64 && shift >= 16; shift -= 2) {
+  for (int shift = 30; n > 64 && need < kFew && shift >= 16; shift -= 2) {
     const uint32_t t1 = bound | 1u << shift, t2 = bound | 2u << shift, t3 = bound | 3u << shift;
-    const int c1 = __popcll(__ballot(top >= t1)), c2 = __popcll(__ballot(top >= t2)), c3 = __popcll(__ballot(top >= t3));
+    const int c1 = count(t1), c2 = count(t2), c3 = count(t3);
     bound = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : bound;
     if ((c3 >= need ? c3 : c2 >= need ? c2 : c1) == need) break;
   }
@@ -342,7 +351,7 @@ __device__ __forceinline__ void choose_wave(const SelectParams& p, const uint32_
     for (int u = 0; u < 4; ++u) {
       const unsigned long long who = __ballot(k[u] >= bound);
       const int to = found + __popcll(who & below);
-      if (k[u] >= bound && to < kFew) team.key[to] = k[u], team.page[to] = i + 64 * u + lane;
+      if (k[u] >= bound && to < kFew) team.key[to] = k[u], team.page[to] = (uint16_t)(i + 64 * u + lane);
       found += __popcll(who);
     }
   }
@@ -624,7 +633,10 @@ struct SelectPlan {
 };
 
 constexpr long long kWaveRow = 2048;  // keys of a row that one wave chooses from
-constexpr size_t kSelectLds = 60 * 1024;
+// The same in decode batches, where the other waves have no row of their own: 200 rows of 8 heads and up to 256 pages
+// take 34 us by a wave and 38 by the workgroup, 64 rows of up to 1024 pages 25 and 24, 128 of them chosen 34 and 28.
+constexpr long long kWaveDecode = 512;
+constexpr size_t kSelectLds = 58 * 1024;
 constexpr size_t kSelectWorkspace = 256u << 20;  // the split form works through more rows in turns
 
 SelectPlan plan_select(const rpa_sparse_shape_t& s) {
@@ -665,7 +677,8 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
 template <int STEPS>
 int launch_select(const SelectPlan& plan, SelectParams p, hipStream_t stream) {
   if (!plan.split) {
-    const auto kernel = plan.stride <= kWaveRow ? select_kernel<STEPS, true> : select_kernel<STEPS, false>;
+    const bool wave = plan.stride <= (plan.tokens > 1 ? kWaveRow : kWaveDecode);
+    const auto kernel = wave ? select_kernel<STEPS, true> : select_kernel<STEPS, false>;
     kernel<<<(unsigned)(plan.tiles * p.Hkv), kSelectThreads, plan.lds, stream>>>(p);
     return launched("select_pages");
   }
