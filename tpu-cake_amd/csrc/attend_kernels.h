@@ -194,12 +194,9 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int byte = 64 * i + 16 * j;
-        if (FULL || byte < row_bytes) {
-          k[b][i] = load16(src + byte);
-          v[b][i] = load16(src + row_bytes + byte);
-        } else {
-          k[b][i] = v[b][i] = u32x4{0, 0, 0, 0};
-        }
+        const global_bytes from = FULL || byte < row_bytes ? src : zero;
+        k[b][i] = load16(from + byte);
+        v[b][i] = load16(from + row_bytes + byte);
       }
     }
   };
@@ -493,11 +490,10 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int byte = 16 * (member % 8 + 8 * i);
-        k[i] = v[i] = u32x4{0, 0, 0, 0};
-        if (byte < (FULL ? DP * kElem : row_bytes)) {
-          k[i] = load16(src + byte);
-          v[i] = load16(src + row_bytes + byte);
-        }
+        if (byte >= DP * kElem) break;
+        const global_bytes from = FULL || byte < row_bytes ? src : zero;
+        k[i] = load16(from + byte);
+        v[i] = load16(from + row_bytes + byte);
       }
     };
     const auto store = [&](int turn) {
