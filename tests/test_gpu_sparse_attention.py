@@ -128,6 +128,37 @@ def test_chunk_nan_that_other_tokens_see(cuda, kind):
     assert (np.abs(got - want) <= tol)[~bad].all()
 
 
+@pytest.mark.parametrize("kind,dim,group", [("bf16", 128, 4), ("bf16", 64, 8), ("bf16", 256, 16), ("bf16", 40, 3), ("fp8", 128, 1),
+                                            ("fp8", 256, 4), ("fp8", 80, 5)])
+@pytest.mark.parametrize("page,num_pages", [(64, 12), (256, 12), (24, 70), (1, 1100)])
+def test_short_chunks_split_their_lists(cuda, kind, dim, group, page, num_pages):
+    """Three and more workgroups a tile; parts without keys, a decode row and rows past the last token."""
+    b = Batch(dim + page, [1500, 700, 20, 3000], [20, 9, 2, 1], page, group * 2, 2, dim, pad=6)
+    _check(b, num_pages, kind, hole=0.2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_split_chunks_with_pages_listed_twice_and_nan(cuda, kind):
+    """Each part falls back by itself: twice in one token's list, and NaN that one token lists, in different parts."""
+    b = Batch(21, [4000, 900], [30, 8], 64, 8, 2, 128)
+    pool, scales, keys, values = b.pool(kind)
+    picked = b.lists(24, hole=0.0)
+    picked[4, 0, :3] = 2  # three times
+    picked[picked == 40] = -1
+    picked[9, 1, 0] = 40
+    held = pool.view(torch.uint8) if kind == "fp8" else pool
+    held[b.table[0, 40], 3, 2:] = 0x7F if kind == "fp8" else float("nan")  # kv head 1
+    pool = held.view(pool.dtype)
+    kw = dict(sm_scale=0.1, kv_scales=None if scales is None else torch.from_numpy(scales).cuda())
+    got = sparse.sparse_paged_attention(b.q.cuda(), pool.cuda(), i32(picked), *b.meta(), **kw).double().cpu().numpy()
+    bad = np.zeros((b.tokens, 8), bool)
+    bad[9, 4:] = True
+    assert (~np.isfinite(got).all(-1) == bad).all()
+    want = orc.sparse_attention(b.q.double().numpy(), keys, values, picked, b.lens, b.table, b.cu, b.n, 0.1)
+    tol = _tolerance(want, b.q, keys, values, 24 * 64, 0.1)
+    assert (np.abs(got - want) <= tol)[~bad].all()
+
+
 @pytest.mark.parametrize("soft_cap", [None, 20.0, -20.0])
 @pytest.mark.parametrize("sm_scale", [1.0, -0.3, 0.0])
 def test_scales_and_caps(cuda, soft_cap, sm_scale):

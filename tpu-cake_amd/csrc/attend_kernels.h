@@ -424,7 +424,15 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
   const int h = blockIdx.x % p.Hkv;
   const Tile tile = tile_of(p.cu, p.num_seqs, p.kv_lens, p.N, p.T, tp.tokens, blockIdx.x / p.Hkv);
   if (tile.count == 0) return;  // uniform
+  const int split = blockIdx.y;
+  const auto part_of = [&](int t) {  // of a token: as join_kernel reads it
+    return p.parts + (((size_t)(tile.first + t) * p.Hkv + h) * p.splits + split) * (32 + (size_t)p.G * p.D);
+  };
   if (tile.seq < 0 || tile.pos + tile.count <= 0) {
+    if (p.splits > 1) {
+      for (int i = tid; i < tile.count * p.G; i += kThreads) part_of(i / p.G)[2 * (i % p.G) + 1] = 0.f;
+      return;
+    }
     for (int i = tid; i < tile.count * p.G * p.D / 8; i += kThreads) {
       const int t = i / (p.G * p.D / 8), c = i % (p.G * p.D / 8);
       *(u32x4*)(p.out + ((size_t)(tile.first + t) * p.Hkv + h) * p.G * p.D + 8 * c) = u32x4{0, 0, 0, 0};
@@ -674,6 +682,14 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
   const auto write = [&](int only) {
     const float sum = swap_sum(l), g = sum == 0.f ? 0.f : p.v_scale / sum;
     if (!live || group || (only >= 0 && token != only)) return;
+    if (p.splits > 1) {
+      float* const part = part_of(token);
+      if (j == 0) part[2 * head] = m, part[2 * head + 1] = sum;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        if (FULL || 16 * d + 4 * j < p.D) *(f32x4*)(part + 32 + head * p.D + 16 * d + 4 * j) = o[d];
+      return;
+    }
     uint16_t* const row = p.out + (((size_t)(tile.first + token) * p.Hkv + h) * p.G + head) * p.D;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
@@ -715,9 +731,13 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
   for (int i = tid * each; i < min((tid + 1) * each, words); ++i) found.a += __popc(s_bits[i]);
   uint32_t before = scan_pairs<kThreads / 64>(found, total, s_scan).a;
   for (int i = tid * each; i < min((tid + 1) * each, words); ++i) s_before[i] = before, before += __popc(s_bits[i]);
+  const auto rank = [&](int page) { return (int)(s_before[page / 32] + __popc(s_bits[page / 32] & ((1u << (page % 32)) - 1))); };
+  // this workgroup's part of the union
+  const int each_split = ((int)total.a + p.splits - 1) / p.splits, from = split * each_split;
+  const int to = min(from + each_split, (int)total.a);
   reset();
-  for (int first = 0; first < (int)total.a; first += kTilePages) {
-    const int pages = min((int)total.a - first, kTilePages);
+  for (int first = from; first < to; first += kTilePages) {
+    const int pages = min(to - first, kTilePages);
     __syncthreads();
     for (int i = tid; i < pages; i += kThreads) s_entry[i].mask = 0;
     __syncthreads();
@@ -725,7 +745,7 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
       int t;
       const int page = listed(i, t);
       if (page < 0) continue;
-      const int at = (int)(s_before[page / 32] + __popc(s_bits[page / 32] & ((1u << (page % 32)) - 1))) - first;
+      const int at = rank(page) - first;
       if (at < 0 || at >= pages) continue;
       const int old = atomicOr(&s_entry[at].mask, 1 << t);
       if (old >> t & 1) s_flag[0] = 1;
@@ -755,7 +775,8 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
       for (int i = tid; i < pages; i += kThreads) {
         int own;
         const int page = listed(t * p.K + first + i, own);
-        if (page >= 0) entry(i, page, 1 << t);
+        const int at = page >= 0 ? rank(page) : -1;
+        if (at >= from && at < to) entry(i, page, 1 << t);
         else s_entry[i] = {0, 0, 0, 0};
       }
       __syncthreads();
@@ -787,6 +808,7 @@ struct AttendPlan {
 };
 
 constexpr long long kTileFill = 257;   // tiles from which two workgroups share a CU
+constexpr int kTileSplits = 8;
 constexpr long long kAttendFill = 256;  // workgroups below which lists are split: one a CU
 
 AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
@@ -802,6 +824,12 @@ AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
     r.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
     r.tokens = 64 / r.gp;
     r.grid = (((long long)s.num_tokens + r.tokens - 1) / r.tokens + s.max_num_seqs) * s.num_kv_heads;
+    // Few tiles: their unions are split, into parts of at least 256 listed keys, while all parts run at once.  20, 60
+    // and 120 tokens of 32 pages of 64 keys (8 kv heads) take 28, 39 and 40 us, unsplit 59, 60 and 59.
+    long long splits = kAttendFill / r.grid, most = (long long)s.num_pages * s.page_size / 256;
+    splits = splits < most ? splits : most;
+    r.splits = splits < 2 ? 1 : splits < kTileSplits ? (int)splits : kTileSplits;
+    if (r.splits > 1) r.bytes = (size_t)r.rows * r.splits * (32 + (size_t)G * s.head_dim) * 4;
     return r;
   }
   // a workgroup's part: at least 128 keys, one unit a wave, and at most kMaxBlocks blocks
@@ -824,14 +852,14 @@ void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t st
     const auto launch = [&](auto kernel, int groups) {
       const size_t lds = groups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
                          (size_t)((p.PPS + 31) / 32) * 8;
-      kernel<<<(unsigned)plan.grid, 256 * groups, lds, stream>>>(tp);
+      kernel<<<dim3((unsigned)plan.grid, plan.splits), 256 * groups, lds, stream>>>(tp);
     };
     if constexpr (DP == 256) {
       launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
     } else if constexpr (FP8) {
       launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
     } else {
-      if (plan.grid < kTileFill) launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
+      if (plan.grid * plan.splits < kTileFill) launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
       else launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
     }
     return;

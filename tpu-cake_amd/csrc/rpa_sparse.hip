@@ -186,7 +186,7 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
     else launch_attend<128, false, false>(plan, p, s);
   }
   if ((rc = launched("sparse_paged_attention"))) return rc;
-  if (!plan.chunk && plan.splits > 1) {
+  if (plan.splits > 1) {
     join_kernel<<<(unsigned)plan.rows, 256, 0, s>>>(p);
     return launched("sparse_paged_attention (join)");
   }
