@@ -13,6 +13,9 @@
 // Rows choose apart, so rows are what workgroups share nothing of: one row (its up to 16 heads) a
 // workgroup, its keys over four waves, each with its own (m, l, O), joined at the end through LDS.  With
 // few rows the list is split over workgroups as well, and a second launch joins their parts.
+//
+// Measured (8 kv heads of 128, 2048 keys a row): 64 decode rows of 64 heads, 539 MB: 92 us, 5.9 TB/s; 2 rows of an
+// fp8 pool, 8.4 MB: 7.1 us and 3.9 for the join, launches and latency.
 #pragma once
 
 #include "select_kernels.h"

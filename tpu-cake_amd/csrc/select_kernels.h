@@ -14,6 +14,11 @@
 // The index is read once for a row: (2 D + 1) bytes a page and head, 1/32 of a 16-key bf16 page of
 // 128-dim heads; it bounds long contexts.  Short ones are bound by latency (metadata, page ids, index
 // rows, then the counting steps: four dependent round trips).
+//
+// Measured (8 kv heads of 128): 64 decode rows over 4 096 to 65 536 keys in pages of 64, 49 MB of index: 23 us,
+// 2.1 TB/s; 2 rows over half a million keys in pages of 16, 127 MB: scored in 31 us, 4.1 TB/s, chosen in 11.5;
+// a chunk of 1000 tokens over 32 768 keys in pages of 64, 15 MB: 32 us, of which rounding queries, scoring and
+// choosing take a third each.
 #pragma once
 
 #include "page_index.h"
