@@ -267,7 +267,7 @@ __device__ __forceinline__ void widen_bounds(const AppendParams& p, int t0, int 
 // One launch: the first `wide` workgroups (with an index) widen bounds, the others copy rows beside them.  Decode
 // batches are bound by latency: a token a workgroup, or a team.  Long batches are bound by the turnover of
 // workgroups and by runs that start late: eight tokens, and four rounds of teams first.  64 decode tokens of 8 heads
-// of 128 take 5.6 us (launch and two round trips); 7 900 prompt tokens into an fp8 pool, 55 MB, 24 us or 2.3 TB/s.
+// of 128 take 5.6 us (launch and two round trips); 9 000 prompt tokens into an fp8 pool, 55 MB, 24 us or 2.3 TB/s.
 template <bool FP8, int TOKENS>
 __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
   const int block = blockIdx.x, teams = __umulhi(64u, p.chunk_magic);
