@@ -1,6 +1,8 @@
 """The sparse entry points together, as a serving loop runs them: pages are assigned, keys appended,
 pages chosen and attended to, and finished requests give their pages back."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -163,3 +165,84 @@ def test_two_graphs_replay_side_by_side(cuda):
         for _, got, want, _, _ in calls:
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
             got[1].zero_()
+
+
+def test_captured_chunks_with_other_lengths(cuda):
+    """A chunk's choice and attention, lists split over workgroups: captured once, replayed with other lengths and tokens."""
+    n, tokens, width = 3, 40, 64
+    rng = np.random.default_rng(3)
+    pool = torch.randn((n * width, 64, 2 * HKV, DIM), device="cuda").to(torch.bfloat16)
+    index = sparse.PageIndex(torch.randint(-127, 128, (n * width, HKV, 2, DIM), dtype=torch.int8, device="cuda"),
+                             torch.randint(-6, -3, (n * width, HKV), dtype=torch.int8, device="cuda"))
+    q = torch.empty((tokens, HQ, DIM), dtype=torch.bfloat16, device="cuda")
+    lens, table, cu, num = i32([0] * n), i32(rng.permutation(n * width).reshape(n, width)), i32([0] * (n + 1)), i32([n])
+
+    def fill(kv_lens, q_lens):
+        lens.copy_(i32(kv_lens))
+        cu.copy_(i32(np.concatenate([[0], np.cumsum(q_lens)])))
+        q.copy_(torch.from_numpy(rng.standard_normal(q.shape, np.float32)))
+
+    def step():
+        picked = sparse.select_pages(q, index, lens, table, cu, num, page_size=64, num_pages=20)
+        return picked, sparse.sparse_paged_attention(q, pool, picked, lens, table, cu, num, sm_scale=SCALE)
+
+    fill([4000, 100, 9], [30, 1, 1])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step()
+    for kv_lens, q_lens in (([4000, 100, 9], [30, 1, 1]), ([64 * 64, 64, 1], [1, 38, 1]), ([0, 0, 0], [0, 0, 0]), ([700, 3000, 2], [0, 40, 0])):
+        fill(kv_lens, q_lens)
+        want = [x.clone() for x in step()]
+        for _ in range(2):
+            got[1].fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            torch.randn(4096, device="cuda").sum().item()
+
+
+def test_threads_on_streams_of_their_own(cuda):
+    """Two threads at once, split forms, each on its stream: the results of one after the other."""
+    rng = np.random.default_rng(4)
+    jobs = []
+    for rows in (2, 30):
+        pages = 6000
+        q = torch.randn((rows, HQ, DIM), device="cuda").to(torch.bfloat16)
+        pool = torch.randn((pages, 4, 2 * HKV, DIM), device="cuda").to(torch.bfloat16)
+        index = sparse.PageIndex(torch.randint(-127, 128, (pages, HKV, 2, DIM), dtype=torch.int8, device="cuda"),
+                                 torch.randint(-6, -3, (pages, HKV), dtype=torch.int8, device="cuda"))
+        cu = [0, 1, rows]
+        jobs.append((q, pool, index, (i32([11000, 12000]), i32(rng.permutation(pages).reshape(2, -1)), i32(cu), i32([2]))))
+
+    def step(q, pool, index, batch):
+        picked = sparse.select_pages(q, index, *batch, page_size=4, num_pages=300)
+        return picked, sparse.sparse_paged_attention(q, pool, picked, *batch, sm_scale=SCALE)
+
+    want = [step(*job) for job in jobs]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(step(*jobs[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        for x in got[i]:
+            assert torch.equal(x[0], want[i][0]) and torch.equal(x[1], want[i][1])
