@@ -166,7 +166,7 @@ __device__ __forceinline__ void widen_runs(const AppendParams& p, int t, int pag
     for (int i = 0; i < 8; ++i) hi[i] = -__builtin_inff(), lo[i] = __builtin_inff();
     if (from < step) {
       const uint16_t* src = p.k + (t + from) * p.k_token + h * p.k_head + 8 * c;
-#pragma unroll 4
+#pragma unroll 2  // four rows in flight take 17 registers more, and 26 us where two take 25
       for (int r = from; r < run; r += step, src += step * p.k_token) {
         float x[8];
         unpack8(*(const u32x4*)src, x);
@@ -267,7 +267,7 @@ __device__ __forceinline__ void widen_bounds(const AppendParams& p, int t0, int 
 // One launch: the first `wide` workgroups (with an index) widen bounds, the others copy rows beside them.  Decode
 // batches are bound by latency: a token a workgroup, or a team.  Long batches are bound by the turnover of
 // workgroups and by runs that start late: eight tokens, and four rounds of teams first.  64 decode tokens of 8 heads
-// of 128 take 5.6 us (launch and two round trips); 9 000 prompt tokens into an fp8 pool, 55 MB, 24 us or 2.3 TB/s.
+// of 128 take 5.6 us (launch and two round trips); 9 000 prompt tokens into an fp8 pool, 55 MB, 23 us or 2.4 TB/s.
 template <bool FP8, int TOKENS>
 __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
   const int block = blockIdx.x, teams = __umulhi(64u, p.chunk_magic);
