@@ -80,7 +80,7 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
  * an fp8 pool are code * K scale. */
 typedef struct rpa_append_shape {
   int32_t num_tokens;  /* below 2^30 */
-  int32_t num_kv_heads;
+  int32_t num_kv_heads; /* at most 65535 */
   int32_t head_dim;    /* as rpa_shape_t: 256, or a multiple of 8 in [32, 128] (fp8: of 16 in [64, 128]) */
   int32_t total_pages;
   int32_t page_size;

@@ -104,6 +104,10 @@ def test_counts_that_pass_32_bits_are_refused(lib):
     wide = ctypes.byref(_sparse(max_num_seqs=1 << 27))
     assert lib.rpa_select_pages(wide, 1, 1, *FAKE[:9], 1 << 40, None) == -1 and b"max_num_seqs" in lib.rpa_sparse_last_error()
     assert lib.rpa_sparse_workspace_size(wide) == 0
+    heads = ctypes.byref(_append(num_kv_heads=65536))
+    assert lib.rpa_append_kv(heads, *FAKE[:5], 1.0, 1.0, *FAKE[5:7], None) == -2 and b"65535 kv heads" in lib.rpa_sparse_last_error()
+    heads = ctypes.byref(_sparse(num_kv_heads=65536, num_q_heads=65536, num_tokens=1))
+    assert lib.rpa_select_pages(heads, 1, 1, *FAKE[:9], 1 << 40, None) == -2 and b"65535 kv heads" in lib.rpa_sparse_last_error()
 
 
 def _sparse(**kw):

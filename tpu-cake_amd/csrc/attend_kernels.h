@@ -811,7 +811,7 @@ struct AttendPlan {
 };
 
 constexpr long long kTileFill = 257;   // tiles from which two workgroups share a CU
-constexpr int kTileSplits = 8;
+constexpr int kTileSplits = 8;  // 200 tokens of one kv head take 21 us, 26 with 4, 21 with 16
 constexpr long long kAttendFill = 256;  // workgroups below which lists are split: one a CU
 
 AttendPlan plan_attend(const rpa_sparse_shape_t& s) {

@@ -285,6 +285,7 @@ __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
 
 int check_heads(int hkv, int d, int kv_dtype) {
   if (hkv <= 0) return fail(RPA_E_INVALID, "non-positive dimension in shape");
+  if (hkv > 65535) return fail(RPA_E_UNSUPPORTED, "more than 65535 kv heads");  // a launch's y dimension, 32-bit rows
   if (kv_dtype != RPA_KV_BF16 && kv_dtype != RPA_KV_FP8_E4M3)
     return fail(RPA_E_INVALID, "kv_dtype must be RPA_KV_BF16 or RPA_KV_FP8_E4M3");
   const bool fp8 = kv_dtype == RPA_KV_FP8_E4M3;
