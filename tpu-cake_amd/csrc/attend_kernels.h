@@ -5,9 +5,10 @@
 // On v_mfma_f32_16x16x32_bf16, 32 keys at a time: S = K Q^T (A: 16 keys x 32 dims, B: the group's heads as
 // 16 columns), O^T += V^T P^T (A: 16 dims x 32 keys).  A lane's scores are the keys its P operand needs,
 // so P moves between no lanes; V passes through LDS as key rows and comes back transposed
-// (ds_read_b64_tr_b16).  P is split into two bf16 parts, hi = bf16(p) and bf16(p - hi), each with its own
-// MFMA: nothing is rounded to 8 bits, and the second product hides behind the loads.  fp8 codes are exact
-// in bf16; K scales multiply the scores and V scales P, both in fp32.
+// (ds_read_b64_tr_b16).  P is split into three bf16 parts, each the nearest to what the earlier ones leave, with an
+// MFMA each: 24 bits, all that p has, where values cancel too.  Two parts (16 bits) lose what a token's values
+// have in common; the third product hides behind a row's loads and costs 8% of a chunk's tile.  fp8 codes are
+// exact in bf16; K scales multiply the scores and V scales P, both in fp32.
 //
 // Every listed key of a row is read once, 2 D elem bytes at 2 Hkv D elem apart: HBM bounds decode rows.
 // Rows choose apart, so rows are what workgroups share nothing of: one row (its up to 16 heads) a
@@ -81,10 +82,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 
-// Two values as two bf16 each: the nearest ones, and what is left.
-__device__ __forceinline__ u32x2 split_bf16(float a, float b) {
-  const uint32_t hi = pack_bf16(a, b);
-  return u32x2{hi, pack_bf16(a - bf16_lo(hi), b - bf16_hi(hi))};
+// Two values as three bf16 each: the nearest ones, and those nearest to what is left.
+struct Parts {
+  uint32_t of[3];
+};
+__device__ __forceinline__ Parts split_bf16(float a, float b) {
+  Parts p;
+  p.of[0] = pack_bf16(a, b);
+  a -= bf16_lo(p.of[0]), b -= bf16_hi(p.of[0]);
+  p.of[1] = pack_bf16(a, b);
+  p.of[2] = pack_bf16(a - bf16_lo(p.of[1]), b - bf16_hi(p.of[1]));
+  return p;
 }
 
 // A product that rounds by itself: joined with the subtraction of the maximum into one operation, the maximum's own
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) o[d] *= f;
     }
-    u32x4 hi, lo;
+    u32x4 parts[3];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       float e[4];
@@ -281,9 +289,9 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
         l += e[r];
         if (FP8) e[r] *= vs[b][r];
       }
-      const u32x2 first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
-      hi[2 * b] = first[0], hi[2 * b + 1] = second[0];
-      lo[2 * b] = first[1], lo[2 * b + 1] = second[1];
+      const Parts first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) parts[i][2 * b] = first.of[i], parts[i][2 * b + 1] = second.of[i];
     }
     typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
     const uint8_t* vt = tile_v + (4 * j + n / 4) * kRow + 8 * (n % 4);
@@ -292,8 +300,9 @@ __global__ __launch_bounds__(64 * kAttendWaves) void attend_kernel(AttendParams 
       const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
       const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kRow + 32 * d));
       const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
-      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), o[d], 0, 0, 0);
-      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, parts[i]), o[d], 0, 0, 0);
     }
   }
 
@@ -619,7 +628,7 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
 #pragma unroll
           for (int d = 0; d < DP / 16; ++d) o[d] *= f;
         }
-        u32x4 hi, lo;
+        u32x4 parts[3];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           float e[4];
@@ -629,9 +638,9 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
             l += e[r];
             if (FP8) e[r] *= vs[b][r];
           }
-          const u32x2 first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
-          hi[2 * b] = first[0], hi[2 * b + 1] = second[0];
-          lo[2 * b] = first[1], lo[2 * b + 1] = second[1];
+          const Parts first = split_bf16(e[0], e[1]), second = split_bf16(e[2], e[3]);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) parts[i][2 * b] = first.of[i], parts[i][2 * b + 1] = second.of[i];
         }
         typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
         const uint8_t* const vt = kt + 32 * kKRow + (4 * j + n / 4) * kVRow + 8 * (n % 4);
@@ -640,8 +649,9 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
           const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
           const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kVRow + 32 * d));
           const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, hi), o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, parts[i]), o[d], 0, 0, 0);
         }
       }
       if (unit + kGroups < units) store(turn + 1);

@@ -298,9 +298,8 @@ def sparse_paged_attention(
     twice counts twice).
 
     Returns bf16 [T, Hq, D] (or fills ``out``); rows without a key or without a score above -infinity,
-    and rows at or past ``cu_q_lens[num_seqs]``, are zero.  Scores, softmax and sums are fp32 and probabilities keep 16 bits
-    for the product with V; scaled keys and values are not rounded (the dense operator rounds them to
-    bf16).
+    and rows at or past ``cu_q_lens[num_seqs]``, are zero.  Scores, softmax, probabilities and sums are fp32; scaled keys
+    and values are not rounded (the dense operator rounds them, and its probabilities, to bf16).
     """
     sig = (q.shape, q.dtype, q.get_device(), q.stride(),
            kv_pages.shape, kv_pages.dtype, kv_pages.get_device(), kv_pages.is_contiguous(), selected_pages.shape,
