@@ -159,6 +159,45 @@ def test_split_chunks_with_pages_listed_twice_and_nan(cuda, kind):
     assert (np.abs(got - want) <= tol)[~bad].all()
 
 
+@pytest.mark.parametrize("part,value", [(1, float("nan")), (1, float("inf")), (0, float("nan"))])
+@pytest.mark.parametrize("page,lens,num_pages", [(7, (90, 120), 20), (16, (200, 300), 21), (24, (200, 300), 14), (16, (1500, 1300), 70)])
+@pytest.mark.parametrize("repeated", [False, True])
+def test_chunk_scales_that_other_tokens_list(cuda, part, value, page, lens, num_pages, repeated):
+    """One token lists a page whose scale is not finite, at an entry where the others list nothing, past the
+    union's size too: only its row shows it.  The longest lists are split."""
+    b = Batch(page + num_pages, lens, (20, 40), page, 8, 2, 128)
+    pool, scales, keys, values = b.pool("fp8")
+    picked = b.lists(num_pages, hole=0.3)
+    entry = num_pages - 1
+    picked[:, :, entry] = -1
+    picked[:20][picked[:20] == 1] = -1
+    picked[:, :, 2] = -1
+    picked[3, 0, entry] = 1  # page 1 of the first sequence: token 3 alone lists it, for kv head 0
+    picked[18, 1, 2] = 1     # and token 18, for kv head 1
+    if repeated:
+        picked[5, 0, :2], picked[19, 1, :2] = 2, 0  # twice
+    dirty = scales.copy()
+    dirty[b.table[0, 1], :, part] = value
+    kw = dict(sm_scale=0.1, kv_scales=torch.from_numpy(dirty).cuda())
+    got = sparse.sparse_paged_attention(b.q.cuda(), pool.cuda(), i32(picked), *b.meta(), **kw).double().cpu().numpy()
+    bad = np.zeros((b.tokens, 8), bool)
+    bad[3, :4], bad[18, 4:] = True, True
+    assert (~np.isfinite(got).all(-1) == bad).all()
+    want = orc.sparse_attention(b.q.double().numpy(), keys, values, picked, b.lens, b.table, b.cu, b.n, 0.1)
+    tol = _tolerance(want, b.q, keys, values, num_pages * page, 0.1)
+    assert (np.abs(got - want) <= tol)[~bad].all()
+
+
+@pytest.mark.parametrize("page", [7, 16, 24])
+@pytest.mark.parametrize("num_pages", [9, 80])
+def test_fp8_chunk_pages_listed_twice_beside_holes(cuda, page, num_pages):
+    b = Batch(page, [1400, 1000], [20, 40], page, 8, 2, 64)
+    picked = b.lists(num_pages, hole=0.4)
+    for t in range(0, 60, 3):
+        picked[t, t % 2, [1, 6, 8]] = 2, -1, 2
+    _check(b, num_pages, "fp8", picked=picked)
+
+
 @pytest.mark.parametrize("soft_cap", [None, 20.0, -20.0])
 @pytest.mark.parametrize("sm_scale", [1.0, -0.3, 0.0])
 def test_scales_and_caps(cuda, soft_cap, sm_scale):

@@ -789,8 +789,12 @@ __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGrou
         int own;
         const int page = listed(t * p.K + first + i, own);
         const int at = page >= 0 ? rank(page) : -1;
-        if (at >= from && at < to) entry(i, page, 1 << t);
-        else s_entry[i] = {0, 0, 0, 0};
+        if (at >= from && at < to) {
+          entry(i, page, 1 << t);
+        } else {  // 32 keys may hold some of this entry's: their weights of 0 meet its scales
+          s_entry[i] = {0, 0, 0, 0};
+          if (FP8) s_scale[2 * i] = s_scale[2 * i + 1] = 1.f;
+        }
       }
       __syncthreads();
       attend(pages, tile.pos + t);
