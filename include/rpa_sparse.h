@@ -9,6 +9,8 @@
  *
  * Out-of-range metadata (page ids, slots, lengths) is never dereferenced; the kernels set a bit of
  * the device's error word for it (rpa_sparse_read_error_word).
+ * Offsets (cu_q_lens) that decrease or lie outside [0, num_tokens] set none: the calls stay within
+ * their tensors, and which rows get a result is not defined.
  */
 #ifndef RPA_SPARSE_H_
 #define RPA_SPARSE_H_

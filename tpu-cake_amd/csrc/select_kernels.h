@@ -50,7 +50,7 @@ struct Place {
 };
 
 // The sequence of token t and its position there: the number of sequences that end at or before t (cu
-// is non-decreasing; anything else stays in range).  One round trip to memory where there are up to 64
+// is non-decreasing; anything else stays in range, and a negative length counts as 0).  One round trip to memory where there are up to 64
 // sequences, a lane each, or where token t is all of sequence t (a decode batch): all of that is loaded
 // at once.  Otherwise a 64-ary search, two more for up to 4096 sequences and the ends' own.
 __device__ __forceinline__ Place place_of(const int32_t* cu, const int32_t* num_seqs, const int32_t* kv_lens, int N, int t) {
@@ -61,9 +61,9 @@ __device__ __forceinline__ Place place_of(const int32_t* cu, const int32_t* num_
   if (N <= 64) {
     const int lo = __popcll(__ballot(lane < n && end0 <= t));
     const int begin = __shfl(begin0, lo & 63), end = __shfl(end0, lo & 63), len = __shfl(len0, lo & 63);
-    return lo >= n || t < begin || t >= end ? Place{-1, -1} : Place{lo, len - (end - t)};
+    return lo >= n || t < begin || t >= end ? Place{-1, -1} : Place{lo, max(len, 0) - (end - t)};
   }
-  if (t < n && begin0 == t && end0 == t + 1) return {t, len0 - 1};  // uniform: the same words in all lanes
+  if (t < n && begin0 == t && end0 == t + 1) return {t, max(len0, 0) - 1};  // uniform: the same words in all lanes
   int lo = 0, len = n;  // the answer is in [lo, lo + len]
   while (len > 0) {
     const int step = (len + 63) / 64;
@@ -75,12 +75,13 @@ __device__ __forceinline__ Place place_of(const int32_t* cu, const int32_t* num_
   }
   if (lo >= n) return {-1, -1};
   const int begin = cu[lo], end = cu[lo + 1];
-  return t < begin || t >= end ? Place{-1, -1} : Place{lo, kv_lens[lo] - (end - t)};
+  return t < begin || t >= end ? Place{-1, -1} : Place{lo, max(kv_lens[lo], 0) - (end - t)};
 }
 
 // The index-th tile of `size` (a power of two) consecutive tokens of one sequence: sequences in order,
 // ceil(q_len / size) tiles each, then the tokens past the last (seq -1).  There are at most
-// ceil(T / size) + N tiles.  count: its tokens, pos: its first token's position.
+// ceil(T / size) + N tiles.  count: its tokens, pos: its first token's position.  Offsets are taken into [0, T]
+// and sums of tiles saturate, so whatever cu holds, first .. first + count are tokens of the call.
 struct Tile {
   int seq, first, count, pos;
 };
@@ -94,28 +95,29 @@ __device__ __forceinline__ Tile tile_of(const int32_t* cu, const int32_t* num_se
   const int lane = threadIdx.x % 64, shift = __builtin_ctz(size);
   int begin = cu[min(lane, N - 1)], end = cu[min(lane, N - 1) + 1], len = kv_lens[min(lane, N - 1)];
   const int n = min(max(*num_seqs, 0), N);
-  int before = 0;  // tiles of the sequences before this window's
+  const auto token = [T](int c) { return min(max(c, 0), T); };
+  uint32_t before = 0;  // tiles of the sequences before this window's
   for (int base = 0; base < n; base += 64) {
-    const int s = base + lane;
-    const int own = s < n && end > begin ? (end - begin + size - 1) >> shift : 0;
-    int upto = own;
+    const int s = base + lane, from = token(begin), to = token(end);
+    const uint32_t own = s < n && to > from ? (uint32_t)(to - from + size - 1) >> shift : 0u;
+    uint32_t upto = own;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int o = __shfl_up(upto, d);
-      upto += lane >= d ? o : 0;
+      const uint32_t o = __shfl_up(upto, d);
+      upto = sat_add(upto, lane >= d ? o : 0u);
     }
-    const int here = __popcll(__ballot(before + upto <= index));  // sequences of the window that lie before
+    const int here = __popcll(__ballot(before + upto <= (uint32_t)index));  // sequences of the window that lie before
     if (here < 64) {
-      const int b = __shfl(begin, here), e = __shfl(end, here), l = __shfl(len, here);
-      const int first = b + ((index - before - __shfl(upto - own, here)) << shift);
-      return {base + here, first, first < 0 ? 0 : max(min(min(size, e - first), T - first), 0), l - (e - first)};
+      if (here) before += __shfl(upto, here - 1);
+      const int e = __shfl(end, here), first = __shfl(from, here) + (int)(((uint32_t)index - before) << shift);
+      return {base + here, first, min(size, __shfl(to, here) - first), max(__shfl(len, here), 0) - (e - first)};
     }
     before += __shfl(upto, 63);
     const int next = min(s + 64, N - 1);
     begin = cu[next], end = cu[next + 1], len = kv_lens[next];
   }
-  const int first = (n ? max(cu[n], 0) : 0) + ((index - before) << shift);
-  return {-1, first, max(min(size, T - first), 0), -1};
+  const long long first = (n ? token(cu[n]) : 0) + ((long long)((uint32_t)index - before) << shift);
+  return {-1, (int)min(first, (long long)T), (int)max(min((long long)size, T - first), 0ll), -1};
 }
 
 // The newest page of a token at `pos` (-1: it sees no key).
