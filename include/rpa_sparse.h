@@ -45,8 +45,8 @@ int rpa_sparse_read_error_word(int32_t* host_word, int32_t clear, void* stream);
  * The pool's free pages are a stack: free_pages[0 .. free_count).  A request holds the first
  * ceil(len / page_size) entries of its page_table row. */
 typedef struct rpa_paging_shape {
-  int32_t num_requests;  /* N = page_table.shape[0] */
-  int32_t pages_per_seq; /* PPS = page_table.shape[1] */
+  int32_t num_requests;  /* N = page_table.shape[0], at most 2^31 - 2^16 - 1 */
+  int32_t pages_per_seq; /* PPS = page_table.shape[1], at most 2^31 - 2^16 - 1 */
   int32_t page_size;     /* S */
   int32_t free_capacity; /* F = free_pages.shape[0], below 2^30 */
   int32_t max_tokens;    /* rows of slot_mapping and positions, below 2^30 */
@@ -108,7 +108,8 @@ int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void*
  * kv_lens[i] - (cu_q_lens[i + 1] - t) and sees the keys up to there. */
 typedef struct rpa_sparse_shape {
   int32_t num_tokens, num_q_heads, num_kv_heads, head_dim;
-  int32_t total_pages, page_size, max_num_seqs, pages_per_seq;
+  int32_t total_pages, page_size, max_num_seqs;
+  int32_t pages_per_seq; /* at most 2^31 - 2^16 - 1, as num_pages */
   int32_t kv_dtype;  /* of the pool; ignored by rpa_select_pages apart from its head dims */
   int32_t num_pages; /* entries of a row of the list */
   int64_t q_token_stride, q_head_stride; /* of q [num_tokens, num_q_heads, head_dim], in values */

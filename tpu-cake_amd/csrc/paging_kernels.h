@@ -222,6 +222,8 @@ int check_paging(const rpa_paging_shape_t* s) {
     return fail(RPA_E_INVALID, "non-positive dimension in shape");
   if ((long long)s->pages_per_seq * s->page_size > 0x7fffffffll)
     return fail(RPA_E_INVALID, "pages_per_seq * page_size overflows int32");
+  if (s->num_requests > kMostIndex || s->pages_per_seq > kMostIndex)
+    return fail(RPA_E_UNSUPPORTED, "num_requests and pages_per_seq must be at most 2^31 - 2^16 - 1");
   if (s->free_capacity >= (int)kSumCap || s->max_tokens >= (int)kSumCap || s->max_tokens < 0)
     return fail(RPA_E_INVALID, "free_capacity and max_tokens must be below 2^30");
   return RPA_OK;

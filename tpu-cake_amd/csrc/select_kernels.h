@@ -624,6 +624,8 @@ int check_sparse(const rpa_sparse_shape_t* s) {
     return fail(RPA_E_INVALID, "num_tokens * num_kv_heads overflows int32");
   if (s->num_tokens + 16ll * s->max_num_seqs > 0x7fffffffll)
     return fail(RPA_E_INVALID, "num_tokens + 16 * max_num_seqs overflows int32");
+  if (s->pages_per_seq > kMostIndex || s->num_pages > kMostIndex)
+    return fail(RPA_E_UNSUPPORTED, "pages_per_seq and num_pages must be at most 2^31 - 2^16 - 1");
   if (s->num_q_heads / s->num_kv_heads > 256) return fail(RPA_E_UNSUPPORTED, "more than 256 query heads per kv head");
   return RPA_OK;
 }

@@ -98,6 +98,9 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 // ---- host side ----
+// The most entries of what a kernel's loop walks in 32 bits: an index steps by less than 2^16.
+constexpr int kMostIndex = 0x7fffffff - 0x10000;
+
 // The message of the thread's last failure: a fixed buffer, so that reporting one cannot throw.
 thread_local char g_last_error[256];
 
