@@ -50,6 +50,29 @@ def test_lists_and_tables_that_an_index_would_pass(lib, field):
     assert lib.rpa_select_workspace_size(ctypes.byref(_sparse(pages_per_seq=MOST))) > 0
 
 
+def test_launches_of_2_to_the_32_threads(lib):
+    """HIP takes fewer along a dimension; calls that would need more say so."""
+    rows = _sparse(num_tokens=1 << 22, max_num_seqs=1 << 22, num_kv_heads=1, num_q_heads=1)  # a workgroup a row
+    assert _select(lib, rows) == -2 and b"one launch" in lib.rpa_sparse_last_error()
+    rows = _sparse(num_tokens=1 << 24, max_num_seqs=1 << 24, num_kv_heads=1, num_q_heads=1)
+    assert _attend(lib, rows) == -2 and b"one launch" in lib.rpa_sparse_last_error()
+    tiles = _sparse(num_tokens=1 << 26, num_kv_heads=2, num_q_heads=2)
+    assert _select(lib, tiles) == -2 and b"one launch" in lib.rpa_sparse_last_error()
+    assert _attend(lib, tiles) == -2 and b"one launch" in lib.rpa_sparse_last_error()
+    tokens = _sparse_lib.RpaAppendShape((1 << 30) - 1, 8, 128, 64, 16, 0, 1024, 128, 1024, 128)
+    assert lib.rpa_append_kv(ctypes.byref(tokens), *FAKE[:4], None, 1.0, 1.0, *FAKE[5:7], None) == -2
+    assert b"one launch" in lib.rpa_sparse_last_error()
+    assert lib.rpa_release_pages(ctypes.byref(_paging(num_requests=1 << 28)), *FAKE[:7], None) == -2
+    assert b"one launch" in lib.rpa_sparse_last_error()
+
+
+def test_split_choices_stay_below_them_in_turns(lib):
+    """Tiny rows whose queries pass the LDS, so that the workspace alone would take 2^22 of them at once."""
+    shape = _sparse(num_tokens=20000, max_num_seqs=20000, num_kv_heads=1024, num_q_heads=1024 * 256, head_dim=256)
+    rows = lib.rpa_select_workspace_size(ctypes.byref(shape)) // 64  # 16 keys of 4 bytes each
+    assert 0 < rows * 1024 < 2**32 and rows % 1024 == 0
+
+
 @pytest.mark.parametrize("field", ["num_requests", "pages_per_seq"])
 def test_requests_that_an_index_would_pass(lib, field):
     for count in (MOST + 1, 2**31 - 1):

@@ -818,6 +818,7 @@ int check_attend(const rpa_sparse_shape_t* s) {
 struct AttendPlan {
   bool chunk;           // tiles of tokens
   int tokens, gp;       // of a tile
+  int groups;           // of four waves each
   long long grid;       // its workgroups
   int tiles, width, subs, per, splits;
   long long blocks, rows;
@@ -847,6 +848,7 @@ AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
     splits = splits < most ? splits : most;
     r.splits = splits < 2 ? 1 : splits < kTileSplits ? (int)splits : kTileSplits;
     if (r.splits > 1) r.bytes = (size_t)r.rows * r.splits * (32 + (size_t)G * s.head_dim) * 4;
+    r.groups = s.head_dim > 128 || (s.kv_dtype == RPA_KV_BF16 && r.grid * r.splits >= kTileFill) ? 2 : 3;
     return r;
   }
   // a workgroup's part: at least 128 keys, one unit a wave, and at most kMaxBlocks blocks
@@ -866,18 +868,18 @@ void launch_attend(const AttendPlan& plan, const AttendParams& p, hipStream_t st
   if (plan.chunk) {
     const TileParams tp = {p, plan.tokens, plan.gp, plan.gp == 4 ? 2 : plan.gp == 8 ? 3 : 4,
                            (uint32_t)(0x100000000ull / plan.subs + 1)};
-    const auto launch = [&](auto kernel, int groups) {
-      const size_t lds = groups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
+    const auto launch = [&](auto kernel) {
+      const size_t lds = plan.groups * 2 * 32 * (size_t)(DP * 4 + 48) + kTilePages * (sizeof(TileEntry) + (FP8 ? 8 : 0)) +
                          (size_t)((p.PPS + 31) / 32) * 8;
-      kernel<<<dim3((unsigned)plan.grid, plan.splits), 256 * groups, lds, stream>>>(tp);
+      kernel<<<dim3((unsigned)plan.grid, plan.splits), 256 * plan.groups, lds, stream>>>(tp);
     };
     if constexpr (DP == 256) {
-      launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
+      launch(attend_tile_kernel<DP, FULL, FP8, 2>);
     } else if constexpr (FP8) {
-      launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
+      launch(attend_tile_kernel<DP, FULL, FP8, 3>);
     } else {
-      if (plan.grid * plan.splits < kTileFill) launch(attend_tile_kernel<DP, FULL, FP8, 3>, 3);
-      else launch(attend_tile_kernel<DP, FULL, FP8, 2>, 2);
+      if (plan.groups == 3) launch(attend_tile_kernel<DP, FULL, FP8, 3>);
+      else launch(attend_tile_kernel<DP, FULL, FP8, 2>);
     }
     return;
   }

@@ -69,6 +69,7 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
   const ReleaseParams p = {cached_lens, finished, page_table, free_pages, free_count, cached_lens_out, free_count_out,
                            shape->num_requests, shape->pages_per_seq, shape->page_size, shape->free_capacity};
   const int grid = (shape->num_requests - 1) / kReleaseSlice + 1;
+  if (const int many = check_launch(grid, kReleaseThreads)) return many;
   release_kernel<<<grid, kReleaseThreads, 0, (hipStream_t)stream>>>(p);
   return launched("release_pages");
 }
@@ -96,10 +97,12 @@ int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void*
                           shape->num_kv_heads, shape->head_dim, shape->page_size, wide,
                           (uint32_t)(0x100000000ull / chunks + 1), (uint32_t)(0x100000000ull / (2 * chunks) + 1)};
   const int threads = 64 * (shape->num_kv_heads < 8 ? shape->num_kv_heads : 8);
+  const int grid = wide + (shape->num_tokens - 1) / tokens + 1;
+  if ((rc = check_launch(grid, threads))) return rc;
   const auto kernel = shape->kv_dtype == RPA_KV_FP8_E4M3
                           ? (tokens > 1 ? append_kernel<true, kAppendTokens> : append_kernel<true, 1>)
                           : (tokens > 1 ? append_kernel<false, kAppendTokens> : append_kernel<false, 1>);
-  kernel<<<wide + (shape->num_tokens - 1) / tokens + 1, threads, 0, (hipStream_t)stream>>>(p);
+  kernel<<<grid, threads, 0, (hipStream_t)stream>>>(p);
   return launched("append_kv");
 }
 
@@ -157,6 +160,9 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
   const AttendPlan plan = plan_attend(*shape);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  if ((rc = check_launch(plan.chunk ? plan.grid : plan.rows, plan.chunk ? 256 * plan.groups : 64 * kAttendWaves)) ||
+      (plan.splits > 1 && (rc = check_launch(plan.rows, 256))))
+    return rc;
   const float cap = options->soft_cap < 0.f ? -options->soft_cap : options->soft_cap;
   AttendParams p = {};
   p.q = (const uint16_t*)q, p.kv = (const uint8_t*)kv_pages, p.scales = kv_scales;

@@ -676,7 +676,9 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
   r.tiles = r.tokens == 1 ? s.num_tokens : ((long long)s.num_tokens + r.tokens - 1) / r.tokens + s.max_num_seqs;
   if (r.split) {
     const long long tile = r.tokens * (long long)s.num_kv_heads * keys, most = (long long)kSelectWorkspace / tile;
+    const long long launch = kMostThreads / 1024 / (r.tokens * (long long)s.num_kv_heads);  // of choosing; at least 3
     r.batch = most < 1 ? 1 : most > 65535 ? 65535 : most;
+    if (r.batch > launch) r.batch = launch;
     if (r.batch > r.tiles) r.batch = r.tiles;
     r.bytes = (size_t)(r.batch * tile);
   }
@@ -686,6 +688,7 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
 template <int STEPS>
 int launch_select(const SelectPlan& plan, SelectParams p, hipStream_t stream) {
   if (!plan.split) {
+    if (const int rc = check_launch(plan.tiles * p.Hkv, kSelectThreads)) return rc;
     const bool wave = plan.stride <= (plan.tokens > 1 ? kWaveRow : kWaveDecode);
     const auto kernel = wave ? select_kernel<STEPS, true> : select_kernel<STEPS, false>;
     kernel<<<(unsigned)(plan.tiles * p.Hkv), kSelectThreads, plan.lds, stream>>>(p);

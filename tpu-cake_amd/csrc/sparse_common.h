@@ -112,6 +112,14 @@ __attribute__((format(printf, 2, 3))) int fail(int code, const char* format, ...
   return code;
 }
 
+// HIP launches fewer than 2^32 threads along a dimension.
+constexpr long long kMostThreads = (1ll << 32) - 1;
+
+int check_launch(long long groups, int threads) {
+  if (groups > kMostThreads / threads) return fail(RPA_E_UNSUPPORTED, "more rows than one launch takes");
+  return RPA_OK;
+}
+
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(RPA_E_HIP, "%s: %s", what, hipGetErrorString(e));
