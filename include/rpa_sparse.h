@@ -37,8 +37,9 @@ enum {
 int rpa_sparse_abi_version(void);
 const char* rpa_sparse_last_error(void);
 
-/* The current device's error word: the bits of every call since it was last cleared.  Waits for
- * the stream; `clear` != 0 sets it to 0 afterwards. */
+/* The current device's error word: the bits of every call since they were last cleared.  Waits for
+ * the stream; `clear` != 0 takes back the bits it returns, and no others that calls on other streams
+ * set meanwhile. */
 int rpa_sparse_read_error_word(int32_t* host_word, int32_t clear, void* stream);
 
 /* ---- page allocation -------------------------------------------------------------------------

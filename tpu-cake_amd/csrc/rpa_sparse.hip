@@ -21,15 +21,15 @@ const char* rpa_sparse_last_error(void) { return g_last_error; }
 int rpa_sparse_read_error_word(int32_t* host_word, int32_t clear, void* stream) {
   if (!host_word) return fail(RPA_E_INVALID, "host_word is NULL");
   const hipStream_t s = (hipStream_t)stream;
-  const int32_t zero = 0;
   if (hipMemcpyFromSymbolAsync(host_word, HIP_SYMBOL(g_error_word), sizeof(int32_t), 0, hipMemcpyDeviceToHost, s) !=
           hipSuccess ||
       hipStreamSynchronize(s) != hipSuccess)
     return fail(RPA_E_HIP, "reading the error word failed");
-  if (clear && (hipMemcpyToSymbolAsync(HIP_SYMBOL(g_error_word), &zero, sizeof zero, 0, hipMemcpyHostToDevice, s) !=
-                    hipSuccess ||
-                hipStreamSynchronize(s) != hipSuccess))
-    return fail(RPA_E_HIP, "clearing the error word failed");
+  if (clear && *host_word) {
+    clear_error_kernel<<<1, 1, 0, s>>>(*host_word);
+    if (hipGetLastError() != hipSuccess || hipStreamSynchronize(s) != hipSuccess)
+      return fail(RPA_E_HIP, "clearing the error word failed");
+  }
   return RPA_OK;
 }
 

@@ -21,6 +21,9 @@ __device__ int32_t g_error_word;
 
 __device__ __forceinline__ void flag_error(int bits) { atomicOr(&g_error_word, bits); }
 
+// Takes back the bits that a caller has read; other streams' kernels may set others meanwhile.
+__global__ void clear_error_kernel(int bits) { atomicAnd(&g_error_word, ~bits); }
+
 __device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b > 0); }
 
 constexpr uint32_t kSumCap = 1u << 30;  // sums saturate here: limits (pages, tokens) are below this

@@ -91,7 +91,8 @@ def check(rc: int) -> None:
 
 def read_error_word(device=None, *, clear: bool = False) -> int:
     """The error word of ``device`` (default: the current one): bits ``ERR_PAGE``, ``ERR_SLOT``,
-    ``ERR_LEN``, ``ERR_FREE`` of all calls since it was last cleared.  Waits for the current stream."""
+    ``ERR_LEN``, ``ERR_FREE`` of all calls since they were last cleared.  Waits for the current stream;
+    ``clear`` takes back the bits it returns."""
     import torch
 
     word = _i32(0)
