@@ -117,7 +117,8 @@ typedef struct rpa_sparse_shape {
 } rpa_sparse_shape_t;
 
 /* For each token and kv head the logical pages (indices into its sequence's page table row) whose
- * keys can score highest, ascending, -1 past the last: int32 [num_tokens, num_kv_heads, num_pages].
+ * keys can score highest, ascending, -1 past the last: int32 [num_tokens, num_kv_heads, num_pages], apart
+ * from the inputs.
  * A token sees the pages 0 .. position / page_size.  The first `sink_pages` and the last
  * `recent_pages` of them are always chosen (sink_pages + recent_pages <= num_pages), the others by
  *   score(p) = 2^exponent(p) * max over the group's heads g of sum_d max(qh_gd hi_d, qh_gd lo_d)
@@ -140,7 +141,7 @@ typedef struct rpa_sparse_options {
  * its kv head: selected_pages int32 [num_tokens, num_kv_heads, num_pages], logical pages in any order,
  * entries outside the token's pages (-1) list nothing, a page listed twice counts twice.  Keys and values
  * of an fp8 pool are code * scale, not rounded; kv_scales as in rpa.h or NULL.
- * out bf16 [num_tokens, num_q_heads, head_dim], contiguous; rows without a key or without a score
+ * out bf16 [num_tokens, num_q_heads, head_dim], contiguous, apart from the inputs; rows without a key or without a score
  * above -infinity, and rows at or past cu_q_lens[num_seqs], are zero. */
 size_t rpa_sparse_workspace_size(const rpa_sparse_shape_t* shape);
 int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse_options_t* options, const void* q,

@@ -43,8 +43,18 @@ int rpa_assign_pages(const rpa_paging_shape_t* shape, const int32_t* cached_lens
       !free_count_out || (shape->free_capacity && !free_pages) ||
       (shape->max_tokens && (!slot_mapping || !positions)))
     return fail(RPA_E_INVALID, "NULL tensor pointer");
-  if (kv_lens == cached_lens || kv_lens == new_tokens || free_count_out == free_count)
-    return fail(RPA_E_INVALID, "outputs must not overlap the inputs");
+  const long long N = shape->num_requests, most = shape->max_tokens;
+  const Memory in[] = {{"cached_lens", cached_lens, 4 * N}, {"new_tokens", new_tokens, 4 * N},
+                       {"page_table", page_table, 4 * N * shape->pages_per_seq},
+                       {"free_pages", free_pages, 4ll * shape->free_capacity}, {"free_count", free_count, 4}};
+  const Memory out[] = {{"kv_lens", kv_lens, 4 * N}, {"cu_q_lens", cu_q_lens, 4 * (N + 1)}, {"num_seqs", num_seqs, 4},
+                        {"slot_mapping", slot_mapping, 4 * most}, {"positions", positions, 4 * most},
+                        {"free_count_out", free_count_out, 4}};
+  for (const Memory& o : out) {
+    if (const int bad = check_separate(o, in)) return bad;
+    for (const Memory* other = out; other != &o; ++other)
+      if (meets(*other, o)) return fail(RPA_E_INVALID, "%s overlaps %s: outputs need memory of their own", o.name, other->name);
+  }
   const AssignParams p = {cached_lens, new_tokens, page_table, free_pages, free_count, kv_lens, cu_q_lens, num_seqs,
                           slot_mapping, positions, free_count_out, shape->num_requests, shape->pages_per_seq,
                           shape->page_size, shape->free_capacity, shape->max_tokens};
@@ -64,8 +74,13 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
   if (!cached_lens || !finished || !page_table || !free_count || !cached_lens_out || !free_count_out ||
       (shape->free_capacity && !free_pages))
     return fail(RPA_E_INVALID, "NULL tensor pointer");
-  if (cached_lens_out == cached_lens || free_count_out == free_count)
-    return fail(RPA_E_INVALID, "outputs must not overlap the inputs");
+  const long long N = shape->num_requests;
+  const Memory in[] = {{"cached_lens", cached_lens, 4 * N}, {"finished", finished, N},
+                       {"page_table", page_table, 4 * N * shape->pages_per_seq},
+                       {"free_pages", free_pages, 4ll * shape->free_capacity}, {"free_count", free_count, 4}};
+  const Memory lens = {"cached_lens_out", cached_lens_out, 4 * N}, count = {"free_count_out", free_count_out, 4};
+  int bad = check_separate(lens, in);
+  if (bad || (bad = check_separate(count, in)) || (bad = check_separate(count, {lens}))) return bad;
   const ReleaseParams p = {cached_lens, finished, page_table, free_pages, free_count, cached_lens_out, free_count_out,
                            shape->num_requests, shape->pages_per_seq, shape->page_size, shape->free_capacity};
   const int grid = (shape->num_requests - 1) / kReleaseSlice + 1;
@@ -126,6 +141,13 @@ int rpa_select_pages(const rpa_sparse_shape_t* shape, int32_t sink_pages, int32_
   const SelectPlan plan = plan_select(*shape);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  const long long T = shape->num_tokens, Hkv = shape->num_kv_heads, D = shape->head_dim, N = shape->max_num_seqs;
+  const Memory in[] = {rows_of("q", q, T, shape->num_q_heads, D, shape->q_token_stride, shape->q_head_stride),
+                       {"bounds", bounds, shape->total_pages * Hkv * 2 * D}, {"exponents", exponents, shape->total_pages * Hkv},
+                       {"kv_lens", kv_lens, 4 * N}, {"page_indices", page_indices, 4 * N * shape->pages_per_seq},
+                       {"cu_q_lens", cu_q_lens, 4 * (N + 1)}, {"num_seqs", num_seqs, 4},
+                       {"workspace", workspace, (long long)plan.bytes}};
+  if ((rc = check_separate({"selected_pages", selected_pages, 4 * T * Hkv * shape->num_pages}, in))) return rc;
   const SelectParams p = {(const uint16_t*)q, bounds, exponents, kv_lens, page_indices, cu_q_lens, num_seqs, selected_pages,
                           (uint32_t*)workspace, shape->q_token_stride, shape->q_head_stride, shape->num_tokens,
                           shape->num_kv_heads, shape->num_q_heads / shape->num_kv_heads, shape->head_dim,
@@ -156,10 +178,18 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
   if (kv_scales && !fp8) return fail(RPA_E_INVALID, "kv_scales requires fp8 kv_pages");
   if ((rc = check_strides("q", q, shape->q_token_stride, shape->q_head_stride))) return rc;
   if (!aligned16(kv_pages) || !aligned16(out)) return fail(RPA_E_INVALID, "kv_pages and out must be 16-byte aligned");
-  if (out == q) return fail(RPA_E_INVALID, "out must not be q");
   const AttendPlan plan = plan_attend(*shape);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  const long long T = shape->num_tokens, Hq = shape->num_q_heads, Hkv = shape->num_kv_heads, D = shape->head_dim;
+  const long long N = shape->max_num_seqs, pool = (long long)shape->total_pages * shape->page_size;
+  const Memory in[] = {rows_of("q", q, T, Hq, D, shape->q_token_stride, shape->q_head_stride),
+                       {"kv_pages", kv_pages, pool * 2 * Hkv * D * (fp8 ? 1 : 2)},
+                       {"kv_scales", kv_scales, 8 * shape->total_pages * Hkv},
+                       {"selected_pages", selected_pages, 4 * T * Hkv * shape->num_pages}, {"kv_lens", kv_lens, 4 * N},
+                       {"page_indices", page_indices, 4 * N * shape->pages_per_seq}, {"cu_q_lens", cu_q_lens, 4 * (N + 1)},
+                       {"num_seqs", num_seqs, 4}, {"workspace", workspace, (long long)plan.bytes}};
+  if ((rc = check_separate({"out", out, 2 * T * Hq * D}, in))) return rc;
   if ((rc = check_launch(plan.chunk ? plan.grid : plan.rows, plan.chunk ? 256 * plan.groups : 64 * kAttendWaves)) ||
       (plan.splits > 1 && (rc = check_launch(plan.rows, 256))))
     return rc;
@@ -178,7 +208,6 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
   p.scale = options->sm_scale * options->k_scale * (cap != 0.f ? 1.f : kLog2e), p.cap = cap;
   p.v_scale = options->v_scale;
   const hipStream_t s = (hipStream_t)stream;
-  const int D = p.D;
   if (fp8) {
     if (D == 256) launch_attend<256, true, true>(plan, p, s);
     else if (D == 128) launch_attend<128, true, true>(plan, p, s);

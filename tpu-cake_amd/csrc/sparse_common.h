@@ -123,6 +123,36 @@ int check_launch(long long groups, int threads) {
   return RPA_OK;
 }
 
+// Memory of a call: `outer` blocks, `step` bytes apart, of `bytes` each.
+struct Memory {
+  const char* name;
+  const void* at;
+  long long bytes, outer = 1, step = 0;
+};
+
+// Rows [tokens, heads, dim] of 16 bits; strides in values.  Blocks are what lies within the larger stride.
+Memory rows_of(const char* name, const void* at, long long tokens, long long heads, long long dim, long long token, long long head) {
+  const bool by_token = token >= head;
+  const long long inner = by_token ? (heads - 1) * head : (tokens - 1) * token;
+  return {name, at, 2 * (inner + dim), by_token ? tokens : heads, 2 * (by_token ? token : head)};
+}
+
+bool meets(const Memory& a, const Memory& out) {  // out: one block
+  if (!a.at || !out.at || a.bytes <= 0 || out.bytes <= 0) return false;
+  const long long from = (long long)((uintptr_t)out.at - (uintptr_t)a.at);  // of out, from a's first byte on
+  // the first block that ends behind out's first byte
+  const long long k = from < a.bytes ? 0 : a.step > 0 ? (from - a.bytes) / a.step + 1 : a.outer;
+  return k < a.outer && k * a.step < from + out.bytes;
+}
+
+// Workgroups run in no order: what a call writes must not lie in what it reads, nor in another output.
+template <int N>
+int check_separate(const Memory& out, const Memory (&others)[N]) {
+  for (const Memory& m : others)
+    if (meets(m, out)) return fail(RPA_E_INVALID, "%s overlaps %s: outputs need memory of their own", out.name, m.name);
+  return RPA_OK;
+}
+
 int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(RPA_E_HIP, "%s: %s", what, hipGetErrorString(e));

@@ -107,6 +107,28 @@ def _index(index, pages, heads, dim, device) -> PageIndex:
     return index
 
 
+def _blocks(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """A tensor's memory as (first byte, bytes of a block, blocks, bytes from one to the next): one block if contiguous,
+    else (rows [T, H, D]) what lies within the larger stride."""
+    size = t.element_size()
+    if t.is_contiguous():
+        return t.data_ptr(), t.numel() * size, 1, 0
+    (inner, count), (outer, blocks) = sorted(((t.stride(0), t.shape[0]), (t.stride(1), t.shape[1])))
+    return t.data_ptr(), ((count - 1) * inner + t.shape[2]) * size, blocks, outer * size
+
+
+def _separate(name: str, out: torch.Tensor, ins: dict) -> None:
+    """Refuses an output whose memory an input has a part of: workgroups run in no order."""
+    for other, t in ins.items():
+        if t is None or not t.numel() or not out.numel():
+            continue
+        first, size, blocks, step = _blocks(t)
+        start = out.data_ptr() - first
+        behind = 0 if start < size else (start - size) // step + 1 if step else blocks  # the first that ends after out begins
+        if behind < blocks and behind * step < start + out.numel() * out.element_size():
+            raise ValueError(f"{name} overlaps {other}: outputs need memory of their own")
+
+
 def preflight_append(slot_mapping: torch.Tensor, kv_pages: torch.Tensor) -> None:
     """Host check of what ``append_kv`` takes for granted: every slot is -1 or a row of the pool, no row
     is written twice, and the new rows of a page are consecutive tokens at consecutive slots.  Reads
@@ -263,6 +285,8 @@ def select_pages(
         out = kv_lens.new_empty(out_shape)
     else:
         _tensor("out", out, torch.int32, out_shape, q.device)
+        _separate("out", out, {"q": q, "index.bounds": bounds, "index.exponents": exponents, "kv_lens": kv_lens,
+                               "page_indices": page_indices, "cu_q_lens": cu_q_lens, "num_seqs": num_seqs})
     if dev != _get_device():
         with torch.cuda.device(dev):
             return select_pages(q, index, kv_lens, page_indices, cu_q_lens, num_seqs, page_size=page_size, num_pages=num_pages,
@@ -337,8 +361,8 @@ def sparse_paged_attention(
         out = q.new_empty(q.shape)
     else:
         _tensor("out", out, torch.bfloat16, q.shape, q.device)
-        if out.data_ptr() == q.data_ptr():
-            raise ValueError("out must be a tensor of its own")
+        _separate("out", out, {"q": q, "kv_pages": kv_pages, "selected_pages": selected_pages, "kv_lens": kv_lens,
+                               "page_indices": page_indices, "cu_q_lens": cu_q_lens, "num_seqs": num_seqs, "kv_scales": kv_scales})
     if dev != _get_device():
         with torch.cuda.device(dev):
             return sparse_paged_attention(q, kv_pages, selected_pages, kv_lens, page_indices, cu_q_lens, num_seqs,
