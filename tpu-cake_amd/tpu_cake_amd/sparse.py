@@ -103,7 +103,7 @@ def _index(index, pages, heads, dim, device) -> PageIndex:
     if not (isinstance(index, tuple) and len(index) == 2):
         raise TypeError("index must be a PageIndex")
     _tensor("index.bounds", index[0], torch.int8, (pages, heads, 2, dim), device)
-    _tensor("index.exponents", index[1], torch.int8, (index[0].shape[0], index[0].shape[1]), device)
+    _tensor("index.exponents", index[1], torch.int8, (index[0].shape[0], index[0].shape[1]), index[0].device)
     return index
 
 
