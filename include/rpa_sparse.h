@@ -97,6 +97,7 @@ typedef struct rpa_append_shape {
  * e4m3(x / scale), saturated, with the scale of the row's page and head in kv_scales (float
  * [total_pages, num_kv_heads, 2]) or, where that is NULL, k_scale and v_scale, positive and finite
  * (ignored for bf16).
+ * keys and values must not lie in the rows that are written.
  * bounds and exponents: the pool's index, or both NULL.  A page whose row 0 is written starts its
  * bounds anew, other pages' widen.  The slots (other than -1) have to differ, and the new rows of one
  * page have to be consecutive tokens at consecutive slots. */
@@ -117,7 +118,7 @@ typedef struct rpa_sparse_shape {
 } rpa_sparse_shape_t;
 
 /* For each token and kv head the logical pages (indices into its sequence's page table row) whose
- * keys can score highest, ascending, -1 past the last: int32 [num_tokens, num_kv_heads, num_pages], apart
+ * keys are estimated to score highest, ascending, -1 past the last: int32 [num_tokens, num_kv_heads, num_pages], apart
  * from the inputs.
  * A token sees the pages 0 .. position / page_size.  The first `sink_pages` and the last
  * `recent_pages` of them are always chosen (sink_pages + recent_pages <= num_pages), the others by

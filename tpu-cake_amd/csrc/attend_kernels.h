@@ -7,16 +7,17 @@
 // so P moves between no lanes; V passes through LDS as key rows and comes back transposed
 // (ds_read_b64_tr_b16).  P is split into three bf16 parts, each the nearest to what the earlier ones leave, with an
 // MFMA each: 24 bits, all that p has, where values cancel too.  Two parts (16 bits) lose what a token's values
-// have in common; the third product hides behind a row's loads and costs 8% of a chunk's tile.  fp8 codes are
-// exact in bf16; K scales multiply the scores and V scales P, both in fp32.
+// have in common; the third product hides behind a row's loads and takes a chunk's tiles from 92 to 100 us, in fp8
+// pools from 104 to 123.  fp8 codes are exact in bf16; K scales multiply the scores and V scales P, both in fp32.
 //
 // Every listed key of a row is read once, 2 D elem bytes at 2 Hkv D elem apart: HBM bounds decode rows.
 // Rows choose apart, so rows are what workgroups share nothing of: one row (its up to 16 heads) a
 // workgroup, its keys over four waves, each with its own (m, l, O), joined at the end through LDS.  With
 // few rows the list is split over workgroups as well, and a second launch joins their parts.
 //
-// Measured (8 kv heads of 128, 2048 keys a row): 64 decode rows of 64 heads, 539 MB: 92 us, 5.9 TB/s; 2 rows of an
-// fp8 pool, 8.4 MB: 7.1 us and 3.9 for the join, launches and latency.
+// Measured (8 kv heads of 128, 2048 keys a row): 64 decode rows of 64 heads, 539 MB: 92 us, 5.9 TB/s; of an fp8 pool,
+// 271 MB: 59 us, 4.6 TB/s; 2 rows of an fp8 pool, 8.4 MB: 7.4 us and 4.0 for the join, launches and latency.  A plain
+// read of 2 GiB reaches 6.3 TB/s.
 #pragma once
 
 #include "select_kernels.h"
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendParams p) {
 // LDS, for all of them.  Neighbouring tokens choose mostly the same pages (in the measured chunk 16 tokens of
 // 32 pages each name 44 to 48), so the L2 gives up a tenth of the bytes that rows of their own would ask
 // for, and every wave multiplies whole 16-column tiles.  Per 32 keys the four waves read 64 KB of K and V out
-// of LDS (512 cycles at 128 B a cycle) beside 384 cycles of MFMA each.  A key counts for a column if its page
+// of LDS (512 cycles at 128 B a cycle) beside 512 cycles of MFMA each.  A key counts for a column if its page
 // is on the token's own list and it is not past the token's position; a wave passes over 32 keys that none of
 // its columns counts.  A page one token lists and another does not may hold infinities or NaN, and P = 0 does
 // not silence those: where an output is not finite the tile is done again token by token, each reading its own
@@ -404,11 +405,13 @@ struct alignas(16) TileEntry {
 };
 
 // kGroups groups of four waves take every kGroups-th 32 keys and join at the end.  A turn is bound by what a SIMD
-// issues (24 MFMA of 16 cycles and some 120 VALU instructions a wave), by its chain of LDS reads, products and
-// exponentials and by waiting for the slowest wave, not by memory: 500 tokens of 32 pages of 64 keys (32 heads, 8
-// kv heads, 128 dims) take 100 us with 3 groups, one workgroup a CU, and 92 with 2 groups of 128 registers, two
-// workgroups a CU; 2000 tokens 264 and 228; 60 and 250 tokens, too few to fill a CU twice, 60 and 79.  fp8 needs
-// registers for its conversion, 104 us with 3 groups, and spills with 2; 256 dims fill the LDS with one workgroup.
+// issues (32 MFMA of 16 cycles and, by the counters, 198 VALU and 34 LDS instructions a wave), by its chain of LDS
+// reads, products and exponentials and by waiting for the slowest wave, not by memory: 500 tokens of 32 pages of 64 keys
+// beside 5 decode rows (32 heads, 8 kv heads, 128 dims; 304 workgroups) take 112 us with 3 groups, one workgroup a CU,
+// and 103 with 2 groups of 128 registers, two workgroups a CU; 700 tokens 125 and 111, 1000 125 and 113, 2000 243 and
+// 212; of those that do not fill a CU twice, 60 tokens 25 and 28, 250 tokens 65 and 84.  128 bf16 dims do not fit 128
+// registers: 36 are spilled, 104 bytes a lane, which writes 9.5 MB of the 13.8 that 505 tokens write.  fp8, which converts
+// as well, would spill 69 and keeps 3 groups (123 us); 256 dims fill the LDS with one workgroup.
 template <int DP, bool FULL, bool FP8, int kGroups>
 __global__ __launch_bounds__(256 * kGroups, DP < 256 && kGroups == 2 ? 4 : kGroups) void attend_tile_kernel(TileParams tp) {
   const AttendParams& p = tp.a;
@@ -826,7 +829,7 @@ struct AttendPlan {
 };
 
 constexpr long long kTileFill = 257;   // tiles from which two workgroups share a CU
-constexpr int kTileSplits = 8;  // 200 tokens of one kv head take 21 us, 26 with 4, 21 with 16
+constexpr int kTileSplits = 8;  // 200 tokens of one kv head take 23 us, 28 with 4, 23 with 16
 constexpr long long kAttendFill = 256;  // workgroups below which lists are split: one a CU
 
 AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
@@ -837,13 +840,18 @@ AttendPlan plan_attend(const rpa_sparse_shape_t& s) {
   r.width = s.page_size <= 64 ? s.page_size : 64;
   r.subs = (s.page_size + r.width - 1) / r.width;
   r.blocks = (long long)s.num_pages * r.subs;
+  // Tiles or rows, by the tokens a table row has: lengths are on the GPU, so rows without tokens count too, and a table
+  // with many of them takes rows where tiles would be faster.  A lone token's tile costs as much as sixteen's.  In us, as
+  // tiles and as rows (32 heads, 8 kv heads, 128 dims, lists of 32 pages of 64 keys): 64 sequences of 2 tokens 123 and 124,
+  // of 3 131 and 179; 64 decode rows beside a chunk of 16 181 and 121, of 66 (two a row) 188 and 174, of 200 208 and 286; 200
+  // beside 200 (just below two) 380 and 452; 16 beside 8 72 and 40; 8 sequences of 4 33 and 35.
   if (s.num_tokens > 2 * s.max_num_seqs && G <= 16 && s.pages_per_seq <= kTileColumns && r.subs < kTileParts) {
     r.chunk = true;
     r.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
     r.tokens = 64 / r.gp;
     r.grid = (((long long)s.num_tokens + r.tokens - 1) / r.tokens + s.max_num_seqs) * s.num_kv_heads;
     // Few tiles: their unions are split, into parts of at least 256 listed keys, while all parts run at once.  20, 60
-    // and 120 tokens of 32 pages of 64 keys (8 kv heads) take 28, 39 and 40 us, unsplit 59, 60 and 59.
+    // and 120 tokens of 32 pages of 64 keys (8 kv heads) take 21, 25 and 34 us, unsplit 62, 63 and 64.
     long long splits = kAttendFill / r.grid, most = (long long)s.num_pages * s.page_size / 256;
     splits = splits < most ? splits : most;
     r.splits = splits < 2 ? 1 : splits < kTileSplits ? (int)splits : kTileSplits;

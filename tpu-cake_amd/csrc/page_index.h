@@ -267,7 +267,9 @@ __device__ __forceinline__ void widen_bounds(const AppendParams& p, int t0, int 
 // One launch: the first `wide` workgroups (with an index) widen bounds, the others copy rows beside them.  Decode
 // batches are bound by latency: a token a workgroup, or a team.  Long batches are bound by the turnover of
 // workgroups and by runs that start late: eight tokens, and four rounds of teams first.  64 decode tokens of 8 heads
-// of 128 take 5.6 us (launch and two round trips); 9 000 prompt tokens into an fp8 pool, 55 MB, 23 us or 2.4 TB/s.
+// of 128 take 5.3 us (launch and two round trips); 9 000 prompt tokens into an fp8 pool, 55 MB, 24.6 us or 2.2 TB/s, into
+// a bf16 pool, 74 MB, 21.3 us or 3.5 TB/s.  K is read twice, by the workgroups that copy and by those that widen: 54 MB are
+// fetched where 37 would do.
 template <bool FP8, int TOKENS>
 __global__ __launch_bounds__(512) void append_kernel(AppendParams p) {
   const int block = blockIdx.x, teams = __umulhi(64u, p.chunk_magic);

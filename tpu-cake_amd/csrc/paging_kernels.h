@@ -7,14 +7,16 @@
 // the number of pages taken before request i: its j-th new page is free[count - 1 - (P(i) - need(i)) - j].
 //
 // A step's metadata is tens of bytes a request: launches and dependent loads bound it, not bandwidth.
-// So one launch does everything.  Every workgroup writes kTokens entries of the slot map and sums over
+// So one launch does everything.  Every workgroup writes an entry of the slot map a thread and sums over
 // the requests itself, 4 to a thread, until its tokens are covered; workgroup 0 sums over all of them
 // and writes the per-request outputs.  Repeating the sums costs a read of 8 N bytes from the L2 for
 // each workgroup; a second launch that read them back would cost more than that for N up to thousands.
 // The outputs do not overlap the inputs, as the workgroups read the inputs at different times.
 //
-// Measured: 64 requests 4.3 us (an empty launch takes 2 to 3), 4096 requests and 65 000 tokens 10.4 us: the
-// four turns of two sums, 1.5 us each, and the slot map's dependent reads (owner, page).  Release: 3.0 and 4.4 us.
+// Measured: 64 requests 4.4 us (an empty launch takes 2 to 3), 4096 requests and 65 000 tokens 10.4 us.  That is one turn
+// of workgroups of 1024 threads, which takes 8.8 us with no token at all, where 1024 requests in workgroups of 256 take
+// 5.4 (four barriers over 16 waves instead of 4, and sums over 16 parts a thread); 8192 requests, two turns, take 15.8.
+// Tokens add 1.2: the slot map's dependent reads (owner, page).  Release: 3.1 and 4.2 us.
 #pragma once
 
 #include "sparse_common.h"
@@ -84,8 +86,9 @@ __global__ __launch_bounds__(THREADS) void assign_kernel(AssignParams p) {
     for (int k = 0; k < kItems; ++k) {
       taken[k] = (int)pre.a;
       pre = {sat_add(pre.a, min((uint32_t)need[k], kSumCap)), sat_add(pre.b, min((uint32_t)q[k], kSumCap))};
-      // selects, not branches: with branches this compiler (clang 22, ROCm 7.2) kept the old q[0] for
-      // requests turned down for their pages alone
+      // selects, not branches: of `if (!admitted) q[k] = 0, need[k] = 0` with short-circuited conditions clang 22 (ROCm 7.2)
+      // makes right IR but, for k = 0, code that clears q and need only where the first two conditions fail and does
+      // nothing where the third does: requests turned down for their pages alone kept their tokens
       const bool admitted =
           valid[k] & (pre.b <= (uint32_t)p.max_tokens) & ((need[k] == 0) | (pre.a <= (uint32_t)count));
       q[k] = admitted ? q[k] : 0;

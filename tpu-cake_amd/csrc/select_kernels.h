@@ -1,8 +1,8 @@
 // The choice of pages: for each (token, kv head) the pages whose keys can score highest.
 //
 // Mathematics: the group's queries are rounded to int8 on a grid 2^f they share (f as the index's
-// exponents), qh.  A key x of page p has q . x <= sum_d max(q_d hi_d, q_d lo_d), so with the index's
-// int8 bounds the score is
+// exponents), qh.  A key x of page p has q . x <= sum_d max(q_d hi_d, q_d lo_d); the score estimates that bound from qh,
+// so a query below half a step of the group's grid counts as 0 and the head with the largest scores decides:
 //     s(p) = 2^e(p) max_g sum_d max(qh_gd hi_d, qh_gd lo_d) = 2^e(p) max_g ([qh+ ; qh-] . [hi ; lo])_g,
 // qh+ = max(qh, 0), qh- = min(qh, 0): one int8 product of length 2 D a page and head, on
 // v_mfma_i32_16x16x64_i8.  |sum| <= 127^2 D < 2^24, so it is exact in int32 and as fp32, and the
@@ -15,10 +15,10 @@
 // 128-dim heads; it bounds long contexts.  Short ones are bound by latency (metadata, page ids, index
 // rows, then the counting steps: four dependent round trips).
 //
-// Measured (8 kv heads of 128): 64 decode rows over 4 096 to 65 536 keys in pages of 64, 49 MB of index: 23 us,
-// 2.1 TB/s; 2 rows over half a million keys in pages of 16, 127 MB: scored in 31 us, 4.1 TB/s, chosen in 11.5;
-// a chunk of 1000 tokens over 32 768 keys in pages of 64, 15 MB: 32 us, of which rounding queries, scoring and
-// choosing take a third each.
+// Measured (8 kv heads of 128): 64 decode rows over 4 096 to 65 536 keys in pages of 64, 49 MB of index: 24 us,
+// 2.1 TB/s; 2 rows over half a million keys in pages of 16, 127 MB: scored in 31 us, 4.1 TB/s, chosen in 12;
+// a chunk of 1000 tokens over 32 768 keys in pages of 64, 15 MB: 35 us, of which rounding queries, scoring and
+// choosing take a third each.  256 dims spill 5 or 6 registers of the 64 that two workgroups a CU leave.
 #pragma once
 
 #include "page_index.h"
@@ -656,6 +656,9 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
   r.steps = need <= 2 ? 2 : need <= 4 ? 4 : 8;
   const size_t row = r.steps * 64 + 16, keys = (size_t)r.stride * 4;
   const long long rows = (long long)s.num_tokens * s.num_kv_heads;
+  // Tiles or rows, by the tokens a table row has, as the attention (32 heads, 8 kv heads, 32 768 keys in pages of 64; us as
+  // tiles and as rows): 64 decode rows beside a chunk of 16 29 and 25, of 66 29 and 34, of 200 29 and 56; 64 sequences of 2
+  // tokens 21 and 32.
   r.tile = s.num_tokens > 2 * s.max_num_seqs && G <= 16;
   if (r.tile) {
     r.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
@@ -670,6 +673,9 @@ SelectPlan plan_select(const rpa_sparse_shape_t& s) {
   } else {
     r.gp = (G + 15) / 16 * 16;
     r.tokens = 1;
+    // Few rows of long tables are split over workgroups: 32 rows of up to 2048 pages take 20 us split and 26 whole, 128 rows
+    // 26 and 26; of up to 8192 pages 128 rows 67 and 108, 248 rows 121 and 123.  248 rows of up to 2048 pages would be
+    // faster whole, 34 us where they take 43.
     r.split = r.gp * row + keys > kSelectLds || (rows < 256 && r.stride > 1024);
     r.lds = r.gp * row + (r.split ? 0 : keys);
   }

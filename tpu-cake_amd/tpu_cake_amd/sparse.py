@@ -7,8 +7,9 @@ sequence, here each token and kv head reads the keys of ``num_pages`` pages.
 * ``append_kv`` writes a step's new keys and values to the slots that ``paging.assign_pages`` gave
   them, and keeps the pool's **page index**: for each page and kv head the largest and smallest
   value of every dimension of the page's keys, 2 * head_dim bytes.
-* ``select_pages`` bounds every page's scores for a token from the index alone and chooses the pages
-  with the highest bounds; the first and the newest pages are always among them.
+* ``select_pages`` estimates the highest score that a page's keys can have for a token, from the index
+  alone, and chooses the pages with the highest estimates; the first and the newest pages are always
+  among them.
 * ``sparse_paged_attention`` attends to the keys of the listed pages, up to the token's position.
 
 Decode rows (one token a sequence), prompt chunks and mixes of them are one call each.  All tensors
@@ -242,14 +243,15 @@ def select_pages(
     (columns of the sequence's ``page_indices`` row), ascending, -1 past the last.
 
     A token sees the pages up to its own (position // page_size).  The first ``sink_pages`` and the last
-    ``recent_pages`` of them are always chosen; the others by the bound that the index gives for the
-    group's queries, rounded to int8,
+    ``recent_pages`` of them are always chosen; the others by an estimate of their highest score, of
+    the index's bounds and the group's queries, rounded to int8 on one grid,
 
         score(p) = 2**exponent(p) * max_g sum_d max(q_gd * hi_d, q_gd * lo_d),
 
     the highest first and of equal scores the earlier page.  Scores are whole numbers times a power of
-    two: the choice does not depend on an order of summation.  Tokens at or past ``cu_q_lens[num_seqs]``
-    get no page.
+    two: the choice does not depend on an order of summation.  A head whose queries are all below 1/254 of
+    the group's largest counts as 0, and the head with the largest scores decides.  Tokens at or past
+    ``cu_q_lens[num_seqs]`` get no page.
     """
     bounds, exponents = index
     sig = (q.shape, q.dtype, q.get_device(), q.stride(), bounds.shape, bounds.dtype, bounds.get_device(), bounds.is_contiguous(),
