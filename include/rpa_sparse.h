@@ -74,6 +74,13 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
                       const int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
                       int32_t* cached_lens_out, int32_t* free_count_out, void* stream);
 
+/* Cuts requests longer than `limit` to `budget` tokens (1 <= budget <= limit): their length becomes budget in
+ * cached_lens_out, dropped_out is dropped int32 [N] plus the tokens that went (the others' as they are), and the pages
+ * past those of budget tokens are pushed on the free stack, in order.  max_tokens of the shape is ignored. */
+int rpa_trim_pages(const rpa_paging_shape_t* shape, int32_t budget, int32_t limit, const int32_t* cached_lens,
+                   const int32_t* dropped, const int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
+                   int32_t* cached_lens_out, int32_t* dropped_out, int32_t* free_count_out, void* stream);
+
 /* ---- K/V append and the page index ------------------------------------------------------------
  * The page index of a pool: bounds int8 [total_pages, num_kv_heads, 2, head_dim] (of every dimension
  * the largest, then the smallest value of the page's keys) and exponents int8 [total_pages,

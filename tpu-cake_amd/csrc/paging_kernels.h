@@ -155,13 +155,18 @@ struct ReleaseParams {
   const int32_t* free_count;
   int32_t *cached_out, *free_out;
   int N, PPS, S, F;
+  const int32_t* dropped;  // the trim's: requests longer than `limit` are cut to `budget`
+  int32_t* dropped_out;
+  int budget, limit;
 };
 
 constexpr int kReleaseThreads = 1024;
 constexpr int kReleaseSlice = 64;  // requests per workgroup
 
 // A workgroup owns a slice of the requests: it sums the pages that earlier requests give back, then
-// copies its own, a wave for each finished request.
+// copies its own, a wave for each finished request.  The trim (TRIM) gives back the pages of a request past
+// its budget's instead: sums and stack are the same.
+template <bool TRIM>
 __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams p) {
   __shared__ uint32_t s_sum[kReleaseThreads / 64];
   __shared__ uint32_t s_off[kReleaseSlice];
@@ -169,14 +174,16 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const int i0 = blockIdx.x * kReleaseSlice;
   const long long capacity = (long long)p.PPS * p.S;
+  const int first = TRIM ? ceil_div(p.budget, p.S) : 0;  // the first page that goes
+  const auto gone = [&](int i, int len) { return TRIM ? len > p.limit : p.finished[i] != 0; };
   const auto pages_of = [&](bool finished, int len) {
-    return !finished || len <= 0 ? 0 : ceil_div((int)min((long long)len, capacity), p.S);
+    return !finished || len <= 0 ? 0 : max(ceil_div((int)min((long long)len, capacity), p.S) - first, 0);
   };
   uint32_t before = 0;
 #pragma unroll 4
   for (int i = tid; i < i0; i += kReleaseThreads) {
-    const bool finished = p.finished[i];
-    const int len = p.cached[i];  // beside it, not after it
+    const int len = p.cached[i];
+    const bool finished = gone(i, len);  // loaded beside it, not after it
     before = sat_add(before, (uint32_t)pages_of(finished, len));
   }
   for (int d = 32; d; d /= 2) before = sat_add(before, __shfl_xor(before, d));
@@ -187,8 +194,8 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
     for (int w = 0; w < kReleaseThreads / 64; ++w) before = sat_add(before, s_sum[w]);
     const int i = i0 + lane;
     const bool live = i < p.N;
-    const bool finished = live && p.finished[i];
     const int len = live ? p.cached[i] : 0;
+    const bool finished = live && gone(i, len);
     const int pages = pages_of(finished, len);
     uint32_t inc = (uint32_t)pages;
     for (int d = 1; d < 64; d *= 2) {
@@ -198,8 +205,9 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
     s_pages[lane] = pages;
     s_off[lane] = sat_add(before, inc - (uint32_t)pages);
     if (live) {
-      if (finished && (len < 0 || len > capacity)) flag_error(RPA_SPARSE_ERR_LEN);
-      p.cached_out[i] = finished ? 0 : len;
+      if ((TRIM || finished) && (len < 0 || len > capacity)) flag_error(RPA_SPARSE_ERR_LEN);
+      p.cached_out[i] = finished ? (TRIM ? p.budget : 0) : len;
+      if (TRIM) p.dropped_out[i] = p.dropped[i] + (finished ? len - p.budget : 0);
     }
     if (i0 + kReleaseSlice >= p.N && lane == 63) {
       const long long end = (long long)max(*p.free_count, 0) + sat_add(before, inc);
@@ -212,7 +220,7 @@ __global__ __launch_bounds__(kReleaseThreads) void release_kernel(ReleaseParams 
   for (int r = wave; r < kReleaseSlice; r += kReleaseThreads / 64) {
     const int pages = s_pages[r];
     if (pages == 0) continue;
-    const int32_t* row = p.table + (size_t)(i0 + r) * p.PPS;
+    const int32_t* row = p.table + (size_t)(i0 + r) * p.PPS + first;
     const long long to = count + s_off[r];
     for (int j = lane; j < pages; j += 64)
       if (to + j < p.F) p.free_pages[to + j] = row[j];

@@ -82,11 +82,40 @@ int rpa_release_pages(const rpa_paging_shape_t* shape, const int32_t* cached_len
   int bad = check_separate(lens, in);
   if (bad || (bad = check_separate(count, in)) || (bad = check_separate(count, {lens}))) return bad;
   const ReleaseParams p = {cached_lens, finished, page_table, free_pages, free_count, cached_lens_out, free_count_out,
-                           shape->num_requests, shape->pages_per_seq, shape->page_size, shape->free_capacity};
+                           shape->num_requests, shape->pages_per_seq, shape->page_size, shape->free_capacity,
+                           nullptr, nullptr, 0, 0};
   const int grid = (shape->num_requests - 1) / kReleaseSlice + 1;
   if (const int many = check_launch(grid, kReleaseThreads)) return many;
-  release_kernel<<<grid, kReleaseThreads, 0, (hipStream_t)stream>>>(p);
+  release_kernel<false><<<grid, kReleaseThreads, 0, (hipStream_t)stream>>>(p);
   return launched("release_pages");
+}
+
+int rpa_trim_pages(const rpa_paging_shape_t* shape, int32_t budget, int32_t limit, const int32_t* cached_lens,
+                   const int32_t* dropped, const int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
+                   int32_t* cached_lens_out, int32_t* dropped_out, int32_t* free_count_out, void* stream) {
+  const int rc = check_paging(shape);
+  if (rc) return rc;
+  if (budget < 1 || limit < budget) return fail(RPA_E_INVALID, "budget must be positive and limit at least budget");
+  if (!cached_lens || !dropped || !page_table || !free_count || !cached_lens_out || !dropped_out || !free_count_out ||
+      (shape->free_capacity && !free_pages))
+    return fail(RPA_E_INVALID, "NULL tensor pointer");
+  const long long N = shape->num_requests;
+  const Memory in[] = {{"cached_lens", cached_lens, 4 * N}, {"dropped", dropped, 4 * N},
+                       {"page_table", page_table, 4 * N * shape->pages_per_seq},
+                       {"free_pages", free_pages, 4ll * shape->free_capacity}, {"free_count", free_count, 4}};
+  const Memory lens = {"cached_lens_out", cached_lens_out, 4 * N}, count = {"free_count_out", free_count_out, 4};
+  const Memory gone = {"dropped_out", dropped_out, 4 * N};
+  int bad = check_separate(lens, in);
+  if (bad || (bad = check_separate(gone, in)) || (bad = check_separate(count, in)) || (bad = check_separate(gone, {lens})) ||
+      (bad = check_separate(count, {lens, gone})))
+    return bad;
+  const ReleaseParams p = {cached_lens, nullptr, page_table, free_pages, free_count, cached_lens_out, free_count_out,
+                           shape->num_requests, shape->pages_per_seq, shape->page_size, shape->free_capacity,
+                           dropped, dropped_out, budget, limit};
+  const int grid = (shape->num_requests - 1) / kReleaseSlice + 1;
+  if (const int many = check_launch(grid, kReleaseThreads)) return many;
+  release_kernel<true><<<grid, kReleaseThreads, 0, (hipStream_t)stream>>>(p);
+  return launched("trim_pages");
 }
 
 int rpa_append_kv(const rpa_append_shape_t* shape, const void* keys, const void* values, const int32_t* slot_mapping,

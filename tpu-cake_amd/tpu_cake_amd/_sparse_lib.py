@@ -43,6 +43,7 @@ _SIGNATURES = {
     "rpa_sparse_read_error_word": (ctypes.c_int, [ctypes.POINTER(_i32), _i32, _vp]),
     "rpa_assign_pages": (ctypes.c_int, [ctypes.POINTER(RpaPagingShape)] + [_vp] * 12),
     "rpa_release_pages": (ctypes.c_int, [ctypes.POINTER(RpaPagingShape)] + [_vp] * 8),
+    "rpa_trim_pages": (ctypes.c_int, [ctypes.POINTER(RpaPagingShape)] + [_i32] * 2 + [_vp] * 9),
     "rpa_append_kv": (ctypes.c_int, [ctypes.POINTER(RpaAppendShape)] + [_vp] * 5 + [ctypes.c_float] * 2 + [_vp] * 3),
     "rpa_select_workspace_size": (_sz, [ctypes.POINTER(RpaSparseShape)]),
     "rpa_select_pages": (ctypes.c_int, [ctypes.POINTER(RpaSparseShape), _i32, _i32] + [_vp] * 9 + [_sz, _vp]),

@@ -4,12 +4,13 @@ The pool's free pages are a stack (``free_pages[:free_count]``); a request holds
 ``ceil(len / page_size)`` entries of its ``page_table`` row.  ``assign_pages`` gives each request the
 pages of its new tokens and writes what ``ops.ragged_paged_attention`` and the entry points of
 ``sparse`` take: lengths, cumulative query lengths, the slot of every new token (``sparse.append_kv``)
-and its position.  ``release_pages`` takes the pages of finished requests back.  Nothing is read on
-the host, so a serving loop's step needs no synchronisation and can be captured into a graph.
+and its position.  ``release_pages`` takes the pages of finished requests back, ``trim_pages`` those of
+requests that ``eviction`` cut to their budget.  Nothing is read on the host, so a serving loop's step
+needs no synchronisation and can be captured into a graph.
 
 All tensors are contiguous int32 tensors on one GPU.  What a call reads is never written by it,
 except new entries of ``page_table`` (``assign_pages``) and of ``free_pages`` above its count
-(``release_pages``): lengths and counts come back in tensors of their own, the caller's next inputs.
+(``release_pages``, ``trim_pages``): lengths and counts come back in tensors of their own, the caller's next inputs.
 """
 
 from __future__ import annotations
@@ -181,6 +182,65 @@ def release_pages(
             return release_pages(cached_lens, finished, page_table, free_pages, free_count, page_size=page_size, out=out)
     rc = fn(shape, cached_lens.data_ptr(), finished.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(),
             free_count.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), _current_stream(dev))
+    if rc:
+        _sparse_lib.check(rc)
+    return tuple(out)
+
+
+def trim_pages(
+    cached_lens: torch.Tensor,  # i32[N]
+    dropped: torch.Tensor,      # i32[N]: tokens that each request's cache has lost so far
+    page_table: torch.Tensor,   # i32[N, pages_per_seq]
+    free_pages: torch.Tensor,   # i32[F], entries above the count written in place
+    free_count: torch.Tensor,   # i32[1]
+    *,
+    page_size: int,
+    budget: int,
+    limit: int | None = None,   # budget where it is None
+    out: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts the requests longer than ``limit`` to ``budget`` tokens and pushes the pages that they no longer need on
+    the free stack, in order; returns (lengths, dropped tokens, the new count).
+
+    The step after ``eviction.choose_moves`` and ``eviction.move_rows`` with the same budget and limit, which bring
+    the rows to keep into the first ``budget``: once for all the layers that share the page table.  Pages past
+    ``free_pages``' capacity are dropped and set ``ERR_FREE``, lengths that are negative or past the table ``ERR_LEN``.
+    """
+    sig = (page_table.shape, page_table.dtype, page_table.get_device(), page_table.is_contiguous(),
+           cached_lens.shape, cached_lens.dtype, cached_lens.get_device(), cached_lens.is_contiguous(),
+           dropped.shape, dropped.dtype, dropped.get_device(), dropped.is_contiguous(),
+           free_pages.shape, free_pages.dtype, free_pages.get_device(), free_pages.is_contiguous(),
+           free_count.shape, free_count.dtype, free_count.get_device(), free_count.is_contiguous(), page_size, budget, limit, "trim")
+    plan = _plans.get(sig)
+    if plan is None:
+        n = page_table.shape[0]
+        i32 = torch.int32
+        _check({"page_table": (page_table, (None, None), i32), "cached_lens": (cached_lens, (n,), i32),
+                "dropped": (dropped, (n,), i32), "free_pages": (free_pages, (None,), i32),
+                "free_count": (free_count, (1,), i32)}, page_table, n, page_size)
+        if free_pages.numel() >= 1 << 30:
+            raise ValueError("free_pages must have fewer than 2^30 entries")
+        most = budget if limit is None else limit
+        for name, x, least in (("budget", budget, 1), ("limit", most, budget)):
+            if not (isinstance(x, int) and least <= x < 1 << 31):
+                raise ValueError(f"{name}={x!r} must be an int of at least {least}")
+        plan = _keep(sig, (_sparse_lib.RpaPagingShape(n, page_table.shape[1], page_size, free_pages.numel(), 0), [n, n, 1], most,
+                           _sparse_lib.load().rpa_trim_pages))
+    shape, sizes, most, fn = plan
+    dev = page_table.get_device()
+    if out is None:
+        out = _parts(page_table.new_empty(2 * sizes[0] + 1), sizes)
+    else:
+        names = {"out lengths": out[0], "out dropped": out[1], "out count": out[2]}
+        _check({k: (t, (n,), torch.int32) for (k, t), n in zip(names.items(), sizes)}, page_table, 1, page_size)
+        _separate(names, {"cached_lens": cached_lens, "dropped": dropped, "page_table": page_table,
+                          "free_pages": free_pages, "free_count": free_count})
+    if dev != _get_device():
+        with torch.cuda.device(dev):
+            return trim_pages(cached_lens, dropped, page_table, free_pages, free_count, page_size=page_size, budget=budget,
+                              limit=limit, out=out)
+    rc = fn(shape, budget, most, cached_lens.data_ptr(), dropped.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(),
+            free_count.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), _current_stream(dev))
     if rc:
         _sparse_lib.check(rc)
     return tuple(out)
