@@ -1,0 +1,541 @@
+// Attention over a paged cache that accounts for the weight each key got.
+//
+// Mathematics: o_t = sum_x p_tx v_x, p_tx = 2^(s_tx - m_t) / l_t over the keys x up to token t's position (log2 domain),
+// and for each key the sum of p_tx over the step's tokens and the group's heads.  The row's maximum m and sum l are
+// known only once every key has been seen, so weights take the scores a second time.
+#pragma once
+
+#include "attend_kernels.h"
+
+namespace rpa_sparse {
+namespace {
+
+// v / d for 0 <= v < 2^31: (v * m) >> (31 + s) with s = ceil(log2 d), m = floor(2^(31 + s) / d) + 1.  m d is past
+// 2^(31 + s) by at most 2^s, so the quotient is exact.
+struct Divisor {
+  uint32_t m;
+  int shift;
+};
+Divisor divisor(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return {(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), 31 + s};
+}
+__device__ __forceinline__ int div_by(int v, Divisor d) { return (int)(((uint64_t)(uint32_t)v * d.m) >> d.shift); }
+
+constexpr int kWeighWaves = 4, kWeighThreads = 64 * kWeighWaves;
+constexpr int kBlockKeys = 256;  // keys of a block of rows' work: two units of 32 for each wave
+constexpr int kWeighKeys = 128;  // keys whose weights a workgroup sums at once
+
+struct WeighParams {
+  const uint16_t* q;
+  const uint8_t* kv;
+  const float* scales;
+  const int32_t *kv_lens, *table, *cu, *num_seqs, *dropped;
+  float* weights;
+  int32_t* positions;
+  uint16_t* out;
+  float2* stats;  // (m, 1 / l) of every token and head
+  float* parts;   // two for each workgroup: (m, l) of 16 rows, then the rows' O
+  long long q_token, q_head;
+  int T, Hkv, G, D, P, S, N, PPS;
+  int tiles;      // 16-head tiles of a group
+  Divisor page, group;
+  float scale, cap, v_scale, decay;  // scale: of q.k; times log2 e where cap is 0
+};
+
+struct Sequence {
+  int first, tokens, keys;  // its first token, its tokens, its keys
+};
+
+// Sequence i, its offsets taken into [0, T] and its length into the page table.
+__device__ __forceinline__ Sequence sequence_at(const WeighParams& p, int i, bool flag = false) {
+  const int begin = min(max(p.cu[i], 0), p.T), end = min(max(p.cu[i + 1], 0), p.T), len = max(p.kv_lens[i], 0);
+  const int capacity = p.PPS * p.S;
+  if (flag && len > capacity && end > begin) flag_error(RPA_SPARSE_ERR_LEN);
+  return {begin, max(end - begin, 0), min(len, capacity)};
+}
+
+// Where a workgroup's share of all the work begins: sequences in order, `amount(i)` units of work each, the total in
+// shares of equal size.
+struct Share {
+  long long from, to;  // units
+  int seq;             // that `from` lies in
+  long long before;    // units of the sequences before it
+};
+
+template <typename Amount>
+__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount) {
+  __shared__ long long s_sum[kWeighWaves];
+  __shared__ Share s_share;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int each = (n + kWeighThreads - 1) / kWeighThreads, i0 = min(tid * each, n), i1 = min(i0 + each, n);
+  long long own = 0;
+  for (int i = i0; i < i1; ++i) own += amount(i);
+  long long upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long long o = __shfl_up(upto, d);
+    upto += lane >= d ? o : 0;
+  }
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kWeighWaves; ++w) {
+    upto += w < wave ? s_sum[w] : 0;
+    total += s_sum[w];
+  }
+  const long long each_share = (total + count - 1) / count, from = min(index * each_share, total);
+  const long long to = min(from + each_share, total);
+  long long before = upto - own;
+  if (from < to && from >= before && from < upto) {
+    int i = i0;
+    for (;; ++i) {
+      const long long a = amount(i);
+      if (from < before + a) break;
+      before += a;
+    }
+    s_share = {from, to, i, before};
+  }
+  __syncthreads();
+  return from < to ? s_share : Share{0, 0, 0, 0};
+}
+
+// The blocks of keys of one row of sequence i; sequence n stands for the tokens past the last one.
+__device__ __forceinline__ int row_blocks(const Sequence& s) { return max((s.keys + kBlockKeys - 1) / kBlockKeys, 1); }
+
+__device__ __forceinline__ Sequence row_sequence(const WeighParams& p, int n, int i) {
+  if (i < n) return sequence_at(p, i);
+  const int end = n ? min(max(p.cu[n], 0), p.T) : 0;
+  return {end, p.T - end, 0};
+}
+
+// Rows: a token's heads, up to 16 of one kv head.  Their keys come in blocks, blocks of all rows in shares, one a
+// workgroup: a long sequence's rows are spread over as many workgroups as their blocks need, and short ones' share a workgroup.
+// A row that a workgroup does not have whole leaves a part: the first in the workgroup's slot 0, the last in slot 1.
+template <int DP, bool FULL, bool FP8>
+__global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p) {
+  constexpr int kRow = DP * 2 + 32;
+  constexpr int kWave = 32 * kRow;
+  constexpr int kORow = DP + 4;
+  constexpr int kElem = FP8 ? 1 : 2;
+  constexpr int kLoads = DP * kElem / 64;
+  constexpr int kSteps = DP / 32;
+  static_assert(16 * kORow * 4 <= kWave, "O rows fit the wave's V region");
+  __shared__ __align__(16) uint8_t s_v[kWeighWaves * kWave];
+  __shared__ float s_m[kWeighWaves][16], s_l[kWeighWaves][16];
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
+  const int count = min(max(*p.num_seqs, 0), p.N);
+  const int heads = p.Hkv * p.tiles;
+  Share share = share_of(count + 1, blockIdx.x, gridDim.x, [&](int i) {
+    const Sequence s = row_sequence(p, count, i);
+    return (long long)s.tokens * heads * row_blocks(s);
+  });
+  if (share.from == share.to) return;
+
+  const int row_bytes = p.D * kElem;
+  const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
+  const global_bytes zero = zero_row();
+  uint8_t* const tile_v = s_v + wave * kWave;
+  int seq = share.seq;
+  Sequence s = row_sequence(p, count, seq);
+  long long before = share.before, at = share.from;
+  while (at < share.to) {
+    int blocks = row_blocks(s);
+    while (at >= before + (long long)s.tokens * heads * blocks) {
+      before += (long long)s.tokens * heads * blocks;
+      s = row_sequence(p, count, ++seq);
+      blocks = row_blocks(s);
+    }
+    const long long row = (at - before) / blocks;
+    const int first_block = (int)(at - before - row * blocks);
+    const int end_block = (int)min((long long)blocks, first_block + (share.to - at));
+    const int token = (int)(row / heads), head_tile = (int)(row - (long long)token * heads), h = head_tile / p.tiles;
+    const int tile = head_tile - h * p.tiles, t = s.first + token;
+    const int keys = max(s.keys - (s.tokens - 1 - token), 0);
+    const bool known = seq < count;
+    const int32_t* const table = p.table + (size_t)(known ? seq : 0) * p.PPS;
+
+    bf16x8 q[kSteps];
+    {
+      const int head = tile * 16 + n;
+      const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + head) * p.q_head;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int dim = FP8 ? 64 * (i / 2) + 16 * j + 8 * (i % 2) : 32 * i + 8 * j;
+        u32x4 w = {0, 0, 0, 0};
+        if (head < p.G && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+        q[i] = __builtin_bit_cast(bf16x8, w);
+      }
+    }
+    const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
+    const int end_key = min(keys, end_block * kBlockKeys), end_unit = (end_key + 31) / 32;
+    int slots[2];
+    u32x4 k[2][kLoads], v[2][kLoads];
+    uint32_t seen[2];
+    float ks[2], vs[2];  // fp8: the scales of key n of the 16
+    const auto find = [&](int unit) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int key = unit * 32 + 16 * b + n;
+        int slot = -1;
+        if (key < end_key) {
+          const int page = div_by(key, p.page), id = table[page];
+          if (id >= 0 && id < p.P) slot = id * p.S + (key - page * p.S);
+          else flag_error(RPA_SPARSE_ERR_PAGE);
+        }
+        slots[b] = slot;
+      }
+    };
+    const auto load = [&] {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bool ok = slots[b] >= 0;
+        seen[b] = (uint32_t)__ballot(ok) & 0xffffu;
+        const global_bytes src = ok ? rows + (uint32_t)slots[b] * row_stride : zero;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int byte = 64 * i + 16 * j;
+          const global_bytes from = FULL || byte < row_bytes ? src : zero;
+          k[b][i] = load16(from + byte);
+          v[b][i] = load16(from + row_bytes + byte);
+        }
+        if (FP8) {
+          const float* scale = p.scales && ok ? p.scales + ((size_t)div_by(slots[b], p.page) * p.Hkv + h) * 2 : nullptr;
+          ks[b] = scale ? scale[0] : 1.f, vs[b] = scale ? scale[1] : 1.f;
+        }
+      }
+    };
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = kLowest, l = 0.f;
+    int unit = first_block * (kBlockKeys / 32) + wave;
+    if (unit < end_unit) find(unit), load();
+    for (; unit < end_unit; unit += kWeighWaves) {
+      f32x4 sc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        sc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const u32x4 a = FP8 ? bf16_of_codes(k[b][i / 2][2 * (i % 2)], k[b][i / 2][2 * (i % 2) + 1]) : k[b][FP8 ? 0 : i];
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], sc[b], 0, 0, 0);
+        }
+      }
+      wave_fence();  // the last unit's V has been read
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          uint8_t* dst = tile_v + (16 * b + n) * kRow + (FP8 ? 128 * i + 32 * j : 64 * i + 16 * j);
+          if (FP8) {
+            *(u32x4*)dst = bf16_of_codes(v[b][i][0], v[b][i][1]);
+            *(u32x4*)(dst + 16) = bf16_of_codes(v[b][i][2], v[b][i][3]);
+          } else {
+            *(u32x4*)dst = v[b][i];
+          }
+        }
+      wave_fence();
+      const bool whole = (seen[0] & seen[1]) == 0xffffu;
+      const uint32_t here[2] = {seen[0] >> (4 * j), seen[1] >> (4 * j)};
+      float vk[2][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sc[b][r] = scaled(sc[b][r], FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale);
+          vk[b][r] = FP8 ? __shfl(vs[b], 4 * j + r) : 1.f;
+        }
+      if (unit + kWeighWaves < end_unit) find(unit + kWeighWaves), load();
+      if (p.cap != 0.f) cap_scores(sc, p.cap);
+      if (!whole) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[b][r] = here[b] >> r & 1 ? sc[b][r] : -__builtin_inff();
+      }
+      float top = max_of(max_of(max_of(sc[0][0], sc[0][1]), max_of(sc[0][2], sc[0][3])),
+                         max_of(max_of(sc[1][0], sc[1][1]), max_of(sc[1][2], sc[1][3])));
+      if (__ballot(top > m + kRescale)) {
+        top = swap_max(top);
+        const float next = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) o[d] *= f;
+      }
+      u32x4 parts[3];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = __builtin_amdgcn_exp2f(sc[b][r] - m);
+          l += e[r];
+          if (FP8) e[r] *= vk[b][r];
+        }
+        const Parts lo = split_bf16(e[0], e[1]), hi = split_bf16(e[2], e[3]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) parts[i][2 * b] = lo.of[i], parts[i][2 * b + 1] = hi.of[i];
+      }
+      typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+      const uint8_t* vt = tile_v + (4 * j + n / 4) * kRow + 8 * (n % 4);
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
+        const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kRow + 32 * d));
+        const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, parts[i]), o[d], 0, 0, 0);
+      }
+    }
+
+    // join the waves
+    l = swap_sum(l);
+    if (j == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+    __syncthreads();  // every wave is done with its V, too
+    float all = s_m[0][n];
+#pragma unroll
+    for (int w = 1; w < kWeighWaves; ++w) all = fmaxf(all, s_m[w][n]);
+    const float f = __builtin_amdgcn_exp2f(m - all);
+    float* const mine = (float*)tile_v + n * kORow;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) *(f32x4*)(mine + 16 * d + 4 * j) = o[d] * f;
+    __syncthreads();
+    const bool own = first_block == 0 && end_block == blocks;
+    const int live = min(p.G - tile * 16, 16), quads = p.D / 4;
+    float* const part = p.parts + (2 * (size_t)blockIdx.x + (at > share.from)) * (32 + 16 * (size_t)p.D);
+    for (int i = tid; i < live * quads; i += kWeighThreads) {
+      const int r = i / quads, d = i % quads * 4;
+      float top = s_m[0][r], sum = 0.f;
+#pragma unroll
+      for (int w = 1; w < kWeighWaves; ++w) top = fmaxf(top, s_m[w][r]);
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWeighWaves; ++w) {
+        sum += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
+        x += *(const f32x4*)((const float*)(s_v + w * kWave) + r * kORow + d);
+      }
+      if (!own) {
+        if (d == 0) part[2 * r] = top, part[2 * r + 1] = sum;
+        *(f32x4*)(part + 32 + r * p.D + d) = x;
+        continue;
+      }
+      const size_t to = (size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r;
+      const float g = sum == 0.f ? 0.f : p.v_scale / sum;
+      if (d == 0) p.stats[to] = {top, sum == 0.f ? 0.f : 1.f / sum};
+      *(u32x2*)(p.out + to * p.D + d) =
+          sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x[0] * g, x[1] * g), pack_bf16(x[2] * g, x[3] * g)};
+    }
+    __syncthreads();  // the next row's V
+    at += end_block - first_block;
+  }
+}
+
+// Joins the parts of rows that several workgroups had: one workgroup for each share, which takes the row that ends in
+// it and began before it.
+__global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(WeighParams p) {
+  const int count = min(max(*p.num_seqs, 0), p.N), heads = p.Hkv * p.tiles;
+  const Share share = share_of(count + 1, blockIdx.x, gridDim.x, [&](int i) {
+    const Sequence s = row_sequence(p, count, i);
+    return (long long)s.tokens * heads * row_blocks(s);
+  });
+  if (share.from == share.to) return;
+  const Sequence s = row_sequence(p, count, share.seq);
+  const int blocks = row_blocks(s);
+  const long long row = (share.from - share.before) / blocks, begin = share.before + row * blocks, end = begin + blocks;
+  if (begin == share.from || end > share.to) return;  // uniform
+  const long long each = share.from / blockIdx.x;  // every share before the last has as many; block 0 begins a row
+  const int first = (int)(begin / each), last = blockIdx.x;
+  const int token = (int)(row / heads), head_tile = (int)(row - (long long)token * heads), h = head_tile / p.tiles;
+  const int tile = head_tile - h * p.tiles, t = s.first + token;
+  const int live = min(p.G - tile * 16, 16), quads = p.D / 4;
+  const size_t stride = 32 + 16 * (size_t)p.D;
+  for (int i = threadIdx.x; i < live * quads; i += kWeighThreads) {
+    const int r = i / quads, d = i % quads * 4;
+    float top = kLowest, sum = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int w = first; w <= last; ++w) {
+      const float* part = p.parts + (2 * (size_t)w + (w == first && begin % each != 0)) * stride;
+      const float m = part[2 * r], l = part[2 * r + 1];
+      if (l == 0.f) continue;
+      const f32x4 o = *(const f32x4*)(part + 32 + r * p.D + d);
+      const float next = fmaxf(top, m), mine = __builtin_amdgcn_exp2f(top - next), its = __builtin_amdgcn_exp2f(m - next);
+      top = next;
+      sum = sum * mine + l * its;
+      x = x * mine + o * its;
+    }
+    const size_t to = (size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r;
+    const float g = sum == 0.f ? 0.f : p.v_scale / sum;
+    if (d == 0) p.stats[to] = {top, sum == 0.f ? 0.f : 1.f / sum};
+    *(u32x2*)(p.out + to * p.D + d) =
+        sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x[0] * g, x[1] * g), pack_bf16(x[2] * g, x[3] * g)};
+  }
+}
+
+// The weights of a sequence's keys, kWeighKeys at a time for a kv head, 32 a wave: the scores once more, from K held in
+// registers and every row (token, head) that sees one of the keys, 16 columns at a time.
+template <int DP, bool FULL, bool FP8>
+__global__ __launch_bounds__(kWeighThreads) void weigh_keys_kernel(WeighParams p) {
+  constexpr int kElem = FP8 ? 1 : 2;
+  constexpr int kLoads = DP * kElem / 64;
+  constexpr int kSteps = DP / 32;
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
+  const int count = min(max(*p.num_seqs, 0), p.N);
+  const auto blocks_of = [](const Sequence& s) { return s.tokens ? (s.keys + kWeighKeys - 1) / kWeighKeys : 0; };
+  const Share share = share_of(count, blockIdx.x, gridDim.x, [&](int i) {
+    return (long long)blocks_of(sequence_at(p, i, true)) * p.Hkv;
+  });
+  const int row_bytes = p.D * kElem;
+  const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
+  const global_bytes zero = zero_row();
+  int seq = share.seq;
+  long long before = share.before;
+  for (long long at = share.from; at < share.to; ++at) {
+    Sequence s = sequence_at(p, seq);
+    while (at >= before + (long long)blocks_of(s) * p.Hkv) {
+      before += (long long)blocks_of(s) * p.Hkv;
+      s = sequence_at(p, ++seq);
+    }
+    const int blocks = blocks_of(s), h = (int)((at - before) / blocks), first = (int)((at - before) - (long long)h * blocks) * kWeighKeys;
+    const int32_t* const table = p.table + (size_t)seq * p.PPS;
+    const int key0 = first + 32 * wave;
+    if (key0 >= s.keys) continue;  // no barrier follows
+    const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
+    bf16x8 k[2][kSteps];
+    float ks[2];
+    const auto slot_of = [&](int key) {
+      if (key >= s.keys) return -1;
+      const int page = div_by(key, p.page), id = table[page];
+      return id >= 0 && id < p.P ? id * p.S + (key - page * p.S) : -1;
+    };
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int slot = slot_of(key0 + 16 * b + n);
+      const global_bytes src = slot >= 0 ? rows + (uint32_t)slot * row_stride : zero;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int byte = 64 * i + 16 * j;
+        const u32x4 w = load16((FULL || byte < row_bytes ? src : zero) + byte);
+        if (FP8) {
+          k[b][2 * i] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[0], w[1]));
+          k[b][2 * i + 1] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[2], w[3]));
+        } else {
+          k[b][i] = __builtin_bit_cast(bf16x8, w);
+        }
+      }
+      ks[b] = FP8 && p.scales && slot >= 0 ? p.scales[((size_t)div_by(slot, p.page) * p.Hkv + h) * 2] : 1.f;
+    }
+    float scale[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) scale[b][r] = FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale;
+    const int old = s.keys - s.tokens;  // keys before the step's
+    const int end = s.tokens * p.G;
+    float sum[2][4] = {};
+    for (int base = max(key0 - old, 0) * p.G; base < end; base += 16) {
+      const int row = base + n, token = div_by(min(row, end - 1), p.group), g = row - token * p.G, t = s.first + token;
+      const bool live = row < end;
+      const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + g) * p.q_head;
+      f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int dim = FP8 ? 64 * (i / 2) + 16 * j + 8 * (i % 2) : 32 * i + 8 * j;
+        u32x4 w = {0, 0, 0, 0};
+        if (live && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][i], __builtin_bit_cast(bf16x8, w), sc[b], 0, 0, 0);
+      }
+      const float2 stat = live ? p.stats[(size_t)t * p.Hkv * p.G + h * p.G + g] : float2{0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[b][r] = scaled(sc[b][r], scale[b][r]);
+      if (p.cap != 0.f) cap_scores(sc, p.cap);
+      const int last = live ? old + token : -1;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(sc[b][r] - stat.x);
+          sum[b][r] += key0 + 16 * b + 4 * j + r <= last && stat.y != 0.f ? e * stat.y : 0.f;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        for (int d = 1; d < 16; d *= 2) sum[b][r] += __shfl_xor(sum[b][r], d);
+    // lane n of each j: key n / 4 * 16 ... of the 8 keys a lane has, lane n < 8 writes the n-th
+    if (n < 8) {
+      const int b = n / 4, r = n % 4;
+      float x = 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x = u == n ? sum[u / 4][u % 4] : x;
+      const int key = key0 + 16 * b + 4 * j + r, slot = slot_of(key);
+      if (slot >= 0) {
+        const int page = div_by(slot, p.page);
+        const size_t to = ((size_t)page * p.Hkv + h) * p.S + (slot - page * p.S);
+        if (key >= old) p.positions[to] = (p.dropped ? p.dropped[seq] : 0) + key;
+        else if (p.decay != 0.f) x += p.decay * p.weights[to];
+        p.weights[to] = x;
+      }
+    }
+  }
+}
+
+// ---- host side ----
+int check_weigh(const rpa_weigh_shape_t* s) {
+  if (!s) return fail(RPA_E_INVALID, "shape is NULL");
+  rpa_sparse_shape_t t = {s->num_tokens, s->num_q_heads, s->num_kv_heads, s->head_dim, s->total_pages, s->page_size,
+                          s->max_num_seqs, s->pages_per_seq, s->kv_dtype, 1, s->q_token_stride, s->q_head_stride};
+  const int rc = check_sparse(&t);
+  if (rc) return rc;
+  if ((long long)s->num_tokens * s->num_q_heads > kMostIndex)
+    return fail(RPA_E_INVALID, "num_tokens * num_q_heads must be at most 2^31 - 2^16 - 1");
+  if ((long long)s->pages_per_seq * s->page_size > kMostIndex || s->max_num_seqs > kMostIndex)
+    return fail(RPA_E_INVALID, "pages_per_seq * page_size and max_num_seqs must be at most 2^31 - 2^16 - 1");
+  return RPA_OK;
+}
+
+struct WeighPlan {
+  int tiles, rows_grid, keys_grid;
+  size_t stats, bytes;
+};
+
+constexpr int kRowsGrid = 768, kKeysGrid = 2048;
+
+WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
+  WeighPlan r = {};
+  r.tiles = (s.num_q_heads / s.num_kv_heads + 15) / 16;
+  const auto most = [](long long a, long long b) { return a > 0 && b > LLONG_MAX / a ? LLONG_MAX : a * b; };
+  const long long capacity = (long long)s.pages_per_seq * s.page_size;
+  const long long rows = (long long)s.num_tokens * s.num_kv_heads * r.tiles;
+  const long long work = most(rows, capacity / kBlockKeys + 1);
+  r.rows_grid = (int)(work < kRowsGrid ? work : kRowsGrid);
+  const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
+  const long long blocks = most(seqs * s.num_kv_heads, capacity / kWeighKeys + 1);
+  r.keys_grid = (int)(blocks < kKeysGrid ? blocks : kKeysGrid);
+  r.stats = ((size_t)s.num_tokens * s.num_q_heads * sizeof(float2) + 15) / 16 * 16;
+  r.bytes = r.stats + (size_t)r.rows_grid * 2 * (32 + 16 * (size_t)s.head_dim) * 4;
+  return r;
+}
+
+template <int DP, bool FULL, bool FP8>
+int launch_weigh(const WeighPlan& plan, const WeighParams& p, hipStream_t stream) {
+  weigh_rows_kernel<DP, FULL, FP8><<<plan.rows_grid, kWeighThreads, 0, stream>>>(p);
+  int rc = launched("weighed_attention");
+  if (rc) return rc;
+  weigh_join_kernel<<<plan.rows_grid, kWeighThreads, 0, stream>>>(p);
+  if ((rc = launched("weighed_attention (join)"))) return rc;
+  weigh_keys_kernel<DP, FULL, FP8><<<plan.keys_grid, kWeighThreads, 0, stream>>>(p);
+  return launched("weighed_attention (keys)");
+}
+
+}  // namespace
+}  // namespace rpa_sparse

@@ -8,7 +8,7 @@ reference's fused-plan surface (``tpu_cake_amd.fused``); the v1 Inkling decode
 contract (``experiment inkling-rpa``) runs through ``tpu_cake_amd.inkling``.
 """
 
-from . import fused, inkling, paging, sparse  # noqa: F401
+from . import eviction, fused, inkling, paging, rotary, sparse  # noqa: F401
 
 from .ops import (  # noqa: F401
     DEFAULT_MASK_VALUE,
@@ -27,9 +27,11 @@ __all__ = [
     "CapturedCalls",
     "DEFAULT_MASK_VALUE",
     "PreparedCall",
+    "eviction",
     "fused",
     "inkling",
     "paging",
+    "rotary",
     "sparse",
     "dynamic_validate_inputs",
     "gather_kv",

@@ -1,4 +1,4 @@
-"""Build ``librpa.so`` and ``librpa_sparse.so`` for gfx950 in-tree with hipcc (``python -m tpu_cake_amd.build``).
+"""Build ``librpa.so``, ``librpa_sparse.so`` and ``librpa_bounded.so`` for gfx950 in-tree with hipcc (``python -m tpu_cake_amd.build``).
 
 Also builds ``librpa_timeline.so``: the same sources with ``-DRPA_TIMELINE``, whose attention
 kernel records a per-workgroup timeline (read by ``tpu_cake_amd.timeline``); the product path
@@ -20,8 +20,10 @@ INCLUDE = ROOT / "include"
 SOURCES = [CSRC / "rpa_kernels.hip"]
 HEADERS = [CSRC / "rpa_schedule.h", INCLUDE / "rpa.h"]
 SPARSE_SOURCES = [CSRC / "rpa_sparse.hip"]  # page allocation, K/V append, sparse attention (include/rpa_sparse.h)
+BOUNDED_SOURCES = [CSRC / "rpa_bounded.hip"]  # rotation, weighed attention, eviction (include/rpa_bounded.h)
 OUTPUT = PKG / "librpa.so"
 SPARSE_OUTPUT = PKG / "librpa_sparse.so"
+BOUNDED_OUTPUT = PKG / "librpa_bounded.so"
 TIMELINE_OUTPUT = PKG / "librpa_timeline.so"
 ARCH = "gfx950"
 
@@ -33,13 +35,13 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-def sparse_command(output: pathlib.Path = SPARSE_OUTPUT) -> list[str]:
-    """As ``command``, without its no-NaN assumption: what the append and the choice of pages do
+def sparse_command(output: pathlib.Path = SPARSE_OUTPUT, sources: list[pathlib.Path] | None = None) -> list[str]:
+    """As ``command``, without its no-NaN assumption: what the append and the choices of pages and of rows do
     with NaN inputs is defined."""
     return [
         hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-        f"-I{INCLUDE}", f"-I{CSRC}", *[str(s) for s in SPARSE_SOURCES], "-o", str(output),
+        f"-I{INCLUDE}", f"-I{CSRC}", *[str(s) for s in sources or SPARSE_SOURCES], "-o", str(output),
     ]
 
 
@@ -74,10 +76,11 @@ def _finish(job, verbose: bool) -> pathlib.Path:
 
 
 def build(verbose: bool = False, timeline: bool = True) -> pathlib.Path:
-    """Compile every HIP source into ``librpa.so`` and ``librpa_sparse.so`` (always recompiles), and
+    """Compile every HIP source into ``librpa.so``, ``librpa_sparse.so`` and ``librpa_bounded.so`` (always recompiles), and
     (``timeline``) the timeline variant beside them, the compilations in parallel.  Returns the path
     of ``librpa.so``."""
-    jobs = [_start(OUTPUT, command, []), _start(SPARSE_OUTPUT, sparse_command)]
+    jobs = [_start(OUTPUT, command, []), _start(SPARSE_OUTPUT, sparse_command),
+            _start(BOUNDED_OUTPUT, sparse_command, BOUNDED_SOURCES)]
     if timeline:
         jobs.append(_start(TIMELINE_OUTPUT, command, ["-DRPA_TIMELINE"]))
     out = [_finish(j, verbose) for j in jobs]
