@@ -149,7 +149,9 @@ int rpa_weighed_attention(const rpa_weigh_shape_t* shape, const rpa_weigh_option
   p.q_token = s.q_token_stride, p.q_head = s.q_head_stride;
   p.T = s.num_tokens, p.Hkv = s.num_kv_heads, p.G = s.num_q_heads / s.num_kv_heads, p.D = s.head_dim;
   p.P = s.total_pages, p.S = s.page_size, p.N = s.max_num_seqs, p.PPS = s.pages_per_seq;
-  p.chunk = plan.tiles_grid > 0, p.tile_parts = (float*)((uint8_t*)workspace + plan.stats + plan.parts);
+  p.chunk = plan.tiles_grid > 0, p.score_room = plan.score_room;
+  p.scores = (float*)((uint8_t*)workspace + plan.stats + plan.parts);
+  p.tile_parts = (float*)((uint8_t*)workspace + plan.stats + plan.parts + plan.scores);
   p.tiles = plan.tiles, p.page = divisor(s.page_size), p.group = divisor(p.G);
   p.scale = options->sm_scale * options->k_scale * (cap != 0.f ? 1.f : kLog2e), p.cap = cap;
   p.v_scale = options->v_scale, p.decay = options->decay;

@@ -25,7 +25,6 @@ __device__ __forceinline__ int div_by(int v, Divisor d) { return (int)(((uint64_
 
 constexpr int kWeighWaves = 4, kWeighThreads = 64 * kWeighWaves;
 constexpr int kBlockKeys = 256;  // keys of a block of rows' work: two units of 32 for each wave
-constexpr int kWeighKeys = 128;  // keys whose weights a workgroup sums at once
 
 struct WeighParams {
   const uint16_t* q;
@@ -36,6 +35,8 @@ struct WeighParams {
   int32_t* positions;
   uint16_t* out;
   float2* stats;  // (m, 1 / l) of every token and head
+  float* scores;
+  long long score_room;  // blocks of 16 keys
   float* parts;   // two for each workgroup: (m, l) of 16 rows, then the rows' O
   long long q_token, q_head;
   int T, Hkv, G, D, P, S, N, PPS;
@@ -64,44 +65,58 @@ struct Share {
   long long from, to;  // units
   int seq;             // that `from` lies in
   long long before;    // units of the sequences before it
+  long long scores;    // and their blocks of scores
 };
 
-template <typename Amount>
-__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount) {
-  __shared__ long long s_sum[kWeighWaves];
+template <typename Amount, typename Scores>
+__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount, Scores scores) {
+  __shared__ long long s_sum[kWeighWaves], s_scores[kWeighWaves];
   __shared__ Share s_share;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const int each = (n + kWeighThreads - 1) / kWeighThreads, i0 = min(tid * each, n), i1 = min(i0 + each, n);
-  long long own = 0;
-  for (int i = i0; i < i1; ++i) own += amount(i);
-  long long upto = own;
+  long long own = 0, mine = 0;
+  for (int i = i0; i < i1; ++i) own += amount(i), mine += scores(i);
+  long long upto = own, stored = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const long long o = __shfl_up(upto, d);
-    upto += lane >= d ? o : 0;
+    const long long o = __shfl_up(upto, d), u = __shfl_up(stored, d);
+    upto += lane >= d ? o : 0, stored += lane >= d ? u : 0;
   }
-  if (lane == 63) s_sum[wave] = upto;
+  if (lane == 63) s_sum[wave] = upto, s_scores[wave] = stored;
   __syncthreads();
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < kWeighWaves; ++w) {
-    upto += w < wave ? s_sum[w] : 0;
+    upto += w < wave ? s_sum[w] : 0, stored += w < wave ? s_scores[w] : 0;
     total += s_sum[w];
   }
   const long long each_share = (total + count - 1) / count, from = min(index * each_share, total);
   const long long to = min(from + each_share, total);
   long long before = upto - own;
+  stored -= mine;
   if (from < to && from >= before && from < upto) {
     int i = i0;
     for (;; ++i) {
       const long long a = amount(i);
       if (from < before + a) break;
-      before += a;
+      before += a, stored += scores(i);
     }
-    s_share = {from, to, i, before};
+    s_share = {from, to, i, before, stored};
   }
   __syncthreads();
-  return from < to ? s_share : Share{0, 0, 0, 0};
+  return from < to ? s_share : Share{0, 0, 0, 0, 0};
+}
+template <typename Amount>
+__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount) {
+  return share_of(n, index, count, amount, [](int) { return 0ll; });
+}
+
+// Scores of a sequence with one token, which its weights take instead of K once more: blocks of 16 keys, of which
+// [kv head][head of the group][key].  They are kept while they fit the workspace, which holds all that distinct pages can
+// have.
+__device__ __forceinline__ long long score_blocks(const Sequence& s) { return s.tokens == 1 ? (s.keys + 15) / 16 : 0; }
+__device__ __forceinline__ bool scores_fit(const WeighParams& p, const Sequence& s, long long before) {
+  return s.tokens == 1 && before + score_blocks(s) <= p.score_room;
 }
 
 // The blocks of keys of one row of sequence i; sequence n stands for the tokens past the last one.
@@ -134,10 +149,13 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
   const int count = min(max(*p.num_seqs, 0), p.N);
   const int heads = p.Hkv * p.tiles;
-  Share share = share_of(count + 1, blockIdx.x, gridDim.x, [&](int i) {
-    const Sequence s = row_sequence(p, count, i);
-    return (long long)s.tokens * heads * row_blocks(s);
-  });
+  const Share share = share_of(
+      count + 1, blockIdx.x, gridDim.x,
+      [&](int i) {
+        const Sequence s = row_sequence(p, count, i);
+        return (long long)s.tokens * heads * row_blocks(s);
+      },
+      [&](int i) { return i < count ? score_blocks(sequence_at(p, i)) : 0ll; });
   if (share.from == share.to) return;
 
   const int row_bytes = p.D * kElem;
@@ -146,11 +164,12 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
   uint8_t* const tile_v = s_v + wave * kWave;
   int seq = share.seq;
   Sequence s = row_sequence(p, count, seq);
-  long long before = share.before, at = share.from;
+  long long before = share.before, at = share.from, score_at = share.scores;
   while (at < share.to) {
     int blocks = row_blocks(s);
     while (at >= before + (long long)s.tokens * heads * blocks) {
       before += (long long)s.tokens * heads * blocks;
+      score_at += seq < count ? score_blocks(s) : 0;
       s = row_sequence(p, count, ++seq);
       blocks = row_blocks(s);
     }
@@ -177,7 +196,9 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
     }
     const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
     const int end_key = min(keys, end_block * kBlockKeys), end_unit = (end_key + 31) / 32;
-    int slots[2];
+    const bool keep = known && scores_fit(p, s, score_at);
+    float* const scores = p.scores + ((size_t)score_at * p.Hkv + h) * p.G * 16 + (tile * 16 + n) * 16 + 4 * j;
+    int ids[2];  // the pages of key n and n + 16 of a unit: found a turn before its keys are loaded
     u32x4 k[2][kLoads], v[2][kLoads];
     uint32_t seen[2];
     float ks[2], vs[2];  // fp8: the scales of key n of the 16
@@ -185,21 +206,18 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int key = unit * 32 + 16 * b + n;
-        int slot = -1;
-        if (key < end_key) {
-          const int page = div_by(key, p.page), id = table[page];
-          if (id >= 0 && id < p.P) slot = id * p.S + (key - page * p.S);
-          else flag_error(RPA_SPARSE_ERR_PAGE);
-        }
-        slots[b] = slot;
+        ids[b] = key < end_key ? table[div_by(key, p.page)] : -1;
       }
     };
-    const auto load = [&] {
+    const auto load = [&](int unit) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const bool ok = slots[b] >= 0;
+        const int key = unit * 32 + 16 * b + n, id = ids[b];
+        const bool ok = key < end_key && id >= 0 && id < p.P;
+        if (key < end_key && !ok) flag_error(RPA_SPARSE_ERR_PAGE);
         seen[b] = (uint32_t)__ballot(ok) & 0xffffu;
-        const global_bytes src = ok ? rows + (uint32_t)slots[b] * row_stride : zero;
+        const int slot = ok ? id * p.S + (key - div_by(key, p.page) * p.S) : 0;
+        const global_bytes src = ok ? rows + (uint32_t)slot * row_stride : zero;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
           const int byte = 64 * i + 16 * j;
@@ -208,17 +226,18 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
           v[b][i] = load16(from + row_bytes + byte);
         }
         if (FP8) {
-          const float* scale = p.scales && ok ? p.scales + ((size_t)div_by(slots[b], p.page) * p.Hkv + h) * 2 : nullptr;
+          const float* scale = p.scales && ok ? p.scales + ((size_t)id * p.Hkv + h) * 2 : nullptr;
           ks[b] = scale ? scale[0] : 1.f, vs[b] = scale ? scale[1] : 1.f;
         }
       }
+      if (unit + kWeighWaves < end_unit) find(unit + kWeighWaves);
     };
     f32x4 o[DP / 16];
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kLowest, l = 0.f;
     int unit = first_block * (kBlockKeys / 32) + wave;
-    if (unit < end_unit) find(unit), load();
+    if (unit < end_unit) find(unit), load(unit);
     for (; unit < end_unit; unit += kWeighWaves) {
       f32x4 sc[2];
 #pragma unroll
@@ -254,13 +273,19 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
           sc[b][r] = scaled(sc[b][r], FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale);
           vk[b][r] = FP8 ? __shfl(vs[b], 4 * j + r) : 1.f;
         }
-      if (unit + kWeighWaves < end_unit) find(unit + kWeighWaves), load();
+      if (unit + kWeighWaves < end_unit) load(unit + kWeighWaves);
       if (p.cap != 0.f) cap_scores(sc, p.cap);
       if (!whole) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[b][r] = here[b] >> r & 1 ? sc[b][r] : -__builtin_inff();
+      }
+      if (keep) {  // uniform
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (tile * 16 + n < p.G && unit * 32 + 16 * b < end_key)
+            *(f32x4*)(scores + (size_t)(2 * unit + b) * p.Hkv * p.G * 16) = sc[b];
       }
       float top = max_of(max_of(max_of(sc[0][0], sc[0][1]), max_of(sc[0][2], sc[0][3])),
                          max_of(max_of(sc[1][0], sc[1][1]), max_of(sc[1][2], sc[1][3])));
@@ -734,114 +759,198 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_join_tiles_kernel(WeighPa
   }
 }
 
-// The weights of a sequence's keys, kWeighKeys at a time for a kv head, 32 a wave: the scores once more, from K held in
-// registers and every row (token, head) that sees one of the keys, 16 columns at a time.
+// The weights of a sequence's keys, a block of them for a kv head at a time.  Of a sequence with one token the scores are
+// there, and its block is kScoreKeys.  Of others a block is kWeighKeys, 64 a wave, whose K stays in registers as the
+// products' A operand while every row (token, head) that sees one of them passes through LDS, kWeighRows at a time: the
+// scores once more.  A lane sums its keys over its columns, and lanes meet once at the end.
+constexpr int kScoreKeys = 1024, kWeighRows = 32;
+
 template <int DP, bool FULL, bool FP8>
-__global__ __launch_bounds__(kWeighThreads) void weigh_keys_kernel(WeighParams p) {
+__global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParams p) {
   constexpr int kElem = FP8 ? 1 : 2;
-  constexpr int kLoads = DP * kElem / 64;
-  constexpr int kSteps = DP / 32;
-  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
-  const int count = min(max(*p.num_seqs, 0), p.N);
-  const auto blocks_of = [](const Sequence& s) { return s.tokens ? (s.keys + kWeighKeys - 1) / kWeighKeys : 0; };
-  const Share share = share_of(count, blockIdx.x, gridDim.x, [&](int i) {
-    return (long long)blocks_of(sequence_at(p, i, true)) * p.Hkv;
-  });
+  constexpr int kSteps = DP / 16;
+  constexpr int kWave = DP > 128 ? 32 : 64, kBlocks = kWave / 32;  // keys of a wave
+  constexpr int kKeys = kWave * kWeighWaves;
+  constexpr int kRow = DP * 2 + 16;
+  constexpr int kLoads = kWeighRows * DP * 2 / 16 / kWeighThreads;
+  __shared__ __align__(16) uint8_t s_q[2][kWeighRows * kRow];
+  __shared__ float2 s_stat[2][kWeighRows];
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
+  const int count = min(max(*p.num_seqs, 0), p.N), index = share_index();
+  const auto blocks_of = [&](const Sequence& s) {
+    const int keys = s.tokens == 1 ? kScoreKeys : kKeys;
+    return s.tokens ? (s.keys + keys - 1) / keys : 0;
+  };
+  const Share share = share_of(
+      count, index, gridDim.x, [&](int i) { return (long long)blocks_of(sequence_at(p, i, true)) * p.Hkv; },
+      [&](int i) { return score_blocks(sequence_at(p, i)); });
+  if (share.from == share.to) return;
   const int row_bytes = p.D * kElem;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
   const global_bytes zero = zero_row();
   int seq = share.seq;
-  long long before = share.before;
+  Sequence s = sequence_at(p, seq);
+  long long before = share.before, score_at = share.scores;
   for (long long at = share.from; at < share.to; ++at) {
-    Sequence s = sequence_at(p, seq);
     while (at >= before + (long long)blocks_of(s) * p.Hkv) {
       before += (long long)blocks_of(s) * p.Hkv;
+      score_at += score_blocks(s);
       s = sequence_at(p, ++seq);
     }
-    const int blocks = blocks_of(s), h = (int)((at - before) / blocks), first = (int)((at - before) - (long long)h * blocks) * kWeighKeys;
+    const int blocks = blocks_of(s), h = (int)((at - before) / blocks), block = (int)((at - before) - (long long)h * blocks);
     const int32_t* const table = p.table + (size_t)seq * p.PPS;
-    const int key0 = first + 32 * wave;
-    if (key0 >= s.keys) continue;  // no barrier follows
-    const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
-    bf16x8 k[2][kSteps];
-    float ks[2];
-    const auto slot_of = [&](int key) {
-      if (key >= s.keys) return -1;
-      const int page = div_by(key, p.page), id = table[page];
-      return id >= 0 && id < p.P ? id * p.S + (key - page * p.S) : -1;
-    };
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int slot = slot_of(key0 + 16 * b + n);
-      const global_bytes src = slot >= 0 ? rows + (uint32_t)slot * row_stride : zero;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int byte = 64 * i + 16 * j;
-        const u32x4 w = load16((FULL || byte < row_bytes ? src : zero) + byte);
-        if (FP8) {
-          k[b][2 * i] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[0], w[1]));
-          k[b][2 * i + 1] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[2], w[3]));
-        } else {
-          k[b][i] = __builtin_bit_cast(bf16x8, w);
-        }
-      }
-      ks[b] = FP8 && p.scales && slot >= 0 ? p.scales[((size_t)div_by(slot, p.page) * p.Hkv + h) * 2] : 1.f;
-    }
-    float scale[2][4];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) scale[b][r] = FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale;
     const int old = s.keys - s.tokens;  // keys before the step's
-    const int end = s.tokens * p.G;
-    float sum[2][4] = {};
-    for (int base = max(key0 - old, 0) * p.G; base < end; base += 16) {
-      const int row = base + n, token = div_by(min(row, end - 1), p.group), g = row - token * p.G, t = s.first + token;
-      const bool live = row < end;
-      const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + g) * p.q_head;
-      f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // adds x to a key's weight
+    const auto add = [&](int key, float x) {
+      const int page = div_by(key, p.page), id = table[page];
+      if (id < 0 || id >= p.P) return;
+      const size_t to = ((size_t)id * p.Hkv + h) * p.S + (key - page * p.S);
+      if (key >= old) p.positions[to] = (p.dropped ? p.dropped[seq] : 0) + key;
+      else if (p.decay != 0.f) x += p.decay * p.weights[to];
+      p.weights[to] = x;
+    };
+    const bool kept = scores_fit(p, s, score_at);
+    if (kept) {
+      const float2* const stat = p.stats + (size_t)s.first * p.Hkv * p.G + h * p.G;
+      const int key0 = block * kScoreKeys + 4 * tid;  // this thread's four keys
+      if (key0 < s.keys) {
+        const float* from = p.scores + (((size_t)score_at + key0 / 16) * p.Hkv + h) * p.G * 16 + key0 % 16;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int g = 0; g < p.G; ++g) {
+          const f32x4 x = *(const f32x4*)(from + g * 16);
+          const float2 st = stat[g];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int dim = FP8 ? 64 * (i / 2) + 16 * j + 8 * (i % 2) : 32 * i + 8 * j;
-        u32x4 w = {0, 0, 0, 0};
-        if (live && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][i], __builtin_bit_cast(bf16x8, w), sc[b], 0, 0, 0);
-      }
-      const float2 stat = live ? p.stats[(size_t)t * p.Hkv * p.G + h * p.G + g] : float2{0.f, 0.f};
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[b][r] = scaled(sc[b][r], scale[b][r]);
-      if (p.cap != 0.f) cap_scores(sc, p.cap);
-      const int last = live ? old + token : -1;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(sc[b][r] - stat.x);
-          sum[b][r] += key0 + 16 * b + 4 * j + r <= last && stat.y != 0.f ? e * stat.y : 0.f;
+          for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(x[r] - st.x) * st.y;
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (key0 + r < s.keys) add(key0 + r, sum[r]);
+      }
+      continue;
     }
+    // a sequence with one token whose scores did not fit: its block in parts
+    const int first_key = block * (s.tokens == 1 ? kScoreKeys : kKeys);
+    const int end_key = min(s.keys, first_key + (s.tokens == 1 ? kScoreKeys : kKeys));
+    for (int part = first_key; part < end_key; part += kKeys) {
+      const int key0 = part + kWave * wave;
+      const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
+      const auto slot_of = [&](int key) {
+        if (key >= s.keys) return -1;
+        const int page = div_by(key, p.page), id = table[page];
+        return id >= 0 && id < p.P ? id * p.S + (key - page * p.S) : -1;
+      };
+      bf16x8 k[kBlocks][kSteps];
+      float ks[kBlocks];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < kBlocks; ++b) {
+        const int slot = slot_of(key0 + 32 * b + n);
+        const global_bytes src = slot >= 0 ? rows + (uint32_t)slot * row_stride : zero;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        for (int d = 1; d < 16; d *= 2) sum[b][r] += __shfl_xor(sum[b][r], d);
-    // lane n of each j: key n / 4 * 16 ... of the 8 keys a lane has, lane n < 8 writes the n-th
-    if (n < 8) {
-      const int b = n / 4, r = n % 4;
-      float x = 0.f;
+        for (int i = 0; i < kSteps; ++i) {
+          const int dim = 16 * i + 8 * half;
+          const global_bytes from = FULL || dim < p.D ? src : zero;
+          if (FP8) {
+            typedef const __attribute__((address_space(1))) u32x2* global_u32x2;
+            const u32x2 w = *(global_u32x2)(from + dim);
+            k[b][i] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[0], w[1]));
+          } else {
+            k[b][i] = __builtin_bit_cast(bf16x8, load16(from + 2 * dim));
+          }
+        }
+        ks[b] = FP8 && p.scales && slot >= 0 ? p.scales[((size_t)div_by(slot, p.page) * p.Hkv + h) * 2] : 1.f;
+      }
+      const int end_row = s.tokens * p.G, begin_row = max(part - old, 0) * p.G;
+      u32x4 w[kLoads];
+      float2 st = {0.f, 0.f};
+      const auto load = [&](int base) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x = u == n ? sum[u / 4][u % 4] : x;
-      const int key = key0 + 16 * b + 4 * j + r, slot = slot_of(key);
-      if (slot >= 0) {
-        const int page = div_by(slot, p.page);
-        const size_t to = ((size_t)page * p.Hkv + h) * p.S + (slot - page * p.S);
-        if (key >= old) p.positions[to] = (p.dropped ? p.dropped[seq] : 0) + key;
-        else if (p.decay != 0.f) x += p.decay * p.weights[to];
-        p.weights[to] = x;
+        for (int i = 0; i < kLoads; ++i) {
+          constexpr int kChunks = DP * 2 / 16;
+          const int row = base + tid / kChunks + i * (kWeighThreads / kChunks), dim = tid % kChunks * 8;
+          const int token = div_by(min(row, end_row - 1), p.group), g = min(row, end_row - 1) - token * p.G;
+          w[i] = u32x4{0, 0, 0, 0};
+          if (row < end_row && (FULL || dim < p.D))
+            w[i] = *(const u32x4*)(p.q + (s.first + token) * p.q_token + ((long long)h * p.G + g) * p.q_head + dim);
+        }
+        if (tid < kWeighRows) {
+          const int row = base + tid, token = div_by(min(row, end_row - 1), p.group), g = min(row, end_row - 1) - token * p.G;
+          st = row < end_row ? p.stats[(size_t)(s.first + token) * p.Hkv * p.G + h * p.G + g] : float2{0.f, 0.f};
+        }
+      };
+      const auto store = [&](int turn) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          constexpr int kChunks = DP * 2 / 16;
+          *(u32x4*)(s_q[turn & 1] + (tid / kChunks + i * (kWeighThreads / kChunks)) * kRow + tid % kChunks * 16) = w[i];
+        }
+        if (tid < kWeighRows) s_stat[turn & 1][tid] = st;
+      };
+      float sum[kBlocks][16];
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[b][r] = 0.f;
+      __syncthreads();  // the last use of LDS
+      load(begin_row), store(0);
+      __syncthreads();
+      int turn = 0;
+#pragma unroll 1
+      for (int base = begin_row; base < end_row; base += kWeighRows, ++turn) {
+        if (base + kWeighRows < end_row) load(base + kWeighRows);
+        const int first = div_by(base, p.group), last = div_by(min(base + kWeighRows, end_row) - 1, p.group);  // tokens
+        if (key0 <= old + last && key0 < s.keys) {  // uniform
+          const float2 stat = s_stat[turn & 1][n];
+          const bool whole = key0 + kWave - 1 <= old + first && base + kWeighRows <= end_row;
+          const int token = div_by(min(base + n, end_row - 1), p.group), seen = base + n < end_row ? old + token : -1;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            f32x16 sc;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+              const u32x4 x = *(const u32x4*)(s_q[turn & 1] + n * kRow + 32 * i + 16 * half);
+              sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b][i], __builtin_bit_cast(bf16x8, x), sc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              float scale = p.scale;
+              if (FP8) scale *= __shfl(ks[b], 8 * (r / 4) + 4 * half + r % 4);
+              sc[r] = scaled(sc[r], scale);
+            }
+            if (p.cap != 0.f) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sc[r] = scaled(p.cap * tanhf(sc[r] / p.cap), kLog2e);
+            }
+            if (whole) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sum[b][r] += __builtin_amdgcn_exp2f(sc[r] - stat.x) * stat.y;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(sc[r] - stat.x) * stat.y;
+                sum[b][r] += key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= seen ? e : 0.f;
+              }
+            }
+          }
+        }
+        if (base + kWeighRows < end_row) store(turn + 1);
+        __syncthreads();
+      }
+      // over the 32 columns: lane n then has key n's
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        float mine = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = sum[b][r];
+#pragma unroll
+          for (int d = 1; d < 32; d *= 2) x += __shfl_xor(x, d);
+          mine = n == r ? x : mine;
+        }
+        const int key = key0 + 32 * b + 8 * (n / 4) + 4 * half + n % 4;
+        if (n < 16 && key < s.keys) add(key, mine);
       }
     }
   }
@@ -863,7 +972,8 @@ int check_weigh(const rpa_weigh_shape_t* s) {
 
 struct WeighPlan {
   int tiles, rows_grid, tiles_grid, keys_grid;  // tiles_grid 0: rows only
-  size_t stats, parts, bytes;
+  long long score_room;
+  size_t stats, parts, scores, bytes;
 };
 
 constexpr int kRowsGrid = 768, kTilesGrid = 512, kKeysGrid = 2048;
@@ -877,11 +987,15 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const long long work = most(rows, capacity / kBlockKeys + 1);
   r.rows_grid = (int)(work < kRowsGrid ? work : kRowsGrid);
   const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
-  const long long blocks = most(seqs * s.num_kv_heads, capacity / kWeighKeys + 1);
+  const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1);
   r.keys_grid = (int)(blocks < kKeysGrid ? blocks : kKeysGrid);
   r.stats = ((size_t)s.num_tokens * s.num_q_heads * sizeof(float2) + 15) / 16 * 16;
   r.parts = (size_t)r.rows_grid * 2 * (32 + 16 * (size_t)s.head_dim) * 4;
-  r.bytes = r.stats + r.parts;
+  // of sequences with one token: their own keys, and no more than the pool holds
+  const long long pool = (long long)s.total_pages * s.page_size / 16 + seqs, keys = most(seqs, capacity / 16 + 1);
+  r.score_room = pool < keys ? pool : keys;
+  r.scores = (size_t)r.score_room * s.num_q_heads * 64;
+  r.bytes = r.stats + r.parts + r.scores;
   const int group = s.num_q_heads / s.num_kv_heads;
   // sums of tiles' keys stay in 64 bits
   const bool fits = most(4 * ((long long)s.num_tokens * group + group), capacity) < 1ll << 62;
