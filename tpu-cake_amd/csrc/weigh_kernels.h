@@ -62,14 +62,17 @@ __device__ __forceinline__ Sequence sequence_at(const WeighParams& p, int i, boo
 // Where a workgroup's share of all the work begins: sequences in order, `amount(i)` units of work each, the total in
 // shares of equal size.
 struct Share {
+  int index;           // of the shares in order
   long long from, to;  // units
   int seq;             // that `from` lies in
   long long before;    // units of the sequences before it
   long long scores;    // and their blocks of scores
 };
 
-template <typename Amount, typename Scores>
-__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount, Scores scores) {
+// NEAR: XCDs take workgroups in turn; neighbouring shares, which read the same keys, go to one of them.
+template <bool NEAR, typename Amount, typename Scores>
+__device__ __forceinline__ Share share_of(int n, Amount amount, Scores scores) {
+  const int count = gridDim.x;
   __shared__ long long s_sum[kWeighWaves], s_scores[kWeighWaves];
   __shared__ Share s_share;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
@@ -90,7 +93,13 @@ __device__ __forceinline__ Share share_of(int n, int index, int count, Amount am
     upto += w < wave ? s_sum[w] : 0, stored += w < wave ? s_scores[w] : 0;
     total += s_sum[w];
   }
-  const long long each_share = (total + count - 1) / count, from = min(index * each_share, total);
+  const long long each_share = (total + count - 1) / count;
+  int index = blockIdx.x;
+  if (NEAR && total) {
+    const int used = (int)((total + each_share - 1) / each_share), xcd = index % 8;
+    index = index < used ? xcd * (used / 8) + min(xcd, used % 8) + index / 8 : count;
+  }
+  const long long from = min(index * each_share, total);
   const long long to = min(from + each_share, total);
   long long before = upto - own;
   stored -= mine;
@@ -101,14 +110,14 @@ __device__ __forceinline__ Share share_of(int n, int index, int count, Amount am
       if (from < before + a) break;
       before += a, stored += scores(i);
     }
-    s_share = {from, to, i, before, stored};
+    s_share = {index, from, to, i, before, stored};
   }
   __syncthreads();
-  return from < to ? s_share : Share{0, 0, 0, 0, 0};
+  return from < to ? s_share : Share{0, 0, 0, 0, 0, 0};
 }
-template <typename Amount>
-__device__ __forceinline__ Share share_of(int n, int index, int count, Amount amount) {
-  return share_of(n, index, count, amount, [](int) { return 0ll; });
+template <bool NEAR, typename Amount>
+__device__ __forceinline__ Share share_of(int n, Amount amount) {
+  return share_of<NEAR>(n, amount, [](int) { return 0ll; });
 }
 
 // Scores of a sequence with one token, which its weights take instead of K once more: blocks of 16 keys, of which
@@ -149,8 +158,8 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
   const int count = min(max(*p.num_seqs, 0), p.N);
   const int heads = p.Hkv * p.tiles;
-  const Share share = share_of(
-      count + 1, blockIdx.x, gridDim.x,
+  const Share share = share_of<false>(
+      count + 1,
       [&](int i) {
         const Sequence s = row_sequence(p, count, i);
         return (long long)s.tokens * heads * row_blocks(s);
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(WeighParams p
 // it and began before it.
 __global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(WeighParams p) {
   const int count = min(max(*p.num_seqs, 0), p.N), heads = p.Hkv * p.tiles;
-  const Share share = share_of(count + 1, blockIdx.x, gridDim.x, [&](int i) {
+  const Share share = share_of<false>(count + 1, [&](int i) {
     const Sequence s = row_sequence(p, count, i);
     return (long long)s.tokens * heads * row_blocks(s);
   });
@@ -446,12 +455,6 @@ __device__ __forceinline__ TileOf tile_at(const WeighParams& p, const Sequence& 
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// XCDs take workgroups in turn; neighbouring shares, which read the same keys, go to one of them.
-__device__ __forceinline__ int share_index() {
-  const int per = gridDim.x / 8;
-  return gridDim.x % 8 ? blockIdx.x : blockIdx.x % 8 * per + blockIdx.x / 8;
-}
-
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_kernel(WeighParams p) {
   constexpr int kKeys = DP > 128 ? 32 : 64;  // of a turn
@@ -467,8 +470,8 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
   __shared__ float s_ks[2][kKeys], s_vs[2][kKeys];
   __shared__ int s_bad, s_again;
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
-  const int count = min(max(*p.num_seqs, 0), p.N), index = share_index();
-  const Share share = share_of(count, index, gridDim.x, [&](int i) { return tile_slots(p, sequence_at(p, i)) * p.Hkv; });
+  const int count = min(max(*p.num_seqs, 0), p.N);
+  const Share share = share_of<true>(count, [&](int i) { return tile_slots(p, sequence_at(p, i)) * p.Hkv; });
   if (share.from == share.to) return;
   const int row_bytes = p.D * kElem;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
       }
     };
     const bool own = tile.slot == 0 && end_slot == tile.slots;
-    float* const part = p.tile_parts + (2 * (size_t)index + (at > share.from)) * (kColumns * (2 + (size_t)p.D));
+    float* const part = p.tile_parts + (2 * (size_t)share.index + (at > share.from)) * (kColumns * (2 + (size_t)p.D));
     // The columns' results: those of token `only`, or all (-1).
     const auto write = [&](int only) {
       const float sum = l + __shfl_xor(l, 32);
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
 // Joins the parts of tiles, as weigh_join_kernel those of rows; kColumns / gridDim.y columns a workgroup.
 __global__ __launch_bounds__(kWeighThreads) void weigh_join_tiles_kernel(WeighParams p) {
   const int count = min(max(*p.num_seqs, 0), p.N), index = blockIdx.x;
-  const Share share = share_of(count, index, gridDim.x, [&](int i) { return tile_slots(p, sequence_at(p, i)) * p.Hkv; });
+  const Share share = share_of<false>(count, [&](int i) { return tile_slots(p, sequence_at(p, i)) * p.Hkv; });
   if (share.from == share.to) return;
   const Sequence s = sequence_at(p, share.seq);
   const long long per_head = tile_slots(p, s);
@@ -776,13 +779,13 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
   __shared__ __align__(16) uint8_t s_q[2][kWeighRows * kRow];
   __shared__ float2 s_stat[2][kWeighRows];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
-  const int count = min(max(*p.num_seqs, 0), p.N), index = share_index();
+  const int count = min(max(*p.num_seqs, 0), p.N);
   const auto blocks_of = [&](const Sequence& s) {
     const int keys = s.tokens == 1 ? kScoreKeys : kKeys;
     return s.tokens ? (s.keys + keys - 1) / keys : 0;
   };
-  const Share share = share_of(
-      count, index, gridDim.x, [&](int i) { return (long long)blocks_of(sequence_at(p, i, true)) * p.Hkv; },
+  const Share share = share_of<true>(
+      count, [&](int i) { return (long long)blocks_of(sequence_at(p, i, true)) * p.Hkv; },
       [&](int i) { return score_blocks(sequence_at(p, i)); });
   if (share.from == share.to) return;
   const int row_bytes = p.D * kElem;
