@@ -23,8 +23,13 @@ Divisor divisor(int d) {
 }
 __device__ __forceinline__ int div_by(int v, Divisor d) { return (int)(((uint64_t)(uint32_t)v * d.m) >> d.shift); }
 
+// A load that nothing else will want.
+__device__ __forceinline__ u32x4 load16_once(global_bytes at) {
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)at);
+}
+
 constexpr int kWeighWaves = 4, kWeighThreads = 64 * kWeighWaves;
-constexpr int kBlockKeys = 256;  // keys of a block of rows' work: two units of 32 for each wave
+constexpr int kMostWaves = 8;  // of a workgroup of rows
 
 struct WeighParams {
   const uint16_t* q;
@@ -41,7 +46,10 @@ struct WeighParams {
   long long q_token, q_head;
   int T, Hkv, G, D, P, S, N, PPS;
   int tiles;      // 16-head tiles of a group
+  int near, ways; // rows: kv heads of a workgroup, waves that share a head's keys
+  int block_shift;  // log2 of the keys of a block of rows' work: two units of 32 for each wave of a head
   int rows_grid, tiles_grid;  // workgroups of rows and of tiles
+  int one_page;   // 32 keys from a multiple of 32 on lie in one page
   int quads;      // four neighbouring weights from a multiple of four on are 16 aligned bytes
   int chunk;      // sequences of more than one token are done in tiles
   float* tile_parts;  // of tiles: two for each workgroup, (m, l) of kColumns columns, then their O
@@ -70,10 +78,10 @@ __device__ __forceinline__ bool scores_fit(const WeighParams& p, const Sequence&
 }
 
 // Rows' work: the blocks of keys of a row, and those of all rows of a sequence.
-__device__ __forceinline__ int row_blocks(const Sequence& s) { return max((s.keys + kBlockKeys - 1) / kBlockKeys, 1); }
+__device__ __forceinline__ int row_blocks(const WeighParams& p, const Sequence& s) { return max((s.keys + (1 << p.block_shift) - 1) >> p.block_shift, 1); }
 __device__ __forceinline__ bool in_tiles(const WeighParams& p, const Sequence& s, bool pad) { return p.chunk && s.tokens > 1 && !pad; }
 __device__ __forceinline__ long long row_units(const WeighParams& p, const Sequence& s, bool pad) {
-  return in_tiles(p, s, pad) ? 0 : (long long)s.tokens * p.Hkv * p.tiles * row_blocks(s);
+  return in_tiles(p, s, pad) ? 0 : (long long)s.tokens * (p.Hkv / p.near) * p.tiles * row_blocks(p, s);
 }
 
 // A workgroup's share of all the work: sequences in order, and behind them (`pad`) the tokens past the last one; the
@@ -98,10 +106,10 @@ __device__ __forceinline__ Sequence work_sequence(const WeighParams& p, int coun
 // go to one of them.
 template <bool NEAR, typename Amount>
 __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int blocks, Amount amount, bool flag = false) {
-  __shared__ long long s_sum[3][kWeighWaves];
+  __shared__ long long s_sum[3][kMostWaves];
   __shared__ Share s_share;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, capacity = p.PPS * p.S;
-  const int each = p.N / kWeighThreads + 1, i0 = min(tid * each, p.N + 1), i1 = min(i0 + each, p.N + 1);
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, waves = blockDim.x / 64, capacity = p.PPS * p.S;
+  const int each = p.N / (int)blockDim.x + 1, i0 = min(tid * each, p.N + 1), i1 = min(i0 + each, p.N + 1);
   // the first of this thread's sequences, loaded beside their number
   const int c0 = p.cu[min(i0, p.N)], c1 = p.cu[min(i0 + 1, p.N)], len0 = p.kv_lens[min(i0, p.N - 1)];
   const int count = min(max(*p.num_seqs, 0), p.N);
@@ -133,8 +141,7 @@ __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int b
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 3; ++u)
-#pragma unroll
-    for (int w = 0; w < kWeighWaves; ++w) {
+    for (int w = 0; w < waves; ++w) {
       upto[u] += w < wave ? s_sum[u][w] : 0;
       total[u] += s_sum[u][w];
     }
@@ -158,30 +165,38 @@ __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int b
   return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0};
 }
 
-// Rows: a token's heads, up to 16 of one kv head.  Their keys come in blocks, blocks of all rows in shares, one a
-// workgroup: a long sequence's rows are spread over as many workgroups as their blocks need, and short ones' share a workgroup.
-// A row that a workgroup does not have whole leaves a part: the first in the workgroup's slot 0, the last in slot 1.
+// Rows: a token's heads, up to 16 of one kv head, as the columns of v_mfma_f32_16x16x32_bf16.  A workgroup takes the rows of
+// `near` kv heads, a wave each (where there are few, `ways` waves share a head's keys): a key's rows of all these heads
+// lie together, and the waves walk the same keys.  Keys come in blocks, the blocks of all rows in shares, one a workgroup: a long sequence's rows are spread over as
+// many workgroups as their blocks need, and short ones' share a workgroup.  A row that a workgroup does not have whole leaves a
+// part: the first in the workgroup's slot 0, the last in slot 1.
+//
+// bf16: a wave reads a key's K and V row, which lie together, in whole lines, a unit of 32 keys ahead, and takes both through
+// LDS; fp8 K comes straight into the product's operand, 64 bytes of 16 keys at a time.
 template <int DP, bool FULL, bool FP8>
-__global__ __launch_bounds__(kWeighThreads, DP == 256 ? (FP8 ? 2 : 1) : DP > 64 ? 3 : 4) void weigh_rows_kernel(WeighParams p) {
-  constexpr int kRow = DP * 2 + 32;
-  constexpr int kWave = 32 * kRow;
+__global__ __launch_bounds__(DP == 256 && !FP8 ? 256 : 64 * kMostWaves, DP == 256 && !FP8 ? 1 : DP == 64 ? 4 : 2) void weigh_rows_kernel(WeighParams p) {
+  constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;
+  constexpr int kV = FP8 ? 0 : 32 * kKRow;             // V behind K
+  constexpr int kWave = kV + 32 * kVRow;               // a wave's LDS; later its 16 rows of O in fp32
   constexpr int kORow = DP + 4;
   constexpr int kElem = FP8 ? 1 : 2;
-  constexpr int kLoads = DP * kElem / 64;
   constexpr int kSteps = DP / 32;
-  static_assert(16 * kORow * 4 <= kWave, "O rows fit the wave's V region");
-  __shared__ __align__(16) uint8_t s_v[kWeighWaves * kWave];
-  __shared__ float s_m[kWeighWaves][16], s_l[kWeighWaves][16];
+  constexpr int kChunks = DP / 4, kApart = 64 / kChunks, kLoads = 32 / kApart;  // bf16: chunks of a key, keys of a load
+  constexpr int kCodes = DP / 64;                      // fp8: loads of a lane for a key row's K (or V)
+  constexpr int kSets = FP8 ? 2 : 1;
+  static_assert(16 * kORow * 4 <= kWave, "O rows fit the wave's region");
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ float s_m[kMostWaves][16], s_l[kMostWaves][16];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
-  const int heads = p.Hkv * p.tiles;
+  const int threads = blockDim.x, groups = p.Hkv / p.near;
   const Share share =
       share_of<false>(p, blockIdx.x, gridDim.x, [&](const Sequence& s, bool pad) { return row_units(p, s, pad); });
   if (share.from == share.to) return;
 
-  const int row_bytes = p.D * kElem;
+  const int row_bytes = p.D * kElem, mine = wave % p.near, way = wave / p.near;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
   const global_bytes zero = zero_row();
-  uint8_t* const tile_v = s_v + wave * kWave;
+  uint8_t* const own_lds = lds + wave * kWave;
   const int count = share.count;
   int seq = share.seq;
   Sequence s = share.s;
@@ -192,12 +207,12 @@ __global__ __launch_bounds__(kWeighThreads, DP == 256 ? (FP8 ? 2 : 1) : DP > 64 
       score_at += seq < count ? score_blocks(s) : 0;
       s = work_sequence(p, count, ++seq);
     }
-    const int blocks = row_blocks(s);
+    const int blocks = row_blocks(p, s);
     const long long row = (at - before) / blocks;
     const int first_block = (int)(at - before - row * blocks);
     const int end_block = (int)min((long long)blocks, first_block + (share.to - at));
-    const int token = (int)(row / heads), head_tile = (int)(row - (long long)token * heads), h = head_tile / p.tiles;
-    const int tile = head_tile - h * p.tiles, t = s.first + token;
+    const int token = (int)(row / (groups * p.tiles)), group_tile = (int)(row - (long long)token * (groups * p.tiles));
+    const int h = group_tile / p.tiles * p.near + mine, tile = group_tile % p.tiles, t = s.first + token;
     const int keys = max(s.keys - (s.tokens - 1 - token), 0);
     const bool known = seq < count;
     const int32_t* const table = p.table + (size_t)(known ? seq : 0) * p.PPS;
@@ -215,97 +230,137 @@ __global__ __launch_bounds__(kWeighThreads, DP == 256 ? (FP8 ? 2 : 1) : DP > 64 
       }
     }
     const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
-    const int end_key = min(keys, end_block * kBlockKeys), end_unit = (end_key + 31) / 32;
+    const int end_key = (int)min((long long)keys, (long long)end_block << p.block_shift), end_unit = (end_key + 31) / 32;
     const bool keep = known && scores_fit(p, s, score_at);
-    float* const scores = p.scores + ((size_t)score_at * p.Hkv + h) * p.G * 16 + (tile * 16 + n) * 16 + 4 * j;
-    int ids[2];  // the pages of key n and n + 16 of a unit: found a turn before its keys are loaded
-    u32x4 k[2][kLoads], v[2][kLoads];
-    uint32_t seen[2];
-    float ks[2], vs[2];  // fp8: the scales of key n of the 16
-    const auto find = [&](int unit) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int key = unit * 32 + 16 * b + n;
-        ids[b] = key < end_key ? table[div_by(key, p.page)] : -1;
-      }
+    float* const scores = p.scores + ((size_t)score_at * p.Hkv + h) * p.G * 16;
+    // Loads in flight: of bf16 the unit after the one in LDS, of fp8 (half the bytes) two units.
+    struct {
+      u32x4 w[FP8 ? 4 * kCodes : kLoads];
+      int id;            // the page of key lane % 32, found before the set's last unit was loaded
+      uint32_t seen;     // which keys of the loaded unit exist
+      float ks, vs;      // fp8: the scales of key lane % 32
+    } set[kSets];
+    const auto find = [&](int x, int unit) {
+      const int key = max(min(unit * 32 + lane % 32, end_key - 1), 0);
+      set[x].id = table[div_by(key, p.page)];
     };
-    const auto load = [&](int unit) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int key = unit * 32 + 16 * b + n, id = ids[b];
-        const bool ok = key < end_key && id >= 0 && id < p.P;
-        if (key < end_key && !ok) flag_error(RPA_SPARSE_ERR_PAGE);
-        seen[b] = (uint32_t)__ballot(ok) & 0xffffu;
-        const int slot = ok ? id * p.S + (key - div_by(key, p.page) * p.S) : 0;
-        const global_bytes src = ok ? rows + (uint32_t)slot * row_stride : zero;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int byte = 64 * i + 16 * j;
-          const global_bytes from = FULL || byte < row_bytes ? src : zero;
-          k[b][i] = load16(from + byte);
-          v[b][i] = load16(from + row_bytes + byte);
+    const auto load = [&](int x, int unit) {
+      const int key = unit * 32 + lane % 32, id = set[x].id;
+      u32x4* const w = set[x].w;
+      const bool ok = key < end_key && id >= 0 && id < p.P;
+      if (key < end_key && !ok) flag_error(RPA_SPARSE_ERR_PAGE);
+      const int slot = ok ? id * p.S + (key - div_by(key, p.page) * p.S) : -1;
+      const uint32_t seen = set[x].seen = (uint32_t)__ballot(ok);
+      if (FP8) {
+        if (p.scales) {
+          const float2 scale = *(const float2*)(p.scales + ((size_t)(ok ? id : 0) * p.Hkv + h) * 2);
+          set[x].ks = ok ? scale.x : 1.f, set[x].vs = ok ? scale.y : 1.f;
+        } else {
+          set[x].ks = set[x].vs = 1.f;
         }
-        if (FP8) {
-          const float* scale = p.scales && ok ? p.scales + ((size_t)id * p.Hkv + h) * 2 : nullptr;
-          ks[b] = scale ? scale[0] : 1.f, vs[b] = scale ? scale[1] : 1.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int at_slot = __shfl(slot, 16 * b + n);
+          const global_bytes src = at_slot >= 0 ? rows + (uint32_t)at_slot * row_stride : zero;
+#pragma unroll
+          for (int i = 0; i < kCodes; ++i) {
+            const int byte = 64 * i + 16 * j;
+            const global_bytes from = FULL || byte < row_bytes ? src : zero;
+            w[2 * kCodes * b + i] = load16_once(from + byte);
+            w[2 * kCodes * b + kCodes + i] = load16_once(from + row_bytes + byte);
+          }
+        }
+      } else {
+        const int c = lane % kChunks, part = c >= kChunks / 2, byte = 16 * (c - part * (kChunks / 2));
+        const bool inside = FULL || byte < row_bytes;
+        if (p.one_page && seen == 0xffffffffu) {  // uniform: 32 keys that lie together
+          const global_bytes src = rows + (uint32_t)__builtin_amdgcn_readfirstlane(slot) * row_stride;
+          const uint32_t off = (uint32_t)(lane / kChunks) * (uint32_t)row_stride + part * row_bytes + byte;
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i)
+            w[i] = load16_once(inside ? src + (uint64_t)(i * kApart) * row_stride + off : zero + byte);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int at_slot = __shfl(slot, kApart * i + lane / kChunks);
+            w[i] = load16_once(inside && at_slot >= 0 ? rows + (uint32_t)at_slot * row_stride + part * row_bytes + byte : zero + byte);
+          }
         }
       }
-      if (unit + kWeighWaves < end_unit) find(unit + kWeighWaves);
+      find(x, unit + kSets * p.ways);
+    };
+    const auto store = [&] {  // bf16: the loaded unit's K and V
+      const int c = lane % kChunks, part = c >= kChunks / 2;
+      uint8_t* const dst = own_lds + (part ? kV + lane / kChunks * kVRow + 16 * (c - kChunks / 2) : lane / kChunks * kKRow + 16 * c);
+      const int step = kApart * (part ? kVRow : kKRow);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) *(u32x4*)(dst + i * step) = set[0].w[i];
     };
     f32x4 o[DP / 16];
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kLowest, l = 0.f;
-    int unit = first_block * (kBlockKeys / 32) + wave;
-    if (unit < end_unit) find(unit), load(unit);
-    for (; unit < end_unit; unit += kWeighWaves) {
+    uint32_t here = 0;
+    // One unit's keys, of fp8 those in set x; its loads' successors leave in between.
+    const auto take = [&](int x, int unit) {
       f32x4 sc[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         sc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-          const u32x4 a = FP8 ? bf16_of_codes(k[b][i / 2][2 * (i % 2)], k[b][i / 2][2 * (i % 2) + 1]) : k[b][FP8 ? 0 : i];
+          u32x4 a;
+          if (FP8) a = bf16_of_codes(set[x].w[2 * kCodes * b + i / 2][2 * (i % 2)], set[x].w[2 * kCodes * b + i / 2][2 * (i % 2) + 1]);
+          else a = *(const u32x4*)(own_lds + (16 * b + n) * kKRow + 64 * i + 16 * j);
           sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), q[i], sc[b], 0, 0, 0);
         }
       }
-      wave_fence();  // the last unit's V has been read
+      // Scores leave after the loads of the next unit, by buffer stores, which drop what lies past their end (heads that are
+      // none, or all of it): no branch, so the compiler knows that they follow the loads and waits for those alone.
+      const auto keep_scores = [&] {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          uint8_t* dst = tile_v + (16 * b + n) * kRow + (FP8 ? 128 * i + 32 * j : 64 * i + 16 * j);
-          if (FP8) {
-            *(u32x4*)dst = bf16_of_codes(v[b][i][0], v[b][i][1]);
-            *(u32x4*)(dst + 16) = bf16_of_codes(v[b][i][2], v[b][i][3]);
-          } else {
-            *(u32x4*)dst = v[b][i];
-          }
+        for (int b = 0; b < 2; ++b) {
+          const bool write = keep && unit * 32 + 16 * b < end_key;  // uniform
+          const auto to = __builtin_amdgcn_make_buffer_rsrc(scores + (size_t)(2 * unit + b) * p.Hkv * p.G * 16, 0,
+                                                            write ? p.G * 64 : 0, 0x00027000);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sc[b]), to, (tile * 16 + n) * 64 + 16 * j, 0, 0);
         }
-      wave_fence();
-      const bool whole = (seen[0] & seen[1]) == 0xffffu;
-      const uint32_t here[2] = {seen[0] >> (4 * j), seen[1] >> (4 * j)};
+      };
       float vk[2][4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sc[b][r] = scaled(sc[b][r], FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale);
-          vk[b][r] = FP8 ? __shfl(vs[b], 4 * j + r) : 1.f;
-        }
-      if (unit + kWeighWaves < end_unit) load(unit + kWeighWaves);
-      if (p.cap != 0.f) cap_scores(sc, p.cap);
-      if (!whole) {
+      if (FP8) {
+        here = set[x].seen;
+        wave_fence();  // the last unit's V has been read
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[b][r] = here[b] >> r & 1 ? sc[b][r] : -__builtin_inff();
+          for (int i = 0; i < kCodes; ++i) {
+            uint8_t* dst = own_lds + (16 * b + n) * kVRow + 128 * i + 32 * j;
+            const u32x4 y = set[x].w[2 * kCodes * b + kCodes + i];
+            *(u32x4*)dst = bf16_of_codes(y[0], y[1]);
+            *(u32x4*)(dst + 16) = bf16_of_codes(y[2], y[3]);
+          }
+        wave_fence();
+        const float ks = set[x].ks, vs = set[x].vs;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            sc[b][r] = scaled(sc[b][r], p.scale * __shfl(ks, 16 * b + 4 * j + r));
+            vk[b][r] = __shfl(vs, 16 * b + 4 * j + r);
+          }
+        if (unit + kSets * p.ways < end_unit) load(x, unit + kSets * p.ways);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[b][r] = scaled(sc[b][r], p.scale);
       }
-      if (keep) {  // uniform
+      if (p.cap != 0.f) cap_scores(sc, p.cap);
+      if (here != 0xffffffffu) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          if (tile * 16 + n < p.G && unit * 32 + 16 * b < end_key)
-            *(f32x4*)(scores + (size_t)(2 * unit + b) * p.Hkv * p.G * 16) = sc[b];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[b][r] = here >> (16 * b + 4 * j + r) & 1 ? sc[b][r] : -__builtin_inff();
       }
       float top = max_of(max_of(max_of(sc[0][0], sc[0][1]), max_of(sc[0][2], sc[0][3])),
                          max_of(max_of(sc[1][0], sc[1][1]), max_of(sc[1][2], sc[1][3])));
@@ -331,57 +386,112 @@ __global__ __launch_bounds__(kWeighThreads, DP == 256 ? (FP8 ? 2 : 1) : DP > 64 
 #pragma unroll
         for (int i = 0; i < 3; ++i) parts[i][2 * b] = lo.of[i], parts[i][2 * b + 1] = hi.of[i];
       }
+      if (FP8) keep_scores();
       typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
-      const uint8_t* vt = tile_v + (4 * j + n / 4) * kRow + 8 * (n % 4);
+      const uint8_t* vt = own_lds + kV + (4 * j + n / 4) * kVRow + 8 * (n % 4);
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 32 * d));
-        const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kRow + 32 * d));
+        const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vt + 16 * kVRow + 32 * d));
         const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int i = 0; i < 3; ++i)
           o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, parts[i]), o[d], 0, 0, 0);
       }
+      if (!FP8) {
+        if (unit + p.ways < end_unit) {
+          wave_fence();
+          here = set[0].seen;
+          store();
+          if (unit + 2 * p.ways < end_unit) load(0, unit + 2 * p.ways);
+        }
+        keep_scores();
+      }
+    };
+    const int first_unit = first_block << (p.block_shift - 5);
+    int unit = first_unit + way;
+#pragma unroll
+    for (int x = 0; x < kSets; ++x) find(x, unit + x * p.ways);
+    // Waited for on every path into the loop, and the queries, loaded before, with them: on one where the compiler saw the
+    // queries still under way, every turn would wait for all that is.
+#pragma unroll
+    for (int x = 0; x < kSets; ++x) asm volatile("" : "+v"(set[x].id));
+#pragma unroll
+    for (int x = 0; x < kSets; ++x)
+      if (unit + x * p.ways < end_unit) load(x, unit + x * p.ways);
+    if (!FP8 && unit < end_unit) {
+      wave_fence();
+      here = set[0].seen;
+      store();
+      if (unit + p.ways < end_unit) load(0, unit + p.ways);
     }
+    if (!FP8) {
+      const auto none = __builtin_amdgcn_make_buffer_rsrc(scores, 0, 0, 0x00027000);
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, none, 0, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, none, 16, 0, 0);
+    }
+    for (; unit < end_unit; unit += kSets * p.ways)
+#pragma unroll
+      for (int x = 0; x < kSets; ++x)
+        if (unit + x * p.ways < end_unit) take(x, unit + x * p.ways);
 
-    // join the waves
-    l = swap_sum(l);
-    if (j == 0) s_m[wave][n] = m, s_l[wave][n] = l;
-    __syncthreads();  // every wave is done with its V, too
-    float all = s_m[0][n];
-#pragma unroll
-    for (int w = 1; w < kWeighWaves; ++w) all = fmaxf(all, s_m[w][n]);
-    const float f = __builtin_amdgcn_exp2f(m - all);
-    float* const mine = (float*)tile_v + n * kORow;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) *(f32x4*)(mine + 16 * d + 4 * j) = o[d] * f;
-    __syncthreads();
     const bool own = first_block == 0 && end_block == blocks;
-    const int live = min(p.G - tile * 16, 16), quads = p.D / 4;
-    float* const part = p.parts + (2 * (size_t)blockIdx.x + (at > share.from)) * (32 + 16 * (size_t)p.D);
-    for (int i = tid; i < live * quads; i += kWeighThreads) {
-      const int r = i / quads, d = i % quads * 4;
-      float top = s_m[0][r], sum = 0.f;
+    const int live = min(p.G - tile * 16, 16);
+    float* const part = p.parts + ((2 * (size_t)blockIdx.x + (at > share.from)) * p.near) * (32 + 16 * (size_t)p.D);
+    l = swap_sum(l);
+    if (p.ways == 1) {  // the wave has all of the row
+      if (n < live) {
+        float* const to = part + mine * (32 + 16 * (size_t)p.D);
+        const size_t to_row = (size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + n;
+        const float g = l == 0.f ? 0.f : p.v_scale / l;
+        if (j == 0 && own) p.stats[to_row] = {m, l == 0.f ? 0.f : 1.f / l};
+        if (j == 0 && !own) to[2 * n] = m, to[2 * n + 1] = l;
 #pragma unroll
-      for (int w = 1; w < kWeighWaves; ++w) top = fmaxf(top, s_m[w][r]);
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < DP / 16; ++d) {
+          const int dim = 16 * d + 4 * j;
+          if (!FULL && dim >= p.D) break;
+          if (own)
+            *(u32x2*)(p.out + to_row * p.D + dim) =
+                l == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(o[d][0] * g, o[d][1] * g), pack_bf16(o[d][2] * g, o[d][3] * g)};
+          else
+            *(f32x4*)(to + 32 + n * p.D + dim) = o[d];
+        }
+      }
+    } else {
+      if (j == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+      __syncthreads();  // every wave is done with its V, too
+      float all = kLowest;
+      for (int x = 0; x < p.ways; ++x) all = fmaxf(all, s_m[x * p.near + mine][n]);
+      const float f = __builtin_amdgcn_exp2f(m - all);
+      float* const rows_o = (float*)own_lds + n * kORow;
 #pragma unroll
-      for (int w = 0; w < kWeighWaves; ++w) {
-        sum += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
-        x += *(const f32x4*)((const float*)(s_v + w * kWave) + r * kORow + d);
+      for (int d = 0; d < DP / 16; ++d) *(f32x4*)(rows_o + 16 * d + 4 * j) = o[d] * f;
+      __syncthreads();
+      const int quads = p.D / 4;
+      for (int i = tid; i < p.near * live * quads; i += threads) {
+        const int head = i / (live * quads), r = (i - head * live * quads) / quads, d = i % quads * 4;
+        float top = kLowest, sum = 0.f;
+        for (int x = 0; x < p.ways; ++x) top = fmaxf(top, s_m[x * p.near + head][r]);
+        f32x4 x4 = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < p.ways; ++x) {
+          const int from = x * p.near + head;
+          sum += s_l[from][r] * __builtin_amdgcn_exp2f(s_m[from][r] - top);
+          x4 += *(const f32x4*)((const float*)(lds + from * kWave) + r * kORow + d);
+        }
+        if (!own) {
+          float* const to = part + head * (32 + 16 * (size_t)p.D);
+          if (d == 0) to[2 * r] = top, to[2 * r + 1] = sum;
+          *(f32x4*)(to + 32 + r * p.D + d) = x4;
+          continue;
+        }
+        const size_t to_row = (size_t)t * p.Hkv * p.G + (h - mine + head) * p.G + tile * 16 + r;
+        const float g = sum == 0.f ? 0.f : p.v_scale / sum;
+        if (d == 0) p.stats[to_row] = {top, sum == 0.f ? 0.f : 1.f / sum};
+        *(u32x2*)(p.out + to_row * p.D + d) =
+            sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x4[0] * g, x4[1] * g), pack_bf16(x4[2] * g, x4[3] * g)};
       }
-      if (!own) {
-        if (d == 0) part[2 * r] = top, part[2 * r + 1] = sum;
-        *(f32x4*)(part + 32 + r * p.D + d) = x;
-        continue;
-      }
-      const size_t to = (size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r;
-      const float g = sum == 0.f ? 0.f : p.v_scale / sum;
-      if (d == 0) p.stats[to] = {top, sum == 0.f ? 0.f : 1.f / sum};
-      *(u32x2*)(p.out + to * p.D + d) =
-          sum == 0.f ? u32x2{0, 0} : u32x2{pack_bf16(x[0] * g, x[1] * g), pack_bf16(x[2] * g, x[3] * g)};
+      __syncthreads();  // the next row's LDS
     }
-    __syncthreads();  // the next row's V
     at += end_block - first_block;
   }
 }
@@ -397,34 +507,39 @@ __device__ __forceinline__ RowParts row_parts(const WeighParams& p, long long to
   const int first = (int)(begin / each);
   return {first, (int)((begin + blocks - 1) / each), begin != first * each};
 }
-__device__ __forceinline__ const float* row_part(const WeighParams& p, const RowParts& r, int w) {
-  return p.parts + (2 * (size_t)w + (w == r.first && r.late)) * (32 + 16 * (size_t)p.D);
+// head: of the `near` ones
+__device__ __forceinline__ const float* row_part(const WeighParams& p, const RowParts& r, int w, int head) {
+  return p.parts + ((2 * (size_t)w + (w == r.first && r.late)) * p.near + head) * (32 + 16 * (size_t)p.D);
 }
 
-// Joins a row's parts: the workgroup of the share that the row ends in, if it began before it.
+// Joins a row's parts, for the share that the row ends in, if it began before it: a workgroup a kv head.  Four dims of a
+// head are a thread's, or, of many parts, 8 threads', a share of the parts each.
 __device__ __forceinline__ void join_rows(const WeighParams& p, int block) {
-  constexpr int kParts = 8;
-  const Share share = share_of<false>(p, block, p.rows_grid, [&](const Sequence& s, bool pad) { return row_units(p, s, pad); });
+  constexpr int kParts = 4;
+  const int head = block % p.near;
+  const Share share =
+      share_of<false>(p, block / p.near, p.rows_grid, [&](const Sequence& s, bool pad) { return row_units(p, s, pad); });
   if (share.from == share.to) return;
   const Sequence s = share.s;
-  const int blocks = row_blocks(s), heads = p.Hkv * p.tiles;
+  const int blocks = row_blocks(p, s), groups = p.Hkv / p.near;
   const long long row = (share.from - share.before) / blocks, begin = share.before + row * blocks;
   if (begin == share.from || begin + blocks > share.to) return;  // uniform
   const RowParts parts = row_parts(p, share.row_total, begin, blocks);
-  const int token = (int)(row / heads), head_tile = (int)(row - (long long)token * heads), h = head_tile / p.tiles;
-  const int tile = head_tile - h * p.tiles, t = s.first + token;
-  const int live = min(p.G - tile * 16, 16), quads = p.D / 4;
-  for (int i = threadIdx.x; i < live * quads; i += kWeighThreads) {
+  const int token = (int)(row / (groups * p.tiles)), group_tile = (int)(row - (long long)token * (groups * p.tiles));
+  const int h = group_tile / p.tiles * p.near + head, tile = group_tile % p.tiles, t = s.first + token;
+  const int live = min(p.G - tile * 16, 16), quads = p.D / 4, lanes = parts.last - parts.first > 8 ? 8 : 1;
+  for (int i0 = 0; i0 < live * quads; i0 += kWeighThreads / lanes) {
+    const int i = min(i0 + (int)threadIdx.x / lanes, live * quads - 1), lane = threadIdx.x % lanes;
     const int r = i / quads, d = i % quads * 4;
     float top = kLowest, sum = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int w = parts.first; w <= parts.last; w += kParts) {
+    for (int w = parts.first + lane; w <= parts.last; w += kParts * lanes) {
       float m[kParts], l[kParts];
       f32x4 o[kParts];
 #pragma unroll
       for (int u = 0; u < kParts; ++u) {
-        const float* part = row_part(p, parts, min(w + u, parts.last));
-        m[u] = part[2 * r], l[u] = w + u <= parts.last ? part[2 * r + 1] : 0.f;
+        const float* part = row_part(p, parts, min(w + u * lanes, parts.last), head);
+        m[u] = part[2 * r], l[u] = w + u * lanes <= parts.last ? part[2 * r + 1] : 0.f;
         o[u] = *(const f32x4*)(part + 32 + r * p.D + d);
       }
 #pragma unroll
@@ -436,6 +551,18 @@ __device__ __forceinline__ void join_rows(const WeighParams& p, int block) {
         x = x * mine + o[u] * its;
       }
     }
+    for (int e = 1; e < lanes; e *= 2) {
+      const float m = __shfl_xor(top, e), l = __shfl_xor(sum, e);
+      f32x4 o;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = __shfl_xor(x[u], e);
+      const float next = fmaxf(top, m), mine = __builtin_amdgcn_exp2f(top - next), its = __builtin_amdgcn_exp2f(m - next);
+      top = next;
+      // a side without keys has no O
+      sum = sum * mine + l * its;
+      x = (sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * mine + o * its);
+    }
+    if (lane || i0 + (int)threadIdx.x / lanes >= live * quads) continue;
     const size_t to = (size_t)t * p.Hkv * p.G + h * p.G + tile * 16 + r;
     const float g = sum == 0.f ? 0.f : p.v_scale / sum;
     *(u32x2*)(p.out + to * p.D + d) =
@@ -457,14 +584,14 @@ __device__ __forceinline__ void add_weight(const WeighParams& p, int seq, int h,
 // parts, by `lanes` neighbouring lanes (a power of two), each a share of them.
 __device__ __forceinline__ float2 row_stat(const WeighParams& p, const Share& share, const Sequence& s, long long rows_before, int token,
                                            int h, int g, int lane, int lanes) {
-  const int blocks = row_blocks(s);
-  const long long begin = rows_before + (((long long)token * p.Hkv + h) * p.tiles + g / 16) * blocks;
+  const int blocks = row_blocks(p, s);
+  const long long begin = rows_before + (((long long)token * (p.Hkv / p.near) + h / p.near) * p.tiles + g / 16) * blocks;
   const RowParts parts = row_parts(p, share.row_total, begin, blocks);
   if (parts.first == parts.last) return p.stats[(size_t)(s.first + token) * p.Hkv * p.G + h * p.G + g];
   float top = kLowest, sum = 0.f;
 #pragma unroll 4
   for (int w = parts.first + lane; w <= parts.last; w += lanes) {
-    const float* part = row_part(p, parts, w) + 2 * (g % 16);
+    const float* part = row_part(p, parts, w, h % p.near) + 2 * (g % 16);
     const float m = part[0], l = part[1];
     const float next = l == 0.f ? top : fmaxf(top, m);
     sum = sum * __builtin_amdgcn_exp2f(top - next) + (l == 0.f ? 0.f : l * __builtin_amdgcn_exp2f(m - next));

@@ -9,12 +9,12 @@ namespace {
 // Prompt chunks: tiles of kColumns columns, the (token, head) rows of one sequence and kv head in order, 32 a wave, on
 // v_mfma_f32_32x32x16_bf16: S = K Q^T (32 keys x 32 columns), O^T += V^T P^T.  A tile's keys pass through LDS once for
 // its four waves, two buffers in turn.  A lane's scores are the keys its P operand needs, as in rows.  Tiles' keys come in
-// slots of about kBlockKeys, slots in shares, as blocks of rows do.
-constexpr int kColumns = 128;
+// slots of about kSlotKeys, slots in shares, as blocks of rows do.
+constexpr int kColumns = 128, kSlotKeys = 256;
 
 // Slots of a (sequence, head)'s first j tiles, by the keys that the tiles see: old + kColumns (j' + 1) / G each.
 __device__ __forceinline__ long long slots_before(const WeighParams& p, int old, long long j) {
-  return j + (2 * j * old * p.G + kColumns * j * (j + 1)) / (2 * kBlockKeys * p.G);
+  return j + (2 * j * old * p.G + kColumns * j * (j + 1)) / (2 * kSlotKeys * p.G);
 }
 __device__ __forceinline__ long long tiles_of(const WeighParams& p, const Sequence& s) {
   return ((long long)s.tokens * p.G + kColumns - 1) / kColumns;
@@ -370,10 +370,10 @@ __device__ __forceinline__ void join_tiles(const WeighParams& p, int block) {
 // What follows rows and tiles, one launch: the joins, and the weights of the sequences that rows did.
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams p) {
-  const int block = blockIdx.x, weigh = gridDim.x - p.rows_grid - p.tiles_grid * kJoinTiles;
+  const int block = blockIdx.x, rows = p.rows_grid * p.near, weigh = gridDim.x - rows - p.tiles_grid * kJoinTiles;
   if (block < weigh) weigh_rows<DP, FULL, FP8>(p, block, weigh);
-  else if (block < weigh + p.rows_grid) join_rows(p, block - weigh);
-  else join_tiles(p, block - weigh - p.rows_grid);
+  else if (block < weigh + rows) join_rows(p, block - weigh);
+  else join_tiles(p, block - weigh - rows);
 }
 
 // The weights of the sequences that tiles did, kKeys keys of a kv head at a time, 64 a wave, whose K stays in registers
@@ -547,7 +547,8 @@ int check_weigh(const rpa_weigh_shape_t* s) {
 }
 
 struct WeighPlan {
-  int tiles, rows_grid, tiles_grid, weigh_grid, keys_grid;  // tiles_grid 0: rows only
+  int tiles, near, ways, block_shift, rows_grid, tiles_grid, weigh_grid, keys_grid;  // tiles_grid 0: rows only
+  size_t rows_lds;
   long long score_room;
   size_t stats, parts, scores, bytes;
 };
@@ -560,16 +561,25 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const auto most = [](long long a, long long b) { return a > 0 && b > LLONG_MAX / a ? LLONG_MAX : a * b; };
   const long long capacity = (long long)s.pages_per_seq * s.page_size;
   const long long rows = (long long)s.num_tokens * s.num_kv_heads * r.tiles;
-  const long long work = most(rows, capacity / kBlockKeys + 1);
-  // as many workgroups as the card holds at once, by the registers of a row
-  const long long most_rows = s.head_dim <= 64 ? 1024 : s.head_dim <= 128 ? 768 : s.kv_dtype == RPA_KV_BF16 ? 256 : 512;
-  r.rows_grid = (int)(work < most_rows ? work : most_rows);
+  // rows: the waves of a workgroup, as many as its LDS takes, over neighbouring kv heads, then over a head's keys
+  const bool fp8 = s.kv_dtype == RPA_KV_FP8_E4M3;
+  const int dims = s.head_dim <= 64 ? 64 : s.head_dim <= 128 ? 128 : 256, waves = dims == 256 && !fp8 ? 4 : kMostWaves;
+  r.near = waves;
+  while (s.num_kv_heads % r.near) --r.near;
+  r.ways = 1;
+  while (2 * r.ways * r.near <= waves) r.ways *= 2;
+  r.block_shift = 6;
+  while ((1 << r.block_shift) < 64 * r.ways) ++r.block_shift;
+  r.rows_lds = (size_t)r.near * r.ways * 32 * (dims * 2 + 32 + (fp8 ? 0 : dims * 2 + 16));
+  // as many workgroups as the card holds at once
+  const long long work = most(rows / r.near, (capacity >> r.block_shift) + 1), fill_rows = dims == 64 ? 512 : 256;
+  r.rows_grid = (int)(work < fill_rows ? work : fill_rows);
   const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
   const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1);
   r.keys_grid = (int)(blocks < kKeysGrid ? blocks : kKeysGrid);
   r.weigh_grid = (int)(blocks < kWeighGrid ? blocks : kWeighGrid);
   r.stats = ((size_t)s.num_tokens * s.num_q_heads * sizeof(float2) + 15) / 16 * 16;
-  r.parts = (size_t)r.rows_grid * 2 * (32 + 16 * (size_t)s.head_dim) * 4;
+  r.parts = (size_t)r.rows_grid * 2 * r.near * (32 + 16 * (size_t)s.head_dim) * 4;
   // of sequences with one token: their own keys, and no more than the pool holds
   const long long pool = (long long)s.total_pages * s.page_size / 16 + seqs, keys = most(seqs, capacity / 16 + 1);
   r.score_room = pool < keys ? pool : keys;
@@ -580,7 +590,7 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const bool fits = most(4 * ((long long)s.num_tokens * group + group), capacity) < 1ll << 62;
   if (s.num_tokens > 2 * s.max_num_seqs && fits) {
     const long long tiles = ((long long)s.num_tokens * group + kColumns - 1) / kColumns + seqs;
-    const long long slots = most(tiles * s.num_kv_heads, capacity / kBlockKeys + 2), fill = s.head_dim > 128 ? 256 : kTilesGrid;
+    const long long slots = most(tiles * s.num_kv_heads, capacity / kSlotKeys + 2), fill = s.head_dim > 128 ? 256 : kTilesGrid;
     r.tiles_grid = (int)(slots < fill ? slots : fill);
     r.bytes += (size_t)r.tiles_grid * 2 * kColumns * (2 + (size_t)s.head_dim) * 4;
   }
@@ -589,7 +599,7 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
 
 template <int DP, bool FULL, bool FP8>
 int launch_weigh(const WeighPlan& plan, const WeighParams& p, hipStream_t stream) {
-  weigh_rows_kernel<DP, FULL, FP8><<<plan.rows_grid, kWeighThreads, 0, stream>>>(p);
+  weigh_rows_kernel<DP, FULL, FP8><<<plan.rows_grid, 64 * plan.near * plan.ways, plan.rows_lds, stream>>>(p);
   int rc = launched("weighed_attention");
   if (rc) return rc;
   if (plan.tiles_grid) {
@@ -598,7 +608,7 @@ int launch_weigh(const WeighPlan& plan, const WeighParams& p, hipStream_t stream
     if ((rc = launched("weighed_attention (tiles)"))) return rc;
   }
   weigh_finish_kernel<DP, FULL, FP8>
-      <<<plan.weigh_grid + plan.rows_grid + plan.tiles_grid * kJoinTiles, kWeighThreads, 0, stream>>>(p);
+      <<<plan.weigh_grid + plan.rows_grid * plan.near + plan.tiles_grid * kJoinTiles, kWeighThreads, 0, stream>>>(p);
   if ((rc = launched("weighed_attention (finish)")) || !plan.tiles_grid) return rc;
   weigh_keys_kernel<DP, FULL, FP8><<<plan.keys_grid, kWeighThreads, 0, stream>>>(p);
   return launched("weighed_attention (keys)");
