@@ -151,6 +151,7 @@ int rpa_weighed_attention(const rpa_weigh_shape_t* shape, const rpa_weigh_option
   p.P = s.total_pages, p.S = s.page_size, p.N = s.max_num_seqs, p.PPS = s.pages_per_seq;
   p.near = plan.near, p.ways = plan.ways, p.block_shift = plan.block_shift, p.one_page = s.page_size % 32 == 0;
   p.rows_grid = plan.rows_grid, p.tiles_grid = plan.tiles_grid;
+  p.joins = (JoinOf*)((uint8_t*)workspace + plan.joins);
   p.quads = s.page_size % 4 == 0 && aligned16(weights);
   p.chunk = plan.tiles_grid > 0, p.score_room = plan.score_room;
   p.scores = (float*)((uint8_t*)workspace + plan.stats + plan.parts);

@@ -42,6 +42,7 @@ struct WeighParams {
   float2* stats;  // (m, 1 / l) of every token and head
   float* scores;
   long long score_room;  // blocks of 16 keys
+  struct JoinOf* joins;  // for each workgroup of rows, then of tiles
   float* parts;   // two for each workgroup: (m, l) of 16 rows, then the rows' O
   long long q_token, q_head;
   int T, Hkv, G, D, P, S, N, PPS;
@@ -55,6 +56,16 @@ struct WeighParams {
   float* tile_parts;  // of tiles: two for each workgroup, (m, l) of kColumns columns, then their O
   Divisor page, group;
   float scale, cap, v_scale, decay;  // scale: of q.k; times log2 e where cap is 0
+};
+
+// What a workgroup leaves to be joined: the row (of `near` kv heads from h on) or tile that ends in its share and began in
+// workgroup `first`'s; first -1: none.
+struct alignas(32) JoinOf {
+  int first;
+  int late;  // the first one's part is its slot 1
+  int t, h;  // rows: the token; tiles: the sequence's first
+  int tile;  // rows: of 16 heads; tiles: of kColumns columns
+  int rows;  // tiles: the sequence's rows
 };
 
 struct Sequence {
@@ -165,6 +176,22 @@ __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int b
   return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0};
 }
 
+// The parts of a row that several workgroups had: those of workgroups first .. last.
+struct RowParts {
+  int first, last;
+  bool late;  // the first one's is its slot 1
+};
+// begin: the row's first unit.
+__device__ __forceinline__ RowParts row_parts(const WeighParams& p, long long total, long long begin, int blocks) {
+  const long long each = (total + p.rows_grid - 1) / p.rows_grid;
+  const int first = (int)(begin / each);
+  return {first, (int)((begin + blocks - 1) / each), begin != first * each};
+}
+// head: of the `near` ones
+__device__ __forceinline__ const float* row_part(const WeighParams& p, const RowParts& r, int w, int head) {
+  return p.parts + ((2 * (size_t)w + (w == r.first && r.late)) * p.near + head) * (32 + 16 * (size_t)p.D);
+}
+
 // Rows: a token's heads, up to 16 of one kv head, as the columns of v_mfma_f32_16x16x32_bf16.  A workgroup takes the rows of
 // `near` kv heads, a wave each (where there are few, `ways` waves share a head's keys): a key's rows of all these heads
 // lie together, and the waves walk the same keys.  Keys come in blocks, the blocks of all rows in shares, one a workgroup: a long sequence's rows are spread over as
@@ -191,7 +218,10 @@ __global__ __launch_bounds__(DP == 256 && !FP8 ? 256 : 64 * kMostWaves, DP == 25
   const int threads = blockDim.x, groups = p.Hkv / p.near;
   const Share share =
       share_of<false>(p, blockIdx.x, gridDim.x, [&](const Sequence& s, bool pad) { return row_units(p, s, pad); });
-  if (share.from == share.to) return;
+  if (share.from == share.to) {
+    if (tid == 0) p.joins[blockIdx.x].first = -1;
+    return;
+  }
 
   const int row_bytes = p.D * kElem, mine = wave % p.near, way = wave / p.near;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
@@ -436,6 +466,10 @@ __global__ __launch_bounds__(DP == 256 && !FP8 ? 256 : 64 * kMostWaves, DP == 25
         if (unit + x * p.ways < end_unit) take(x, unit + x * p.ways);
 
     const bool own = first_block == 0 && end_block == blocks;
+    if (at == share.from && tid == 0) {
+      const RowParts r = row_parts(p, share.row_total, at - first_block, blocks);
+      p.joins[blockIdx.x] = {first_block && end_block == blocks ? r.first : -1, r.late, t, h - mine, tile, 0};
+    }
     const int live = min(p.G - tile * 16, 16);
     float* const part = p.parts + ((2 * (size_t)blockIdx.x + (at > share.from)) * p.near) * (32 + 16 * (size_t)p.D);
     l = swap_sum(l);
@@ -496,37 +530,15 @@ __global__ __launch_bounds__(DP == 256 && !FP8 ? 256 : 64 * kMostWaves, DP == 25
   }
 }
 
-// The parts of a row that several workgroups had: those of workgroups first .. last.
-struct RowParts {
-  int first, last;
-  bool late;  // the first one's is its slot 1
-};
-// begin: the row's first unit.
-__device__ __forceinline__ RowParts row_parts(const WeighParams& p, long long total, long long begin, int blocks) {
-  const long long each = (total + p.rows_grid - 1) / p.rows_grid;
-  const int first = (int)(begin / each);
-  return {first, (int)((begin + blocks - 1) / each), begin != first * each};
-}
-// head: of the `near` ones
-__device__ __forceinline__ const float* row_part(const WeighParams& p, const RowParts& r, int w, int head) {
-  return p.parts + ((2 * (size_t)w + (w == r.first && r.late)) * p.near + head) * (32 + 16 * (size_t)p.D);
-}
-
-// Joins a row's parts, for the share that the row ends in, if it began before it: a workgroup a kv head.  Four dims of a
-// head are a thread's, or, of many parts, 8 threads', a share of the parts each.
+// Joins a row's parts, a workgroup a kv head.  Four dims of a head are a thread's, or, of many parts, 8 threads', a share
+// of the parts each.
 __device__ __forceinline__ void join_rows(const WeighParams& p, int block) {
   constexpr int kParts = 4;
   const int head = block % p.near;
-  const Share share =
-      share_of<false>(p, block / p.near, p.rows_grid, [&](const Sequence& s, bool pad) { return row_units(p, s, pad); });
-  if (share.from == share.to) return;
-  const Sequence s = share.s;
-  const int blocks = row_blocks(p, s), groups = p.Hkv / p.near;
-  const long long row = (share.from - share.before) / blocks, begin = share.before + row * blocks;
-  if (begin == share.from || begin + blocks > share.to) return;  // uniform
-  const RowParts parts = row_parts(p, share.row_total, begin, blocks);
-  const int token = (int)(row / (groups * p.tiles)), group_tile = (int)(row - (long long)token * (groups * p.tiles));
-  const int h = group_tile / p.tiles * p.near + head, tile = group_tile % p.tiles, t = s.first + token;
+  const JoinOf join = p.joins[block / p.near];
+  if (join.first < 0) return;  // uniform
+  const RowParts parts = {join.first, block / p.near, join.late != 0};
+  const int h = join.h + head, tile = join.tile, t = join.t;
   const int live = min(p.G - tile * 16, 16), quads = p.D / 4, lanes = parts.last - parts.first > 8 ? 8 : 1;
   for (int i0 = 0; i0 < live * quads; i0 += kWeighThreads / lanes) {
     const int i = min(i0 + (int)threadIdx.x / lanes, live * quads - 1), lane = threadIdx.x % lanes;
@@ -605,10 +617,11 @@ __device__ __forceinline__ float2 row_stat(const WeighParams& p, const Share& sh
   return {top, sum == 0.f ? 0.f : 1.f / sum};
 }
 
-// The weights of the sequences that rows did, a block of keys of a kv head at a time.  Of a sequence with one token the
-// scores are there; a thread sums four keys over the group's heads.  Of one with more (a batch with few tokens that has
-// such a sequence), or whose scores did not fit, K is multiplied once more, 32 keys a wave with 16 rows (token, head) at a time.
-constexpr int kScoreKeys = 1024, kRowKeys = 32 * kWeighWaves;
+// The weights of the sequences that rows did.  Of a sequence with one token the scores are there: a workgroup takes
+// kScoreKeys keys of as many kv heads as make 256 rows, a wave a head at a time, a lane four keys, summed over the group's
+// heads.  Of one with more (a batch with few tokens that has such a sequence), or whose scores did not fit, K is multiplied
+// once more, 32 keys a wave with 16 rows (token, head) at a time.
+constexpr int kScoreKeys = 256, kRowKeys = 32 * kWeighWaves;
 
 template <int DP, bool FULL, bool FP8>
 __device__ __forceinline__ void weigh_rows(const WeighParams& p, int block, int blocks) {
@@ -617,14 +630,15 @@ __device__ __forceinline__ void weigh_rows(const WeighParams& p, int block, int 
   constexpr int kSteps = DP / 32;
   __shared__ float2 s_stat[256];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 16, j = lane / 16;
+  const int heads = min(p.Hkv, 256 / p.G), chunks = (p.Hkv + heads - 1) / heads;  // G is at most 256
   const auto items = [&](const Sequence& s, bool pad) {
     if (pad || !s.tokens || in_tiles(p, s, pad)) return 0ll;
-    const int keys = s.tokens == 1 ? kScoreKeys : kRowKeys;
-    return (long long)((s.keys + keys - 1) / keys) * p.Hkv;
+    return s.tokens == 1 ? (long long)((s.keys + kScoreKeys - 1) / kScoreKeys) * chunks
+                         : (long long)((s.keys + kRowKeys - 1) / kRowKeys) * p.Hkv;
   };
   const Share share = share_of<true>(p, block, blocks, items, true);
   if (share.from == share.to) return;
-  int seq = share.seq, stat_of = -1;  // stat_of: the sequence and head that s_stat holds
+  int seq = share.seq, stat_of = -1;  // stat_of: the sequence and head that s_stat begins with
   Sequence s = share.s;
   long long before = share.before, score_at = share.scores, rows_at = share.rows;
   for (long long at = share.from; at < share.to; ++at) {
@@ -634,119 +648,127 @@ __device__ __forceinline__ void weigh_rows(const WeighParams& p, int block, int 
       s = work_sequence(p, share.count, ++seq);
       stat_of = -1;
     }
-    const int of_head = (int)(items(s, false) / p.Hkv), h = (int)((at - before) / of_head), part = (int)((at - before) - (long long)h * of_head);
+    const bool one = s.tokens == 1;
+    const int keys_of = one ? kScoreKeys : kRowKeys, of_head = (s.keys + keys_of - 1) / keys_of;
+    const int head_chunk = (int)((at - before) / of_head), part = (int)((at - before) - (long long)head_chunk * of_head);
+    const int h0 = one ? head_chunk * heads : head_chunk, h1 = one ? min(h0 + heads, p.Hkv) : h0 + 1;
     const int old = s.keys - s.tokens;  // keys before the step's
-    const bool kept = scores_fit(p, s, score_at);
-    if (kept) {
-      const int key0 = part * kScoreKeys + 4 * tid;  // this thread's four keys
-      const float* from = p.scores + (((size_t)score_at + key0 / 16) * p.Hkv + h) * p.G * 16 + key0 % 16;
-      const bool four = p.quads && key0 + 4 <= old;  // in one page, none of them new
+    if (scores_fit(p, s, score_at)) {
+      const int key0 = part * kScoreKeys + 4 * lane;  // this lane's four keys
+      const bool four = p.quads && key0 + 4 <= old;   // in one page, none of them new
       const int page = div_by(key0, p.page), id = four ? p.table[(size_t)seq * p.PPS + page] : -1;
-      if (stat_of != h) {
+      if (stat_of != h0) {
         __syncthreads();  // the last use of s_stat
-        const int width = p.G <= 32 ? 8 : 1;
-        if (tid < p.G * width) {  // lanes of a head stay together
-          const float2 st = row_stat(p, share, s, rows_at, 0, h, tid / width, tid % width, width);
-          if (tid % width == 0) s_stat[tid / width] = st;
+        const int of = (h1 - h0) * p.G, width = of <= 32 ? 8 : of <= 64 ? 4 : of <= 128 ? 2 : 1;
+        if (tid < of * width) {  // lanes of a row stay together
+          const int r = tid / width;
+          const float2 st = row_stat(p, share, s, rows_at, 0, h0 + r / p.G, r % p.G, tid % width, width);
+          if (tid % width == 0) s_stat[r] = st;
         }
         __syncthreads();
-        stat_of = h;
+        stat_of = h0;
       }
       if (key0 < s.keys) {
         const bool whole = four && id >= 0 && id < p.P;
-        float* const to = p.weights + ((size_t)(whole ? id : 0) * p.Hkv + h) * p.S + (key0 - page * p.S);
-        f32x4 was = {0.f, 0.f, 0.f, 0.f};
-        if (whole && p.decay != 0.f) was = *(const f32x4*)to;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int g = 0; g < p.G; ++g) {
-          const f32x4 x = *(const f32x4*)(from + g * 16);
-          const float2 st = s_stat[g];
+        for (int h = h0 + wave; h < h1; h += kWeighWaves) {
+          const float* const from = p.scores + (((size_t)score_at + key0 / 16) * p.Hkv + h) * p.G * 16 + key0 % 16;
+          const float2* const stat = s_stat + (h - h0) * p.G;
+          float* const to = p.weights + ((size_t)(whole ? id : 0) * p.Hkv + h) * p.S + (key0 - page * p.S);
+          f32x4 was = {0.f, 0.f, 0.f, 0.f};
+          if (whole && p.decay != 0.f) was = *(const f32x4*)to;
+          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+          for (int g = 0; g < p.G; ++g) {
+            const f32x4 x = *(const f32x4*)(from + g * 16);
+            const float2 st = stat[g];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(x[r] - st.x) * st.y;
-        }
-        if (whole) {
-          if (p.decay != 0.f) sum += p.decay * was;
-          *(f32x4*)to = sum;
-        } else if (!four) {
+            for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(x[r] - st.x) * st.y;
+          }
+          if (whole) {
+            if (p.decay != 0.f) sum += p.decay * was;
+            *(f32x4*)to = sum;
+          } else if (!four) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (key0 + r < s.keys) add_weight(p, seq, h, old, key0 + r, sum[r]);
+            for (int r = 0; r < 4; ++r)
+              if (key0 + r < s.keys) add_weight(p, seq, h, old, key0 + r, sum[r]);
+          }
         }
       }
       continue;
     }
-    const int32_t* const table = p.table + (size_t)seq * p.PPS;
-    const int row_bytes = p.D * kElem;
-    const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
-    const global_bytes zero = zero_row(), rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
-    const int first = part * (s.tokens == 1 ? kScoreKeys : kRowKeys), last = min(first + (s.tokens == 1 ? kScoreKeys : kRowKeys), s.keys);
-    for (int key0 = first + 32 * wave; key0 < last; key0 += kRowKeys) {  // no barrier in here
-      bf16x8 k[2][kSteps];
-      float ks[2];
+    for (int h = h0; h < h1; ++h) {  // no barrier in here
+      const int32_t* const table = p.table + (size_t)seq * p.PPS;
+      const int row_bytes = p.D * kElem;
+      const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
+      const global_bytes zero = zero_row(), rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
+      const int first = part * keys_of, last = min(first + keys_of, s.keys);
+      for (int key0 = first + 32 * wave; key0 < last; key0 += kRowKeys) {
+        bf16x8 k[2][kSteps];
+        float ks[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int key = key0 + 16 * b + n, page = div_by(min(key, last - 1), p.page), id = table[page];
-        const bool ok = key < last && id >= 0 && id < p.P;
-        const global_bytes src = ok ? rows + (uint32_t)(id * p.S + (key - page * p.S)) * row_stride : zero;
+        for (int b = 0; b < 2; ++b) {
+          const int key = key0 + 16 * b + n, page = div_by(min(key, last - 1), p.page), id = table[page];
+          const bool ok = key < last && id >= 0 && id < p.P;
+          const global_bytes src = ok ? rows + (uint32_t)(id * p.S + (key - page * p.S)) * row_stride : zero;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int byte = 64 * i + 16 * j;
-          const u32x4 w = load16((FULL || byte < row_bytes ? src : zero) + byte);
-          if (FP8) {
-            k[b][2 * i] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[0], w[1]));
-            k[b][2 * i + 1] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[2], w[3]));
-          } else {
-            k[b][i] = __builtin_bit_cast(bf16x8, w);
+          for (int i = 0; i < kLoads; ++i) {
+            const int byte = 64 * i + 16 * j;
+            const u32x4 w = load16((FULL || byte < row_bytes ? src : zero) + byte);
+            if (FP8) {
+              k[b][2 * i] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[0], w[1]));
+              k[b][2 * i + 1] = __builtin_bit_cast(bf16x8, bf16_of_codes(w[2], w[3]));
+            } else {
+              k[b][i] = __builtin_bit_cast(bf16x8, w);
+            }
           }
+          ks[b] = FP8 && p.scales && ok ? p.scales[((size_t)id * p.Hkv + h) * 2] : 1.f;
         }
-        ks[b] = FP8 && p.scales && ok ? p.scales[((size_t)id * p.Hkv + h) * 2] : 1.f;
-      }
-      float scale[2][4], sum[2][4] = {};
+        float scale[2][4], sum[2][4] = {};
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) scale[b][r] = FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale;
-      const int end = s.tokens * p.G;
-      for (int base = max(key0 - old, 0) * p.G; base < end; base += 16) {
-        const int row = min(base + n, end - 1), token = div_by(row, p.group), g = row - token * p.G, t = s.first + token;
-        const bool live = base + n < end;
-        const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + g) * p.q_head;
-        f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          for (int r = 0; r < 4; ++r) scale[b][r] = FP8 ? p.scale * __shfl(ks[b], 4 * j + r) : p.scale;
+        const int end = s.tokens * p.G;
+        for (int base = max(key0 - old, 0) * p.G; base < end; base += 16) {
+          const int row = min(base + n, end - 1), token = div_by(row, p.group), g = row - token * p.G, t = s.first + token;
+          const bool live = base + n < end;
+          const uint16_t* src = p.q + t * p.q_token + ((long long)h * p.G + g) * p.q_head;
+          f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int dim = FP8 ? 64 * (i / 2) + 16 * j + 8 * (i % 2) : 32 * i + 8 * j;
-          u32x4 w = {0, 0, 0, 0};
-          if (live && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+          for (int i = 0; i < kSteps; ++i) {
+            const int dim = FP8 ? 64 * (i / 2) + 16 * j + 8 * (i % 2) : 32 * i + 8 * j;
+            u32x4 w = {0, 0, 0, 0};
+            if (live && (FULL || dim < p.D)) w = *(const u32x4*)(src + dim);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+              sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][i], __builtin_bit_cast(bf16x8, w), sc[b], 0, 0, 0);
+          }
+          const float2 stat = row_stat(p, share, s, rows_at, token, h, g, 0, 1);
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-            sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][i], __builtin_bit_cast(bf16x8, w), sc[b], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[b][r] = scaled(sc[b][r], scale[b][r]);
+          if (p.cap != 0.f) cap_scores(sc, p.cap);
+          const int seen = live ? old + token : -1;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float e = __builtin_amdgcn_exp2f(sc[b][r] - stat.x) * stat.y;
+              sum[b][r] += key0 + 16 * b + 4 * j + r <= seen ? e : 0.f;
+            }
         }
-        const float2 stat = row_stat(p, share, s, rows_at, token, h, g, 0, 1);
+        float mine = 0.f;  // lane n < 8: of key 16 (n / 4) + 4 j + n % 4
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int u = 0; u < 8; ++u) {
+          float x = sum[u / 4][u % 4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[b][r] = scaled(sc[b][r], scale[b][r]);
-        if (p.cap != 0.f) cap_scores(sc, p.cap);
-        const int seen = live ? old + token : -1;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = __builtin_amdgcn_exp2f(sc[b][r] - stat.x) * stat.y;
-            sum[b][r] += key0 + 16 * b + 4 * j + r <= seen ? e : 0.f;
-          }
+          for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d);
+          mine = n == u ? x : mine;
+        }
+        const int key = key0 + 16 * (n / 4) + 4 * j + n % 4;
+        if (n < 8 && key < last) add_weight(p, seq, h, old, key, mine);
       }
-      float mine = 0.f;  // lane n < 8: of key 16 (n / 4) + 4 j + n % 4
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        float x = sum[u / 4][u % 4];
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d);
-        mine = n == u ? x : mine;
-      }
-      const int key = key0 + 16 * (n / 4) + 4 * j + n % 4;
-      if (n < 8 && key < last) add_weight(p, seq, h, old, key, mine);
     }
   }
 }

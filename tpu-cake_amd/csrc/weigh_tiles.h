@@ -65,7 +65,11 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
   __shared__ int s_bad, s_again;
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
   const Share share = share_of<true>(p, blockIdx.x, gridDim.x, [&](const Sequence& s, bool pad) { return all_slots(p, s, pad); });
-  if (share.from == share.to) return;
+  JoinOf* const joins = p.joins + p.rows_grid;
+  if (share.from == share.to) {  // a share of nothing keeps its workgroup's place
+    if (tid == 0) joins[blockIdx.x].first = -1;
+    return;
+  }
   const int row_bytes = p.D * kElem;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
   const global_bytes zero = zero_row();
@@ -256,6 +260,14 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
       }
     };
     const bool own = tile.slot == 0 && end_slot == tile.slots;
+    if (at == share.from && tid == 0) {
+      JoinOf join = {-1, 0, s.first, h, tile.j, s.tokens * p.G};
+      if (tile.slot && end_slot == tile.slots) {
+        const long long each = share.from / share.index, begin = at - tile.slot;  // a share before this one has `each`
+        join.first = (int)(begin / each), join.late = begin % each != 0;
+      }
+      joins[share.index] = join;
+    }
     float* const part = p.tile_parts + (2 * (size_t)share.index + (at > share.from)) * (kColumns * (2 + (size_t)p.D));
     // The columns' results: those of token `only`, or all (-1).
     const auto write = [&](int only) {
@@ -321,23 +333,16 @@ constexpr int kJoinTiles = 8;
 
 __device__ __forceinline__ void join_tiles(const WeighParams& p, int block) {
   constexpr int kParts = 8;
-  const int index = block / kJoinTiles;
-  const Share share = share_of<false>(p, index, p.tiles_grid, [&](const Sequence& s, bool pad) { return all_slots(p, s, pad); });
-  if (share.from == share.to) return;
-  const Sequence s = share.s;
-  const long long per_head = tile_slots(p, s);
-  const int h = (int)((share.from - share.before) / per_head);
-  const TileOf tile = tile_at(p, s, share.from - share.before - h * per_head);
-  const long long begin = share.from - tile.slot, end = begin + tile.slots;
-  if (begin == share.from || end > share.to) return;  // uniform
-  const long long each = share.from / index;
-  const int first = (int)(begin / each), last = index;
+  const int last = block / kJoinTiles;
+  const JoinOf join = p.joins[p.rows_grid + last];
+  if (join.first < 0) return;  // uniform
+  const int first = join.first, h = join.h;
   const int columns = kColumns / kJoinTiles, c0 = block % kJoinTiles * columns, quads = p.D / 4;
   const size_t stride = kColumns * (2 + (size_t)p.D);
-  const auto part_of = [&](int w) { return p.tile_parts + (2 * (size_t)w + (w == first && begin % each != 0)) * stride; };
+  const auto part_of = [&](int w) { return p.tile_parts + (2 * (size_t)w + (w == first && join.late)) * stride; };
   for (int i = threadIdx.x; i < columns * quads; i += kWeighThreads) {
-    const int c = c0 + i / quads, d = i % quads * 4, row = tile.j * kColumns + c;
-    if (row >= s.tokens * p.G) break;
+    const int c = c0 + i / quads, d = i % quads * 4, row = join.tile * kColumns + c;
+    if (row >= join.rows) break;
     float top = kLowest, sum = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     for (int w = first; w <= last; w += kParts) {
@@ -359,7 +364,7 @@ __device__ __forceinline__ void join_tiles(const WeighParams& p, int block) {
       }
     }
     const int token = div_by(row, p.group), g = row - token * p.G;
-    const size_t to = (size_t)(s.first + token) * p.Hkv * p.G + h * p.G + g;
+    const size_t to = (size_t)(join.t + token) * p.Hkv * p.G + h * p.G + g;
     const float f = sum == 0.f ? 0.f : p.v_scale / sum;
     if (d == 0) p.stats[to] = {top, sum == 0.f ? 0.f : 1.f / sum};
     *(u32x2*)(p.out + to * p.D + d) =
@@ -370,10 +375,10 @@ __device__ __forceinline__ void join_tiles(const WeighParams& p, int block) {
 // What follows rows and tiles, one launch: the joins, and the weights of the sequences that rows did.
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams p) {
-  const int block = blockIdx.x, rows = p.rows_grid * p.near, weigh = gridDim.x - rows - p.tiles_grid * kJoinTiles;
-  if (block < weigh) weigh_rows<DP, FULL, FP8>(p, block, weigh);
-  else if (block < weigh + rows) join_rows(p, block - weigh);
-  else join_tiles(p, block - weigh - rows);
+  const int block = blockIdx.x, rows = p.rows_grid * p.near, tiles = p.tiles_grid * kJoinTiles;
+  if (block < rows) join_rows(p, block);
+  else if (block < rows + tiles) join_tiles(p, block - rows);
+  else weigh_rows<DP, FULL, FP8>(p, block - rows - tiles, gridDim.x - rows - tiles);
 }
 
 // The weights of the sequences that tiles did, kKeys keys of a kv head at a time, 64 a wave, whose K stays in registers
@@ -550,7 +555,7 @@ struct WeighPlan {
   int tiles, near, ways, block_shift, rows_grid, tiles_grid, weigh_grid, keys_grid;  // tiles_grid 0: rows only
   size_t rows_lds;
   long long score_room;
-  size_t stats, parts, scores, bytes;
+  size_t stats, parts, scores, joins, bytes;
 };
 
 constexpr int kTilesGrid = 512, kWeighGrid = 1280, kKeysGrid = 2048;
@@ -594,6 +599,8 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
     r.tiles_grid = (int)(slots < fill ? slots : fill);
     r.bytes += (size_t)r.tiles_grid * 2 * kColumns * (2 + (size_t)s.head_dim) * 4;
   }
+  r.joins = (r.bytes + 31) / 32 * 32;
+  r.bytes = r.joins + (size_t)(r.rows_grid + r.tiles_grid) * sizeof(JoinOf);
   return r;
 }
 
