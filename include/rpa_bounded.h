@@ -111,9 +111,10 @@ typedef struct rpa_choose_shape {
  * row below it that is not kept: moves int32 [max_num_seqs, num_kv_heads, max_moves, 2] holds the two
  * slots (page * page_size + row), to and from, and -1 past the last.  A list that needs more than max_moves
  * entries (never with max_moves >= budget) is cut short and sets RPA_SPARSE_ERR_LEN. */
+size_t rpa_choose_workspace_size(const rpa_choose_shape_t* shape);
 int rpa_choose_moves(const rpa_choose_shape_t* shape, const float* weights, const int32_t* positions,
                      const int32_t* kv_lens, const int32_t* page_indices, const int32_t* num_seqs,
-                     const int32_t* dropped, int32_t* moves, void* stream);
+                     const int32_t* dropped, int32_t* moves, void* workspace, size_t workspace_bytes, void* stream);
 
 typedef struct rpa_move_shape {
   int32_t num_lists; /* sequences of the lists */

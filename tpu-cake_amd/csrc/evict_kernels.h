@@ -2,7 +2,7 @@
 //
 // Mathematics: a row's key is its weight as an unsigned whole number of the same order (0 for NaN), the largest of all for
 // rows that stay in any case.  The budget-th largest key of a (sequence, head) is found digit by digit: counts of the
-// next eight bits over the rows that share the bits so far, four times.  Rows above it stay, and of the rows at it
+// next bits over the rows that share the bits so far, four times.  Rows above it stay, and of the rows at it
 // the lowest ones, as many as fit.  Kept rows at or past `budget` and rows below it that go are equally many: the i-th of the
 // one take the places of the i-th of the other.  Counts are whole numbers, so nothing depends on an order.
 //
@@ -20,85 +20,236 @@ struct ChooseParams {
   const float* weights;
   const int32_t *positions, *kv_lens, *table, *num_seqs, *dropped;
   int32_t* moves;
+  uint32_t* keys;    // of rows past kChooseRows: for each (sequence, head) `stride` keys, then `counts`' blocks
+  uint32_t* counts;  // 2048 for each block of kKeyRows
+  long long stride;
   int N, PPS, Hkv, P, S, budget, limit, sinks, recent, M;
+  int first;         // the launch's first sequence
+  int room;          // keys that fit a workgroup's LDS
+  int quads;         // four neighbouring entries from a multiple of four on are 16 aligned bytes of one page
 };
 
 // The order of weights as whole numbers, 0 for NaN; zeros of both signs are equal.
 __device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? ordered(w + 0.f) : 0u; }
 
-constexpr int kChooseThreads = 1024;
+constexpr int kChooseRows = 32768;  // rows of a sequence whose keys fit LDS
+constexpr int kKeyRows = 4096;      // rows of a workgroup that makes a longer one's keys
+constexpr int kDigits = 2048;       // 11 bits, 11 bits, 10 bits
 
-// One workgroup a (kv head, sequence).
-__global__ __launch_bounds__(kChooseThreads) void choose_rows_kernel(ChooseParams p) {
-  constexpr int kWaves = kChooseThreads / 64;
-  __shared__ uint32_t s_count[256];
-  __shared__ Pair s_scan[kWaves];
-  __shared__ uint32_t s_found[2];
-  const int tid = threadIdx.x;
-  const int h = blockIdx.x % p.Hkv, seq = blockIdx.x / p.Hkv;
-  int32_t* const list = p.moves + ((size_t)seq * p.Hkv + h) * p.M * 2;
-  const long long capacity = (long long)p.PPS * p.S;
-  int n = seq < *p.num_seqs ? p.kv_lens[seq] : 0;
-  const long long end = (long long)n + (p.dropped ? p.dropped[seq] : 0);
-  if (n > capacity) {
-    if (tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
-    n = (int)capacity;
-  }
-  int done = 0;  // entries of the list
-  if (n > p.limit && n > p.budget) {  // uniform
-    const int32_t* const table = p.table + (size_t)seq * p.PPS;
-    const auto slot_of = [&](int row) {  // -1: no such page
-      const int page = table[row / p.S];
-      return page >= 0 && page < p.P ? page * p.S + row % p.S : -1;
-    };
-    const auto key_of = [&](int row) {
-      const int slot = slot_of(row);
-      if (slot < 0) {
+// A sequence that is cut: its rows (0: it is not), and the position past its last.
+struct Cut {
+  int rows;
+  long long end;
+};
+__device__ __forceinline__ Cut cut_of(const ChooseParams& p, int seq, bool flag) {
+  const int count = *p.num_seqs, len = p.kv_lens[seq], gone = p.dropped ? p.dropped[seq] : 0;
+  const int capacity = p.PPS * p.S;
+  const int n = p.first + seq < count ? len : 0;
+  if (flag && n > capacity) flag_error(RPA_SPARSE_ERR_LEN);
+  return {n > p.limit && min(n, capacity) > p.budget ? min(n, capacity) : 0, (long long)n + gone};
+}
+
+// Four rows' keys, from `row` (a multiple of four) on; rows from n on are 0.
+__device__ __forceinline__ u32x4 keys_at(const ChooseParams& p, const int32_t* table, int h, const Cut& cut, int row) {
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  int at[4] = {0, 0, 0, 0};
+  bool ok[4] = {false, false, false, false};
+  if (p.quads) {
+    const int page = row < cut.rows ? table[row / p.S] : -1;
+    if (page >= 0 && page < p.P) {
+      const size_t from = ((size_t)page * p.Hkv + h) * p.S + row % p.S;
+      const f32x4 x = *(const f32x4*)(p.weights + from);
+      const i32x4 y = *(const i32x4*)(p.positions + from);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = x[i], at[i] = y[i], ok[i] = row + i < cut.rows;
+    } else if (row < cut.rows) {
+      flag_error(RPA_SPARSE_ERR_PAGE);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (row + i >= cut.rows) continue;
+      const int page = table[(row + i) / p.S];
+      if (page < 0 || page >= p.P) {
         flag_error(RPA_SPARSE_ERR_PAGE);
-        return 0u;
+        continue;
       }
-      const size_t at = ((size_t)(slot / p.S) * p.Hkv + h) * p.S + slot % p.S;
-      const int position = p.positions[at];
-      return position < p.sinks || position >= end - p.recent ? 0xffffffffu : weight_key(p.weights[at]);
-    };
-    uint32_t prefix = 0, rank = p.budget;  // the rank-th largest of the keys that begin with prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kChooseThreads) s_count[i] = 0;
-      __syncthreads();
-      for (int row = tid; row < n; row += kChooseThreads) {
-        const uint32_t key = key_of(row);
-        if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&s_count[key >> shift & 255], 1u);
+      const size_t from = ((size_t)page * p.Hkv + h) * p.S + (row + i) % p.S;
+      w[i] = p.weights[from], at[i] = p.positions[from], ok[i] = true;
+    }
+  }
+  u32x4 key;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    key[i] = !ok[i] ? 0u : at[i] < p.sinks || at[i] >= cut.end - p.recent ? 0xffffffffu : weight_key(w[i]);
+  return key;
+}
+
+// Keys of long sequences, and how many of a block's rows have each first digit.
+__global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
+  __shared__ uint32_t s_count[kDigits];
+  const int tid = threadIdx.x, h = blockIdx.y % p.Hkv, seq = blockIdx.y / p.Hkv, first = blockIdx.x * kKeyRows;
+  const Cut cut = cut_of(p, seq, false);
+  if (cut.rows <= p.room || first >= cut.rows) return;  // uniform
+  for (int i = tid; i < kDigits; i += 256) s_count[i] = 0;
+  __syncthreads();
+  uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
+#pragma unroll
+  for (int i = 0; i < kKeyRows / 1024; ++i) {
+    const int row = first + 1024 * i + 4 * tid;
+    const u32x4 key = keys_at(p, p.table + (size_t)seq * p.PPS, h, cut, row);
+    if (row < cut.rows) *(u32x4*)(keys + row) = key;  // a multiple of four is there
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (row + u < cut.rows) atomicAdd(&s_count[key[u] >> 21], 1u);
+  }
+  __syncthreads();
+  uint32_t* const counts = p.counts + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * kDigits;
+  for (int i = tid; i < kDigits; i += 256) counts[i] = s_count[i];
+}
+
+// One workgroup a (kv head, sequence).  A step's loads are of 256 rows a wave, four neighbouring rows a lane.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void choose_rows_kernel(ChooseParams p, int blocks) {
+  constexpr int kWaves = THREADS / 64, kBins = kDigits / THREADS;
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ uint32_t s_count[kDigits];
+  __shared__ uint32_t s_sum[kWaves], s_found[2];
+  __shared__ uint32_t s_waves[kWaves][4];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int h = blockIdx.x % p.Hkv, seq = blockIdx.x / p.Hkv;
+  int32_t* const list = p.moves + (size_t)blockIdx.x * p.M * 2;
+  const Cut cut = cut_of(p, seq, tid == 0);
+  const int n = cut.rows;
+  int done = 0;  // entries of the list
+  if (n) {       // uniform
+    const int32_t* const table = p.table + (size_t)seq * p.PPS;
+    const bool inside = n <= p.room;
+    const uint32_t* const far = p.keys + (size_t)blockIdx.x * p.stride;
+    const auto load = [&](int row) { return inside ? *(const u32x4*)(s_keys + row) : *(const u32x4*)(far + row); };
+    // the digits of the budget-th largest key, one after another; rank: which one it is of the keys that begin with them
+    uint32_t prefix = 0, rank = p.budget;
+    for (int shift = 21, bits = 11; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1, bits = shift ? 11 : 10) {
+      const bool first = shift == 21;
+      if (first && !inside) {
+        for (int i = tid; i < kDigits; i += THREADS) {
+          uint32_t sum = 0;
+          for (int b = 0; b < (n + kKeyRows - 1) / kKeyRows; ++b) sum += p.counts[((size_t)blockIdx.x * blocks + b) * kDigits + i];
+          s_count[i] = sum;
+        }
+      } else {
+        for (int i = tid; i < kDigits; i += THREADS) s_count[i] = 0;
+        __syncthreads();
+        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
+          u32x4 key;
+          if (first) {
+            key = keys_at(p, table, h, cut, row);
+            *(u32x4*)(s_keys + row) = key;
+          } else {
+            key = load(row);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (row + u < n && (first || key[u] >> (shift + bits) == prefix)) atomicAdd(&s_count[key[u] >> shift & ((1u << bits) - 1)], 1u);
+        }
       }
       __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0;
-        int d = 255;
-        while (d > 0 && above + s_count[d] < rank) above += s_count[d--];
-        s_found[0] = prefix << 8 | d, s_found[1] = rank - above;
+      // the largest digits first: thread 0 has the last kBins
+      uint32_t own = 0;
+      const int top = kDigits - 1 - tid * kBins;
+#pragma unroll
+      for (int i = 0; i < kBins; ++i) own += s_count[top - i];
+      uint32_t upto = own;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = __shfl_up(upto, d);
+        upto += lane >= d ? o : 0u;
+      }
+      if (lane == 63) s_sum[wave] = upto;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) upto += s_sum[w];
+      if (upto - own < rank && rank <= upto) {
+        uint32_t above = upto - own;
+        int d = top;
+        while (above + s_count[d] < rank) above += s_count[d--];
+        s_found[0] = prefix << bits | d, s_found[1] = rank - above;
       }
       __syncthreads();
       prefix = s_found[0], rank = s_found[1];
     }
-    // rank: how many of the rows at this very key stay
-    uint32_t equal = 0, late = 0, holes = 0;
-    for (int base = 0; base < n; base += kChooseThreads) {
-      const int row = base + tid;
-      const uint32_t key = row < n ? key_of(row) : 0u;
-      const bool same = row < n && key == prefix;
-      Pair total;
-      Pair before = scan_pairs<kWaves>({same, 0}, total, s_scan);
-      const bool kept = row < n && (key > prefix || (same && equal + before.a < rank));
-      equal += total.a;
-      const bool comes = kept && row >= p.budget, goes = row < n && !kept && row < p.budget;
-      before = scan_pairs<kWaves>({comes, goes}, total, s_scan);
-      if (comes && late + before.a < (uint32_t)p.M) list[2 * (late + before.a) + 1] = slot_of(row);
-      if (goes && holes + before.b < (uint32_t)p.M) list[2 * (holes + before.b)] = slot_of(row);
-      late += total.a, holes += total.b;
+    // rank: how many of the rows at this very key stay, the lowest.  Every wave has a stretch of rows.
+    const int stretch = ((n + kWaves - 1) / kWaves + 255) / 256 * 256, from = min(wave * stretch, n), to = min(from + stretch, n);
+    uint32_t same_low = 0, same_high = 0, more = 0, less = 0;  // rows at the key before the budget and past it; above and past; below and before
+#pragma unroll 4
+    for (int row = from + 4 * lane; row < to; row += 256) {
+      const u32x4 key = load(row);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (row + u >= n) continue;
+        const bool low = row + u < p.budget, same = key[u] == prefix;
+        same_low += same && low, same_high += same && !low;
+        more += key[u] > prefix && !low, less += key[u] < prefix && low;
+      }
     }
-    if (late > (uint32_t)p.M && tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
-    done = (int)min(late, (uint32_t)p.M);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      same_low += __shfl_xor(same_low, d), same_high += __shfl_xor(same_high, d);
+      more += __shfl_xor(more, d), less += __shfl_xor(less, d);
+    }
+    if (lane == 0) s_waves[wave][0] = same_low, s_waves[wave][1] = same_high, s_waves[wave][2] = more, s_waves[wave][3] = less;
+    __syncthreads();
+    uint32_t all_low = 0, low = 0, high = 0, late = 0, holes = 0, all_late = 0, all_high = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) low += s_waves[w][0], high += s_waves[w][1], late += s_waves[w][2], holes += s_waves[w][3];
+      all_low += s_waves[w][0], all_high += s_waves[w][1], all_late += s_waves[w][2];
+    }
+    // rows at the key that stay: the first `rank`, before the budget first
+    const uint32_t stay_low = min(rank, all_low);
+    uint32_t same = low + high;  // seen so far
+    late += min(rank, same) > stay_low ? min(rank, same) - stay_low : 0u;
+    holes += low - min(rank, low);
+    all_late += min(rank, all_low + all_high) - stay_low;
+    const auto slot_of = [&](int row) {  // -1: no such page
+      const int page = table[row / p.S];
+      return page >= 0 && page < p.P ? page * p.S + row % p.S : -1;
+    };
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll 2
+    for (int base = from; base < to; base += 256) {
+      const int row = base + 4 * lane;
+      const u32x4 key = row < to ? load(row) : u32x4{0, 0, 0, 0};
+      uint32_t mine = same;  // rows at the key before this lane's
+      bool is[4];
+      uint32_t count = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        is[u] = row < to && row + u < n && key[u] == prefix;
+        const uint64_t votes = __ballot(is[u]);
+        mine += __popcll(votes & below), count += __popcll(votes);
+      }
+      same += count;
+      bool comes[4], goes[4];
+      uint32_t late_at = late, hole_at = holes;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool there = row < to && row + u < n, kept = there && (key[u] > prefix || (is[u] && mine < rank));
+        mine += is[u];
+        comes[u] = kept && row + u >= p.budget, goes[u] = there && !kept && row + u < p.budget;
+        const uint64_t a = __ballot(comes[u]), b = __ballot(goes[u]);
+        late_at += __popcll(a & below), hole_at += __popcll(b & below);
+        late += __popcll(a), holes += __popcll(b);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (comes[u] && late_at < (uint32_t)p.M) list[2 * (size_t)late_at + 1] = slot_of(row + u);
+        if (goes[u] && hole_at < (uint32_t)p.M) list[2 * (size_t)hole_at] = slot_of(row + u);
+        late_at += comes[u], hole_at += goes[u];
+      }
+    }
+    if (all_late > (uint32_t)p.M && tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
+    done = (int)min(all_late, (uint32_t)p.M);
   }
-  for (long long i = 2ll * done + tid; i < 2ll * p.M; i += kChooseThreads) list[i] = -1;
+  for (long long i = 2ll * done + tid; i < 2ll * p.M; i += THREADS) list[i] = -1;
 }
 
 struct MoveParams {
@@ -166,7 +317,30 @@ int check_choose(const rpa_choose_shape_t* s) {
   if (s->sinks < 0 || s->recent < 0 || (long long)s->sinks + s->recent > s->budget)
     return fail(RPA_E_INVALID, "sinks and recent must not be negative nor more than the budget together");
   if (s->max_moves >= 1 << 30) return fail(RPA_E_INVALID, "max_moves must be below 2^30");
-  return check_launch((long long)s->max_num_seqs * s->num_kv_heads, kChooseThreads);
+  if ((long long)s->max_num_seqs * s->num_kv_heads > 0x7fffffff / 1024)
+    return fail(RPA_E_UNSUPPORTED, "more lists than one launch takes");
+  return RPA_OK;
+}
+
+struct ChoosePlan {
+  int threads, room, blocks;  // blocks 0: all keys fit LDS
+  long long stride;
+  size_t keys, bytes;
+};
+
+// Small workgroups where a sequence's rows are few: their barriers cost less.
+ChoosePlan plan_choose(const rpa_choose_shape_t& s) {
+  ChoosePlan r = {};
+  const long long capacity = (long long)s.pages_per_seq * s.page_size;
+  r.threads = capacity <= 8192 ? 256 : 1024;
+  r.room = (int)((capacity < kChooseRows ? capacity : kChooseRows) + 3) / 4 * 4;
+  if (capacity > kChooseRows) {
+    r.blocks = (int)((capacity + kKeyRows - 1) / kKeyRows);
+    r.stride = (capacity + 3) / 4 * 4;
+    r.keys = (size_t)s.max_num_seqs * s.num_kv_heads * r.stride * 4;
+    r.bytes = r.keys + (size_t)s.max_num_seqs * s.num_kv_heads * r.blocks * kDigits * 4;
+  }
+  return r;
 }
 
 int check_move(const rpa_move_shape_t* s) {

@@ -173,22 +173,48 @@ int rpa_weighed_attention(const rpa_weigh_shape_t* shape, const rpa_weigh_option
   return launch_weigh<128, false, false>(plan, p, stream_);
 }
 
+size_t rpa_choose_workspace_size(const rpa_choose_shape_t* shape) {
+  return check_choose(shape) == RPA_OK ? plan_choose(*shape).bytes : 0;
+}
+
 int rpa_choose_moves(const rpa_choose_shape_t* shape, const float* weights, const int32_t* positions,
                      const int32_t* kv_lens, const int32_t* page_indices, const int32_t* num_seqs,
-                     const int32_t* dropped, int32_t* moves, void* stream) {
+                     const int32_t* dropped, int32_t* moves, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_choose(shape);
   if (rc) return rc;
   if (!weights || !positions || !kv_lens || !page_indices || !num_seqs || !moves)
     return fail(RPA_E_INVALID, "NULL tensor pointer");
   const rpa_choose_shape_t& s = *shape;
+  const ChoosePlan plan = plan_choose(s);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
+    return fail(RPA_E_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const long long N = s.max_num_seqs, slots = (long long)s.total_pages * s.page_size * s.num_kv_heads;
   const Memory in[] = {{"weights", weights, 4 * slots}, {"positions", positions, 4 * slots}, {"kv_lens", kv_lens, 4 * N},
                        {"page_indices", page_indices, 4 * N * s.pages_per_seq}, {"num_seqs", num_seqs, 4},
-                       {"dropped", dropped, 4 * N}};
+                       {"dropped", dropped, 4 * N}, {"workspace", workspace, (long long)plan.bytes}};
   if ((rc = check_separate({"moves", moves, 8 * N * s.num_kv_heads * s.max_moves}, in))) return rc;
-  const ChooseParams p = {weights, positions, kv_lens, page_indices, num_seqs, dropped, moves, s.max_num_seqs, s.pages_per_seq,
-                          s.num_kv_heads, s.total_pages, s.page_size, s.budget, s.limit, s.sinks, s.recent, s.max_moves};
-  choose_rows_kernel<<<(unsigned)(N * s.num_kv_heads), kChooseThreads, 0, (hipStream_t)stream>>>(p);
+  ChooseParams p = {};
+  p.weights = weights, p.positions = positions, p.kv_lens = kv_lens, p.table = page_indices, p.num_seqs = num_seqs;
+  p.dropped = dropped, p.moves = moves, p.keys = (uint32_t*)workspace, p.stride = plan.stride;
+  p.counts = (uint32_t*)((uint8_t*)workspace + plan.keys);
+  p.N = s.max_num_seqs, p.PPS = s.pages_per_seq, p.Hkv = s.num_kv_heads, p.P = s.total_pages, p.S = s.page_size;
+  p.budget = s.budget, p.limit = s.limit, p.sinks = s.sinks, p.recent = s.recent, p.M = s.max_moves;
+  p.room = plan.room, p.quads = s.page_size % 4 == 0 && aligned16(weights) && aligned16(positions);
+  const unsigned lists = (unsigned)(N * s.num_kv_heads);
+  const hipStream_t stream_ = (hipStream_t)stream;
+  if (plan.blocks) {
+    for (unsigned first = 0; first < lists; first += 65535 / s.num_kv_heads * s.num_kv_heads) {  // a launch's y dimension
+      ChooseParams part = p;
+      const unsigned seqs = first / s.num_kv_heads, step = 65535 / s.num_kv_heads * s.num_kv_heads;
+      part.kv_lens += seqs, part.table += (size_t)seqs * s.pages_per_seq, part.dropped += dropped ? seqs : 0;
+      part.keys += first * (size_t)plan.stride, part.counts += (size_t)first * plan.blocks * kDigits, part.first = (int)seqs;
+      choose_keys_kernel<<<dim3(plan.blocks, lists - first < step ? lists - first : step), 256, 0, stream_>>>(part);
+      if ((rc = launched("choose_moves (keys)"))) return rc;
+    }
+  }
+  const size_t lds = (size_t)plan.room * 4;
+  if (plan.threads == 256) choose_rows_kernel<256><<<lists, 256, lds, stream_>>>(p, plan.blocks);
+  else choose_rows_kernel<1024><<<lists, 1024, lds, stream_>>>(p, plan.blocks);
   return launched("choose_moves");
 }
 

@@ -42,7 +42,8 @@ _SIGNATURES = {
     "rpa_weigh_workspace_size": (_sz, [ctypes.POINTER(RpaWeighShape)]),
     "rpa_weighed_attention": (ctypes.c_int, [ctypes.POINTER(RpaWeighShape), ctypes.POINTER(RpaWeighOptions)] + [_vp] * 12
                               + [_sz, _vp]),
-    "rpa_choose_moves": (ctypes.c_int, [ctypes.POINTER(RpaChooseShape)] + [_vp] * 8),
+    "rpa_choose_workspace_size": (_sz, [ctypes.POINTER(RpaChooseShape)]),
+    "rpa_choose_moves": (ctypes.c_int, [ctypes.POINTER(RpaChooseShape)] + [_vp] * 8 + [_sz, _vp]),
     "rpa_move_rows": (ctypes.c_int, [ctypes.POINTER(RpaMoveShape)] + [_vp] * 6),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -201,8 +201,9 @@ def choose_moves(
         if sinks + recent > budget:
             raise ValueError(f"sinks={sinks} and recent={recent} exceed budget={budget}")
         shape = _bounded_lib.RpaChooseShape(n, width, heads, pages, page_size, budget, most, sinks, recent, room)
-        plan = _keep(sig, (shape, (n, heads, room, 2), _bounded_lib.load().rpa_choose_moves))
-    shape, out_shape, fn = plan
+        lib = _bounded_lib.load()
+        plan = _keep(sig, (shape, (n, heads, room, 2), int(lib.rpa_choose_workspace_size(ctypes.byref(shape))), lib.rpa_choose_moves))
+    shape, out_shape, need, fn = plan
     dev = kv_lens.get_device()
     if out is None:
         out = kv_lens.new_empty(out_shape)
@@ -214,8 +215,10 @@ def choose_moves(
         with torch.cuda.device(dev):
             return choose_moves(ledger, kv_lens, page_indices, num_seqs, budget=budget, recent=recent, sinks=sinks, limit=limit,
                                 dropped=dropped, max_moves=max_moves, out=out)
+    scratch = torch.empty(need, dtype=torch.uint8, device=kv_lens.device) if need else None
     rc = fn(shape, ledger[0].data_ptr(), ledger[1].data_ptr(), kv_lens.data_ptr(), page_indices.data_ptr(), num_seqs.data_ptr(),
-            None if dropped is None else dropped.data_ptr(), out.data_ptr(), _current_stream(dev))
+            None if dropped is None else dropped.data_ptr(), out.data_ptr(), scratch.data_ptr() if need else None, need,
+            _current_stream(dev))
     if rc:
         _bounded_lib.check(rc)
     return out
