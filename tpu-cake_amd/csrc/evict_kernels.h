@@ -258,48 +258,79 @@ struct MoveParams {
   uint8_t* kv;
   float* weights;
   int32_t* positions;
-  long long entries, rows;  // of all lists; P * S
-  int M, Hkv, D, S, chunks;  // chunks: 16 bytes each, of a head's key and value row
+  long long rows;            // P * S
+  int entries;               // of all lists
+  int M, Hkv, S, chunks;     // chunks: 16 bytes each, of a head's key and value row, which lie together
 };
 
-// A wave takes entries of the lists, its lanes 16 bytes of a head's key and value row, which lie together.
-template <bool FP8>
+constexpr int kMoveEntries = 16;  // of a wave
+
+// A wave takes kMoveEntries entries of the lists: their slots, scales and ledger entries a lane each, then their rows,
+// LANES lanes a row, four loads in flight.
+template <bool FP8, int LANES>
 __global__ __launch_bounds__(256) void move_kernel(MoveParams p) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const long long entry = (long long)blockIdx.x * 4 + wave;
-  if (entry >= p.entries) return;
-  const int h = (int)(entry / p.M % p.Hkv);
-  const int to = p.moves[2 * entry], from = p.moves[2 * entry + 1];
-  if (to < 0 || from < 0) return;
-  if (to >= p.rows || from >= p.rows) {
-    if (lane == 0) flag_error(RPA_SPARSE_ERR_SLOT);
-    return;
+  constexpr int kRows = 64 / LANES, kTurns = kMoveEntries / kRows, kHold = kTurns < 4 ? kTurns : 4;
+  const int lane = threadIdx.x % 64, first = (blockIdx.x * 4 + threadIdx.x / 64) * kMoveEntries;
+  const int entry = first + lane;
+  int to = -1, from = -1, h = 0;
+  if (lane < kMoveEntries && entry < p.entries) {
+    const u32x2 slots = *(const u32x2*)(p.moves + 2 * (size_t)entry);
+    to = (int)slots[0], from = (int)slots[1];
+    h = entry / p.M % p.Hkv;
   }
-  const size_t row_bytes = 16ull * p.chunks;
-  const uint8_t* const src = p.kv + ((size_t)from * p.Hkv + h) * row_bytes;
-  uint8_t* const dst = p.kv + ((size_t)to * p.Hkv + h) * row_bytes;
-  const size_t head_from = (size_t)(from / p.S) * p.Hkv + h, head_to = (size_t)(to / p.S) * p.Hkv + h;
-  for (int c = lane; c < p.chunks; c += 64) {
-    u32x4 w = *(const u32x4*)(src + 16 * c);
+  bool live = to >= 0 && from >= 0;
+  if (live && (to >= p.rows || from >= p.rows)) {
+    flag_error(RPA_SPARSE_ERR_SLOT);
+    live = false;
+  }
+  if (!__ballot(live)) return;
+  float ratio_from[2] = {1.f, 1.f}, ratio_to[2] = {1.f, 1.f};  // the K and V scales there and here
+  if (live) {
+    const size_t head_from = (size_t)(from / p.S) * p.Hkv + h, head_to = (size_t)(to / p.S) * p.Hkv + h;
+    const size_t a = head_from * p.S + from % p.S, b = head_to * p.S + to % p.S;
+    const float weight = p.weights[a];
+    const int position = p.positions[a];
     if (FP8 && p.scales) {
-      const int part = 2 * c >= p.chunks;
-      const float there = p.scales[2 * head_from + part], here = p.scales[2 * head_to + part];
-      if (there != here) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ratio_from[i] = p.scales[2 * head_from + i], ratio_to[i] = p.scales[2 * head_to + i];
+    }
+    p.weights[b] = weight;
+    p.positions[b] = position;
+  }
+  const int c = lane % LANES, part = 2 * c >= p.chunks;
+  const size_t row_bytes = 16ull * p.chunks;
+#pragma unroll
+  for (int turn = 0; turn < kTurns; turn += kHold) {
+    u32x4 w[kHold];
+    int dst[kHold], head[kHold];
+    float there[kHold], here[kHold];
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+      const int e = (turn + u) * kRows + lane / LANES;
+      const int src = __shfl(from, e), place = __shfl(live ? to : -1, e);
+      dst[u] = c < p.chunks ? place : -1;
+      head[u] = __shfl(h, e);
+      if (FP8) {
+        const float k0 = __shfl(ratio_from[0], e), v0 = __shfl(ratio_from[1], e);
+        const float k1 = __shfl(ratio_to[0], e), v1 = __shfl(ratio_to[1], e);
+        there[u] = part ? v0 : k0, here[u] = part ? v1 : k1;
+      }
+      if (dst[u] >= 0) w[u] = *(const u32x4*)(p.kv + ((size_t)src * p.Hkv + head[u]) * row_bytes + 16 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+      if (dst[u] < 0) continue;
+      if (FP8 && there[u] != here[u]) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          fp8_values(u32x2{w[2 * i], w[2 * i + 1]}, there, x);
-          const u32x2 codes = fp8_codes(x, here);
-          w[2 * i] = codes[0], w[2 * i + 1] = codes[1];
+          fp8_values(u32x2{w[u][2 * i], w[u][2 * i + 1]}, there[u], x);
+          const u32x2 codes = fp8_codes(x, here[u]);
+          w[u][2 * i] = codes[0], w[u][2 * i + 1] = codes[1];
         }
       }
+      *(u32x4*)(p.kv + ((size_t)dst[u] * p.Hkv + head[u]) * row_bytes + 16 * c) = w[u];
     }
-    *(u32x4*)(dst + 16 * c) = w;
-  }
-  if (lane == 0) {
-    const size_t a = head_from * p.S + from % p.S, b = head_to * p.S + to % p.S;
-    p.weights[b] = p.weights[a];
-    p.positions[b] = p.positions[a];
   }
 }
 
@@ -349,7 +380,7 @@ int check_move(const rpa_move_shape_t* s) {
   int rc = check_heads(s->num_kv_heads, s->head_dim, s->kv_dtype);
   if (rc || (rc = check_pool(s->total_pages, s->page_size))) return rc;
   const __int128 entries = (__int128)s->num_lists * s->num_kv_heads * s->max_moves;
-  if (entries > 4 * (kMostThreads / 256)) return fail(RPA_E_UNSUPPORTED, "more rows than one launch takes");
+  if (entries > kMostIndex) return fail(RPA_E_UNSUPPORTED, "more rows than one launch takes");
   return RPA_OK;
 }
 

@@ -96,13 +96,25 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p) {
     const float2 x = turn ? turned[c * V + i] : float2{1.f, 0.f};
     cosine[i] = x.x, sine[i] = x.y;
   }
-  for (int base = part * teams; base < rows; base += p.parts * teams) {
-    const int row = base + mine;
-    const bool ok = inside && row < rows, query = row < p.Hq;
+  // a turn's rows, loaded a turn ahead
+  const auto row_at = [&](int base) { return base + mine; };
+  const auto load = [&](int base, Word& wa, Word& wb) {
+    const int row = row_at(base);
+    const bool query = row < p.Hq;
     const int head = query ? row : row - p.Hq;
     const uint16_t* const src = query ? p.q + t * p.q_token + head * p.q_head : p.k + t * p.k_token + head * p.k_head;
-    Word wa = {}, wb = {};
-    if (ok && live) wa = *(const Word*)(src + a), wb = *(const Word*)(src + b);
+    wa = Word{}, wb = Word{};
+    if (inside && row < rows && live) wa = *(const Word*)(src + a), wb = *(const Word*)(src + b);
+  };
+  const int step = p.parts * teams;
+  Word next_a, next_b;
+  load(part * teams, next_a, next_b);
+  for (int base = part * teams; base < rows; base += step) {
+    const int row = row_at(base);
+    const bool ok = inside && row < rows, query = row < p.Hq;
+    const int head = query ? row : row - p.Hq;
+    Word wa = next_a, wb = next_b;
+    if (base + step < rows) load(base + step, next_a, next_b);
     float x[V], y[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {

@@ -236,11 +236,12 @@ int rpa_move_rows(const rpa_move_shape_t* shape, const int32_t* moves, const flo
   if ((rc = check_separate(rows, in)) || (rc = check_separate(sums, in)) || (rc = check_separate(places, in)) ||
       (rc = check_separate(rows, {sums, places})) || (rc = check_separate(sums, {places})))
     return rc;
-  const MoveParams p = {moves, kv_scales, (uint8_t*)kv_pages, weights, positions, entries, pool, s.max_moves, s.num_kv_heads,
-                        s.head_dim, s.page_size, (int)(row / 16)};
-  const unsigned grid = (unsigned)((entries + 3) / 4);
-  if (fp8) move_kernel<true><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-  else move_kernel<false><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+  const MoveParams p = {moves, kv_scales, (uint8_t*)kv_pages, weights, positions, pool, (int)entries, s.max_moves, s.num_kv_heads,
+                        s.page_size, (int)(row / 16)};
+  const unsigned grid = (unsigned)((entries + 4 * kMoveEntries - 1) / (4 * kMoveEntries));
+  const auto kernel = fp8 ? (p.chunks <= 16 ? move_kernel<true, 16> : move_kernel<true, 32>)
+                          : (p.chunks <= 16 ? move_kernel<false, 16> : p.chunks <= 32 ? move_kernel<false, 32> : move_kernel<false, 64>);
+  kernel<<<grid, 256, 0, (hipStream_t)stream>>>(p);
   return launched("move_rows");
 }
 
