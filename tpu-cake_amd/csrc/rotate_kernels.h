@@ -86,35 +86,28 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p) {
     turned[i] = x;
   }
   wave_fence();
-  // this lane's values: V from `a` on and V from `b` on
+  // This lane's values: V from `a` on and V from `b` on, both in order over the lanes, so that a load takes whole lines.  In the
+  // half layout they are pairs' two sides, interleaved each holds V / 2 pairs.
+  const int half = p.D / 2, plain = c - pairs / V;  // plain: of the lanes that hold what is not turned
   const bool inside = c < p.D / (2 * V), turns = INTERLEAVED || c * V < pairs;
-  const int a = INTERLEAVED || !turns ? 2 * V * c : c * V, b = INTERLEAVED || !turns ? a + V : pairs + c * V;
+  const int a = turns ? V * c : p.R + V * plain;
+  const int b = INTERLEAVED ? half + V * c : turns ? pairs + V * c : p.R + (p.D - p.R) / 2 + V * plain;
   float cosine[V], sine[V];
+  bool turn[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const bool turn = c * V + i < pairs;
-    const float2 x = turn ? turned[c * V + i] : float2{1.f, 0.f};
+    const int pair = INTERLEAVED ? (i < V / 2 ? a / 2 + i : b / 2 + i - V / 2) : c * V + i;
+    turn[i] = pair < pairs;
+    const float2 x = turn[i] ? turned[pair] : float2{1.f, 0.f};
     cosine[i] = x.x, sine[i] = x.y;
   }
-  // a turn's rows, loaded a turn ahead
-  const auto row_at = [&](int base) { return base + mine; };
-  const auto load = [&](int base, Word& wa, Word& wb) {
-    const int row = row_at(base);
-    const bool query = row < p.Hq;
-    const int head = query ? row : row - p.Hq;
-    const uint16_t* const src = query ? p.q + t * p.q_token + head * p.q_head : p.k + t * p.k_token + head * p.k_head;
-    wa = Word{}, wb = Word{};
-    if (inside && row < rows && live) wa = *(const Word*)(src + a), wb = *(const Word*)(src + b);
-  };
-  const int step = p.parts * teams;
-  Word next_a, next_b;
-  load(part * teams, next_a, next_b);
-  for (int base = part * teams; base < rows; base += step) {
-    const int row = row_at(base);
+  for (int base = part * teams; base < rows; base += p.parts * teams) {
+    const int row = base + mine;
     const bool ok = inside && row < rows, query = row < p.Hq;
     const int head = query ? row : row - p.Hq;
-    Word wa = next_a, wb = next_b;
-    if (base + step < rows) load(base + step, next_a, next_b);
+    const uint16_t* const src = query ? p.q + t * p.q_token + head * p.q_head : p.k + t * p.k_token + head * p.k_head;
+    Word wa = {}, wb = {};
+    if (ok && live) wa = *(const Word*)(src + a), wb = *(const Word*)(src + b);
     float x[V], y[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -148,8 +141,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateParams p) {
       for (int i = 0; i < V; ++i) {
         float* const z = i < V / 2 ? x + 2 * i : y + 2 * i - V;
         const float u = z[0], v = z[1];
-        const bool turn = c * V + i < pairs;  // others keep infinities that a product with 0 would not
-        z[0] = turn ? u * cosine[i] - v * sine[i] : u, z[1] = turn ? v * cosine[i] + u * sine[i] : v;
+        // others keep infinities that a product with 0 would not
+        z[0] = turn[i] ? u * cosine[i] - v * sine[i] : u, z[1] = turn[i] ? v * cosine[i] + u * sine[i] : v;
       }
     } else if (turns) {
 #pragma unroll
