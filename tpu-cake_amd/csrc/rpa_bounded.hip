@@ -149,7 +149,7 @@ int rpa_weighed_attention(const rpa_weigh_shape_t* shape, const rpa_weigh_option
   p.q_token = s.q_token_stride, p.q_head = s.q_head_stride;
   p.T = s.num_tokens, p.Hkv = s.num_kv_heads, p.G = s.num_q_heads / s.num_kv_heads, p.D = s.head_dim;
   p.P = s.total_pages, p.S = s.page_size, p.N = s.max_num_seqs, p.PPS = s.pages_per_seq;
-  p.near = plan.near, p.ways = plan.ways, p.block_shift = plan.block_shift, p.one_page = s.page_size % 32 == 0;
+  p.near = plan.near, p.ways = plan.ways, p.block_shift = plan.block_shift, p.one_page = s.page_size % 32 == 0, p.few = plan.few;
   p.rows_grid = plan.rows_grid, p.tiles_grid = plan.tiles_grid;
   p.joins = (JoinOf*)((uint8_t*)workspace + plan.joins);
   p.quads = s.page_size % 4 == 0 && aligned16(weights);

@@ -50,6 +50,7 @@ struct WeighParams {
   int near, ways; // rows: kv heads of a workgroup, waves that share a head's keys
   int block_shift;  // log2 of the keys of a block of rows' work: two units of 32 for each wave of a head
   int rows_grid, tiles_grid;  // workgroups of rows and of tiles
+  int few;        // at most kFewSeqs sequences, and all sums of work fit 32 bits
   int one_page;   // 32 keys from a multiple of 32 on lie in one page
   int quads;      // four neighbouring weights from a multiple of four on are 16 aligned bytes
   int chunk;      // sequences of more than one token are done in tiles
@@ -113,10 +114,78 @@ __device__ __forceinline__ Sequence work_sequence(const WeighParams& p, int coun
   return {end, p.T - end, 0};
 }
 
-// amount(sequence, pad): its units.  NEAR: XCDs take workgroups in turn; neighbouring shares, which read the same keys,
-// go to one of them.
+// The index of a workgroup's share, of as many as hold anything.  NEAR: XCDs take workgroups in turn; neighbouring shares,
+// which read the same keys, go to one of them.
+template <bool NEAR>
+__device__ __forceinline__ int share_index(int block, int blocks, int used) {
+  if (!NEAR) return block;
+  const int xcd = block % 8;
+  return block < used ? xcd * (used / 8) + min(xcd, used % 8) + block / 8 : blocks;
+}
+
+// As share_of, where there are at most kFewSeqs sequences and all sums fit 32 bits: each wave by itself, four sequences a
+// lane, without LDS or a barrier.  Four short sequences' call takes 15 us with it, 20 without.
+constexpr int kFewSeqs = 255;
+
+template <bool NEAR, typename Amount>
+__device__ __forceinline__ Share share_of_few(const WeighParams& p, int block, int blocks, Amount amount, bool flag) {
+  constexpr int kEach = (kFewSeqs + 64) / 64;
+  const int lane = threadIdx.x % 64, capacity = p.PPS * p.S, each = p.N / 64 + 1;
+  int c0[kEach], c1[kEach], len[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = min(lane * each + k, p.N);
+    c0[k] = p.cu[i], c1[k] = p.cu[min(i + 1, p.N)], len[k] = p.kv_lens[min(i, p.N - 1)];
+  }
+  const int count = min(max(*p.num_seqs, 0), p.N);
+  Sequence s[kEach];
+  int units[kEach][3], own[3] = {0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = lane * each + k, begin = min(max(c0[k], 0), p.T), end = min(max(c1[k], 0), p.T);
+    const bool ok = k < each && i < count, pad = k < each && i == count;
+    s[k] = {pad && !count ? 0 : begin, ok ? max(end - begin, 0) : pad ? p.T - (count ? begin : 0) : 0, ok ? min(max(len[k], 0), capacity) : 0};
+    if (flag && ok && s[k].tokens && len[k] > capacity) flag_error(RPA_SPARSE_ERR_LEN);
+    units[k][0] = (int)amount(s[k], pad), units[k][1] = ok ? (int)score_blocks(s[k]) : 0, units[k][2] = (int)row_units(p, s[k], pad);
+#pragma unroll
+    for (int u = 0; u < 3; ++u) own[u] += units[k][u];
+  }
+  int upto[3] = {own[0], own[1], own[2]};
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      const int o = __shfl_up(upto[u], d);
+      upto[u] += lane >= d ? o : 0;
+    }
+  const int total = __builtin_amdgcn_readlane(upto[0], 63), row_total = __builtin_amdgcn_readlane(upto[2], 63);
+  const int each_share = (int)(((long long)total + blocks - 1) / blocks);
+  const int index = total ? share_index<NEAR>(block, blocks, (total + each_share - 1) / each_share) : block;
+  const int from = (int)min((long long)index * each_share, (long long)total), to = min(from + each_share, total);
+  if (from >= to) return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0};
+  int before[3] = {upto[0] - own[0], upto[1] - own[1], upto[2] - own[2]}, at = 0;
+  const int hit = __builtin_ctzll(__ballot(from >= before[0] && from < upto[0]));
+  Sequence mine = s[0];
+  bool past = true;  // of the sequences so far
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    past = past && k < each && from >= before[0] + units[k][0];
+    if (past) {
+#pragma unroll
+      for (int u = 0; u < 3; ++u) before[u] += units[k][u];
+      at = k + 1;
+      if (k + 1 < kEach) mine = s[k + 1];
+    }
+  }
+  const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, hit); };
+  return Share{index, from, to, hit * each + of(at), count, {of(mine.first), of(mine.tokens), of(mine.keys)}, of(before[0]), of(before[1]),
+               of(before[2]), row_total};
+}
+
+// amount(sequence, pad): its units.
 template <bool NEAR, typename Amount>
 __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int blocks, Amount amount, bool flag = false) {
+  if (p.few) return share_of_few<NEAR>(p, block, blocks, amount, flag);
   __shared__ long long s_sum[3][kMostWaves];
   __shared__ Share s_share;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, waves = blockDim.x / 64, capacity = p.PPS * p.S;
@@ -157,11 +226,7 @@ __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int b
       total[u] += s_sum[u][w];
     }
   const long long each_share = (total[0] + blocks - 1) / blocks;
-  int index = block;
-  if (NEAR && total[0]) {
-    const int used = (int)((total[0] + each_share - 1) / each_share), xcd = index % 8;
-    index = index < used ? xcd * (used / 8) + min(xcd, used % 8) + index / 8 : blocks;
-  }
+  const int index = total[0] ? share_index<NEAR>(block, blocks, (int)((total[0] + each_share - 1) / each_share)) : block;
   const long long from = min(index * each_share, total[0]), to = min(from + each_share, total[0]);
   if (from < to && from >= upto[0] - own[0] && from < upto[0]) {
     long long before[3] = {upto[0] - own[0], upto[1] - own[1], upto[2] - own[2]};

@@ -553,6 +553,7 @@ int check_weigh(const rpa_weigh_shape_t* s) {
 
 struct WeighPlan {
   int tiles, near, ways, block_shift, rows_grid, tiles_grid, weigh_grid, keys_grid;  // tiles_grid 0: rows only
+  bool few;
   size_t rows_lds;
   long long score_room;
   size_t stats, parts, scores, joins, bytes;
@@ -599,6 +600,12 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
     r.tiles_grid = (int)(slots < fill ? slots : fill);
     r.bytes += (size_t)r.tiles_grid * 2 * kColumns * (2 + (size_t)s.head_dim) * 4;
   }
+  // the largest that share_of's sums can be, whatever the offsets say: each sequence may claim all tokens
+  const long long claims = most(s.max_num_seqs, s.num_tokens);
+  const long long by_rows = most(most(claims, s.num_kv_heads / r.near * r.tiles), (capacity >> r.block_shift) + 2);
+  const long long by_tiles = most(most(most(claims, group) / kColumns + s.max_num_seqs, s.num_kv_heads), capacity / kSlotKeys + 2);
+  const long long by_keys = most(most(s.max_num_seqs, s.num_kv_heads), capacity / 16 + 2), limit = 1 << 30;
+  r.few = s.max_num_seqs <= kFewSeqs && by_rows < limit && by_tiles < limit && by_keys < limit;
   r.joins = (r.bytes + 31) / 32 * 32;
   r.bytes = r.joins + (size_t)(r.rows_grid + r.tiles_grid) * sizeof(JoinOf);
   return r;
