@@ -447,15 +447,26 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
     const int end_row = s.tokens * p.G, begin_row = max(part - old, 0) * p.G;
     u32x4 w[kLoads];
     float2 st = {0.f, 0.f};
+    // This thread's rows of a stage, kApart apart, as (token, head) and where they lie: found once, then stepped.
+    constexpr int kChunks = DP * 2 / 16, kApart = kWeighThreads / kChunks;
+    const int dim = tid % kChunks * 8, step_tokens = div_by(kWeighRows, p.group), step_heads = kWeighRows - step_tokens * p.G;
+    const long long step = step_tokens * p.q_token + step_heads * p.q_head, wrap = p.q_token - p.G * p.q_head;
+    const uint16_t* at_q[kLoads];
+    int head[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = begin_row + tid / kChunks + i * kApart, token = div_by(row, p.group);
+      head[i] = row - token * p.G;
+      at_q[i] = p.q + (s.first + token) * p.q_token + ((long long)h * p.G + head[i]) * p.q_head + dim;
+    }
     const auto load = [&](int base) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        constexpr int kChunks = DP * 2 / 16;
-        const int row = base + tid / kChunks + i * (kWeighThreads / kChunks), dim = tid % kChunks * 8;
-        const int token = div_by(min(row, end_row - 1), p.group), g = min(row, end_row - 1) - token * p.G;
         w[i] = u32x4{0, 0, 0, 0};
-        if (row < end_row && (FULL || dim < p.D))
-          w[i] = *(const u32x4*)(p.q + (s.first + token) * p.q_token + ((long long)h * p.G + g) * p.q_head + dim);
+        if (base + tid / kChunks + i * kApart < end_row && (FULL || dim < p.D)) w[i] = *(const u32x4*)at_q[i];
+        head[i] += step_heads;
+        at_q[i] += step;
+        if (head[i] >= p.G) head[i] -= p.G, at_q[i] += wrap;
       }
       if (tid < kWeighRows) {
         const int row = base + tid, token = div_by(min(row, end_row - 1), p.group), g = min(row, end_row - 1) - token * p.G;
@@ -464,10 +475,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
     };
     const auto store = [&](int turn) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        constexpr int kChunks = DP * 2 / 16;
-        *(u32x4*)(s_q[turn & 1] + (tid / kChunks + i * (kWeighThreads / kChunks)) * kRow + tid % kChunks * 16) = w[i];
-      }
+      for (int i = 0; i < kLoads; ++i) *(u32x4*)(s_q[turn & 1] + (tid / kChunks + i * kApart) * kRow + tid % kChunks * 16) = w[i];
       if (tid < kWeighRows) s_stat[turn & 1][tid] = st;
     };
     float sum[kBlocks][16];
@@ -511,16 +519,14 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = scaled(p.cap * tanhf(sc[r] / p.cap), kLog2e);
           }
-          if (whole) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[b][r] += __builtin_amdgcn_exp2f(sc[r] - stat.x) * stat.y;
-          } else {
+          for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(sc[r] - stat.x);
+          if (!whole) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float e = __builtin_amdgcn_exp2f(sc[r] - stat.x) * stat.y;
-              sum[b][r] += key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= seen ? e : 0.f;
-            }
+            for (int r = 0; r < 16; ++r) sc[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= seen ? sc[r] : 0.f;
           }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum[b][r] = __builtin_fmaf(sc[r], stat.y, sum[b][r]);
         }
       }
       if (base + kWeighRows < end_row) store(turn + 1);
