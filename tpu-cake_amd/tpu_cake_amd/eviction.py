@@ -56,10 +56,6 @@ def _keep(sig: tuple, plan: tuple) -> tuple:
     return plan
 
 
-def _key(t):
-    return None if t is None else (t.shape, t.dtype, t.get_device(), t.is_contiguous())
-
-
 def _ledger(ledger, shape, device) -> None:
     if not (isinstance(ledger, tuple) and len(ledger) == 2):
         raise TypeError("ledger must be a Ledger")
@@ -107,9 +103,19 @@ def weighed_attention(
     Scores, softmax, probabilities and sums are fp32; scaled keys and values are not rounded.  The pages of different
     sequences have to differ (``preflight_pages`` checks it on the host).
     """
-    sig = (q.shape, q.dtype, q.get_device(), q.stride(), _key(kv_pages), _key(ledger[0]), _key(ledger[1]), _key(kv_lens),
-           _key(page_indices), _key(cu_q_lens), _key(num_seqs), _key(dropped), _key(kv_scales), sm_scale, soft_cap, decay,
-           k_scale, v_scale)
+    # what the checks go by: written out, as a call costs less than a helper's calls would
+    weights, positions = ledger
+    sig = (q.shape, q.dtype, q.get_device(), q.stride(),
+           kv_pages.shape, kv_pages.dtype, kv_pages.get_device(), kv_pages.is_contiguous(),
+           weights.shape, weights.dtype, weights.get_device(), weights.is_contiguous(),
+           positions.shape, positions.dtype, positions.get_device(), positions.is_contiguous(),
+           kv_lens.shape, kv_lens.dtype, kv_lens.get_device(), kv_lens.is_contiguous(),
+           page_indices.shape, page_indices.dtype, page_indices.get_device(), page_indices.is_contiguous(),
+           cu_q_lens.shape, cu_q_lens.dtype, cu_q_lens.get_device(), cu_q_lens.is_contiguous(),
+           num_seqs.shape, num_seqs.dtype, num_seqs.get_device(), num_seqs.is_contiguous(),
+           None if dropped is None else (dropped.shape, dropped.dtype, dropped.get_device(), dropped.is_contiguous()),
+           None if kv_scales is None else (kv_scales.shape, kv_scales.dtype, kv_scales.get_device(), kv_scales.is_contiguous()),
+           sm_scale, soft_cap, decay, k_scale, v_scale)
     plan = _plans.get(sig)
     if plan is None:
         pages, page_size, heads, dim, code = _pool(kv_pages)
@@ -149,7 +155,7 @@ def weighed_attention(
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     rc = fn(shape, options, q.data_ptr(), kv_pages.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(),
             kv_lens.data_ptr(), page_indices.data_ptr(), cu_q_lens.data_ptr(), num_seqs.data_ptr(),
-            None if dropped is None else dropped.data_ptr(), ledger[0].data_ptr(), ledger[1].data_ptr(), out.data_ptr(),
+            None if dropped is None else dropped.data_ptr(), weights.data_ptr(), positions.data_ptr(), out.data_ptr(),
             scratch.data_ptr() if need else None, need, _current_stream(dev))
     if rc:
         _bounded_lib.check(rc)
@@ -180,8 +186,14 @@ def choose_moves(
     ``max_moves`` may be less where sequences grow by few tokens between two evictions: a sequence of n keys needs
     at most n - budget moves.  A list that needs more is cut short and sets ``ERR_LEN`` in the error word.
     """
-    sig = (_key(ledger[0]), _key(ledger[1]), _key(kv_lens), _key(page_indices), _key(num_seqs), _key(dropped), budget, recent,
-           sinks, limit, max_moves)
+    weights, positions = ledger
+    sig = (weights.shape, weights.dtype, weights.get_device(), weights.is_contiguous(),
+           positions.shape, positions.dtype, positions.get_device(), positions.is_contiguous(),
+           kv_lens.shape, kv_lens.dtype, kv_lens.get_device(), kv_lens.is_contiguous(),
+           page_indices.shape, page_indices.dtype, page_indices.get_device(), page_indices.is_contiguous(),
+           num_seqs.shape, num_seqs.dtype, num_seqs.get_device(), num_seqs.is_contiguous(),
+           None if dropped is None else (dropped.shape, dropped.dtype, dropped.get_device(), dropped.is_contiguous()),
+           budget, recent, sinks, limit, max_moves)
     plan = _plans.get(sig)
     if plan is None:
         _ledger(ledger, (None, None, None), None)
@@ -216,7 +228,7 @@ def choose_moves(
             return choose_moves(ledger, kv_lens, page_indices, num_seqs, budget=budget, recent=recent, sinks=sinks, limit=limit,
                                 dropped=dropped, max_moves=max_moves, out=out)
     scratch = torch.empty(need, dtype=torch.uint8, device=kv_lens.device) if need else None
-    rc = fn(shape, ledger[0].data_ptr(), ledger[1].data_ptr(), kv_lens.data_ptr(), page_indices.data_ptr(), num_seqs.data_ptr(),
+    rc = fn(shape, weights.data_ptr(), positions.data_ptr(), kv_lens.data_ptr(), page_indices.data_ptr(), num_seqs.data_ptr(),
             None if dropped is None else dropped.data_ptr(), out.data_ptr(), scratch.data_ptr() if need else None, need,
             _current_stream(dev))
     if rc:
@@ -238,7 +250,12 @@ def move_rows(
     here), saturated at +-448.  Slots outside the pool are skipped and set ``ERR_SLOT`` in the error word.  No slot that is
     written may be another entry's of the same head, as those of ``choose_moves`` are not.
     """
-    sig = (_key(kv_pages), _key(ledger[0]), _key(ledger[1]), _key(moves), _key(kv_scales))
+    weights, positions = ledger
+    sig = (kv_pages.shape, kv_pages.dtype, kv_pages.get_device(), kv_pages.is_contiguous(),
+           weights.shape, weights.dtype, weights.get_device(), weights.is_contiguous(),
+           positions.shape, positions.dtype, positions.get_device(), positions.is_contiguous(),
+           moves.shape, moves.dtype, moves.get_device(), moves.is_contiguous(),
+           None if kv_scales is None else (kv_scales.shape, kv_scales.dtype, kv_scales.get_device(), kv_scales.is_contiguous()))
     plan = _plans.get(sig)
     if plan is None:
         pages, page_size, heads, dim, code = _pool(kv_pages)
@@ -256,6 +273,6 @@ def move_rows(
         with torch.cuda.device(dev):
             return move_rows(kv_pages, ledger, moves, kv_scales=kv_scales)
     rc = fn(shape, moves.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(), kv_pages.data_ptr(),
-            ledger[0].data_ptr(), ledger[1].data_ptr(), _current_stream(dev))
+            weights.data_ptr(), positions.data_ptr(), _current_stream(dev))
     if rc:
         _bounded_lib.check(rc)

@@ -71,10 +71,6 @@ def _weight(name: str, w, heads: int, dim: int, device):
     return w.dtype, dim if w.dim() == 2 else 0
 
 
-def _key(t):
-    return None if t is None else (t.shape, t.dtype, t.get_device(), t.stride())
-
-
 def rotate_heads(
     q: torch.Tensor,          # bf16 [T, Hq, D]
     k: torch.Tensor,          # bf16 [T, Hkv, D]
@@ -103,15 +99,21 @@ def rotate_heads(
     or past ``cu_q_lens[num_seqs]`` are zero, and left as they are in place; without them every row is done.
     ``rotated`` is a multiple of 8 (``interleaved``: of 2); head dims and strides are those of ``sparse``.
     """
+    # what the checks go by: written out, as a call costs less than a helper's calls would
     sig = (q.shape, q.dtype, q.get_device(), q.stride(), k.shape, k.dtype, k.get_device(), k.stride(),
            positions.shape, positions.dtype, positions.get_device(), positions.is_contiguous(),
            turns.shape, turns.dtype, turns.get_device(), turns.is_contiguous(), interleaved, magnitude, eps,
-           _key(q_weight), _key(k_weight), _key(cu_q_lens), _key(num_seqs), _key(dropped),
-           None if out is None else (_key(out[0]), _key(out[1])))
+           None if q_weight is None else (q_weight.shape, q_weight.dtype, q_weight.get_device(), q_weight.is_contiguous()),
+           None if k_weight is None else (k_weight.shape, k_weight.dtype, k_weight.get_device(), k_weight.is_contiguous()),
+           None if cu_q_lens is None else (cu_q_lens.shape, cu_q_lens.dtype, cu_q_lens.get_device(), cu_q_lens.is_contiguous()),
+           None if num_seqs is None else (num_seqs.shape, num_seqs.dtype, num_seqs.get_device(), num_seqs.is_contiguous()),
+           None if dropped is None else (dropped.shape, dropped.dtype, dropped.get_device(), dropped.is_contiguous()),
+           None if out is None else (out[0].shape, out[0].dtype, out[0].get_device(), out[0].stride(),
+                                     out[1].shape, out[1].dtype, out[1].get_device(), out[1].stride()))
     plan = _plans.get(sig)
     if plan is None:
         i32 = torch.int32
-        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        if q.dim() != 3:
             raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
         device, tokens, dim = q.device, q.shape[0], q.shape[2]
         _tensor("q", q, torch.bfloat16, (tokens, None, dim), None, rows=True)
