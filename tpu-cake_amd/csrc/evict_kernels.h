@@ -22,6 +22,8 @@ struct ChooseParams {
   int32_t* moves;
   uint32_t* keys;    // of rows past kChooseRows: for each (sequence, head) `stride` keys, then `counts`' blocks
   uint32_t* counts;  // 2048 for each block of kKeyRows
+  uint32_t* found;   // of each (sequence, head): the budget-th largest key and how many of the rows at it stay
+  uint32_t* tallies; // a Tally for each block of kKeyRows
   long long stride;
   int N, PPS, Hkv, P, S, budget, limit, sinks, recent, M;
   int first;         // the launch's first sequence
@@ -32,8 +34,11 @@ struct ChooseParams {
 // The order of weights as whole numbers, 0 for NaN; zeros of both signs are equal.
 __device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? ordered(w + 0.f) : 0u; }
 
-constexpr int kChooseRows = 32768;  // rows of a sequence whose keys fit LDS
-constexpr int kKeyRows = 4096;      // rows of a workgroup that makes a longer one's keys
+// Rows of a sequence whose keys fit LDS: one workgroup does all (48 lists of 32768: 35 us, 40 by blocks; 512: 86 and 119).
+// Past them its VALU would be what counts (24 lists of 131072: 132 us), so keys, tallies and lists are made by blocks of
+// kKeyRows and only the digits are found by one workgroup: 62 us, 34 of them the digits.
+constexpr int kChooseRows = 32768;
+constexpr int kKeyRows = 4096;
 constexpr int kDigits = 2048;       // 11 bits, 11 bits, 10 bits
 
 // A sequence that is cut: its rows (0: it is not), and the position past its last.
@@ -85,6 +90,87 @@ __device__ __forceinline__ u32x4 keys_at(const ChooseParams& p, const int32_t* t
   return key;
 }
 
+// Rows at the key before the budget and past it, above it and past, below it and before.
+struct Tally {
+  uint32_t same_low, same_high, more, less;
+
+  __device__ __forceinline__ void rows(int row, const u32x4& key, int n, int budget, uint32_t bound) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (row + u >= n) continue;
+      const bool low = row + u < budget, same = key[u] == bound;
+      same_low += same && low, same_high += same && !low;
+      more += key[u] > bound && !low, less += key[u] < bound && low;
+    }
+  }
+  __device__ __forceinline__ void add(const Tally& o) {
+    same_low += o.same_low, same_high += o.same_high, more += o.more, less += o.less;
+  }
+  __device__ __forceinline__ void of_wave() {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      same_low += __shfl_xor(same_low, d), same_high += __shfl_xor(same_high, d);
+      more += __shfl_xor(more, d), less += __shfl_xor(less, d);
+    }
+  }
+};
+
+// Writes a (sequence, head)'s list from some row on, by one wave.
+struct Lister {
+  int32_t* list;
+  const int32_t* table;
+  uint32_t bound, rank;       // the key, and how many of the rows at it stay, the lowest
+  uint32_t same, late, holes; // rows at the key, rows that move and places for them before the next row
+
+  __device__ __forceinline__ void start(const Tally& before, uint32_t all_low) {
+    const uint32_t stay_low = min(rank, all_low);
+    same = before.same_low + before.same_high;
+    late = before.more + (min(rank, same) > stay_low ? min(rank, same) - stay_low : 0u);
+    holes = before.less + before.same_low - min(rank, before.same_low);
+  }
+  __device__ __forceinline__ uint32_t moved(const Tally& all) const {
+    return all.more + min(rank, all.same_low + all.same_high) - min(rank, all.same_low);
+  }
+  __device__ __forceinline__ void rows(const ChooseParams& p, int row, int lane, const u32x4& key, int end) {  // of the whole wave
+    const auto slot_of = [&](int at) {  // -1: no such page
+      const int page = table[at / p.S];
+      return page >= 0 && page < p.P ? page * p.S + at % p.S : -1;
+    };
+    int slot = -1;  // of the first, where the four are of one page
+    if (p.quads && row < end) slot = slot_of(row);
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t mine = same;  // rows at the key before this lane's
+    bool is[4];
+    uint32_t count = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      is[u] = row + u < end && key[u] == bound;
+      const uint64_t votes = __ballot(is[u]);
+      mine += __popcll(votes & below), count += __popcll(votes);
+    }
+    same += count;
+    bool comes[4], goes[4];
+    uint32_t late_at = late, hole_at = holes;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool there = row + u < end, kept = there && (key[u] > bound || (is[u] && mine < rank));
+      mine += is[u];
+      comes[u] = kept && row + u >= p.budget, goes[u] = there && !kept && row + u < p.budget;
+      const uint64_t a = __ballot(comes[u]), b = __ballot(goes[u]);
+      late_at += __popcll(a & below), hole_at += __popcll(b & below);
+      late += __popcll(a), holes += __popcll(b);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!comes[u] && !goes[u]) continue;
+      const int at = !p.quads ? slot_of(row + u) : slot < 0 ? -1 : slot + u;
+      if (comes[u] && late_at < (uint32_t)p.M) list[2 * (size_t)late_at + 1] = at;
+      if (goes[u] && hole_at < (uint32_t)p.M) list[2 * (size_t)hole_at] = at;
+      late_at += comes[u], hole_at += goes[u];
+    }
+  }
+};
+
 // Keys of long sequences, and how many of a block's rows have each first digit.
 __global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
   __shared__ uint32_t s_count[kDigits];
@@ -108,148 +194,213 @@ __global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
   for (int i = tid; i < kDigits; i += 256) counts[i] = s_count[i];
 }
 
+struct ChooseShared {
+  uint32_t count[kDigits];
+  uint32_t sum[16], found[2], held;
+  Tally waves[16];
+};
+
+// The budget-th largest key, and which one it is of the rows at it: its digits one after another.  INSIDE: all keys fit
+// LDS.  Otherwise choose_keys_kernel has made them, and LDS takes those that have the first digit.
+template <int THREADS, bool INSIDE>
+__device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, int h, const int32_t* table, int blocks,
+                                         uint32_t* s_keys, ChooseShared& sh, uint32_t& prefix, uint32_t& rank) {
+  constexpr int kBins = kDigits / THREADS, kAhead = 8;  // loads of a thread in flight
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut.rows;
+  prefix = 0, rank = p.budget;
+  int held = -1;  // keys in LDS that have the first digit; -1: not there
+  for (int shift = 21, bits = 11; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1, bits = shift ? 11 : 10) {
+    const bool first = shift == 21;
+    const auto count = [&](uint32_t key) { atomicAdd(&sh.count[key >> shift & ((1u << bits) - 1)], 1u); };
+    const auto begins = [&](uint32_t key) { return key >> (shift + bits) == prefix; };
+    if (first && !INSIDE) {
+      const int used = (n + kKeyRows - 1) / kKeyRows;
+      const uint32_t* const from = p.counts + (size_t)blockIdx.x * blocks * kDigits;
+      uint32_t sum[kBins] = {};
+#pragma unroll 16
+      for (int b = 0; b < used; ++b)
+#pragma unroll
+        for (int i = 0; i < kBins; ++i) sum[i] += from[(size_t)b * kDigits + tid * kBins + i];
+#pragma unroll
+      for (int i = 0; i < kBins; ++i) sh.count[tid * kBins + i] = sum[i];
+      if (tid == 0) sh.held = 0;
+    } else {
+      for (int i = tid; i < kDigits; i += THREADS) sh.count[i] = 0;
+      __syncthreads();
+      if (first) {
+        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
+          const u32x4 key = keys_at(p, table, h, cut, row);
+          *(u32x4*)(s_keys + row) = key;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (row + u < n) count(key[u]);
+        }
+      } else if (INSIDE) {
+        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
+          const u32x4 key = *(const u32x4*)(s_keys + row);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (row + u < n && begins(key[u])) count(key[u]);
+        }
+      } else if (held < 0) {
+        const uint32_t* const keys = p.keys + (size_t)blockIdx.x * p.stride;
+        for (int at = 4 * (tid - lane); at < n; at += 4 * THREADS * kAhead) {  // uniform in a wave
+          u32x4 key[kAhead];
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) {
+            const int row = at + 4 * THREADS * x + 4 * lane;
+            if (row < n) key[x] = *(const u32x4*)(keys + row);
+          }
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) {
+            const int row = at + 4 * THREADS * x + 4 * lane;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const bool is = row + u < n && begins(key[x][u]);
+              const uint64_t votes = __ballot(is);
+              if (is) count(key[x][u]);
+              if (shift != 10 || !votes) continue;  // uniform
+              uint32_t place = 0;
+              if (lane == 0) place = atomicAdd(&sh.held, (uint32_t)__popcll(votes));  // their order does not count
+              place = __shfl(place, 0) + __popcll(votes & ((1ull << lane) - 1));
+              if (is && place < (uint32_t)p.room) s_keys[place] = key[x][u];
+            }
+          }
+        }
+      } else {
+        for (int i = tid; i < held; i += THREADS)
+          if (begins(s_keys[i])) count(s_keys[i]);
+      }
+    }
+    __syncthreads();
+    // the largest digits first: thread 0 has the last kBins
+    uint32_t own = 0;
+    const int top = kDigits - 1 - tid * kBins;
+#pragma unroll
+    for (int i = 0; i < kBins; ++i) own += sh.count[top - i];
+    uint32_t upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(upto, d);
+      upto += lane >= d ? o : 0u;
+    }
+    if (lane == 63) sh.sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += sh.sum[w];
+    if (upto - own < rank && rank <= upto) {
+      uint32_t above = upto - own;
+      int d = top;
+      while (above + sh.count[d] < rank) above += sh.count[d--];
+      sh.found[0] = prefix << bits | d, sh.found[1] = rank - above;
+    }
+    __syncthreads();
+    prefix = sh.found[0], rank = sh.found[1];
+    if (!INSIDE && shift == 10) held = sh.held <= (uint32_t)p.room ? (int)sh.held : -1;
+  }
+}
+
+// The list of rows whose keys are in LDS: every wave has a stretch of rows.
+template <int THREADS>
+__device__ __forceinline__ int list_rows(const ChooseParams& p, int n, const uint32_t* s_keys, ChooseShared& sh, Lister out) {
+  constexpr int kWaves = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int stretch = ((n + kWaves - 1) / kWaves + 255) / 256 * 256, from = min(wave * stretch, n), to = min(from + stretch, n);
+  Tally own = {};
+  for (int row = from + 4 * lane; row < to; row += 256) own.rows(row, *(const u32x4*)(s_keys + row), n, p.budget, out.bound);
+  own.of_wave();
+  if (lane == 0) sh.waves[wave] = own;
+  __syncthreads();
+  Tally before = {}, all = {};
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before.add(sh.waves[w]);
+    all.add(sh.waves[w]);
+  }
+  out.start(before, all.same_low);
+  for (int base = from; base < to; base += 256) {
+    const int row = base + 4 * lane;
+    out.rows(p, row, lane, row < to ? *(const u32x4*)(s_keys + row) : u32x4{0, 0, 0, 0}, to);
+  }
+  const uint32_t moved = out.moved(all);
+  if (moved > (uint32_t)p.M && tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
+  return (int)min(moved, (uint32_t)p.M);
+}
+
 // One workgroup a (kv head, sequence).  A step's loads are of 256 rows a wave, four neighbouring rows a lane.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void choose_rows_kernel(ChooseParams p, int blocks) {
-  constexpr int kWaves = THREADS / 64, kBins = kDigits / THREADS;
   extern __shared__ __align__(16) uint32_t s_keys[];
-  __shared__ uint32_t s_count[kDigits];
-  __shared__ uint32_t s_sum[kWaves], s_found[2];
-  __shared__ uint32_t s_waves[kWaves][4];
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  __shared__ ChooseShared s_rest;
   const int h = blockIdx.x % p.Hkv, seq = blockIdx.x / p.Hkv;
+  const int32_t* const table = p.table + (size_t)seq * p.PPS;
   int32_t* const list = p.moves + (size_t)blockIdx.x * p.M * 2;
-  const Cut cut = cut_of(p, seq, tid == 0);
-  const int n = cut.rows;
-  int done = 0;  // entries of the list
-  if (n) {       // uniform
-    const int32_t* const table = p.table + (size_t)seq * p.PPS;
-    const bool inside = n <= p.room;
-    const uint32_t* const far = p.keys + (size_t)blockIdx.x * p.stride;
-    const auto load = [&](int row) { return inside ? *(const u32x4*)(s_keys + row) : *(const u32x4*)(far + row); };
-    // the digits of the budget-th largest key, one after another; rank: which one it is of the keys that begin with them
-    uint32_t prefix = 0, rank = p.budget;
-    for (int shift = 21, bits = 11; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1, bits = shift ? 11 : 10) {
-      const bool first = shift == 21;
-      if (first && !inside) {
-        for (int i = tid; i < kDigits; i += THREADS) {
-          uint32_t sum = 0;
-          for (int b = 0; b < (n + kKeyRows - 1) / kKeyRows; ++b) sum += p.counts[((size_t)blockIdx.x * blocks + b) * kDigits + i];
-          s_count[i] = sum;
-        }
-      } else {
-        for (int i = tid; i < kDigits; i += THREADS) s_count[i] = 0;
-        __syncthreads();
-        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
-          u32x4 key;
-          if (first) {
-            key = keys_at(p, table, h, cut, row);
-            *(u32x4*)(s_keys + row) = key;
-          } else {
-            key = load(row);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (row + u < n && (first || key[u] >> (shift + bits) == prefix)) atomicAdd(&s_count[key[u] >> shift & ((1u << bits) - 1)], 1u);
-        }
-      }
-      __syncthreads();
-      // the largest digits first: thread 0 has the last kBins
-      uint32_t own = 0;
-      const int top = kDigits - 1 - tid * kBins;
-#pragma unroll
-      for (int i = 0; i < kBins; ++i) own += s_count[top - i];
-      uint32_t upto = own;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const uint32_t o = __shfl_up(upto, d);
-        upto += lane >= d ? o : 0u;
-      }
-      if (lane == 63) s_sum[wave] = upto;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) upto += s_sum[w];
-      if (upto - own < rank && rank <= upto) {
-        uint32_t above = upto - own;
-        int d = top;
-        while (above + s_count[d] < rank) above += s_count[d--];
-        s_found[0] = prefix << bits | d, s_found[1] = rank - above;
-      }
-      __syncthreads();
-      prefix = s_found[0], rank = s_found[1];
-    }
-    // rank: how many of the rows at this very key stay, the lowest.  Every wave has a stretch of rows.
-    const int stretch = ((n + kWaves - 1) / kWaves + 255) / 256 * 256, from = min(wave * stretch, n), to = min(from + stretch, n);
-    uint32_t same_low = 0, same_high = 0, more = 0, less = 0;  // rows at the key before the budget and past it; above and past; below and before
-#pragma unroll 4
-    for (int row = from + 4 * lane; row < to; row += 256) {
-      const u32x4 key = load(row);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (row + u >= n) continue;
-        const bool low = row + u < p.budget, same = key[u] == prefix;
-        same_low += same && low, same_high += same && !low;
-        more += key[u] > prefix && !low, less += key[u] < prefix && low;
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      same_low += __shfl_xor(same_low, d), same_high += __shfl_xor(same_high, d);
-      more += __shfl_xor(more, d), less += __shfl_xor(less, d);
-    }
-    if (lane == 0) s_waves[wave][0] = same_low, s_waves[wave][1] = same_high, s_waves[wave][2] = more, s_waves[wave][3] = less;
-    __syncthreads();
-    uint32_t all_low = 0, low = 0, high = 0, late = 0, holes = 0, all_late = 0, all_high = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) low += s_waves[w][0], high += s_waves[w][1], late += s_waves[w][2], holes += s_waves[w][3];
-      all_low += s_waves[w][0], all_high += s_waves[w][1], all_late += s_waves[w][2];
-    }
-    // rows at the key that stay: the first `rank`, before the budget first
-    const uint32_t stay_low = min(rank, all_low);
-    uint32_t same = low + high;  // seen so far
-    late += min(rank, same) > stay_low ? min(rank, same) - stay_low : 0u;
-    holes += low - min(rank, low);
-    all_late += min(rank, all_low + all_high) - stay_low;
-    const auto slot_of = [&](int row) {  // -1: no such page
-      const int page = table[row / p.S];
-      return page >= 0 && page < p.P ? page * p.S + row % p.S : -1;
-    };
-    const uint64_t below = (1ull << lane) - 1;
-#pragma unroll 2
-    for (int base = from; base < to; base += 256) {
-      const int row = base + 4 * lane;
-      const u32x4 key = row < to ? load(row) : u32x4{0, 0, 0, 0};
-      uint32_t mine = same;  // rows at the key before this lane's
-      bool is[4];
-      uint32_t count = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        is[u] = row < to && row + u < n && key[u] == prefix;
-        const uint64_t votes = __ballot(is[u]);
-        mine += __popcll(votes & below), count += __popcll(votes);
-      }
-      same += count;
-      bool comes[4], goes[4];
-      uint32_t late_at = late, hole_at = holes;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool there = row < to && row + u < n, kept = there && (key[u] > prefix || (is[u] && mine < rank));
-        mine += is[u];
-        comes[u] = kept && row + u >= p.budget, goes[u] = there && !kept && row + u < p.budget;
-        const uint64_t a = __ballot(comes[u]), b = __ballot(goes[u]);
-        late_at += __popcll(a & below), hole_at += __popcll(b & below);
-        late += __popcll(a), holes += __popcll(b);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (comes[u] && late_at < (uint32_t)p.M) list[2 * (size_t)late_at + 1] = slot_of(row + u);
-        if (goes[u] && hole_at < (uint32_t)p.M) list[2 * (size_t)hole_at] = slot_of(row + u);
-        late_at += comes[u], hole_at += goes[u];
-      }
-    }
-    if (all_late > (uint32_t)p.M && tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
-    done = (int)min(all_late, (uint32_t)p.M);
+  const Cut cut = cut_of(p, seq, threadIdx.x == 0);
+  uint32_t bound, rank;
+  if (THREADS == 1024 && cut.rows > p.room) {  // the list is choose_list_kernel's
+    find_key<THREADS, THREADS != 1024>(p, cut, h, table, blocks, s_keys, s_rest, bound, rank);
+    if (threadIdx.x == 0) p.found[2 * (size_t)blockIdx.x] = bound, p.found[2 * (size_t)blockIdx.x + 1] = rank;
+    return;
   }
-  for (long long i = 2ll * done + tid; i < 2ll * p.M; i += THREADS) list[i] = -1;
+  int done = 0;  // entries of the list
+  if (cut.rows) {
+    find_key<THREADS, true>(p, cut, h, table, blocks, s_keys, s_rest, bound, rank);
+    done = list_rows<THREADS>(p, cut.rows, s_keys, s_rest, Lister{list, table, bound, rank});
+  }
+  for (long long i = 2ll * done + threadIdx.x; i < 2ll * p.M; i += THREADS) list[i] = -1;
+}
+
+// Long sequences' lists, by blocks of kKeyRows: a wave has a quarter of a block.  First the blocks' tallies, then,
+// with those of the blocks before, the list.
+template <bool LIST>
+__global__ __launch_bounds__(256) void choose_list_kernel(ChooseParams p) {
+  constexpr int kSteps = kKeyRows / 1024;
+  __shared__ Tally s_waves[4], s_before[4], s_all[4];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, seq = blockIdx.y / p.Hkv;
+  const Cut cut = cut_of(p, seq, false);
+  const int n = cut.rows, used = (n + kKeyRows - 1) / kKeyRows, block = blockIdx.x;
+  if (n <= p.room || block >= used) return;  // uniform
+  Tally* const tallies = (Tally*)p.tallies + (size_t)blockIdx.y * gridDim.x;
+  const uint32_t bound = p.found[2 * (size_t)blockIdx.y], rank = p.found[2 * (size_t)blockIdx.y + 1];
+  const uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
+  const int from = block * kKeyRows + wave * (kKeyRows / 4) + 4 * lane;
+  u32x4 key[kSteps];
+#pragma unroll
+  for (int x = 0; x < kSteps; ++x) key[x] = from + 256 * x < n ? *(const u32x4*)(keys + from + 256 * x) : u32x4{0, 0, 0, 0};
+  Tally before = {}, all = {};  // of the blocks
+  if (LIST) {
+    for (int b = tid; b < used; b += 256) {
+      const Tally one = tallies[b];
+      if (b < block) before.add(one);
+      all.add(one);
+    }
+    before.of_wave(), all.of_wave();
+    if (lane == 0) s_before[wave] = before, s_all[wave] = all;
+  }
+  Tally own = {};
+#pragma unroll
+  for (int x = 0; x < kSteps; ++x) own.rows(from + 256 * x, key[x], n, p.budget, bound);
+  own.of_wave();
+  if (lane == 0) s_waves[wave] = own;
+  __syncthreads();
+  if (!LIST) {
+    if (tid) return;
+    for (int w = 1; w < 4; ++w) own.add(s_waves[w]);
+    tallies[block] = own;
+    return;
+  }
+  before = all = Tally{};
+  for (int w = 0; w < 4; ++w) {
+    before.add(s_before[w]), all.add(s_all[w]);
+    if (w < wave) before.add(s_waves[w]);
+  }
+  int32_t* const list = p.moves + (size_t)blockIdx.y * p.M * 2;
+  Lister out = {list, p.table + (size_t)seq * p.PPS, bound, rank};
+  out.start(before, all.same_low);
+#pragma unroll
+  for (int x = 0; x < kSteps; ++x) out.rows(p, from + 256 * x, lane, key[x], n);
+  const uint32_t moved = out.moved(all);
+  if (block == 0 && tid == 0 && moved > (uint32_t)p.M) flag_error(RPA_SPARSE_ERR_LEN);
+  const long long done = min(moved, (uint32_t)p.M);
+  for (long long i = 2 * done + block * 256 + tid; i < 2ll * p.M; i += 256ll * used) list[i] = -1;
 }
 
 struct MoveParams {
@@ -356,20 +507,25 @@ int check_choose(const rpa_choose_shape_t* s) {
 struct ChoosePlan {
   int threads, room, blocks;  // blocks 0: all keys fit LDS
   long long stride;
-  size_t keys, bytes;
+  size_t keys, counts, found, bytes;  // bytes up to the end of each
 };
 
-// Small workgroups where a sequence's rows are few: their barriers cost less.
+// Waves of a workgroup: sixteen while every list has a CU to itself (256 lists of 4096 rows: 13.0 us, 16.6 with four; of
+// 8192: 16.8 and 27.1), four where lists share one (512 of 4096: 24.1 and 19.3; of 8192: 35.0 and 33.2) or rows are
+// few, sixteen again past 8192 rows (512 of 16384: 52 and 57; of 24576: 69 and 137, as LDS holds one list either way).
 ChoosePlan plan_choose(const rpa_choose_shape_t& s) {
   ChoosePlan r = {};
   const long long capacity = (long long)s.pages_per_seq * s.page_size;
-  r.threads = capacity <= 8192 ? 256 : 1024;
+  r.threads = capacity > (s.max_num_seqs * (long long)s.num_kv_heads <= 256 ? 1024 : 8192) ? 1024 : 256;
   r.room = (int)((capacity < kChooseRows ? capacity : kChooseRows) + 3) / 4 * 4;
   if (capacity > kChooseRows) {
     r.blocks = (int)((capacity + kKeyRows - 1) / kKeyRows);
     r.stride = (capacity + 3) / 4 * 4;
     r.keys = (size_t)s.max_num_seqs * s.num_kv_heads * r.stride * 4;
-    r.bytes = r.keys + (size_t)s.max_num_seqs * s.num_kv_heads * r.blocks * kDigits * 4;
+    const size_t lists = (size_t)s.max_num_seqs * s.num_kv_heads;
+    r.counts = r.keys + lists * r.blocks * kDigits * 4;
+    r.found = r.counts + (lists * 8 + 15) / 16 * 16;
+    r.bytes = r.found + lists * r.blocks * sizeof(Tally);
   }
   return r;
 }
