@@ -63,6 +63,21 @@ def test_long_sequences(cuda):
     c.choose(budget=3000, recent=64)
 
 
+@pytest.mark.parametrize("lens,hkv", [([1500] * 20 + [40] * 130, 2), ([9000] + [300] * 140, 2), ([40000] + [500] * 40, 7)])
+def test_many_lists(cuda, lens, hkv):
+    c = Cache(len(lens), lens, 16, hkv)
+    c.choose(budget=200, recent=20, sinks=4, limit=260, max_moves=200)
+
+
+def test_long_sequences_of_one_weight(cuda):
+    """More rows begin with the bound's first digit than LDS holds."""
+    c = Cache(7, [40000, 35000], 16, 2)
+    c.weights[:] = 0.25
+    c.choose(budget=3000, recent=64, sinks=4)
+    c.weights.reshape(-1)[::3] = 0.25000003
+    c.choose(budget=13500, recent=64, max_moves=13500)
+
+
 def test_lists_that_are_too_short(cuda):
     c = Cache(3, [300, 120], 16, 2, ties=True)
     eviction.read_error_word(clear=True)

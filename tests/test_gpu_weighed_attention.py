@@ -194,6 +194,42 @@ def test_many_sequences(cuda):
     _check(b, _state(b))
 
 
+def test_chunks_of_many_sequences(cuda):
+    """More sequences than one wave counts, some of one token."""
+    rng = np.random.default_rng(22)
+    lens = rng.integers(1, 60, 300)
+    new = np.minimum(rng.integers(1, 9, 300), lens)
+    b = Batch(22, lens.tolist(), new.tolist(), 16, 4, 2, 64, spare=3)
+    _check(b, _state(b, "fp8"))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_chunks_in_a_batch_of_few_tokens(cuda, kind):
+    """As many sequences as tokens could be there, but some have more than one."""
+    b = Batch(23, [300, 45, 200, 40], [5, 1, 70, 40], 16, 8, 2, 128, spare=150)
+    _check(b, _state(b, kind))
+
+
+@pytest.mark.parametrize("hq,hkv", [(320, 160), (130, 65), (512, 2)])
+def test_many_heads(cuda, hq, hkv):
+    b = Batch(hq, [70, 300, 5, 16], [1, 1, 1, 1], 16, hq, hkv, 32)
+    _check(b, _state(b))
+
+
+def test_pages_held_twice(cuda):
+    """Sequences that share pages, which the ledger does not allow: the outputs are right, and so are the weights of one
+    that shares none, behind more keys than the pool has."""
+    b = Batch(24, [400, 400, 400, 400, 300], [1] * 5, 16, 8, 2, 64)
+    b.table[1:4] = b.table[0]
+    state = pool, _, keys, values, weights, positions = _state(b)
+    ledger = eviction.Ledger(torch.from_numpy(weights).cuda(), torch.from_numpy(positions).cuda())
+    out = eviction.weighed_attention(b.q.cuda(), pool.cuda(), ledger, *b.meta(), sm_scale=0.125)
+    want = orc.weighed_attention(b.q.double().numpy(), keys, values, weights, positions, b.lens, b.table, b.cu, b.n, 0.125)
+    assert (np.abs(out.double().cpu().numpy() - want[0]) <= 2.0**-8 * np.abs(want[0]) + want[3]).all()
+    rows = b.table[4, :300 // 16]
+    assert (np.abs(ledger.weights.double().cpu().numpy() - want[1])[rows] <= want[4][rows]).all()
+
+
 def test_strided_queries(cuda):
     b = Batch(14, [90, 33], [1, 33], 16, 8, 2, 64)
     wide = torch.zeros((b.tokens, 12, 80), dtype=torch.bfloat16, device="cuda")

@@ -571,7 +571,9 @@ struct WeighPlan {
   size_t stats, parts, scores, joins, bytes;
 };
 
-constexpr int kTilesGrid = 512, kWeighGrid = 1280, kKeysGrid = 2048;
+// Two workgroups a CU hold tiles (two chunks of 777 tokens over 6000 .. 16384 keys: 839 us, 1036 with 256 of them, 849 with
+// 1024); the weights' grids count for little (640 or 2560 of them instead of 1280: 0.5 to 1% more; 1024 or 4096 of keys: the same).
+constexpr int kRowsGrid = 256, kTilesGrid = 512, kWeighGrid = 1280, kKeysGrid = 2048;
 
 WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   WeighPlan r = {};
@@ -589,9 +591,10 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   r.block_shift = 6;
   while ((1 << r.block_shift) < 64 * r.ways) ++r.block_shift;
   r.rows_lds = (size_t)r.near * r.ways * 32 * (dims * 2 + 32 + (fp8 ? 0 : dims * 2 + 16));
-  // as many workgroups as the card holds at once
-  const long long work = most(rows / r.near, (capacity >> r.block_shift) + 1), fill_rows = dims == 64 ? 512 : 256;
-  r.rows_grid = (int)(work < fill_rows ? work : fill_rows);
+  // One workgroup a CU: 64 sequences of 1024 .. 8192 keys, 64 heads of 128 over 8, take 272 us, and 278 with two, whose parts
+  // are twice as many; with 32 heads of 64 148 us and 153.
+  const long long work = most(rows / r.near, (capacity >> r.block_shift) + 1);
+  r.rows_grid = (int)(work < kRowsGrid ? work : kRowsGrid);
   const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
   const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1);
   r.keys_grid = (int)(blocks < kKeysGrid ? blocks : kKeysGrid);
@@ -606,7 +609,10 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const int group = s.num_q_heads / s.num_kv_heads;
   // sums of tiles' keys stay in 64 bits
   const bool fits = most(4 * ((long long)s.num_tokens * group + group), capacity) < 1ll << 62;
-  if (s.num_tokens > 2 * s.max_num_seqs && fits) {
+  // Tiles where some sequence has more than one token for sure.  32 sequences of 4000 keys, 32 heads of 128 over 8: of 2
+  // tokens 226 us, by rows 275; of 4: 231 and 437; of 16: 262 and 1460; one of 65 tokens beside 63 of one: 275 and 479.  A step
+  // of single tokens, which the launches would cost 16 of 228 us, has as many tokens as sequences at most.
+  if (s.num_tokens > s.max_num_seqs && fits) {
     const long long tiles = ((long long)s.num_tokens * group + kColumns - 1) / kColumns + seqs;
     const long long slots = most(tiles * s.num_kv_heads, capacity / kSlotKeys + 2), fill = s.head_dim > 128 ? 256 : kTilesGrid;
     r.tiles_grid = (int)(slots < fill ? slots : fill);
