@@ -266,7 +266,7 @@ __device__ __forceinline__ const float* row_part(const WeighParams& p, const Row
 // bf16: a wave reads a key's K and V row, which lie together, in whole lines, a unit of 32 keys ahead, and takes both through
 // LDS; fp8 K comes straight into the product's operand, 64 bytes of 16 keys at a time.
 template <int DP, bool FULL, bool FP8>
-__global__ __launch_bounds__(DP == 256 && !FP8 ? 256 : 64 * kMostWaves, DP == 256 && !FP8 ? 1 : 2) void weigh_rows_kernel(WeighParams p) {
+__global__ __launch_bounds__(DP == 256 ? 256 : 64 * kMostWaves, DP == 256 ? 1 : 2) void weigh_rows_kernel(WeighParams p) {
   constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;
   constexpr int kV = FP8 ? 0 : 32 * kKRow;             // V behind K
   constexpr int kWave = kV + 32 * kVRow;               // a wave's LDS; later its 16 rows of O in fp32
