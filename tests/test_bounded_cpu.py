@@ -319,7 +319,8 @@ def test_rotate_python_refuses(anywhere, change, message):
 
 
 @pytest.mark.parametrize("change,message", [
-    (dict(soft_cap=0.0), "soft_cap"), (dict(q=_bf(3, 3, 128)), "divisible"), (dict(q=_bf(3, 4, 64)), "q has shape"),
+    (dict(soft_cap=0.0), "soft_cap"), (dict(soft_cap=torch.ones(())), "must be a float"), (dict(sm_scale=torch.ones(())), "must be a float"),
+    (dict(sm_scale=None), "must be a float"), (dict(q=_bf(3, 3, 128)), "divisible"), (dict(q=_bf(3, 4, 64)), "q has shape"),
     (dict(decay=-1.0), "decay"), (dict(decay=float("nan")), "decay"), (dict(decay=float("inf")), "decay"), (dict(dropped=_i(3)), "dropped has shape"),
     (dict(ledger=eviction.Ledger(torch.zeros(4, 2, 8), _i(4, 2, 16))), "ledger.weights has shape"),
     (dict(ledger=eviction.Ledger(torch.zeros(4, 2, 16), _i(4, 2, 8))), "ledger.positions has shape"),

@@ -102,3 +102,65 @@ def test_a_serving_loop(cuda):
                 for p, kx, vx, w in zip(stay, rows[page, off, h, 0], rows[page, off, h, 1], weights[page, h, off]):
                     assert np.array_equal(kx, cache[p][0]) and np.array_equal(vx, cache[p][1]) and abs(w - cache[p][2]) < 1e-4
                 model[i][h] = {p: cache[p] for p in stay}
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_a_captured_step(cuda, kind):
+    """A decode step with everything in one graph, replayed, against the same calls made one by one on a second cache."""
+    rng = np.random.default_rng(1)
+    n, pps, total = 6, 6, 40
+    fp8 = kind == "fp8"
+    turns = rotary.turns_of(rotary.frequencies(DIM))
+    held = rng.integers(20, 48, n)
+    start = torch.from_numpy(rng.standard_normal((total, PAGE, 2 * HKV, DIM), np.float32)).cuda().to(torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    order = rng.permutation(total)
+    pages, rows = -(-held // PAGE), np.zeros((n, pps), np.int64)
+    for i, at in enumerate(np.cumsum(pages) - pages):
+        rows[i, :pages[i]] = order[at:at + pages[i]]
+    used = int(pages.sum())
+
+    class Side:
+        def __init__(self):
+            self.pool = start.clone()
+            self.ledger = eviction.make_ledger(self.pool)
+            self.scales = torch.full((total, HKV, 2), 0.5, device="cuda") if fp8 else None
+            self.table, self.stack = _i32(rows), _i32(np.concatenate([order[used:][::-1], np.zeros(used)]))
+            self.lens, self.dropped, self.count = _i32(held), _i32(np.zeros(n)), _i32([total - used])
+            self.qkv = torch.zeros((n, HQ + 2 * HKV, DIM), dtype=torch.bfloat16, device="cuda")
+            self.out = torch.zeros((n, HQ, DIM), dtype=torch.bfloat16, device="cuda")
+
+        def step(self):
+            meta = paging.assign_pages(self.lens, torch.ones_like(self.lens), self.table, self.stack, self.count, page_size=PAGE, max_tokens=n)
+            q, k, v = self.qkv[:, :HQ], self.qkv[:, HQ:HQ + HKV], self.qkv[:, HQ + HKV:]
+            rotary.rotate_heads(q, k, meta.positions, turns, cu_q_lens=meta.cu_q_lens, num_seqs=meta.num_seqs, dropped=self.dropped, out=(q, k))
+            sparse.append_kv(k, v, self.pool, meta.slot_mapping, **(dict(kv_scales=self.scales) if fp8 else {}))
+            eviction.weighed_attention(q, self.pool, self.ledger, meta.kv_lens, self.table, meta.cu_q_lens, meta.num_seqs,
+                                       dropped=self.dropped, sm_scale=0.125, kv_scales=self.scales, out=self.out)
+            moves = eviction.choose_moves(self.ledger, meta.kv_lens, self.table, meta.num_seqs, budget=BUDGET, recent=RECENT, sinks=SINKS,
+                                          limit=LIMIT, dropped=self.dropped, max_moves=16)
+            eviction.move_rows(self.pool, self.ledger, moves, kv_scales=self.scales)
+            lens, dropped, count = paging.trim_pages(meta.kv_lens, self.dropped, self.table, self.stack, meta.free_count, page_size=PAGE,
+                                                     budget=BUDGET, limit=LIMIT)
+            self.lens.copy_(lens), self.dropped.copy_(dropped), self.count.copy_(count)
+
+        def state(self):
+            return [self.pool.view(torch.uint8), *self.ledger, self.table, self.stack, self.lens, self.dropped, self.count, self.out]
+
+    warm, graphed, eager = Side(), Side(), Side()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        warm.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        graphed.step()
+    for turn in range(30):
+        x = torch.from_numpy(rng.standard_normal((n, HQ + 2 * HKV, DIM), np.float32)).to(torch.bfloat16).cuda()
+        graphed.qkv.copy_(x), eager.qkv.copy_(x)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(graphed.state(), eager.state())), turn
+    assert bool((eager.dropped > 0).all())
+    assert eviction.read_error_word(clear=True) == 0 and paging.read_error_word(clear=True) == 0

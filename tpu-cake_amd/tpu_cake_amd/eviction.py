@@ -126,6 +126,9 @@ def weighed_attention(
         if dropped is not None:
             _tensor("dropped", dropped, torch.int32, (n,), device)
         _scales(kv_scales, k_scale, v_scale, pages, heads, code, device)
+        for name, x in (("sm_scale", sm_scale), ("soft_cap", 1.0 if soft_cap is None else soft_cap)):
+            if not isinstance(x, (int, float)):
+                raise ValueError(f"{name}={x!r} must be a float")
         if soft_cap is not None and soft_cap == 0.0:
             raise ValueError(f"soft_cap={soft_cap} must not be 0.0.")
         if not (isinstance(decay, (int, float)) and 0.0 <= decay < float("inf")):
