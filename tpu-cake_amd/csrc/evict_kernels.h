@@ -9,6 +9,12 @@
 // A cache's rows are in no order for attention, so only what lies past the budget is moved, not everything behind the
 // first gap; the ledger's positions tell the recent rows.  Moves read past the budget and write before it: they
 // do not meet, and a list that is applied twice gives the same.
+//
+// Latency bounds the choice: 512 lists of 2112 rows read 5 MB and take 14.5 us, three passes over keys in LDS with a barrier
+// or two each; 24 lists of 100 000 to 131 072 rows (23 MB, 4 us at 6.3 TB/s) take 62 us in four launches, 34 of them the
+// digits by 24 workgroups (a read of the first digits' counts, then of all keys, by one CU each).  Moves are copies: 64
+// lists of 8 heads, 64 entries each at most, 11 MB, 5.6 us; six fp8 prompts' 2048 entries a head, 49 MB, 7.8 us at
+// 6.3 TB/s, 20: rows of 256 bytes at random places, scales of both pages beside them.
 #pragma once
 
 #include "attend_kernels.h"
@@ -416,6 +422,7 @@ struct MoveParams {
 
 constexpr int kMoveEntries = 16;  // of a wave
 
+// One entry a wave took 57 us where this takes 19 (the six fp8 prompts), as slots, scales and rows are a chain of loads.
 // A wave takes kMoveEntries entries of the lists: their slots, scales and ledger entries a lane each, then their rows,
 // LANES lanes a row, four loads in flight.
 template <bool FP8, int LANES>

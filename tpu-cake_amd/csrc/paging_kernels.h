@@ -16,7 +16,8 @@
 // Measured: 64 requests 4.4 us (an empty launch takes 2 to 3), 4096 requests and 65 000 tokens 10.4 us.  That is one turn
 // of workgroups of 1024 threads, which takes 8.8 us with no token at all, where 1024 requests in workgroups of 256 take
 // 5.4 (four barriers over 16 waves instead of 4, and sums over 16 parts a thread); 8192 requests, two turns, take 15.8.
-// Tokens add 1.2: the slot map's dependent reads (owner, page).  Release: 3.1 and 4.2 us.
+// Tokens add 1.2: the slot map's dependent reads (owner, page).  Release: 3.1 and 4.2 us; trim: 3.7, and 9.8 where 1280
+// of 4096 requests give back up to 1186 pages of 16 each.
 #pragma once
 
 #include "sparse_common.h"

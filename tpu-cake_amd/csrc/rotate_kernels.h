@@ -11,6 +11,11 @@
 // pairs' sines and cosines, pass them through LDS, and each then turns the same pairs of every head.  In the
 // half layout a lane holds V values of each half, so a pair meets in one lane and nothing is exchanged but
 // the norm's sum.
+//
+// 6750 prompt tokens of 64 + 8 heads of 128, half of each turned: 249 MB, 45 us, 5.5 TB/s (a copy of 4 GiB: 4.6; 39.5 us at
+// a plain read's 6.3).  54 us where a lane's two values were not whole lines' parts; rows loaded ahead, nontemporal accesses and
+// an unrolled loop over heads changed nothing.  64 decode tokens: 5 us on the GPU, 10.6 a call, of which 3.5 are the two output
+// tensors and 3.9 the call into the library.
 #pragma once
 
 #include "select_kernels.h"

@@ -3,6 +3,20 @@
 // Mathematics: o_t = sum_x p_tx v_x, p_tx = 2^(s_tx - m_t) / l_t over the keys x up to token t's position (log2 domain),
 // and for each key the sum of p_tx over the step's tokens and the group's heads.  The row's maximum m and sum l are
 // known only once every key has been seen, so weights take the scores a second time.
+//
+// Rows (sequences of one token) leave their scores, 4 bytes a (head, key), and the launch after them makes weights of
+// those; prompt chunks multiply K once more instead, which costs less than what a chunk's scores would weigh.  Launches: rows,
+// tiles (where a step may have chunks), joins of parts with the weights of rows, weights of chunks.
+//
+// HBM bounds rows.  64 sequences of 1024 to 8192 keys, 64 heads of 128 over 8, bf16: 855 MB, 136 us at the 6.3 TB/s of a plain
+// read; 191 us, of which rows 170 (845 MB read, 63 MB of scores written: 5.3 TB/s) and weights 24.  Without their scores
+// rows took 136, without any product 132 to 140: it is the mixed stores that cost.  Two sequences of 245 000 keys, 32
+// heads, fp8 pages of 16: 1.03 GB, 163 us; 277, of which rows 249 (4.3 TB/s; their loads alone take 195, the conversions and
+// the three products of P do not hide entirely) and weights 36.
+//
+// Tried for rows and not kept: loads that stay in the caches (191 us where nontemporal ones take 168); a barrier that
+// keeps the heads' waves at the same keys (195 and 191; fp8 230 and 195 for the loads); scores through LDS, at other
+// places or with other cache policies (the same).
 #pragma once
 
 #include "attend_kernels.h"
@@ -124,7 +138,7 @@ __device__ __forceinline__ int share_index(int block, int blocks, int used) {
 }
 
 // As share_of, where there are at most kFewSeqs sequences and all sums fit 32 bits: each wave by itself, four sequences a
-// lane, without LDS or a barrier.  Four short sequences' call takes 15 us with it, 20 without.
+// lane, without LDS or a barrier.  Four short sequences' call takes 18.0 us with it, 19.5 without.
 constexpr int kFewSeqs = 255;
 
 template <bool NEAR, typename Amount>
@@ -259,12 +273,13 @@ __device__ __forceinline__ const float* row_part(const WeighParams& p, const Row
 
 // Rows: a token's heads, up to 16 of one kv head, as the columns of v_mfma_f32_16x16x32_bf16.  A workgroup takes the rows of
 // `near` kv heads, a wave each (where there are few, `ways` waves share a head's keys): a key's rows of all these heads
-// lie together, and the waves walk the same keys.  Keys come in blocks, the blocks of all rows in shares, one a workgroup: a long sequence's rows are spread over as
-// many workgroups as their blocks need, and short ones' share a workgroup.  A row that a workgroup does not have whole leaves a
-// part: the first in the workgroup's slot 0, the last in slot 1.
+// lie together, and the waves walk the same keys.  Keys come in blocks, the blocks of all rows in equal shares, one a
+// workgroup: a long sequence's rows are spread over as many workgroups as their blocks need, and short ones' share a
+// workgroup.  A row that a workgroup does not have whole leaves a part: the first in the workgroup's slot 0, the last in slot 1.
 //
 // bf16: a wave reads a key's K and V row, which lie together, in whole lines, a unit of 32 keys ahead, and takes both through
-// LDS; fp8 K comes straight into the product's operand, 64 bytes of 16 keys at a time.
+// LDS; fp8 K comes straight into the product's operand, 64 bytes of 16 keys at a time.  P goes into its product in three
+// bf16 parts, 24 bits: rounded to one it would be off by 2^-9, and two lose what large values leave of small differences.
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(DP == 256 ? 256 : 64 * kMostWaves, DP == 256 ? 1 : 2) void weigh_rows_kernel(WeighParams p) {
   constexpr int kKRow = DP * 2 + 16, kVRow = DP * 2 + 32;

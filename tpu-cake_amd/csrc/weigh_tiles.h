@@ -9,7 +9,13 @@ namespace {
 // Prompt chunks: tiles of kColumns columns, the (token, head) rows of one sequence and kv head in order, 32 a wave, on
 // v_mfma_f32_32x32x16_bf16: S = K Q^T (32 keys x 32 columns), O^T += V^T P^T.  A tile's keys pass through LDS once for
 // its four waves, two buffers in turn.  A lane's scores are the keys its P operand needs, as in rows.  Tiles' keys come in
-// slots of about kSlotKeys, slots in shares, as blocks of rows do.
+// slots of about kSlotKeys, slots in shares, as blocks of rows do, and shares of the same keys go to one XCD.
+//
+// Products bound it: two chunks of 777 tokens over 6000 to 16384 keys, 32 heads of 128 over 8, take 193 GFLOP for scores and
+// output, 176 us at the 1.1 PFLOP/s of a large bf16 product; P in three parts makes 387 of them, 352 us.  434 us, 0.89
+// PFLOP/s of what is issued.  Spread over XCDs at random the whole call took 1097 us where neighbours on one take 809;
+// products before the other wave's softmax (s_setprio) 450 where 476; a turn's products and exponentials pipelined in software took
+// the same 432 and spilled registers.
 constexpr int kColumns = 128, kSlotKeys = 256;
 
 // Slots of a (sequence, head)'s first j tiles, by the keys that the tiles see: old + kColumns (j' + 1) / G each.
@@ -374,7 +380,8 @@ __device__ __forceinline__ void join_tiles(const WeighParams& p, int block) {
   }
 }
 
-// What follows rows and tiles, one launch: the joins, and the weights of the sequences that rows did.
+// What follows rows and tiles, one launch: the joins, and the weights of the sequences that rows did, which wait for
+// neither (they take a row's sum from its parts).
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams p) {
   const int block = blockIdx.x, rows = p.rows_grid * p.near, tiles = p.tiles_grid * kJoinTiles;
@@ -386,6 +393,8 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams
 // The weights of the sequences that tiles did, kKeys keys of a kv head at a time, 64 a wave, whose K stays in registers
 // as the products' A operand while every row (token, head) that sees one of them passes through LDS, kWeighRows at a time:
 // the scores once more.  A lane sums its keys over its columns, and lanes meet once at the end.
+// The two chunks above: 97 GFLOP, 88 us; 160, the exponentials beside the products.  32 keys a wave take 205 to 235 us where 64
+// took 182, as each key pays the rows' reads from LDS.
 constexpr int kWeighRows = 64;
 
 template <int DP, bool FULL, bool FP8>
