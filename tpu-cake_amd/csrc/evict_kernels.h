@@ -11,10 +11,10 @@
 // do not meet, and a list that is applied twice gives the same.
 //
 // Latency bounds the choice: 512 lists of 2112 rows read 5 MB and take 14.5 us, three passes over keys in LDS with a barrier
-// or two each; 24 lists of 100 000 to 131 072 rows (23 MB, 4 us at 6.3 TB/s) take 62 us in four launches, 34 of them the
-// digits by 24 workgroups (a read of the first digits' counts, then of all keys, by one CU each).  Moves are copies: 64
-// lists of 8 heads, 64 entries each at most, 11 MB, 5.6 us; six fp8 prompts' 2048 entries a head, 49 MB, 7.8 us at
-// 6.3 TB/s, 20: rows of 256 bytes at random places, scales of both pages beside them.
+// or two each; 24 lists of 105 000 to 126 000 rows (23 MB, 4 us at 6.3 TB/s) take 48 us: keys and their first digits 14,
+// the digits 10 + 4 + 7, tallies 5, the list 12.  Moves are copies: 64 lists of 8 heads, 64 entries each at most, 11 MB, 5.6 us;
+// six fp8 prompts' 2048 entries a head, 49 MB, 7.8 us at 6.3 TB/s, 20: rows of 256 bytes at random places, scales of both
+// pages beside them.
 #pragma once
 
 #include "attend_kernels.h"
@@ -28,7 +28,9 @@ struct ChooseParams {
   int32_t* moves;
   uint32_t* keys;    // of rows past kChooseRows: for each (sequence, head) `stride` keys, then `counts`' blocks
   uint32_t* counts;  // 2048 for each block of kKeyRows
-  uint32_t* found;   // of each (sequence, head): the budget-th largest key and how many of the rows at it stay
+  uint32_t* found;   // of each (sequence, head): the budget-th largest key (first its first digit) and its rank among those
+  uint32_t* near;    // the keys that have the first digit: those of each kSegment rows at their beginning,
+  uint32_t* held;    // so many
   uint32_t* tallies; // a Tally for each block of kKeyRows
   long long stride;
   int N, PPS, Hkv, P, S, budget, limit, sinks, recent, M;
@@ -40,11 +42,12 @@ struct ChooseParams {
 // The order of weights as whole numbers, 0 for NaN; zeros of both signs are equal.
 __device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? ordered(w + 0.f) : 0u; }
 
-// Rows of a sequence whose keys fit LDS: one workgroup does all (48 lists of 32768: 35 us, 40 by blocks; 512: 86 and 119).
-// Past them its VALU would be what counts (24 lists of 131072: 132 us), so keys, tallies and lists are made by blocks of
-// kKeyRows and only the digits are found by one workgroup: 62 us, 34 of them the digits.
+// Rows of a sequence whose keys fit LDS: one workgroup does all (48 lists of 32768: 36 us, 37 by blocks; 512: 92 and 119; of
+// 16384: 23 and 33, 53 and 82).  Past them its VALU would be what counts (24 lists of 131072: 132 us), so all that goes over
+// rows is done by blocks of kKeyRows, and one workgroup a list sums the blocks' counts and goes over the keys that share
+// the first digit: 48 us in six launches.
 constexpr int kChooseRows = 32768;
-constexpr int kKeyRows = 4096;
+constexpr int kKeyRows = 4096, kSegment = kKeyRows / 4;  // a wave's rows of a block
 constexpr int kDigits = 2048;       // 11 bits, 11 bits, 10 bits
 
 // A sequence that is cut: its rows (0: it is not), and the position past its last.
@@ -202,107 +205,140 @@ __global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
 
 struct ChooseShared {
   uint32_t count[kDigits];
-  uint32_t sum[16], found[2], held;
+  uint32_t sum[16], found[2];
   Tally waves[16];
 };
 
-// The budget-th largest key, and which one it is of the rows at it: its digits one after another.  INSIDE: all keys fit
-// LDS.  Otherwise choose_keys_kernel has made them, and LDS takes those that have the first digit.
-template <int THREADS, bool INSIDE>
-__device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, int h, const int32_t* table, int blocks,
-                                         uint32_t* s_keys, ChooseShared& sh, uint32_t& prefix, uint32_t& rank) {
-  constexpr int kBins = kDigits / THREADS, kAhead = 8;  // loads of a thread in flight
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut.rows;
+// The digit at which the counts, from the largest digit on, reach `rank`; `prefix` takes it on, `rank` counts on from there.
+template <int THREADS>
+__device__ __forceinline__ void next_digit(ChooseShared& sh, int bits, uint32_t& prefix, uint32_t& rank) {
+  constexpr int kBins = kDigits / THREADS;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  __syncthreads();
+  uint32_t own = 0;
+  const int top = kDigits - 1 - tid * kBins;  // thread 0 has the last kBins
+#pragma unroll
+  for (int i = 0; i < kBins; ++i) own += sh.count[top - i];
+  uint32_t upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = __shfl_up(upto, d);
+    upto += lane >= d ? o : 0u;
+  }
+  if (lane == 63) sh.sum[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += sh.sum[w];
+  if (upto - own < rank && rank <= upto) {
+    uint32_t above = upto - own;
+    int d = top;
+    while (above + sh.count[d] < rank) above += sh.count[d--];
+    sh.found[0] = prefix << bits | d, sh.found[1] = rank - above;
+  }
+  __syncthreads();
+  prefix = sh.found[0], rank = sh.found[1];
+}
+
+// The budget-th largest of keys in LDS, and which one it is of the rows at it: its digits one after another.
+template <int THREADS>
+__device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, int h, const int32_t* table, uint32_t* s_keys,
+                                         ChooseShared& sh, uint32_t& prefix, uint32_t& rank) {
+  const int tid = threadIdx.x, n = cut.rows;
   prefix = 0, rank = p.budget;
-  int held = -1;  // keys in LDS that have the first digit; -1: not there
   for (int shift = 21, bits = 11; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1, bits = shift ? 11 : 10) {
-    const bool first = shift == 21;
-    const auto count = [&](uint32_t key) { atomicAdd(&sh.count[key >> shift & ((1u << bits) - 1)], 1u); };
-    const auto begins = [&](uint32_t key) { return key >> (shift + bits) == prefix; };
-    if (first && !INSIDE) {
-      const int used = (n + kKeyRows - 1) / kKeyRows;
-      const uint32_t* const from = p.counts + (size_t)blockIdx.x * blocks * kDigits;
-      uint32_t sum[kBins] = {};
-#pragma unroll 16
-      for (int b = 0; b < used; ++b)
-#pragma unroll
-        for (int i = 0; i < kBins; ++i) sum[i] += from[(size_t)b * kDigits + tid * kBins + i];
-#pragma unroll
-      for (int i = 0; i < kBins; ++i) sh.count[tid * kBins + i] = sum[i];
-      if (tid == 0) sh.held = 0;
-    } else {
-      for (int i = tid; i < kDigits; i += THREADS) sh.count[i] = 0;
-      __syncthreads();
-      if (first) {
-        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
-          const u32x4 key = keys_at(p, table, h, cut, row);
-          *(u32x4*)(s_keys + row) = key;
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (row + u < n) count(key[u]);
-        }
-      } else if (INSIDE) {
-        for (int row = 4 * tid; row < n; row += 4 * THREADS) {
-          const u32x4 key = *(const u32x4*)(s_keys + row);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (row + u < n && begins(key[u])) count(key[u]);
-        }
-      } else if (held < 0) {
-        const uint32_t* const keys = p.keys + (size_t)blockIdx.x * p.stride;
-        for (int at = 4 * (tid - lane); at < n; at += 4 * THREADS * kAhead) {  // uniform in a wave
-          u32x4 key[kAhead];
-#pragma unroll
-          for (int x = 0; x < kAhead; ++x) {
-            const int row = at + 4 * THREADS * x + 4 * lane;
-            if (row < n) key[x] = *(const u32x4*)(keys + row);
-          }
-#pragma unroll
-          for (int x = 0; x < kAhead; ++x) {
-            const int row = at + 4 * THREADS * x + 4 * lane;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const bool is = row + u < n && begins(key[x][u]);
-              const uint64_t votes = __ballot(is);
-              if (is) count(key[x][u]);
-              if (shift != 10 || !votes) continue;  // uniform
-              uint32_t place = 0;
-              if (lane == 0) place = atomicAdd(&sh.held, (uint32_t)__popcll(votes));  // their order does not count
-              place = __shfl(place, 0) + __popcll(votes & ((1ull << lane) - 1));
-              if (is && place < (uint32_t)p.room) s_keys[place] = key[x][u];
-            }
-          }
-        }
+    for (int i = tid; i < kDigits; i += THREADS) sh.count[i] = 0;
+    __syncthreads();
+    for (int row = 4 * tid; row < n; row += 4 * THREADS) {
+      u32x4 key;
+      if (shift == 21) {
+        key = keys_at(p, table, h, cut, row);
+        *(u32x4*)(s_keys + row) = key;
       } else {
-        for (int i = tid; i < held; i += THREADS)
-          if (begins(s_keys[i])) count(s_keys[i]);
+        key = *(const u32x4*)(s_keys + row);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (row + u < n && (shift == 21 || key[u] >> (shift + bits) == prefix))
+          atomicAdd(&sh.count[key[u] >> shift & ((1u << bits) - 1)], 1u);
+    }
+    next_digit<THREADS>(sh, bits, prefix, rank);
+  }
+}
+
+// Of a long sequence: the first digit, from the blocks' counts.
+template <int THREADS>
+__device__ __forceinline__ void first_digit(const ChooseParams& p, int n, int blocks, ChooseShared& sh) {
+  constexpr int kBins = kDigits / THREADS;
+  const int tid = threadIdx.x, used = (n + kKeyRows - 1) / kKeyRows;
+  const uint32_t* const from = p.counts + (size_t)blockIdx.x * blocks * kDigits + tid * kBins;
+  uint32_t sum[kBins] = {};
+#pragma unroll 16
+  for (int b = 0; b < used; ++b)
+#pragma unroll
+    for (int i = 0; i < kBins; ++i) sum[i] += from[(size_t)b * kDigits + i];
+#pragma unroll
+  for (int i = 0; i < kBins; ++i) sh.count[tid * kBins + i] = sum[i];
+  uint32_t prefix = 0, rank = p.budget;
+  next_digit<THREADS>(sh, 11, prefix, rank);
+  if (tid == 0) p.found[2 * (size_t)blockIdx.x] = prefix, p.found[2 * (size_t)blockIdx.x + 1] = rank;
+}
+
+// Long sequences: the keys that have it, each wave's at the beginning of its rows'.
+__global__ __launch_bounds__(256) void choose_near_kernel(ChooseParams p) {
+  const int lane = threadIdx.x % 64, segment = blockIdx.x * 4 + threadIdx.x / 64, from = segment * kSegment + 4 * lane;
+  const int n = cut_of(p, blockIdx.y / p.Hkv, false).rows;
+  if (n <= p.room || segment * kSegment >= n) return;
+  const uint32_t prefix = p.found[2 * (size_t)blockIdx.y];
+  const uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
+  uint32_t* const to = p.near + (size_t)blockIdx.y * p.stride + segment * kSegment;
+  u32x4 key[kSegment / 256];
+#pragma unroll
+  for (int x = 0; x < kSegment / 256; ++x)
+    if (from + 256 * x < n) key[x] = *(const u32x4*)(keys + from + 256 * x);
+  uint32_t held = 0;
+#pragma unroll
+  for (int x = 0; x < kSegment / 256; ++x)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool is = from + 256 * x + u < n && key[x][u] >> 21 == prefix;
+      const uint64_t votes = __ballot(is);
+      if (is) to[held + __popcll(votes & ((1ull << lane) - 1))] = key[x][u];
+      held += __popcll(votes);
+    }
+  if (lane == 0) p.held[(size_t)blockIdx.y * gridDim.x * 4 + segment] = held;
+}
+
+// Long sequences: the other digits, from those keys, a segment a wave at a time.
+__global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p, int blocks) {
+  constexpr int kAhead = 8;  // segments whose first keys are in flight
+  __shared__ ChooseShared sh;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut_of(p, blockIdx.x / p.Hkv, false).rows;
+  if (n <= p.room) return;  // uniform
+  const int segments = (n + kSegment - 1) / kSegment;
+  const uint32_t *const held = p.held + (size_t)blockIdx.x * blocks * 4, *const keys = p.near + (size_t)blockIdx.x * p.stride;
+  uint32_t prefix = p.found[2 * (size_t)blockIdx.x], rank = p.found[2 * (size_t)blockIdx.x + 1];
+  for (int shift = 10, bits = 11; shift >= 0; shift -= 10, bits = 10) {
+    for (int i = tid; i < kDigits; i += 1024) sh.count[i] = 0;
+    __syncthreads();
+    const auto count = [&](uint32_t key) {
+      if (key >> (shift + bits) == prefix) atomicAdd(&sh.count[key >> shift & ((1u << bits) - 1)], 1u);
+    };
+    for (int base = wave; base < segments; base += 16 * kAhead) {
+      uint32_t most[kAhead], key[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int segment = base + 16 * x;
+        most[x] = segment < segments ? held[segment] : 0;
+        if (segment < segments) key[x] = keys[(size_t)segment * kSegment + lane];  // counted or not: it is there, or near enough
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if ((uint32_t)lane < most[x]) count(key[x]);
+        for (uint32_t i = lane + 64; i < most[x]; i += 64) count(keys[(size_t)(base + 16 * x) * kSegment + i]);
       }
     }
-    __syncthreads();
-    // the largest digits first: thread 0 has the last kBins
-    uint32_t own = 0;
-    const int top = kDigits - 1 - tid * kBins;
-#pragma unroll
-    for (int i = 0; i < kBins; ++i) own += sh.count[top - i];
-    uint32_t upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(upto, d);
-      upto += lane >= d ? o : 0u;
-    }
-    if (lane == 63) sh.sum[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += sh.sum[w];
-    if (upto - own < rank && rank <= upto) {
-      uint32_t above = upto - own;
-      int d = top;
-      while (above + sh.count[d] < rank) above += sh.count[d--];
-      sh.found[0] = prefix << bits | d, sh.found[1] = rank - above;
-    }
-    __syncthreads();
-    prefix = sh.found[0], rank = sh.found[1];
-    if (!INSIDE && shift == 10) held = sh.held <= (uint32_t)p.room ? (int)sh.held : -1;
+    next_digit<1024>(sh, bits, prefix, rank);
   }
+  if (tid == 0) p.found[2 * (size_t)blockIdx.x] = prefix, p.found[2 * (size_t)blockIdx.x + 1] = rank;
 }
 
 // The list of rows whose keys are in LDS: every wave has a stretch of rows.
@@ -341,14 +377,10 @@ __global__ __launch_bounds__(THREADS) void choose_rows_kernel(ChooseParams p, in
   int32_t* const list = p.moves + (size_t)blockIdx.x * p.M * 2;
   const Cut cut = cut_of(p, seq, threadIdx.x == 0);
   uint32_t bound, rank;
-  if (THREADS == 1024 && cut.rows > p.room) {  // the list is choose_list_kernel's
-    find_key<THREADS, THREADS != 1024>(p, cut, h, table, blocks, s_keys, s_rest, bound, rank);
-    if (threadIdx.x == 0) p.found[2 * (size_t)blockIdx.x] = bound, p.found[2 * (size_t)blockIdx.x + 1] = rank;
-    return;
-  }
+  if (THREADS == 1024 && cut.rows > p.room) return first_digit<THREADS>(p, cut.rows, blocks, s_rest);  // the rest by blocks
   int done = 0;  // entries of the list
   if (cut.rows) {
-    find_key<THREADS, true>(p, cut, h, table, blocks, s_keys, s_rest, bound, rank);
+    find_key<THREADS>(p, cut, h, table, s_keys, s_rest, bound, rank);
     done = list_rows<THREADS>(p, cut.rows, s_keys, s_rest, Lister{list, table, bound, rank});
   }
   for (long long i = 2ll * done + threadIdx.x; i < 2ll * p.M; i += THREADS) list[i] = -1;
@@ -514,7 +546,7 @@ int check_choose(const rpa_choose_shape_t* s) {
 struct ChoosePlan {
   int threads, room, blocks;  // blocks 0: all keys fit LDS
   long long stride;
-  size_t keys, counts, found, bytes;  // bytes up to the end of each
+  size_t keys, near, counts, found, held, bytes;  // bytes up to the end of each
 };
 
 // Waves of a workgroup: sixteen while every list has a CU to itself (256 lists of 4096 rows: 13.0 us, 16.6 with four; of
@@ -530,9 +562,11 @@ ChoosePlan plan_choose(const rpa_choose_shape_t& s) {
     r.stride = (capacity + 3) / 4 * 4;
     r.keys = (size_t)s.max_num_seqs * s.num_kv_heads * r.stride * 4;
     const size_t lists = (size_t)s.max_num_seqs * s.num_kv_heads;
-    r.counts = r.keys + lists * r.blocks * kDigits * 4;
+    r.near = 2 * r.keys + 256;  // a wave reads 64 keys of a segment, also past the last one's
+    r.counts = r.near + lists * r.blocks * kDigits * 4;
     r.found = r.counts + (lists * 8 + 15) / 16 * 16;
-    r.bytes = r.found + lists * r.blocks * sizeof(Tally);
+    r.held = r.found + lists * r.blocks * 16;
+    r.bytes = r.held + lists * r.blocks * sizeof(Tally);
   }
   return r;
 }
