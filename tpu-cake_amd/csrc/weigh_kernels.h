@@ -118,7 +118,7 @@ struct Share {
   int seq, count;      // the sequence that `from` lies in, of how many
   Sequence s;
   long long before, scores, rows;  // before it: units, blocks of scores, units of rows
-  long long row_total;
+  long long row_total, total;      // units of rows, and of all the work
 };
 
 // Sequence i of `count`, in the order of the work.
@@ -176,7 +176,7 @@ __device__ __forceinline__ Share share_of_few(const WeighParams& p, int block, i
   const int each_share = (int)(((long long)total + blocks - 1) / blocks);
   const int index = total ? share_index<NEAR>(block, blocks, (total + each_share - 1) / each_share) : block;
   const int from = (int)min((long long)index * each_share, (long long)total), to = min(from + each_share, total);
-  if (from >= to) return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0};
+  if (from >= to) return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0, total};
   int before[3] = {upto[0] - own[0], upto[1] - own[1], upto[2] - own[2]}, at = 0;
   const int hit = __builtin_ctzll(__ballot(from >= before[0] && from < upto[0]));
   Sequence mine = s[0];
@@ -193,7 +193,7 @@ __device__ __forceinline__ Share share_of_few(const WeighParams& p, int block, i
   }
   const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, hit); };
   return Share{index, from, to, hit * each + of(at), count, {of(mine.first), of(mine.tokens), of(mine.keys)}, of(before[0]), of(before[1]),
-               of(before[2]), row_total};
+               of(before[2]), row_total, total};
 }
 
 // amount(sequence, pad): its units.
@@ -248,11 +248,11 @@ __device__ __forceinline__ Share share_of(const WeighParams& p, int block, int b
     Sequence s = sequence(i);
     for (long long a; from >= before[0] + (a = amount(s, i == count)); s = sequence(++i))
       before[0] += a, before[1] += i < count ? score_blocks(s) : 0, before[2] += row_units(p, s, i == count);
-    s_share = {index, from, to, i, count, s, before[0], before[1], before[2], total[2]};
+    s_share = {index, from, to, i, count, s, before[0], before[1], before[2], total[2], total[0]};
   }
   __syncthreads();
   if (from < to) return s_share;
-  return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0};
+  return Share{0, 0, 0, 0, 0, {0, 0, 0}, 0, 0, 0, 0, total[0]};
 }
 
 // The parts of a row that several workgroups had: those of workgroups first .. last.

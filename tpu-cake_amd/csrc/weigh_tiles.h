@@ -390,28 +390,36 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams
   else weigh_rows<DP, FULL, FP8>(p, block - rows - tiles, gridDim.x - rows - tiles);
 }
 
-// The weights of the sequences that tiles did, kKeys keys of a kv head at a time, 64 a wave, whose K stays in registers
+// The weights of the sequences that tiles did, 256 keys of a kv head at a time, 64 a wave, whose K stays in registers
 // as the products' A operand while every row (token, head) that sees one of them passes through LDS, kWeighRows at a time:
 // the scores once more.  A lane sums its keys over its columns, and lanes meet once at the end.
 // The two chunks above: 97 GFLOP, 88 us; 160, the exponentials beside the products.  32 keys a wave take 205 to 235 us where 64
 // took 182, as each key pays the rows' reads from LDS.
-constexpr int kWeighRows = 64;
+//
+// Where keys are few (at most kPairs blocks), two waves share their keys and take 32 of a stage's rows each: one prompt of 2000
+// tokens 360 to 287 us for the whole call, two chunks of 500 over 2000 keys 175 to 160, 200 tokens 68 to 60.
+constexpr int kWeighRows = 64, kPairs = 512;
 
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParams p) {
   constexpr int kElem = FP8 ? 1 : 2;
   constexpr int kSteps = DP / 16;
   constexpr int kWave = DP > 128 ? 32 : 64, kBlocks = kWave / 32;  // keys of a wave
-  constexpr int kKeys = kWave * kWeighWaves;
   constexpr int kRow = DP * 2 + 16;
   constexpr int kLoads = kWeighRows * DP * 2 / 16 / kWeighThreads;
   __shared__ __align__(16) uint8_t s_q[2][kWeighRows * kRow];
   __shared__ float2 s_stat[2][kWeighRows];
+  __shared__ float s_other[kWeighWaves / 2][kBlocks][16][2];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
-  const auto blocks_of = [&](const Sequence& s) { return s.tokens > 1 ? (s.keys + kKeys - 1) / kKeys : 0; };
-  const Share share = share_of<true>(p, blockIdx.x, gridDim.x,
-                                     [&](const Sequence& s, bool pad) { return pad ? 0 : (long long)blocks_of(s) * p.Hkv; });
+  const bool may_pair = (long long)p.N * p.Hkv <= kPairs / 2;  // finding the share a second time costs 4 us
+  int keys_of = kWave * kWeighWaves / (may_pair ? 2 : 1);  // of the workgroup
+  const auto blocks_of = [&](const Sequence& s) { return s.tokens > 1 ? (s.keys + keys_of - 1) / keys_of : 0; };
+  const auto amount = [&](const Sequence& s, bool pad) { return pad ? 0 : (long long)blocks_of(s) * p.Hkv; };
+  Share share = share_of<true>(p, blockIdx.x, gridDim.x, amount);
+  const bool pairs = may_pair && share.total <= kPairs;  // the same for every workgroup
+  if (may_pair && !pairs) keys_of *= 2, share = share_of<true>(p, blockIdx.x, gridDim.x, amount);
   if (share.from == share.to) return;
+  const int of_keys = pairs ? wave % (kWeighWaves / 2) : wave;
   const int row_bytes = p.D * kElem;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
   const global_bytes zero = zero_row();
@@ -426,7 +434,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
     const int blocks = blocks_of(s), h = (int)((at - before) / blocks), block = (int)((at - before) - (long long)h * blocks);
     const int32_t* const table = p.table + (size_t)seq * p.PPS;
     const int old = s.keys - s.tokens;  // keys before the step's
-    const int part = block * kKeys, key0 = part + kWave * wave;
+    const int part = block * keys_of, key0 = part + kWave * of_keys;
     const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
     const auto slot_of = [&](int key) {
       if (key >= s.keys) return -1;
@@ -503,6 +511,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
       for (int sub = 0; sub < kWeighRows; sub += 32) {
         const int row0 = base + sub;
         if (row0 >= end_row) break;  // uniform
+        if (pairs && sub / 32 != wave / (kWeighWaves / 2)) continue;
         const int first = div_by(row0, p.group), last = div_by(min(row0 + 32, end_row) - 1, p.group);  // tokens
         if (key0 > old + last || key0 >= s.keys) continue;  // uniform
         const float2 stat = s_stat[turn & 1][sub + n];
@@ -542,8 +551,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
       __syncthreads();
     }
     // over the 32 columns: lane n then has key n's
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
+    const auto of_block = [&](int b) {
       float mine = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -552,6 +560,22 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
         for (int d = 1; d < 32; d *= 2) x += __shfl_xor(x, d);
         mine = n == r ? x : mine;
       }
+      return mine;
+    };
+    if (pairs) {
+      if (wave != of_keys) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          const float mine = of_block(b);
+          if (n < 16) s_other[of_keys][b][n][half] = mine;
+        }
+      }
+      __syncthreads();
+      if (wave != of_keys) continue;
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const float mine = of_block(b) + (pairs ? s_other[of_keys][b][n % 16][half] : 0.f);
       const int key = key0 + 32 * b + 8 * (n / 4) + 4 * half + n % 4;
       if (n < 16 && key < s.keys) add_weight(p, seq, h, old, key, mine);
     }
