@@ -164,3 +164,33 @@ def test_a_captured_step(cuda, kind):
         assert all(torch.equal(a, b) for a, b in zip(graphed.state(), eager.state())), turn
     assert bool((eager.dropped > 0).all())
     assert eviction.read_error_word(clear=True) == 0 and paging.read_error_word(clear=True) == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_a_pool_past_32_bits(cuda, kind):
+    """The last pages of a pool of more than 2^32 values, against the same pages in a small one."""
+    rng = np.random.default_rng(2)
+    fp8 = kind == "fp8"
+    held, new = np.array([700, 333, 60]), np.array([1, 40, 1])
+    pages = -(-held // 64)
+    small, shift = int(pages.sum()), 140000
+    table = np.zeros((3, int(pages.max())), np.int64)
+    for i, at in enumerate(np.cumsum(pages) - pages):
+        table[i, :pages[i]] = rng.permutation(pages[i]) + at
+    values = torch.from_numpy(rng.standard_normal((small, 64, 4, 128), np.float32)).cuda().to(torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    q = torch.from_numpy(rng.standard_normal((42, 8, 128), np.float32)).to(torch.bfloat16).cuda()
+    got = []
+    for first in (0, shift):
+        pool = torch.empty((first + small, 64, 4, 128), dtype=values.dtype, device="cuda")
+        pool[first:] = values
+        scales = torch.full((first + small, 2, 2), 0.25, device="cuda") if fp8 else None
+        ledger = eviction.make_ledger(pool)
+        at = _i32(table + first)
+        out = eviction.weighed_attention(q, pool, ledger, _i32(held), at, _i32([0, 1, 41, 42]), _i32([3]), sm_scale=0.1, kv_scales=scales)
+        moves = eviction.choose_moves(ledger, _i32(held), at, _i32([3]), budget=50, recent=10, sinks=2)
+        eviction.move_rows(pool, ledger, moves, kv_scales=scales)
+        got.append((out, torch.where(moves < 0, moves, moves - first * 64), *(x[first:].clone() for x in (pool.view(torch.uint8), *ledger))))
+        assert not first or pool.numel() > 2**32
+        del pool
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert eviction.read_error_word(clear=True) == 0

@@ -203,6 +203,18 @@ def test_chunks_of_many_sequences(cuda):
     _check(b, _state(b, "fp8"))
 
 
+@pytest.mark.parametrize("dim,kind", [(128, "bf16"), (256, "bf16"), (40, "bf16"), (128, "fp8"), (256, "fp8"), (112, "fp8")])
+def test_chunks_of_many_lengths(cuda, dim, kind):
+    """Enough rows of the table, or enough keys, that every wave has keys of its own."""
+    rng = np.random.default_rng(25)
+    lens = rng.integers(1, 400, 140)
+    new = np.minimum(rng.integers(1, 20, 140), lens)
+    b = Batch(25, lens.tolist(), new.tolist(), 16, 4, 2, dim)
+    _check(b, _state(b, kind))
+    b = Batch(26, [40000, 300], [3, 70], 64, 4, 2, dim)
+    _check(b, _state(b, kind))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 def test_chunks_in_a_batch_of_few_tokens(cuda, kind):
     """As many sequences as tokens could be there, but some have more than one."""
