@@ -396,9 +396,11 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams
 // The two chunks above: 97 GFLOP, 88 us; 160, the exponentials beside the products.  32 keys a wave take 205 to 235 us where 64
 // took 182, as each key pays the rows' reads from LDS.
 //
-// Where keys are few (at most kPairs blocks), two waves share their keys and take 32 of a stage's rows each: one prompt of 2000
-// tokens 360 to 287 us for the whole call, two chunks of 500 over 2000 keys 175 to 160, 200 tokens 68 to 60.
-constexpr int kWeighRows = 64, kPairs = 512;
+// Where keys are few (at most kSpread blocks of 64), a workgroup has 64 and its waves take 32 rows each in turn, straight from
+// memory, as no two waves read the same: a prompt of 2000 tokens 363 to 187 us for the whole call, 175 tokens of 16 heads a
+// group over 400 keys 143 to 82, two chunks of 500 over 2000 keys 177 to 150.  With both in one kernel 64 sequences of 8 tokens over
+// 4000 keys take 435 us instead of 408; a launch for each costs all but those 2 to 5 us.
+constexpr int kWeighRows = 64, kSpread = 1024;
 
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParams p) {
@@ -409,17 +411,16 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
   constexpr int kLoads = kWeighRows * DP * 2 / 16 / kWeighThreads;
   __shared__ __align__(16) uint8_t s_q[2][kWeighRows * kRow];
   __shared__ float2 s_stat[2][kWeighRows];
-  __shared__ float s_other[kWeighWaves / 2][kBlocks][16][2];
+  __shared__ float s_other[kWeighWaves][kBlocks][16][2];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
-  const bool may_pair = (long long)p.N * p.Hkv <= kPairs / 2;  // finding the share a second time costs 4 us
-  int keys_of = kWave * kWeighWaves / (may_pair ? 2 : 1);  // of the workgroup
+  const bool may_spread = 4ll * p.N * p.Hkv <= kSpread;  // finding the share a second time costs 4 us
+  int keys_of = kWave * (may_spread ? 1 : kWeighWaves);  // of the workgroup
   const auto blocks_of = [&](const Sequence& s) { return s.tokens > 1 ? (s.keys + keys_of - 1) / keys_of : 0; };
   const auto amount = [&](const Sequence& s, bool pad) { return pad ? 0 : (long long)blocks_of(s) * p.Hkv; };
   Share share = share_of<true>(p, blockIdx.x, gridDim.x, amount);
-  const bool pairs = may_pair && share.total <= kPairs;  // the same for every workgroup
-  if (may_pair && !pairs) keys_of *= 2, share = share_of<true>(p, blockIdx.x, gridDim.x, amount);
+  const bool spread = may_spread && share.total <= kSpread;  // the same for every workgroup
+  if (may_spread && !spread) keys_of *= kWeighWaves, share = share_of<true>(p, blockIdx.x, gridDim.x, amount);
   if (share.from == share.to) return;
-  const int of_keys = pairs ? wave % (kWeighWaves / 2) : wave;
   const int row_bytes = p.D * kElem;
   const uint64_t row_stride = 2ull * p.Hkv * row_bytes;
   const global_bytes zero = zero_row();
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
     const int blocks = blocks_of(s), h = (int)((at - before) / blocks), block = (int)((at - before) - (long long)h * blocks);
     const int32_t* const table = p.table + (size_t)seq * p.PPS;
     const int old = s.keys - s.tokens;  // keys before the step's
-    const int part = block * keys_of, key0 = part + kWave * of_keys;
+    const int part = block * keys_of, key0 = part + (spread ? 0 : kWave * wave);
     const global_bytes rows = (global_bytes)(uint64_t)p.kv + 2 * (size_t)h * row_bytes;
     const auto slot_of = [&](int key) {
       if (key >= s.keys) return -1;
@@ -500,55 +501,66 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[b][r] = 0.f;
-    __syncthreads();  // the last use of LDS
-    load(begin_row), store(0);
-    __syncthreads();
-    int turn = 0;
-#pragma unroll 1
-    for (int base = begin_row; base < end_row; base += kWeighRows, ++turn) {
-      if (base + kWeighRows < end_row) load(base + kWeighRows);
-#pragma unroll 1
-      for (int sub = 0; sub < kWeighRows; sub += 32) {
-        const int row0 = base + sub;
-        if (row0 >= end_row) break;  // uniform
-        if (pairs && sub / 32 != wave / (kWeighWaves / 2)) continue;
-        const int first = div_by(row0, p.group), last = div_by(min(row0 + 32, end_row) - 1, p.group);  // tokens
-        if (key0 > old + last || key0 >= s.keys) continue;  // uniform
-        const float2 stat = s_stat[turn & 1][sub + n];
-        const bool whole = key0 + kWave - 1 <= old + first && row0 + 32 <= end_row;
-        const int token = div_by(min(row0 + n, end_row - 1), p.group), seen = row0 + n < end_row ? old + token : -1;
+    // 32 rows from row0 on; x(i): this lane's row, dims 16 i + 8 half on
+    const auto weigh = [&](int row0, const float2 stat, auto x) {
+      const int first = div_by(row0, p.group), last = div_by(min(row0 + 32, end_row) - 1, p.group);  // tokens
+      if (key0 > old + last || key0 >= s.keys) return;  // uniform
+      const bool whole = key0 + kWave - 1 <= old + first && row0 + 32 <= end_row;
+      const int token = div_by(min(row0 + n, end_row - 1), p.group), seen = row0 + n < end_row ? old + token : -1;
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          f32x16 sc;
+      for (int b = 0; b < kBlocks; ++b) {
+        f32x16 sc;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+        for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            const u32x4 x = *(const u32x4*)(s_q[turn & 1] + (sub + n) * kRow + 32 * i + 16 * half);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b][i], __builtin_bit_cast(bf16x8, x), sc, 0, 0, 0);
-          }
+        for (int i = 0; i < kSteps; ++i)
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[b][i], __builtin_bit_cast(bf16x8, x(i)), sc, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float scale = p.scale;
-            if (FP8) scale *= __shfl(ks[b], 8 * (r / 4) + 4 * half + r % 4);
-            sc[r] = scaled(sc[r], scale);
-          }
-          if (p.cap != 0.f) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = scaled(p.cap * tanhf(sc[r] / p.cap), kLog2e);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(sc[r] - stat.x);
-          if (!whole) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= seen ? sc[r] : 0.f;
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum[b][r] = __builtin_fmaf(sc[r], stat.y, sum[b][r]);
+        for (int r = 0; r < 16; ++r) {
+          float scale = p.scale;
+          if (FP8) scale *= __shfl(ks[b], 8 * (r / 4) + 4 * half + r % 4);
+          sc[r] = scaled(sc[r], scale);
         }
+        if (p.cap != 0.f) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[r] = scaled(p.cap * tanhf(sc[r] / p.cap), kLog2e);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(sc[r] - stat.x);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= seen ? sc[r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[b][r] = __builtin_fmaf(sc[r], stat.y, sum[b][r]);
       }
-      if (base + kWeighRows < end_row) store(turn + 1);
+    };
+    __syncthreads();  // the last use of LDS
+    if (spread) {
+#pragma unroll 1
+      for (int row0 = begin_row + 32 * wave; row0 < end_row; row0 += 32 * kWeighWaves) {
+        const int row = min(row0 + n, end_row - 1), token = div_by(row, p.group), g = row - token * p.G;
+        const uint16_t* const src = p.q + (s.first + token) * p.q_token + ((long long)h * p.G + g) * p.q_head + 8 * half;
+        const float2 stat = p.stats[(size_t)(s.first + token) * p.Hkv * p.G + h * p.G + g];
+        u32x4 x[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) x[i] = FULL || 16 * i + 8 * half < p.D ? *(const u32x4*)(src + 16 * i) : u32x4{0, 0, 0, 0};
+        weigh(row0, row0 + n < end_row ? stat : float2{0.f, 0.f}, [&](int i) { return x[i]; });
+      }
+    } else {
+      load(begin_row), store(0);
       __syncthreads();
+      int turn = 0;
+#pragma unroll 1
+      for (int base = begin_row; base < end_row; base += kWeighRows, ++turn) {
+        if (base + kWeighRows < end_row) load(base + kWeighRows);
+#pragma unroll 1
+        for (int sub = 0; sub < kWeighRows && base + sub < end_row; sub += 32)
+          weigh(base + sub, s_stat[turn & 1][sub + n],
+                [&](int i) { return *(const u32x4*)(s_q[turn & 1] + (sub + n) * kRow + 32 * i + 16 * half); });
+        if (base + kWeighRows < end_row) store(turn + 1);
+        __syncthreads();
+      }
     }
     // over the 32 columns: lane n then has key n's
     const auto of_block = [&](int b) {
@@ -562,20 +574,21 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
       }
       return mine;
     };
-    if (pairs) {
-      if (wave != of_keys) {
+    if (spread) {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const float mine = of_block(b);
-          if (n < 16) s_other[of_keys][b][n][half] = mine;
-        }
+      for (int b = 0; b < kBlocks; ++b) {
+        const float mine = of_block(b);
+        if (n < 16) s_other[wave][b][n][half] = mine;
       }
       __syncthreads();
-      if (wave != of_keys) continue;
+      if (wave) continue;
     }
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-      const float mine = of_block(b) + (pairs ? s_other[of_keys][b][n % 16][half] : 0.f);
+      float mine = 0.f;
+      if (!spread) mine = of_block(b);
+      else
+        for (int w = 0; w < kWeighWaves; ++w) mine += s_other[w][b][n % 16][half];
       const int key = key0 + 32 * b + 8 * (n / 4) + 4 * half + n % 4;
       if (n < 16 && key < s.keys) add_weight(p, seq, h, old, key, mine);
     }
@@ -630,8 +643,8 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const long long work = most(rows / r.near, (capacity >> r.block_shift) + 1);
   r.rows_grid = (int)(work < kRowsGrid ? work : kRowsGrid);
   const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
-  const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1);
-  r.keys_grid = (int)(blocks < kKeysGrid ? blocks : kKeysGrid);
+  const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1), spread = most(seqs * s.num_kv_heads, capacity / 64 + 1);
+  r.keys_grid = (int)(spread <= kSpread ? spread : blocks < kKeysGrid ? blocks : kKeysGrid);
   r.weigh_grid = (int)(blocks < kWeighGrid ? blocks : kWeighGrid);
   r.stats = ((size_t)s.num_tokens * s.num_q_heads * sizeof(float2) + 15) / 16 * 16;
   r.parts = (size_t)r.rows_grid * 2 * r.near * (32 + 16 * (size_t)s.head_dim) * 4;
