@@ -502,7 +502,10 @@ __global__ __launch_bounds__(kWeighThreads, 2) void weigh_keys_kernel(WeighParam
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[b][r] = 0.f;
     // 32 rows from row0 on; x(i): this lane's row, dims 16 i + 8 half on
-    const auto weigh = [&](int row0, const float2 stat, auto x) {
+    const auto weigh = [&](int row0, float2 stat, auto x) {
+      // a sum that is NaN goes into the exponentials, which a mask clears; a factor of NaN would reach the keys that the row
+      // does not see, too
+      if (!(stat.y == stat.y)) stat = {stat.y, 1.f};
       const int first = div_by(row0, p.group), last = div_by(min(row0 + 32, end_row) - 1, p.group);  // tokens
       if (key0 > old + last || key0 >= s.keys) return;  // uniform
       const bool whole = key0 + kWave - 1 <= old + first && row0 + 32 <= end_row;
