@@ -1,0 +1,36 @@
+"""Sizes near the ends of 32 bits, which the calls over a bounded cache and its neighbours refuse before any launch: no GPU needed."""
+
+import ctypes
+
+import pytest
+
+from tpu_cake_amd import _bounded_lib, _sparse_lib
+
+FAKE = [ctypes.c_void_p((i + 1) << 44) for i in range(16)]  # far apart and never dereferenced: every call here is refused
+
+
+@pytest.fixture(scope="module", params=["bounded", "sparse"])
+def libs(request):
+    binding = {"bounded": _bounded_lib, "sparse": _sparse_lib}[request.param]
+    if not binding.library_path().exists():
+        from tpu_cake_amd import build
+        build.build()
+    return request.param, binding.load()
+
+
+@pytest.mark.parametrize("pages", [1 << 27, 1 << 28, (1 << 29) + 5, 2**31 - 1])
+def test_outputs_in_the_scales_of_many_pages(libs, pages):
+    """The scales' bytes pass 32 bits from 2^28 pages on: an output within them is refused all the same."""
+    name, lib = libs
+    inside = ctypes.c_void_p(FAKE[2].value + 16 * pages - 256)  # 8 bytes a page and kv head, two heads: their end
+    if name == "bounded":
+        shape = _bounded_lib.RpaWeighShape(4, 8, 2, 128, pages, 1, 4, 8, _bounded_lib.RPA_KV_FP8_E4M3, 0, 1024, 128)
+        options = _bounded_lib.RpaWeighOptions(1.0, 0.0, 1.0, 1.0, 1.0)
+        rc = lib.rpa_weighed_attention(ctypes.byref(shape), ctypes.byref(options), *FAKE[:10], inside, FAKE[11], 1 << 42, None)
+        error = lib.rpa_bounded_last_error()
+    else:
+        shape = _sparse_lib.RpaSparseShape(4, 8, 2, 128, pages, 1, 4, 8, _sparse_lib.RPA_KV_FP8_E4M3, 6, 1024, 128)
+        options = _sparse_lib.RpaSparseOptions(1.0, 0.0, 1.0, 1.0)
+        rc = lib.rpa_sparse_paged_attention(ctypes.byref(shape), ctypes.byref(options), *FAKE[:8], inside, FAKE[9], 1 << 42, None)
+        error = lib.rpa_sparse_last_error()
+    assert rc == -1 and b"out overlaps kv_scales" in error, (rc, error)

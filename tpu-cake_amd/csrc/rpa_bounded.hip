@@ -131,7 +131,7 @@ int rpa_weighed_attention(const rpa_weigh_shape_t* shape, const rpa_weigh_option
   const long long T = s.num_tokens, Hq = s.num_q_heads, Hkv = s.num_kv_heads, D = s.head_dim;
   const long long N = s.max_num_seqs, pool = (long long)s.total_pages * s.page_size;
   const Memory in[] = {rows_of("q", q, T, Hq, D, s.q_token_stride, s.q_head_stride),
-                       {"kv_pages", kv_pages, pool * 2 * Hkv * D * (fp8 ? 1 : 2)}, {"kv_scales", kv_scales, 8 * s.total_pages * Hkv},
+                       {"kv_pages", kv_pages, pool * 2 * Hkv * D * (fp8 ? 1 : 2)}, {"kv_scales", kv_scales, 8ll * s.total_pages * Hkv},
                        {"kv_lens", kv_lens, 4 * N}, {"page_indices", page_indices, 4 * N * s.pages_per_seq},
                        {"cu_q_lens", cu_q_lens, 4 * (N + 1)}, {"num_seqs", num_seqs, 4}, {"dropped", dropped, 4 * N},
                        {"workspace", workspace, (long long)plan.bytes}};

@@ -214,7 +214,7 @@ int rpa_sparse_paged_attention(const rpa_sparse_shape_t* shape, const rpa_sparse
   const long long N = shape->max_num_seqs, pool = (long long)shape->total_pages * shape->page_size;
   const Memory in[] = {rows_of("q", q, T, Hq, D, shape->q_token_stride, shape->q_head_stride),
                        {"kv_pages", kv_pages, pool * 2 * Hkv * D * (fp8 ? 1 : 2)},
-                       {"kv_scales", kv_scales, 8 * shape->total_pages * Hkv},
+                       {"kv_scales", kv_scales, 8ll * shape->total_pages * Hkv},
                        {"selected_pages", selected_pages, 4 * T * Hkv * shape->num_pages}, {"kv_lens", kv_lens, 4 * N},
                        {"page_indices", page_indices, 4 * N * shape->pages_per_seq}, {"cu_q_lens", cu_q_lens, 4 * (N + 1)},
                        {"num_seqs", num_seqs, 4}, {"workspace", workspace, (long long)plan.bytes}};
