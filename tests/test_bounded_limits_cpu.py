@@ -34,3 +34,13 @@ def test_outputs_in_the_scales_of_many_pages(libs, pages):
         rc = lib.rpa_sparse_paged_attention(ctypes.byref(shape), ctypes.byref(options), *FAKE[:8], inside, FAKE[9], 1 << 42, None)
         error = lib.rpa_sparse_last_error()
     assert rc == -1 and b"out overlaps kv_scales" in error, (rc, error)
+
+
+@pytest.mark.parametrize("entries", [(1 << 30, 1, 1), (1 << 15, 1 << 15, 1), (1 << 14, 1 << 14, 4), (2**31 - 1, 1, 1), ((1 << 30) - 63, 1, 1)])
+def test_moves_of_2_to_the_32_threads(entries):
+    """Four threads an entry: HIP takes fewer than 2^32 along a dimension, and the call says so itself."""
+    lists, moves, heads = entries
+    shape = _bounded_lib.RpaMoveShape(lists, moves, heads, 128, 64, 16, 0)
+    lib = _bounded_lib.load()
+    assert lib.rpa_move_rows(ctypes.byref(shape), FAKE[0], None, *FAKE[2:5], None) == -2
+    assert b"one launch" in lib.rpa_bounded_last_error()

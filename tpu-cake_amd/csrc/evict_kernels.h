@@ -571,6 +571,8 @@ ChoosePlan plan_choose(const rpa_choose_shape_t& s) {
   return r;
 }
 
+long long move_groups(long long entries) { return (entries + 4 * kMoveEntries - 1) / (4 * kMoveEntries); }
+
 int check_move(const rpa_move_shape_t* s) {
   if (!s) return fail(RPA_E_INVALID, "shape is NULL");
   if (s->num_lists < 0 || s->max_moves <= 0) return fail(RPA_E_INVALID, "non-positive dimension in shape");
@@ -578,7 +580,7 @@ int check_move(const rpa_move_shape_t* s) {
   if (rc || (rc = check_pool(s->total_pages, s->page_size))) return rc;
   const __int128 entries = (__int128)s->num_lists * s->num_kv_heads * s->max_moves;
   if (entries > kMostIndex) return fail(RPA_E_UNSUPPORTED, "more rows than one launch takes");
-  return RPA_OK;
+  return check_launch(move_groups((long long)entries), 256);
 }
 
 }  // namespace

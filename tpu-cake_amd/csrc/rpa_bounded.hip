@@ -251,7 +251,7 @@ int rpa_move_rows(const rpa_move_shape_t* shape, const int32_t* moves, const flo
     return rc;
   const MoveParams p = {moves, kv_scales, (uint8_t*)kv_pages, weights, positions, pool, (int)entries, s.max_moves, s.num_kv_heads,
                         s.page_size, (int)(row / 16)};
-  const unsigned grid = (unsigned)((entries + 4 * kMoveEntries - 1) / (4 * kMoveEntries));
+  const unsigned grid = (unsigned)move_groups(entries);
   const auto kernel = fp8 ? (p.chunks <= 16 ? move_kernel<true, 16> : move_kernel<true, 32>)
                           : (p.chunks <= 16 ? move_kernel<false, 16> : p.chunks <= 32 ? move_kernel<false, 32> : move_kernel<false, 64>);
   kernel<<<grid, 256, 0, (hipStream_t)stream>>>(p);
