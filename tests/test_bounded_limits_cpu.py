@@ -44,3 +44,13 @@ def test_moves_of_2_to_the_32_threads(entries):
     lib = _bounded_lib.load()
     assert lib.rpa_move_rows(ctypes.byref(shape), FAKE[0], None, *FAKE[2:5], None) == -2
     assert b"one launch" in lib.rpa_bounded_last_error()
+
+
+@pytest.mark.parametrize("seqs,heads,page,pages,width", [(256, 8, 16, 40000, 8192), (64, 8, 16, 8500, 8192), (4096, 1, 64, 1 << 14, 1 << 14),
+                                                         (3, 8, 16, 50000, 7700), (1, 1, 1, 32769, 40000), (2000, 2, 16, 64, 1 << 17)])
+def test_choose_workspaces_follow_the_pool(seqs, heads, page, pages, width):
+    """Keys of long sequences: 10 bytes a row and kv head and what a list's last block rounds up (4095 of 32769 rows at most),
+    of as many rows as the pool has, and 16 bytes a list; the table's width counts for nothing."""
+    shape = _bounded_lib.RpaChooseShape(seqs, width, heads, pages, page, 2048, 2111, 4, 256, 64)
+    size = _bounded_lib.load().rpa_choose_workspace_size(ctypes.byref(shape))
+    assert 0 < size <= 41000 / 4096 * 1.125 * pages * page * heads + 16 * seqs * heads + 64

@@ -26,15 +26,17 @@ struct ChooseParams {
   const float* weights;
   const int32_t *positions, *kv_lens, *table, *num_seqs, *dropped;
   int32_t* moves;
-  uint32_t* keys;    // of rows past kChooseRows: for each (sequence, head) `stride` keys, then `counts`' blocks
-  uint32_t* counts;  // 2048 for each block of kKeyRows
   uint32_t* found;   // of each (sequence, head): the budget-th largest key (first its first digit) and its rank among those
+  struct Long* longs;  // of each sequence
+  // of each block of a long sequence's head, kKeyRows rows:
+  uint32_t* keys;
   uint32_t* near;    // the keys that have the first digit: those of each kSegment rows at their beginning,
   uint32_t* held;    // so many
-  uint32_t* tallies; // a Tally for each block of kKeyRows
-  long long stride;
+  uint32_t* counts;  // kDigits
+  uint32_t* tallies; // a Tally
   int N, PPS, Hkv, P, S, budget, limit, sinks, recent, M;
   int first;         // the launch's first sequence
+  int block_room;    // blocks of a head that the workspace holds
   int room;          // keys that fit a workgroup's LDS
   int quads;         // four neighbouring entries from a multiple of four on are 16 aligned bytes of one page
 };
@@ -50,17 +52,48 @@ constexpr int kChooseRows = 32768;
 constexpr int kKeyRows = 4096, kSegment = kKeyRows / 4;  // a wave's rows of a block
 constexpr int kDigits = 2048;       // 11 bits, 11 bits, 10 bits
 
-// A sequence that is cut: its rows (0: it is not), and the position past its last.
+// The rows of a sequence of `len` keys, 0 where it is not cut.
+__device__ __forceinline__ int rows_cut(const ChooseParams& p, int len) {
+  const int n = min(len, p.PPS * p.S);
+  return len > p.limit && n > p.budget ? n : 0;
+}
+
+// A sequence that is cut: its rows, and the position past its last.
 struct Cut {
   int rows;
   long long end;
 };
 __device__ __forceinline__ Cut cut_of(const ChooseParams& p, int seq, bool flag) {
   const int count = *p.num_seqs, len = p.kv_lens[seq], gone = p.dropped ? p.dropped[seq] : 0;
-  const int capacity = p.PPS * p.S;
-  const int n = p.first + seq < count ? len : 0;
-  if (flag && n > capacity) flag_error(RPA_SPARSE_ERR_LEN);
-  return {n > p.limit && min(n, capacity) > p.budget ? min(n, capacity) : 0, (long long)n + gone};
+  const int n = seq < count ? len : 0;
+  if (flag && n > p.PPS * p.S) flag_error(RPA_SPARSE_ERR_LEN);
+  return {rows_cut(p, n), (long long)n + gone};
+}
+
+// Long sequences' blocks lie one sequence behind the other, so that the workspace holds what the pool's rows need and
+// not what the table has room for (64 requests of 2100 keys with tables of 131072 rows, 8 heads: 672 MB by the table).
+// Distinct pages cannot have more.  A sequence that finds no room all the same, as others hold its pages too, is
+// done by one workgroup a head from the ledger.
+__device__ __forceinline__ int blocks_of(int rows) { return (rows + kKeyRows - 1) / kKeyRows; }
+
+struct Long {
+  int rows;   // 0: all its keys fit LDS, or its blocks have no room
+  int place;  // its first block, of as many as one head has
+  __device__ __forceinline__ size_t block0(const ChooseParams& p, int h) const {
+    return (size_t)place * p.Hkv + (size_t)h * blocks_of(rows);
+  }
+};
+
+// A sequence's, by each wave for itself.
+__device__ __forceinline__ Long long_of(const ChooseParams& p, int seq, int rows) {
+  const int count = *p.num_seqs;
+  long long before = 0;
+  for (int i = threadIdx.x % 64; i < min(seq, count); i += 64) {
+    const int n = rows_cut(p, p.kv_lens[i]);
+    before += n > p.room ? blocks_of(n) : 0;
+  }
+  for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
+  return before + blocks_of(rows) <= p.block_room ? Long{rows, (int)before} : Long{0, 0};
 }
 
 // Four rows' keys, from `row` (a multiple of four) on; rows from n on are 0.
@@ -183,12 +216,20 @@ struct Lister {
 // Keys of long sequences, and how many of a block's rows have each first digit.
 __global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
   __shared__ uint32_t s_count[kDigits];
-  const int tid = threadIdx.x, h = blockIdx.y % p.Hkv, seq = blockIdx.y / p.Hkv, first = blockIdx.x * kKeyRows;
+  const int tid = threadIdx.x, h = blockIdx.y % p.Hkv, seq = p.first + blockIdx.y / p.Hkv, first = blockIdx.x * kKeyRows;
   const Cut cut = cut_of(p, seq, false);
-  if (cut.rows <= p.room || first >= cut.rows) return;  // uniform
+  const bool lead = first == 0 && h == 0;
+  if (cut.rows <= p.room || first >= cut.rows) {  // uniform
+    if (lead && tid == 0) p.longs[seq] = Long{0, 0};
+    return;
+  }
+  const Long its = long_of(p, seq, cut.rows);
+  if (lead && tid == 0) p.longs[seq] = its;
+  if (!its.rows) return;  // uniform
   for (int i = tid; i < kDigits; i += 256) s_count[i] = 0;
   __syncthreads();
-  uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
+  const size_t block0 = its.block0(p, h);
+  uint32_t* const keys = p.keys + block0 * kKeyRows;
 #pragma unroll
   for (int i = 0; i < kKeyRows / 1024; ++i) {
     const int row = first + 1024 * i + 4 * tid;
@@ -199,7 +240,7 @@ __global__ __launch_bounds__(256) void choose_keys_kernel(ChooseParams p) {
       if (row + u < cut.rows) atomicAdd(&s_count[key[u] >> 21], 1u);
   }
   __syncthreads();
-  uint32_t* const counts = p.counts + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * kDigits;
+  uint32_t* const counts = p.counts + (block0 + blockIdx.x) * kDigits;
   for (int i = tid; i < kDigits; i += 256) counts[i] = s_count[i];
 }
 
@@ -238,8 +279,9 @@ __device__ __forceinline__ void next_digit(ChooseShared& sh, int bits, uint32_t&
   prefix = sh.found[0], rank = sh.found[1];
 }
 
-// The budget-th largest of keys in LDS, and which one it is of the rows at it: its digits one after another.
-template <int THREADS>
+// The budget-th largest of keys in LDS (HELD; the first digit brings them there) or of the ledger's, and which one it
+// is of the rows at it: its digits one after another.
+template <int THREADS, bool HELD>
 __device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, int h, const int32_t* table, uint32_t* s_keys,
                                          ChooseShared& sh, uint32_t& prefix, uint32_t& rank) {
   const int tid = threadIdx.x, n = cut.rows;
@@ -249,9 +291,9 @@ __device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, 
     __syncthreads();
     for (int row = 4 * tid; row < n; row += 4 * THREADS) {
       u32x4 key;
-      if (shift == 21) {
+      if (!HELD || shift == 21) {
         key = keys_at(p, table, h, cut, row);
-        *(u32x4*)(s_keys + row) = key;
+        if (HELD) *(u32x4*)(s_keys + row) = key;
       } else {
         key = *(const u32x4*)(s_keys + row);
       }
@@ -264,12 +306,12 @@ __device__ __forceinline__ void find_key(const ChooseParams& p, const Cut& cut, 
   }
 }
 
-// Of a long sequence: the first digit, from the blocks' counts.
+// Of a long sequence: the first digit, from the counts of its blocks from block0 on.
 template <int THREADS>
-__device__ __forceinline__ void first_digit(const ChooseParams& p, int n, int blocks, ChooseShared& sh) {
+__device__ __forceinline__ void first_digit(const ChooseParams& p, int n, size_t block0, ChooseShared& sh) {
   constexpr int kBins = kDigits / THREADS;
-  const int tid = threadIdx.x, used = (n + kKeyRows - 1) / kKeyRows;
-  const uint32_t* const from = p.counts + (size_t)blockIdx.x * blocks * kDigits + tid * kBins;
+  const int tid = threadIdx.x, used = blocks_of(n);
+  const uint32_t* const from = p.counts + block0 * kDigits + tid * kBins;
   uint32_t sum[kBins] = {};
 #pragma unroll 16
   for (int b = 0; b < used; ++b)
@@ -285,11 +327,14 @@ __device__ __forceinline__ void first_digit(const ChooseParams& p, int n, int bl
 // Long sequences: the keys that have it, each wave's at the beginning of its rows'.
 __global__ __launch_bounds__(256) void choose_near_kernel(ChooseParams p) {
   const int lane = threadIdx.x % 64, segment = blockIdx.x * 4 + threadIdx.x / 64, from = segment * kSegment + 4 * lane;
-  const int n = cut_of(p, blockIdx.y / p.Hkv, false).rows;
-  if (n <= p.room || segment * kSegment >= n) return;
-  const uint32_t prefix = p.found[2 * (size_t)blockIdx.y];
-  const uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
-  uint32_t* const to = p.near + (size_t)blockIdx.y * p.stride + segment * kSegment;
+  const int seq = p.first + blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
+  const Long its = p.longs[seq];
+  const uint32_t prefix = p.found[2 * ((size_t)seq * p.Hkv + h)];  // beside it; of no meaning where there are no rows
+  const int n = its.rows;
+  if (segment * kSegment >= n) return;
+  const size_t block0 = its.block0(p, h);
+  const uint32_t* const keys = p.keys + block0 * kKeyRows;
+  uint32_t* const to = p.near + block0 * kKeyRows + segment * kSegment;
   u32x4 key[kSegment / 256];
 #pragma unroll
   for (int x = 0; x < kSegment / 256; ++x)
@@ -304,17 +349,18 @@ __global__ __launch_bounds__(256) void choose_near_kernel(ChooseParams p) {
       if (is) to[held + __popcll(votes & ((1ull << lane) - 1))] = key[x][u];
       held += __popcll(votes);
     }
-  if (lane == 0) p.held[(size_t)blockIdx.y * gridDim.x * 4 + segment] = held;
+  if (lane == 0) p.held[block0 * (kKeyRows / kSegment) + segment] = held;
 }
 
 // Long sequences: the other digits, from those keys, a segment a wave at a time.
-__global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p, int blocks) {
+__global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p) {
   constexpr int kAhead = 8;  // segments whose first keys are in flight
   __shared__ ChooseShared sh;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut_of(p, blockIdx.x / p.Hkv, false).rows;
-  if (n <= p.room) return;  // uniform
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = p.longs[blockIdx.x / p.Hkv].rows;
+  if (!n) return;  // uniform
+  const size_t block0 = p.longs[blockIdx.x / p.Hkv].block0(p, blockIdx.x % p.Hkv);
   const int segments = (n + kSegment - 1) / kSegment;
-  const uint32_t *const held = p.held + (size_t)blockIdx.x * blocks * 4, *const keys = p.near + (size_t)blockIdx.x * p.stride;
+  const uint32_t *const held = p.held + block0 * (kKeyRows / kSegment), *const keys = p.near + block0 * kKeyRows;
   uint32_t prefix = p.found[2 * (size_t)blockIdx.x], rank = p.found[2 * (size_t)blockIdx.x + 1];
   for (int shift = 10, bits = 11; shift >= 0; shift -= 10, bits = 10) {
     for (int i = tid; i < kDigits; i += 1024) sh.count[i] = 0;
@@ -328,7 +374,7 @@ __global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p, int b
       for (int x = 0; x < kAhead; ++x) {
         const int segment = base + 16 * x;
         most[x] = segment < segments ? held[segment] : 0;
-        if (segment < segments) key[x] = keys[(size_t)segment * kSegment + lane];  // counted or not: it is there, or near enough
+        if (segment < segments) key[x] = keys[(size_t)segment * kSegment + lane];  // counted or not: a segment has its room
       }
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
@@ -341,14 +387,15 @@ __global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p, int b
   if (tid == 0) p.found[2 * (size_t)blockIdx.x] = prefix, p.found[2 * (size_t)blockIdx.x + 1] = rank;
 }
 
-// The list of rows whose keys are in LDS: every wave has a stretch of rows.
-template <int THREADS>
-__device__ __forceinline__ int list_rows(const ChooseParams& p, int n, const uint32_t* s_keys, ChooseShared& sh, Lister out) {
+// The list of rows whose keys are in LDS (HELD) or the ledger's: every wave has a stretch of rows.
+template <int THREADS, bool HELD>
+__device__ __forceinline__ int list_rows(const ChooseParams& p, const Cut& cut, int h, const uint32_t* s_keys, ChooseShared& sh, Lister out) {
   constexpr int kWaves = THREADS / 64;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut.rows;
+  const auto key_at = [&](int row) { return HELD ? *(const u32x4*)(s_keys + row) : keys_at(p, out.table, h, cut, row); };
   const int stretch = ((n + kWaves - 1) / kWaves + 255) / 256 * 256, from = min(wave * stretch, n), to = min(from + stretch, n);
   Tally own = {};
-  for (int row = from + 4 * lane; row < to; row += 256) own.rows(row, *(const u32x4*)(s_keys + row), n, p.budget, out.bound);
+  for (int row = from + 4 * lane; row < to; row += 256) own.rows(row, key_at(row), n, p.budget, out.bound);
   own.of_wave();
   if (lane == 0) sh.waves[wave] = own;
   __syncthreads();
@@ -360,7 +407,7 @@ __device__ __forceinline__ int list_rows(const ChooseParams& p, int n, const uin
   out.start(before, all.same_low);
   for (int base = from; base < to; base += 256) {
     const int row = base + 4 * lane;
-    out.rows(p, row, lane, row < to ? *(const u32x4*)(s_keys + row) : u32x4{0, 0, 0, 0}, to);
+    out.rows(p, row, lane, row < to ? key_at(row) : u32x4{0, 0, 0, 0}, to);
   }
   const uint32_t moved = out.moved(all);
   if (moved > (uint32_t)p.M && tid == 0) flag_error(RPA_SPARSE_ERR_LEN);
@@ -369,19 +416,23 @@ __device__ __forceinline__ int list_rows(const ChooseParams& p, int n, const uin
 
 // One workgroup a (kv head, sequence).  A step's loads are of 256 rows a wave, four neighbouring rows a lane.
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void choose_rows_kernel(ChooseParams p, int blocks) {
+__global__ __launch_bounds__(THREADS) void choose_rows_kernel(ChooseParams p) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ ChooseShared s_rest;
   const int h = blockIdx.x % p.Hkv, seq = blockIdx.x / p.Hkv;
   const int32_t* const table = p.table + (size_t)seq * p.PPS;
   int32_t* const list = p.moves + (size_t)blockIdx.x * p.M * 2;
+  const Long its = THREADS == 1024 && p.block_room ? p.longs[seq] : Long{0, 0};
   const Cut cut = cut_of(p, seq, threadIdx.x == 0);
   uint32_t bound, rank;
-  if (THREADS == 1024 && cut.rows > p.room) return first_digit<THREADS>(p, cut.rows, blocks, s_rest);  // the rest by blocks
   int done = 0;  // entries of the list
-  if (cut.rows) {
-    find_key<THREADS>(p, cut, h, table, s_keys, s_rest, bound, rank);
-    done = list_rows<THREADS>(p, cut.rows, s_keys, s_rest, Lister{list, table, bound, rank});
+  if (THREADS == 1024 && cut.rows > p.room) {
+    if (its.rows) return first_digit<THREADS>(p, its.rows, its.block0(p, h), s_rest);  // the rest by blocks
+    find_key<THREADS, false>(p, cut, h, table, s_keys, s_rest, bound, rank);
+    done = list_rows<THREADS, false>(p, cut, h, s_keys, s_rest, Lister{list, table, bound, rank});
+  } else if (cut.rows) {
+    find_key<THREADS, true>(p, cut, h, table, s_keys, s_rest, bound, rank);
+    done = list_rows<THREADS, true>(p, cut, h, s_keys, s_rest, Lister{list, table, bound, rank});
   }
   for (long long i = 2ll * done + threadIdx.x; i < 2ll * p.M; i += THREADS) list[i] = -1;
 }
@@ -392,13 +443,15 @@ template <bool LIST>
 __global__ __launch_bounds__(256) void choose_list_kernel(ChooseParams p) {
   constexpr int kSteps = kKeyRows / 1024;
   __shared__ Tally s_waves[4], s_before[4], s_all[4];
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, seq = blockIdx.y / p.Hkv;
-  const Cut cut = cut_of(p, seq, false);
-  const int n = cut.rows, used = (n + kKeyRows - 1) / kKeyRows, block = blockIdx.x;
-  if (n <= p.room || block >= used) return;  // uniform
-  Tally* const tallies = (Tally*)p.tallies + (size_t)blockIdx.y * gridDim.x;
-  const uint32_t bound = p.found[2 * (size_t)blockIdx.y], rank = p.found[2 * (size_t)blockIdx.y + 1];
-  const uint32_t* const keys = p.keys + (size_t)blockIdx.y * p.stride;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, seq = p.first + blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
+  const Long its = p.longs[seq];
+  const size_t of = (size_t)seq * p.Hkv + h;
+  const uint32_t bound = p.found[2 * of], rank = p.found[2 * of + 1];
+  const int n = its.rows, used = blocks_of(n), block = blockIdx.x;
+  if (block >= used) return;  // uniform
+  const size_t block0 = its.block0(p, h);
+  Tally* const tallies = (Tally*)p.tallies + block0;
+  const uint32_t* const keys = p.keys + block0 * kKeyRows;
   const int from = block * kKeyRows + wave * (kKeyRows / 4) + 4 * lane;
   u32x4 key[kSteps];
 #pragma unroll
@@ -430,7 +483,7 @@ __global__ __launch_bounds__(256) void choose_list_kernel(ChooseParams p) {
     before.add(s_before[w]), all.add(s_all[w]);
     if (w < wave) before.add(s_waves[w]);
   }
-  int32_t* const list = p.moves + (size_t)blockIdx.y * p.M * 2;
+  int32_t* const list = p.moves + of * p.M * 2;
   Lister out = {list, p.table + (size_t)seq * p.PPS, bound, rank};
   out.start(before, all.same_low);
 #pragma unroll
@@ -544,9 +597,9 @@ int check_choose(const rpa_choose_shape_t* s) {
 }
 
 struct ChoosePlan {
-  int threads, room, blocks;  // blocks 0: all keys fit LDS
-  long long stride;
-  size_t keys, near, counts, found, held, bytes;  // bytes up to the end of each
+  int threads, room;
+  int blocks, block_room;  // of the longest sequence that the table has room for (0: all keys fit LDS), and of the workspace
+  size_t longs, keys, near, held, counts, tallies, bytes;  // where each begins
 };
 
 // Waves of a workgroup: sixteen while every list has a CU to itself (256 lists of 4096 rows: 13.0 us, 16.6 with four; of
@@ -558,15 +611,21 @@ ChoosePlan plan_choose(const rpa_choose_shape_t& s) {
   r.threads = capacity > (s.max_num_seqs * (long long)s.num_kv_heads <= 256 ? 1024 : 8192) ? 1024 : 256;
   r.room = (int)((capacity < kChooseRows ? capacity : kChooseRows) + 3) / 4 * 4;
   if (capacity > kChooseRows) {
+    const long long N = s.max_num_seqs, rows = (long long)s.total_pages * s.page_size;
     r.blocks = (int)((capacity + kKeyRows - 1) / kKeyRows);
-    r.stride = (capacity + 3) / 4 * 4;
-    r.keys = (size_t)s.max_num_seqs * s.num_kv_heads * r.stride * 4;
-    const size_t lists = (size_t)s.max_num_seqs * s.num_kv_heads;
-    r.near = 2 * r.keys + 256;  // a wave reads 64 keys of a segment, also past the last one's
-    r.counts = r.near + lists * r.blocks * kDigits * 4;
-    r.found = r.counts + (lists * 8 + 15) / 16 * 16;
-    r.held = r.found + lists * r.blocks * 16;
-    r.bytes = r.held + lists * r.blocks * sizeof(Tally);
+    // distinct pages: long sequences have at most the pool's rows, and each all but one of its blocks whole
+    const long long most = rows / (kChooseRows + 1), longest = N < most ? N : most;
+    const long long by_pool = (rows + (kKeyRows - 1) * longest) / kKeyRows, by_table = N * r.blocks;
+    r.block_room = (int)(by_pool < by_table ? by_pool : by_table);
+    if (!longest) r.block_room = 0;
+    const size_t lists = (size_t)N * s.num_kv_heads, room = (size_t)r.block_room * s.num_kv_heads;
+    r.longs = (lists * 8 + 15) / 16 * 16;
+    r.keys = r.longs + ((size_t)N * sizeof(Long) + 15) / 16 * 16;
+    r.near = r.keys + room * kKeyRows * 4;
+    r.held = r.near + room * kKeyRows * 4;
+    r.counts = r.held + room * (kKeyRows / kSegment) * 4;
+    r.tallies = r.counts + room * kDigits * 4;
+    r.bytes = r.tallies + room * sizeof(Tally);
   }
   return r;
 }

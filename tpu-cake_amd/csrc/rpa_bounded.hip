@@ -195,13 +195,14 @@ int rpa_choose_moves(const rpa_choose_shape_t* shape, const float* weights, cons
   if ((rc = check_separate({"moves", moves, 8 * N * s.num_kv_heads * s.max_moves}, in))) return rc;
   ChooseParams p = {};
   p.weights = weights, p.positions = positions, p.kv_lens = kv_lens, p.table = page_indices, p.num_seqs = num_seqs;
-  p.dropped = dropped, p.moves = moves, p.keys = (uint32_t*)workspace, p.stride = plan.stride;
+  p.dropped = dropped, p.moves = moves;
   uint8_t* const base = (uint8_t*)workspace;
-  p.near = (uint32_t*)(base + plan.keys), p.counts = (uint32_t*)(base + plan.near), p.found = (uint32_t*)(base + plan.counts);
-  p.held = (uint32_t*)(base + plan.found), p.tallies = (uint32_t*)(base + plan.held);
+  p.found = (uint32_t*)base, p.longs = (Long*)(base + plan.longs), p.keys = (uint32_t*)(base + plan.keys);
+  p.near = (uint32_t*)(base + plan.near), p.held = (uint32_t*)(base + plan.held), p.counts = (uint32_t*)(base + plan.counts);
+  p.tallies = (uint32_t*)(base + plan.tallies);
   p.N = s.max_num_seqs, p.PPS = s.pages_per_seq, p.Hkv = s.num_kv_heads, p.P = s.total_pages, p.S = s.page_size;
   p.budget = s.budget, p.limit = s.limit, p.sinks = s.sinks, p.recent = s.recent, p.M = s.max_moves;
-  p.room = plan.room, p.quads = s.page_size % 4 == 0 && aligned16(weights) && aligned16(positions);
+  p.room = plan.room, p.block_room = plan.block_room, p.quads = s.page_size % 4 == 0 && aligned16(weights) && aligned16(positions);
   const unsigned lists = (unsigned)(N * s.num_kv_heads);
   const hipStream_t stream_ = (hipStream_t)stream;
   // a launch of long sequences' blocks: at most 65535 lists
@@ -209,24 +210,19 @@ int rpa_choose_moves(const rpa_choose_shape_t* shape, const float* weights, cons
     const unsigned step = 65535 / s.num_kv_heads * s.num_kv_heads;
     for (unsigned first = 0; first < lists; first += step) {
       ChooseParams part = p;
-      const unsigned seqs = first / s.num_kv_heads;
-      part.kv_lens += seqs, part.table += (size_t)seqs * s.pages_per_seq, part.dropped += dropped ? seqs : 0;
-      part.keys += first * (size_t)plan.stride, part.counts += (size_t)first * plan.blocks * kDigits, part.first = (int)seqs;
-      part.near += first * (size_t)plan.stride, part.held += (size_t)first * plan.blocks * 4;
-      part.found += 2 * (size_t)first, part.tallies += (size_t)first * plan.blocks * (sizeof(Tally) / 4);
-      part.moves += (size_t)first * s.max_moves * 2;
+      part.first = (int)(first / s.num_kv_heads);
       kernel<<<dim3(plan.blocks, lists - first < step ? lists - first : step), 256, 0, stream_>>>(part);
       if (const int bad = launched(name)) return bad;
     }
     return (int)RPA_OK;
   };
   const size_t lds = (size_t)plan.room * 4;
-  if (plan.blocks && (rc = by_blocks(choose_keys_kernel, "choose_moves (keys)"))) return rc;
-  if (plan.threads == 256) choose_rows_kernel<256><<<lists, 256, lds, stream_>>>(p, plan.blocks);
-  else choose_rows_kernel<1024><<<lists, 1024, lds, stream_>>>(p, plan.blocks);
-  if ((rc = launched("choose_moves")) || !plan.blocks) return rc;
+  if (plan.block_room && (rc = by_blocks(choose_keys_kernel, "choose_moves (keys)"))) return rc;
+  if (plan.threads == 256) choose_rows_kernel<256><<<lists, 256, lds, stream_>>>(p);
+  else choose_rows_kernel<1024><<<lists, 1024, lds, stream_>>>(p);
+  if ((rc = launched("choose_moves")) || !plan.block_room) return rc;
   if ((rc = by_blocks(choose_near_kernel, "choose_moves (near keys)"))) return rc;
-  choose_last_kernel<<<lists, 1024, 0, stream_>>>(p, plan.blocks);
+  choose_last_kernel<<<lists, 1024, 0, stream_>>>(p);
   if ((rc = launched("choose_moves (digits)")) || (rc = by_blocks(choose_list_kernel<false>, "choose_moves (tallies)"))) return rc;
   return by_blocks(choose_list_kernel<true>, "choose_moves (list)");
 }
