@@ -55,6 +55,21 @@ __device__ __forceinline__ TileOf tile_at(const WeighParams& p, const Sequence& 
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// Whether 16 bytes of values hold an infinity or NaN.
+template <bool FP8>
+__device__ __forceinline__ bool not_finite(const u32x4& v) {
+  bool is = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (FP8) {  // 0x7f and 0xff: adding 1 to the other seven bits carries into the eighth
+      is |= ((v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    } else {
+      is |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  return is;
+}
+
 template <int DP, bool FULL, bool FP8>
 __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_kernel(WeighParams p) {
   constexpr int kKeys = DP > 128 ? 32 : 64;  // of a turn
@@ -68,7 +83,7 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_slot[4][kKeys];
   __shared__ float s_ks[2][kKeys], s_vs[2][kKeys];
-  __shared__ int s_bad, s_again;
+  __shared__ int s_bad, s_again, s_late;
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), n = lane % 32, half = lane / 32;
   const Share share = share_of<true>(p, blockIdx.x, gridDim.x, [&](const Sequence& s, bool pad) { return all_slots(p, s, pad); });
   JoinOf* const joins = p.joins + p.rows_grid;
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
         if (FP8 && tid < kKeys) s_ks[unit & 1][tid] = ks, s_vs[unit & 1][tid] = vs;
       };
       __syncthreads();  // the last use of LDS
-      if (tid == 0) s_bad = 0;
+      if (tid == 0) s_bad = s_again = s_late = 0;
       __syncthreads();
       if (tid < kKeys && units > 0) {
         keep(0, page_of(0));
@@ -310,7 +325,9 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
         }
     };
     // Keys that some columns see and others do not may hold infinities or NaN as values, which P = 0 does not silence:
-    // where a result is not finite the tile is done again token by token, each reading its own keys only.
+    // where a result is not finite and such a value is there (at most kColumns - 1 keys), the tile is done again token by
+    // token, each reading its own keys only.  Results that are not finite for another reason, a query or a value that all
+    // columns see, stand: 1 + kColumns / G passes would find them again.
     const int first_token = div_by(tile.j * kColumns, p.group);
     const int last_token = div_by(min(tile.j * kColumns + kColumns - 1, end_row - 1), p.group);
 #pragma unroll 1
@@ -323,11 +340,21 @@ __global__ __launch_bounds__(kWeighThreads, DP > 128 ? 1 : 2) void weigh_tiles_k
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) finite &= fabsf(o[d][r]) < __builtin_inff();
-        if (tid == 0) s_again = 0;
+        if (live && !finite) s_again = 1;
         __syncthreads();
-        if (!finite) s_again = 1;
-        __syncthreads();
-        if (s_again) continue;
+        if (s_again) {
+          const int begin = max(from, old + first_token + 1);
+#pragma unroll 1
+          for (int i = tid; i < (to - begin) * kHalf; i += kWeighThreads) {
+            const int key = begin + i / kHalf, byte = 16 * (i % kHalf), page = div_by(key, p.page), id = table[page];
+            if (id < 0 || id >= p.P || byte >= row_bytes) continue;
+            const u32x4 v = load16(rows + (uint32_t)(id * p.S + (key - page * p.S)) * row_stride + row_bytes + byte);
+            if (not_finite<FP8>(v) || (FP8 && p.scales && !(fabsf(p.scales[((size_t)id * p.Hkv + h) * 2 + 1]) < __builtin_inff())))
+              s_late = 1;
+          }
+          __syncthreads();
+          if (s_late) continue;
+        }
       }
       write(all ? -1 : only);
       if (all) break;
