@@ -673,7 +673,8 @@ WeighPlan plan_weigh(const rpa_weigh_shape_t& s) {
   const long long work = most(rows / r.near, (capacity >> r.block_shift) + 1);
   r.rows_grid = (int)(work < kRowsGrid ? work : kRowsGrid);
   const long long seqs = s.num_tokens < s.max_num_seqs ? s.num_tokens : s.max_num_seqs;
-  const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1), spread = most(seqs * s.num_kv_heads, capacity / 64 + 1);
+  const long long blocks = most(seqs * s.num_kv_heads, capacity / 128 + 1);
+  const long long spread = most(seqs * s.num_kv_heads, capacity / (dims == 256 ? 32 : 64) + 1);  // of a wave's keys
   r.keys_grid = (int)(spread <= kSpread ? spread : blocks < kKeysGrid ? blocks : kKeysGrid);
   r.weigh_grid = (int)(blocks < kWeighGrid ? blocks : kWeighGrid);
   r.stats = ((size_t)s.num_tokens * s.num_q_heads * sizeof(float2) + 15) / 16 * 16;
