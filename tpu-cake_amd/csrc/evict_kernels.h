@@ -2,7 +2,7 @@
 //
 // Mathematics: a row's key is its weight as an unsigned whole number of the same order (0 for NaN), the largest of all for
 // rows that stay in any case.  The budget-th largest key of a (sequence, head) is found digit by digit: counts of the
-// next bits over the rows that share the bits so far, four times.  Rows above it stay, and of the rows at it
+// next bits over the rows that share the bits so far, three times.  Rows above it stay, and of the rows at it
 // the lowest ones, as many as fit.  Kept rows at or past `budget` and rows below it that go are equally many: the i-th of the
 // one take the places of the i-th of the other.  Counts are whole numbers, so nothing depends on an order.
 //
@@ -10,11 +10,11 @@
 // first gap; the ledger's positions tell the recent rows.  Moves read past the budget and write before it: they
 // do not meet, and a list that is applied twice gives the same.
 //
-// Latency bounds the choice: 512 lists of 2112 rows read 5 MB and take 14.5 us, three passes over keys in LDS with a barrier
-// or two each; 24 lists of 105 000 to 126 000 rows (23 MB, 4 us at 6.3 TB/s) take 48 us: keys and their first digits 14,
-// the digits 10 + 4 + 7, tallies 5, the list 12.  Moves are copies: 64 lists of 8 heads, 64 entries each at most, 11 MB, 5.6 us;
-// six fp8 prompts' 2048 entries a head, 49 MB, 7.8 us at 6.3 TB/s, 20: rows of 256 bytes at random places, scales of both
-// pages beside them.
+// Latency bounds the choice: 512 lists of 2112 rows read 5 MB and take 15 us, three passes over keys in LDS with a barrier
+// or two each; 24 lists of 105 000 to 126 000 rows (23 MB, 4 us at 6.3 TB/s) take 49 us: keys and their first digits 14,
+// the digits 10 + 4 + 7, tallies 4, the list 12.  Moves are copies: 64 lists of 8 heads, 64 entries each at most, 11 MB, 5.6 us;
+// six fp8 prompts' 2048 entries a head, 49 MB, 7.8 us at 6.3 TB/s, 20 where rows change their scale and 9.6 where all
+// pages have one: a full division a value makes it five times the vector instructions.
 #pragma once
 
 #include "attend_kernels.h"
@@ -47,7 +47,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) { return w == w ? ordere
 // Rows of a sequence whose keys fit LDS: one workgroup does all (48 lists of 32768: 36 us, 37 by blocks; 512: 92 and 119; of
 // 16384: 23 and 33, 53 and 82).  Past them its VALU would be what counts (24 lists of 131072: 132 us), so all that goes over
 // rows is done by blocks of kKeyRows, and one workgroup a list sums the blocks' counts and goes over the keys that share
-// the first digit: 48 us in six launches.
+// the first digit: 49 us in six launches.  Which of them run follows the table's width, the only length the host knows: 512
+// lists of 2112 rows take 15 us in a table as wide and 44 in one of 131072 rows, 22 of them in the rows kernel, whose 128 KB
+// of LDS leave one list a CU, and the rest in launches that find nothing.
 constexpr int kChooseRows = 32768;
 constexpr int kKeyRows = 4096, kSegment = kKeyRows / 4;  // a wave's rows of a block
 constexpr int kDigits = 2048;       // 11 bits, 11 bits, 10 bits
@@ -389,7 +391,8 @@ __global__ __launch_bounds__(1024) void choose_last_kernel(ChooseParams p) {
 
 // The list of rows whose keys are in LDS (HELD) or the ledger's: every wave has a stretch of rows.
 template <int THREADS, bool HELD>
-__device__ __forceinline__ int list_rows(const ChooseParams& p, const Cut& cut, int h, const uint32_t* s_keys, ChooseShared& sh, Lister out) {
+__device__ __forceinline__ int list_rows(const ChooseParams& p, const Cut& cut, int h, const uint32_t* s_keys, ChooseShared& sh,
+                                         Lister out) {
   constexpr int kWaves = THREADS / 64;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n = cut.rows;
   const auto key_at = [&](int row) { return HELD ? *(const u32x4*)(s_keys + row) : keys_at(p, out.table, h, cut, row); };

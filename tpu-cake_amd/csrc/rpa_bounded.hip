@@ -4,8 +4,6 @@
 #include <stdarg.h>
 #include <stdio.h>
 
-#include <type_traits>
-
 #include "rpa_bounded.h"
 
 #include "evict_kernels.h"

@@ -9,10 +9,10 @@
 // tiles (where a step may have chunks), joins of parts with the weights of rows, weights of chunks.
 //
 // HBM bounds rows.  64 sequences of 1024 to 8192 keys, 64 heads of 128 over 8, bf16: 855 MB, 136 us at the 6.3 TB/s of a plain
-// read; 191 to 198 us, of which rows 170 (845 MB read, 63 MB of scores written: 5.3 TB/s) and weights 24.  Without their scores
-// rows took 136, without any product 132 to 140: it is the mixed stores that cost.  Two sequences of 245 000 keys, 32
-// heads, fp8 pages of 16: 1.03 GB, 163 us; 277, of which rows 249 (4.3 TB/s; their loads alone take 195, the conversions and
-// the three products of P do not hide entirely) and weights 36.
+// read; 191 to 198 us, of which rows 170 (845 MB read, 52 MB of scores and 10 MB of parts written: 5.3 TB/s) and weights 24.
+// Without their scores rows took 136, without any product 132 to 140: it is the mixed stores that cost.  Two sequences of
+// 245 000 keys, 32 heads, fp8 pages of 16: 1.03 GB, 163 us; 277, of which rows 249 (4.3 TB/s; their loads alone take 195, the
+// conversions and the three products of P do not hide entirely) and weights 36.
 //
 // Tried for rows and not kept: loads that stay in the caches (191 us where nontemporal ones take 168); a barrier that
 // keeps the heads' waves at the same keys (195 and 191; fp8 230 and 195 for the loads); scores through LDS, at other

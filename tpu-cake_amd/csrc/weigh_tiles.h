@@ -420,13 +420,16 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_finish_kernel(WeighParams
 // The weights of the sequences that tiles did, 256 keys of a kv head at a time, 64 a wave, whose K stays in registers
 // as the products' A operand while every row (token, head) that sees one of them passes through LDS, kWeighRows at a time:
 // the scores once more.  A lane sums its keys over its columns, and lanes meet once at the end.
-// The two chunks above: 97 GFLOP, 88 us; 160, the exponentials beside the products.  32 keys a wave take 205 to 235 us where 64
+// The two chunks above: 97 GFLOP, 88 us; 160, the exponentials beside the products.  fp8 takes 1.4 times as long as bf16 (388 us
+// and 284, two chunks of 777 tokens over 9900 and 15700 keys): a shuffle for each score's scale, and 5 registers spilled; 18 in
+// bf16 heads that do not fill 128 dims, which take what full ones do.  32 keys a wave take 205 to 235 us where 64
 // took 182, as each key pays the rows' reads from LDS.
 //
-// Where keys are few (at most kSpread blocks of 64), a workgroup has 64 and its waves take 32 rows each in turn, straight from
-// memory, as no two waves read the same: a prompt of 2000 tokens 363 to 187 us for the whole call, 175 tokens of 16 heads a
-// group over 400 keys 143 to 82, two chunks of 500 over 2000 keys 177 to 150.  With both in one kernel 64 sequences of 8 tokens over
-// 4000 keys take 435 us instead of 408; a launch for each costs all but those 2 to 5 us.
+// Where keys are few (at most kSpread blocks of a wave's keys: 64, or 32 for heads of 256), a workgroup has one such block and
+// its waves take 32 rows each in turn, straight from memory, as no two waves read the same: a prompt of 2000 tokens 363 to
+// 187 us for the whole call, 175 tokens of 16 heads a group over 400 keys 143 to 82, two chunks of 500 over 2000 keys 177 to
+// 150.  With both in one kernel 64 sequences of 8 tokens over 4000 keys take 435 us instead of 408; a launch for each costs all
+// but those 2 to 5 us.
 constexpr int kWeighRows = 64, kSpread = 1024;
 
 template <int DP, bool FULL, bool FP8>
